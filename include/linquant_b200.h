@@ -40,7 +40,8 @@ typedef enum { LQ_DECAY_NONE = 0, LQ_DECAY_SCALAR = 1, LQ_DECAY_DIAGONAL = 2 } l
 typedef void* lq_stream; /* a cudaStream_t */
 
 int lq_version(void);
-/* sizeof the two descriptor structs as the library was compiled: a binding checks its own layout against these (0 = zoo, 1 = ssd, 2 = workspace) */
+/* sizeof the descriptor structs as the library was compiled: a binding checks its own layout against these (0 = zoo, 1 = ssd,
+ * 2 = workspace, 3 = conv, 4 = scan, 5 = linear, 6 = norm) */
 unsigned long long lq_struct_bytes(int which);
 const char* lq_last_error_string(void);
 
@@ -277,6 +278,94 @@ int lq_ssd_split_rotate_quant(const void* xBC, int dtype, int B, int T, int d_ss
  * in_stride_t, y dense. Replaces kronecker_hadamard_fwd (kernels/hadamard.py:141-179). */
 int lq_kronecker_hadamard(const void* x, void* y, int dtype, int B, int T, int H, int D, long long in_stride_t,
                           const float* signs, lq_stream stream);
+
+/* ------------------------------------------------------------------------------------------------------------
+ * Operators around the recurrence of a layer: short causal convolution, selective scan, INT8 product, norms. Prompts
+ * ("fwd") and single tokens ("step", the cached state updated in place). Activations are f16, bf16 or f32 with contiguous
+ * channels and any token pitch (slices of a wider projection output); parameters are dense fp32. Strides are in elements.
+ * No counterpart in the reference's kernels.
+ * ------------------------------------------------------------------------------------------------------------ */
+typedef struct {
+  int B, T, D, W;              /* W taps (2..4); T = 1 for the step */
+  int dtype;                   /* of x, y and the states */
+  int silu;                    /* y = silu(sum) or the sum itself */
+  long long x_stride_b, x_stride_t;
+  const void* x;               /* [B,T,D] */
+  const float *weight, *bias;  /* [D,W], the last tap on the current token; [D] or null */
+  const void* initial_state;   /* fwd: [B,W-1,D], the inputs ahead of the first token, oldest first; null = zeros */
+  const int* lengths;          /* fwd: [B] tokens that count, clamped to 0..T; the rest of y is zero. null = T everywhere */
+  void* y;                     /* [B,T,D] dense */
+  void* final_state;           /* fwd: [B,W-1,D], the last W-1 inputs, or null */
+  void* state;                 /* step: [n_slots,W-1,D] */
+  const int* slots;            /* step: [B] row of `state` of each sequence, no row twice; one outside 0..n_slots-1 marks an
+                                  idle entry: y is zero and no state is touched. null = row b */
+  int n_slots;
+} lq_conv_problem;
+/* y[t] = act(bias + sum_i weight[i] x[t - W + 1 + i]) per channel */
+int lq_short_conv_fwd(const lq_conv_problem* p, lq_stream stream);
+int lq_short_conv_step(const lq_conv_problem* p, lq_stream stream);
+
+typedef struct {
+  int B, T, D, N, G;           /* D channels in G groups that share B and C; N states a channel (1..256) */
+  int H, P;                    /* step with one decay rate a head: D = H * P; H = 0: one rate per channel and state */
+  int dtype;                   /* of u, dt, z, B, C, y */
+  int state_dtype;             /* step: of `state` */
+  int softplus;                /* dt = clamp(softplus(dt + bias), dt_min, dt_max) or clamp(dt + bias, ..) */
+  float dt_min, dt_max;
+  long long u_stride_b, u_stride_t, dt_stride_b, dt_stride_t, z_stride_b, z_stride_t;
+  long long B_stride_b, B_stride_t, B_stride_g, C_stride_b, C_stride_t, C_stride_g;
+  const void *u, *dt, *z;      /* [B,T,D]; dt of the head form [B,H]; z or null: y *= silu(z) */
+  const void *Bm, *Cm;         /* [B,T,G,N] */
+  const float* A;              /* [D,N], or [H] in the head form: the decay of a step is exp(dt A) */
+  const float *skip, *dt_bias; /* [D] ([H] in the head form; skip also [H,P]) or null: y += skip u */
+  int skip_has_hdim;
+  const float* initial_state;  /* fwd: [B,D,N] or null */
+  const int* lengths;          /* fwd: as above */
+  void* y;                     /* [B,T,D] dense */
+  float* final_state;          /* fwd: [B,D,N] or null */
+  void* state;                 /* step: [n_slots,D,N] */
+  const int* slots;            /* step: as above */
+  int n_slots;
+} lq_scan_problem;
+/* h_t = exp(dt_t A) h_{t-1} + dt_t u_t B_t;  y_t = C_t . h_t + skip u_t;  states in fp32 */
+int lq_selective_scan_fwd(const lq_scan_problem* p, lq_stream stream);
+int lq_selective_scan_step(const lq_scan_problem* p, lq_stream stream);
+
+/* Symmetric INT8 codes of rows: scale = amax / 127, codes by the code rule; rows of codes at a pitch that is a multiple of 16
+ * bytes. A row of zeros has scale 0 and codes 0, one with an infinity or NaN a scale that is not finite. */
+int lq_quantize_rows(const void* x, int dtype, int rows, int D, long long x_stride, int8_t* codes, long long codes_stride, float* scale,
+                     lq_stream stream);
+
+typedef struct {
+  int M, N, K;                 /* K <= 131071: the INT32 sums are exact */
+  int out_dtype;
+  const int8_t *x, *w;         /* [M,K] and [N,K] codes, K contiguous, 16-byte aligned rows (bytes behind K are not used) */
+  long long x_stride, w_stride;
+  const float *x_scale, *w_scale, *bias; /* [M], [N], [N] or null */
+  void* y;                     /* [M,N] dense */
+  int* status;                 /* as in lq_ssd_problem */
+} lq_linear_problem;
+/* y[m,n] = (sum_k x[m,k] w[n,k]) x_scale[m] w_scale[n] + bias[n] */
+int lq_int8_linear(const lq_linear_problem* p, lq_stream stream);
+
+typedef struct {
+  int rows, D, group;          /* group: channels that are normed together (divides D; the gated form only, else D) */
+  int dtype, out_dtype;
+  int residual_f32;            /* the residual stream is fp32, not `dtype` */
+  int gate_first;              /* norm(x silu(gate)) weight, else norm(x) weight silu(gate) */
+  float eps, residual_scale;
+  long long x_stride, residual_stride, gate_stride;
+  const void *x, *residual, *gate;
+  const float *weight, *post_weight, *scale_vec; /* scale_vec [D] or null: a residual scale per channel, times residual_scale */
+  void* y;                     /* [rows,D] dense, or null when codes are wanted */
+  void* residual_out;          /* [rows,D] dense, in the residual's type; required with a residual */
+  int8_t* codes;               /* quantised output: rows at codes_stride bytes, and a scale a row */
+  long long codes_stride;
+  float* scale;
+} lq_norm_problem;
+/* r = residual + residual_scale P(x), P(x) = x or norm(x) post_weight;  y = norm(r) weight  (norm(x) weight without a residual) */
+int lq_rms_norm(const lq_norm_problem* p, lq_stream stream);
+int lq_gated_rms_norm(const lq_norm_problem* p, lq_stream stream);
 
 #ifdef __cplusplus
 }

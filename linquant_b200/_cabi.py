@@ -37,6 +37,33 @@ class ZooWorkspace(C.Structure):
     _fields_ = [(n, C.c_void_p) for n in ("qq", "kl", "kwT", "vlT", "vwT", "hT", "wq", "gc", "u", "fw", "amat", "genv", "gcl", "status")]
 
 
+def _fields(**groups):
+    return [(n, t) for t, names in ((getattr(C, "c_" + k.rstrip("_0123456789")), v) for k, v in groups.items()) for n in names.split()]
+
+
+class ConvProblem(C.Structure):
+    _fields_ = _fields(int="B T D W dtype silu", longlong="x_stride_b x_stride_t",
+                       void_p="x weight bias initial_state lengths y final_state state slots", int_2="n_slots")
+
+
+class ScanProblem(C.Structure):
+    _fields_ = _fields(int="B T D N G H P dtype state_dtype softplus", float="dt_min dt_max",
+                       longlong="u_stride_b u_stride_t dt_stride_b dt_stride_t z_stride_b z_stride_t B_stride_b B_stride_t B_stride_g "
+                                "C_stride_b C_stride_t C_stride_g",
+                       void_p="u dt z Bm Cm A skip dt_bias", int_2="skip_has_hdim",
+                       void_p_2="initial_state lengths y final_state state slots", int_3="n_slots")
+
+
+class LinearProblem(C.Structure):
+    _fields_ = _fields(int="M N K out_dtype", void_p="x w", longlong="x_stride w_stride", void_p_2="x_scale w_scale bias y status")
+
+
+class NormProblem(C.Structure):
+    _fields_ = _fields(int="rows D group dtype out_dtype residual_f32 gate_first", float="eps residual_scale",
+                       longlong="x_stride residual_stride gate_stride",
+                       void_p="x residual gate weight post_weight scale_vec y residual_out codes", longlong_2="codes_stride", void_p_2="scale")
+
+
 class LinQuantError(RuntimeError):
     pass
 

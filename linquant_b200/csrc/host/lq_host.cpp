@@ -375,11 +375,521 @@ PyObject* ssd_fwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// ------------------------------------------------------------------------------------------------ layer operators
+// An activation: on this device, of this type and rank, channels contiguous.
+const at::Tensor& act(const Call& c, PyObject* o, int64_t dim, at::ScalarType t) {
+  const at::Tensor& x = Call::tensor(o);
+  if (x.device() != c.dev || x.dim() != dim || x.scalar_type() != t || (x.size(dim - 1) > 1 && x.stride(dim - 1) != 1)) throw NotPlain{};
+  return x;
+}
+void expect(const at::Tensor& t, at::IntArrayRef shape) {
+  if (t.sizes() != shape) throw NotPlain{};
+}
+int extent(int64_t n) {
+  if (n < 0 || n >= (int64_t(1) << 31)) throw NotPlain{};
+  return (int)n;
+}
+bool flag(PyObject* o) {
+  if (o != Py_True && o != Py_False) throw NotPlain{};
+  return o == Py_True;
+}
+const int* int32(const Call& c, PyObject* o, int64_t n) {  // lengths, slots
+  if (o == Py_None) return nullptr;
+  const at::Tensor& t = Call::tensor(o);
+  if (t.device() != c.dev || t.dim() != 1 || t.size(0) != n || t.scalar_type() != at::kInt || !t.is_contiguous()) throw NotPlain{};
+  return t.const_data_ptr<int>();
+}
+at::Tensor empty(at::IntArrayRef shape, at::ScalarType t, at::Device dev) { return at::detail::empty_cuda(shape, t, dev, std::nullopt); }
+cudaStream_t stream_of(const Call& c) { return c10::cuda::getCurrentCUDAStream(c.dev.index()).stream(); }
+// A tensor whose leading axes are rows at one pitch
+struct Rows {
+  int64_t rows = 1, pitch = 0;
+  explicit Rows(const at::Tensor& t) {
+    const int64_t n = t.dim();
+    if (n < 1 || (t.size(n - 1) > 1 && t.stride(n - 1) != 1)) throw NotPlain{};
+    pitch = t.size(n - 1);
+    bool first = true;
+    for (int64_t i = n - 2; i >= 0; --i) {
+      if (t.size(i) != 1 && t.numel() > 0) {
+        if (first) pitch = t.stride(i);
+        else if (t.stride(i) != rows * pitch) throw NotPlain{};
+        first = false;
+      }
+      rows *= t.size(i);
+    }
+    if (first) pitch = t.size(n - 1);
+  }
+};
+PyObject* pair(PyObject* a, PyObject* b) {
+  PyObject* r = PyTuple_New(2);
+  PyTuple_SET_ITEM(r, 0, a);
+  PyTuple_SET_ITEM(r, 1, b);
+  return r;
+}
+
+// short_conv(x, weight, bias, silu, initial_state, lengths, want_state) -> (y, state or None) | status | None
+PyObject* short_conv(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  try {
+    if (n != 7) throw NotPlain{};
+    Call c;
+    const at::Tensor& x0 = Call::tensor(a[0]);
+    if (!x0.is_cuda() || x0.dim() != 3) throw NotPlain{};
+    c.dev = x0.device();
+    c.keep.reserve(4);
+    c10::cuda::CUDAGuard guard(c.dev);
+    const at::ScalarType t = x0.scalar_type();
+    const at::Tensor &x = act(c, a[0], 3, t), &w = Call::tensor(a[1]);
+    if (w.dim() != 2) throw NotPlain{};
+    const int64_t B = x.size(0), T = x.size(1), D = x.size(2), W = w.size(1);
+    lq_conv_problem p = {};
+    p.B = extent(B); p.T = extent(T); p.D = extent(D); p.W = extent(W);
+    p.dtype = out_code(t);
+    p.silu = flag(a[3]);
+    p.x_stride_b = x.stride(0); p.x_stride_t = x.stride(1);
+    p.x = x.const_data_ptr();
+    p.weight = c.f32(a[1], {D, W}, true);
+    p.bias = c.f32(a[2], {D}, true);
+    if (a[4] != Py_None) {
+      const at::Tensor& s = act(c, a[4], 3, t);
+      expect(s, {B, W - 1, D});
+      if (!s.is_contiguous()) throw NotPlain{};
+      p.initial_state = s.const_data_ptr();
+    }
+    p.lengths = int32(c, a[5], B);
+    const at::Tensor y = empty({B, T, D}, t, c.dev);
+    p.y = y.data_ptr();
+    at::Tensor state;
+    if (flag(a[6])) {
+      state = empty({B, W - 1, D}, t, c.dev);
+      p.final_state = state.data_ptr();
+    }
+    cudaStream_t st = stream_of(c);
+    int e;
+    {
+      NoGil ng;
+      e = lq_short_conv_fwd(&p, st);
+    }
+    if (e != LQ_OK) return PyLong_FromLong(e);
+    return pair(THPVariable_Wrap(y), state.defined() ? THPVariable_Wrap(state) : none());
+  } catch (const NotPlain&) {
+    Py_RETURN_NONE;
+  }
+  END_HANDLE_TH_ERRORS
+}
+
+// short_conv_step(x, state, weight, bias, silu, slots) -> y | status | None
+PyObject* short_conv_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  try {
+    if (n != 6) throw NotPlain{};
+    Call c;
+    const at::Tensor& x0 = Call::tensor(a[0]);
+    if (!x0.is_cuda() || x0.dim() != 2) throw NotPlain{};
+    c.dev = x0.device();
+    c.keep.reserve(4);
+    c10::cuda::CUDAGuard guard(c.dev);
+    const at::ScalarType t = x0.scalar_type();
+    const at::Tensor &x = act(c, a[0], 2, t), &state = act(c, a[1], 3, t);
+    const int64_t B = x.size(0), D = x.size(1), W = state.size(1) + 1;
+    if (state.size(2) != D || !state.is_contiguous()) throw NotPlain{};
+    lq_conv_problem p = {};
+    p.B = extent(B); p.T = 1; p.D = extent(D); p.W = extent(W);
+    p.dtype = out_code(t);
+    p.silu = flag(a[4]);
+    p.x_stride_b = x.stride(0);
+    p.x = x.const_data_ptr();
+    p.weight = c.f32(a[2], {D, W}, true);
+    p.bias = c.f32(a[3], {D}, true);
+    p.state = state.data_ptr();
+    p.n_slots = extent(state.size(0));
+    p.slots = int32(c, a[5], B);
+    const at::Tensor y = empty({B, D}, t, c.dev);
+    p.y = y.data_ptr();
+    cudaStream_t st = stream_of(c);
+    int e;
+    {
+      NoGil ng;
+      e = lq_short_conv_step(&p, st);
+    }
+    return e != LQ_OK ? PyLong_FromLong(e) : THPVariable_Wrap(y);
+  } catch (const NotPlain&) {
+    Py_RETURN_NONE;
+  }
+  END_HANDLE_TH_ERRORS
+}
+
+// selective_scan(u, dt, A, B, C, D, z, dt_bias, softplus, dt_min, dt_max, initial_state, lengths, want_state)
+//   -> (y, state or None) | status | None
+PyObject* selective_scan(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  try {
+    if (n != 14) throw NotPlain{};
+    Call c;
+    const at::Tensor& u0 = Call::tensor(a[0]);
+    if (!u0.is_cuda() || u0.dim() != 3) throw NotPlain{};
+    c.dev = u0.device();
+    c.keep.reserve(8);
+    c10::cuda::CUDAGuard guard(c.dev);
+    const at::ScalarType t = u0.scalar_type();
+    const at::Tensor &u = act(c, a[0], 3, t), &dt = act(c, a[1], 3, t), &Bm = act(c, a[3], 4, t), &Cm = act(c, a[4], 4, t);
+    const int64_t B = u.size(0), T = u.size(1), D = u.size(2), G = Bm.size(2), N = Bm.size(3);
+    expect(dt, u.sizes());
+    expect(Bm, {B, T, G, N});
+    expect(Cm, {B, T, G, N});
+    lq_scan_problem p = {};
+    p.B = extent(B); p.T = extent(T); p.D = extent(D); p.N = extent(N); p.G = extent(G);
+    p.dtype = out_code(t);
+    p.state_dtype = LQ_F32;
+    p.softplus = flag(a[8]);
+    p.dt_min = (float)number(a[9]); p.dt_max = (float)number(a[10]);
+    p.u = u.const_data_ptr(); p.dt = dt.const_data_ptr(); p.Bm = Bm.const_data_ptr(); p.Cm = Cm.const_data_ptr();
+    p.u_stride_b = u.stride(0); p.u_stride_t = u.stride(1);
+    p.dt_stride_b = dt.stride(0); p.dt_stride_t = dt.stride(1);
+    p.B_stride_b = Bm.stride(0); p.B_stride_t = Bm.stride(1); p.B_stride_g = Bm.stride(2);
+    p.C_stride_b = Cm.stride(0); p.C_stride_t = Cm.stride(1); p.C_stride_g = Cm.stride(2);
+    if (a[6] != Py_None) {
+      const at::Tensor& z = act(c, a[6], 3, t);
+      expect(z, u.sizes());
+      p.z = z.const_data_ptr();
+      p.z_stride_b = z.stride(0); p.z_stride_t = z.stride(1);
+    }
+    p.A = c.f32(a[2], {D, N}, true);
+    p.skip = c.f32(a[5], {D}, true);
+    p.dt_bias = c.f32(a[7], {D}, true);
+    p.initial_state = c.f32(a[11], {B, D, N}, true);
+    p.lengths = int32(c, a[12], B);
+    const at::Tensor y = empty({B, T, D}, t, c.dev);
+    p.y = y.data_ptr();
+    at::Tensor state;
+    if (flag(a[13])) {
+      state = empty({B, D, N}, at::kFloat, c.dev);
+      p.final_state = state.data_ptr<float>();
+    }
+    cudaStream_t st = stream_of(c);
+    int e;
+    {
+      NoGil ng;
+      e = lq_selective_scan_fwd(&p, st);
+    }
+    if (e != LQ_OK) return PyLong_FromLong(e);
+    return pair(THPVariable_Wrap(y), state.defined() ? THPVariable_Wrap(state) : none());
+  } catch (const NotPlain&) {
+    Py_RETURN_NONE;
+  }
+  END_HANDLE_TH_ERRORS
+}
+
+// selective_scan_step(state, u, dt, A, B, C, D, z, dt_bias, softplus, dt_min, dt_max, slots) -> y | status | None
+//   u [B,D] with A [D,N], or u [B,H,P] with A [H]
+PyObject* selective_scan_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  try {
+    if (n != 13) throw NotPlain{};
+    Call c;
+    const at::Tensor &s = Call::tensor(a[0]), &u = Call::tensor(a[1]);
+    if (!u.is_cuda() || (u.dim() != 2 && u.dim() != 3)) throw NotPlain{};
+    c.dev = u.device();
+    c.keep.reserve(8);
+    c10::cuda::CUDAGuard guard(c.dev);
+    const bool heads = u.dim() == 3;
+    const at::ScalarType t = u.scalar_type();
+    const at::Tensor &Bm = act(c, a[4], 3, t), &Cm = act(c, a[5], 3, t), &dt = act(c, a[2], 2, t);
+    const int64_t B = u.size(0), H = heads ? u.size(1) : 0, P = heads ? u.size(2) : 0, D = heads ? H * P : u.size(1), G = Bm.size(1), N = Bm.size(2);
+    auto channels = [&](const at::Tensor& x) {  // [B,D] or [B,H,P] with the channels of a token contiguous
+      if (x.device() != c.dev || x.scalar_type() != t || x.sizes() != u.sizes()) throw NotPlain{};
+      if ((x.size(-1) > 1 && x.stride(-1) != 1) || (heads && H > 1 && x.stride(1) != P)) throw NotPlain{};
+      return x.stride(0);
+    };
+    if (s.device() != c.dev || !s.is_contiguous() || s.dim() != u.dim() + 1 || s.size(-1) != N) throw NotPlain{};
+    for (int64_t i = 1; i < u.dim(); ++i)
+      if (s.size(i) != u.size(i)) throw NotPlain{};
+    expect(dt, {B, heads ? H : D});
+    expect(Bm, {B, G, N});
+    expect(Cm, {B, G, N});
+    lq_scan_problem p = {};
+    p.B = extent(B); p.T = 1; p.D = extent(D); p.N = extent(N); p.G = extent(G); p.H = extent(H); p.P = extent(P);
+    p.dtype = out_code(t);
+    p.state_dtype = out_code(s.scalar_type());
+    p.softplus = flag(a[9]);
+    p.dt_min = (float)number(a[10]); p.dt_max = (float)number(a[11]);
+    p.u = u.const_data_ptr(); p.dt = dt.const_data_ptr(); p.Bm = Bm.const_data_ptr(); p.Cm = Cm.const_data_ptr();
+    p.u_stride_b = channels(u);
+    p.dt_stride_b = dt.stride(0);
+    p.B_stride_b = Bm.stride(0); p.B_stride_g = Bm.stride(1);
+    p.C_stride_b = Cm.stride(0); p.C_stride_g = Cm.stride(1);
+    if (a[7] != Py_None) {
+      const at::Tensor& z = Call::tensor(a[7]);
+      p.z_stride_b = channels(z);
+      p.z = z.const_data_ptr();
+    }
+    p.A = heads ? c.f32(a[3], {H}, true) : c.f32(a[3], {D, N}, true);
+    if (a[6] != Py_None) {
+      p.skip_has_hdim = heads && Call::tensor(a[6]).dim() == 2;
+      p.skip = !heads ? c.f32(a[6], {D}, true) : p.skip_has_hdim ? c.f32(a[6], {H, P}, true) : c.f32(a[6], {H}, true);
+    }
+    p.dt_bias = c.f32(a[8], {heads ? H : D}, true);
+    p.state = s.data_ptr();
+    p.n_slots = extent(s.size(0));
+    p.slots = int32(c, a[12], B);
+    const at::Tensor y = empty(u.sizes(), t, c.dev);
+    p.y = y.data_ptr();
+    cudaStream_t st = stream_of(c);
+    int e;
+    {
+      NoGil ng;
+      e = lq_selective_scan_step(&p, st);
+    }
+    return e != LQ_OK ? PyLong_FromLong(e) : THPVariable_Wrap(y);
+  } catch (const NotPlain&) {
+    Py_RETURN_NONE;
+  }
+  END_HANDLE_TH_ERRORS
+}
+
+int64_t codes_pitch(int64_t n) { return (n + 15) / 16 * 16; }
+// [.., n] view of rows at a pitch
+at::Tensor rows_view(const at::Tensor& buf, at::IntArrayRef lead, int64_t n, int64_t pitch) {
+  std::vector<int64_t> sizes(lead.begin(), lead.end()), strides(lead.size());
+  int64_t s = pitch;
+  for (size_t i = lead.size(); i-- > 0;) {
+    strides[i] = s;
+    s *= lead[i];
+  }
+  sizes.push_back(n);
+  strides.push_back(1);
+  return buf.as_strided(sizes, strides);
+}
+at::IntArrayRef lead_of(const at::Tensor& x) { return x.sizes().slice(0, x.dim() - 1); }
+
+// quantize_rows(x) -> (codes, scale) | status | None
+PyObject* quantize_rows(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  try {
+    if (n != 1) throw NotPlain{};
+    Call c;
+    const at::Tensor& x = Call::tensor(a[0]);
+    if (!x.is_cuda()) throw NotPlain{};
+    c.dev = x.device();
+    c10::cuda::CUDAGuard guard(c.dev);
+    const Rows r(x);
+    const int64_t D = x.size(-1), pitch = codes_pitch(D);
+    const int dt = out_code(x.scalar_type()), rows = extent(r.rows), width = extent(D);
+    const at::Tensor codes = empty({r.rows, pitch}, at::kChar, c.dev), scale = empty(lead_of(x), at::kFloat, c.dev);
+    cudaStream_t st = stream_of(c);
+    int e;
+    {
+      NoGil ng;
+      e = lq_quantize_rows(x.const_data_ptr(), dt, rows, width, r.pitch, codes.data_ptr<int8_t>(), pitch, scale.data_ptr<float>(), st);
+    }
+    if (e != LQ_OK) return PyLong_FromLong(e);
+    return pair(THPVariable_Wrap(rows_view(codes, lead_of(x), D, pitch)), THPVariable_Wrap(scale));
+  } catch (const NotPlain&) {
+    Py_RETURN_NONE;
+  }
+  END_HANDLE_TH_ERRORS
+}
+
+// int8_linear(x, w, w_scale, x_scale, bias, out_dtype) -> y | status | None.   x: codes with x_scale, or values
+PyObject* int8_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  try {
+    if (n != 6) throw NotPlain{};
+    Call c;
+    const at::Tensor &x = Call::tensor(a[0]), &w = Call::tensor(a[1]);
+    if (!x.is_cuda() || w.device() != x.device() || w.dim() != 2 || w.scalar_type() != at::kChar) throw NotPlain{};
+    c.dev = x.device();
+    c.keep.reserve(6);
+    c10::cuda::CUDAGuard guard(c.dev);
+    const Rows xr(x), wr(w);
+    const int64_t K = x.size(-1), N = w.size(0);
+    if (w.size(1) != K) throw NotPlain{};
+    lq_linear_problem p = {};
+    p.M = extent(xr.rows); p.N = extent(N); p.K = extent(K);
+    auto aligned_rows = [](const at::Tensor& t, const Rows& r) {
+      if ((reinterpret_cast<uintptr_t>(t.const_data_ptr()) & 15u) || (r.pitch & 15)) {
+        if (r.rows > 1 || (reinterpret_cast<uintptr_t>(t.const_data_ptr()) & 15u)) throw NotPlain{};
+        return codes_pitch(r.pitch);  // one row: its pitch is not used
+      }
+      return r.pitch;
+    };
+    p.w = w.const_data_ptr<int8_t>();
+    p.w_stride = aligned_rows(w, wr);
+    p.w_scale = c.f32(a[2], {N}, true);
+    p.bias = c.f32(a[4], {N}, true);
+    cudaStream_t st = stream_of(c);
+    int dt = -1;
+    int8_t* codes = nullptr;
+    float* scale = nullptr;
+    at::ScalarType ot = at::kBFloat16;
+    if (x.scalar_type() == at::kChar) {
+      p.x = x.const_data_ptr<int8_t>();
+      p.x_stride = aligned_rows(x, xr);
+      if (a[3] == Py_None) throw NotPlain{};
+      p.x_scale = c.f32(a[3], lead_of(x), true);
+    } else {
+      dt = out_code(ot = x.scalar_type());
+      if (a[3] != Py_None) throw NotPlain{};
+      p.x_stride = codes_pitch(K);
+      const at::Tensor& buf = c.hold(scratch(xr.rows * (p.x_stride + 4), c.dev));
+      codes = (int8_t*)aligned(buf);
+      scale = (float*)(codes + xr.rows * p.x_stride);
+      p.x = codes;
+      p.x_scale = scale;
+    }
+    if (a[5] != Py_None) {
+      if (!THPDtype_Check(a[5])) throw NotPlain{};
+      ot = ((THPDtype*)a[5])->scalar_type;
+    }
+    p.out_dtype = out_code(ot);
+    std::vector<int64_t> shape(x.sizes().begin(), x.sizes().end());
+    shape.back() = N;
+    const at::Tensor y = empty(shape, ot, c.dev);
+    p.y = y.data_ptr();
+    p.status = status_word(c.dev);
+    int e = LQ_OK;
+    {
+      NoGil ng;
+      if (codes) e = lq_quantize_rows(x.const_data_ptr(), dt, p.M, p.K, xr.pitch, codes, p.x_stride, scale, st);
+      if (e == LQ_OK) e = lq_int8_linear(&p, st);
+    }
+    return e != LQ_OK ? PyLong_FromLong(e) : THPVariable_Wrap(y);
+  } catch (const NotPlain&) {
+    Py_RETURN_NONE;
+  }
+  END_HANDLE_TH_ERRORS
+}
+
+// rms_norm(x, weight, residual, residual_scale, post_weight, eps, quantize, out_dtype)
+//   -> y or (codes, scale) or None, residual or None
+PyObject* rms_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  try {
+    if (n != 8) throw NotPlain{};
+    Call c;
+    const at::Tensor& x = Call::tensor(a[0]);
+    if (!x.is_cuda()) throw NotPlain{};
+    c.dev = x.device();
+    c.keep.reserve(6);
+    c10::cuda::CUDAGuard guard(c.dev);
+    const Rows r(x);
+    const int64_t D = x.size(-1);
+    const at::ScalarType t = x.scalar_type();
+    lq_norm_problem p = {};
+    p.rows = extent(r.rows); p.D = p.group = extent(D);
+    p.dtype = out_code(t);
+    p.x = x.const_data_ptr(); p.x_stride = r.pitch;
+    p.eps = (float)number(a[5]);
+    p.weight = c.f32(a[1], {D}, true);
+    p.post_weight = c.f32(a[4], {D}, true);
+    p.residual_scale = 1.0f;
+    if (THPVariable_Check(a[3])) p.scale_vec = c.f32(a[3], {D}, true);
+    else p.residual_scale = (float)number(a[3]);
+    at::Tensor res, y, codes, scale;
+    if (a[2] != Py_None) {
+      const at::Tensor& in = Call::tensor(a[2]);
+      if (in.device() != c.dev || in.sizes() != x.sizes() || (in.scalar_type() != t && in.scalar_type() != at::kFloat)) throw NotPlain{};
+      const Rows rr(in);
+      p.residual = in.const_data_ptr(); p.residual_stride = rr.pitch;
+      p.residual_f32 = in.scalar_type() == at::kFloat;
+      res = empty(x.sizes(), in.scalar_type(), c.dev);
+      p.residual_out = res.data_ptr();
+    }
+    const at::ScalarType ot = a[7] == Py_None ? t : THPDtype_Check(a[7]) ? ((THPDtype*)a[7])->scalar_type : throw NotPlain{};
+    p.out_dtype = out_code(ot);
+    const int64_t pitch = codes_pitch(D);
+    if (p.weight && flag(a[6])) {
+      codes = empty({r.rows, pitch}, at::kChar, c.dev);
+      scale = empty(lead_of(x), at::kFloat, c.dev);
+      p.codes = codes.data_ptr<int8_t>(); p.codes_stride = pitch; p.scale = scale.data_ptr<float>();
+    } else if (p.weight) {
+      y = empty(x.sizes(), ot, c.dev);
+      p.y = y.data_ptr();
+    }
+    cudaStream_t st = stream_of(c);
+    int e;
+    {
+      NoGil ng;
+      e = lq_rms_norm(&p, st);
+    }
+    if (e != LQ_OK) return PyLong_FromLong(e);
+    PyObject* out = codes.defined() ? pair(THPVariable_Wrap(rows_view(codes, lead_of(x), D, pitch)), THPVariable_Wrap(scale))
+                    : y.defined()   ? THPVariable_Wrap(y)
+                                    : none();
+    return pair(out, res.defined() ? THPVariable_Wrap(res) : none());
+  } catch (const NotPlain&) {
+    Py_RETURN_NONE;
+  }
+  END_HANDLE_TH_ERRORS
+}
+
+// gated_rms_norm(x, gate, weight, group_size, gate_first, eps, quantize, out_dtype) -> y | (codes, scale) | status | None
+PyObject* gated_rms_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  try {
+    if (n != 8) throw NotPlain{};
+    Call c;
+    const at::Tensor &x = Call::tensor(a[0]), &g = Call::tensor(a[1]);
+    if (!x.is_cuda() || g.device() != x.device() || g.sizes() != x.sizes() || g.scalar_type() != x.scalar_type()) throw NotPlain{};
+    c.dev = x.device();
+    c.keep.reserve(6);
+    c10::cuda::CUDAGuard guard(c.dev);
+    const Rows r(x), gr(g);
+    const int64_t D = x.size(-1), pitch = codes_pitch(D);
+    const at::ScalarType t = x.scalar_type();
+    lq_norm_problem p = {};
+    p.rows = extent(r.rows); p.D = extent(D);
+    p.group = a[3] == Py_None ? p.D : integer(a[3]);
+    p.dtype = out_code(t);
+    p.x = x.const_data_ptr(); p.x_stride = r.pitch;
+    p.gate = g.const_data_ptr(); p.gate_stride = gr.pitch;
+    p.gate_first = flag(a[4]);
+    p.eps = (float)number(a[5]);
+    p.weight = c.f32(a[2], {D}, true);
+    const bool quantize = flag(a[6]), two = quantize && p.group != p.D;  // codes span the groups of a row: fp32 rows between
+    const at::ScalarType ot = two ? at::kFloat : a[7] == Py_None ? t : THPDtype_Check(a[7]) ? ((THPDtype*)a[7])->scalar_type : throw NotPlain{};
+    p.out_dtype = out_code(ot);
+    at::Tensor y, codes, scale;
+    if (quantize) {
+      codes = empty({r.rows, pitch}, at::kChar, c.dev);
+      scale = empty(lead_of(x), at::kFloat, c.dev);
+    }
+    if (!quantize || two) {
+      y = empty(x.sizes(), ot, c.dev);
+      p.y = y.data_ptr();
+    } else {
+      p.codes = codes.data_ptr<int8_t>(); p.codes_stride = pitch; p.scale = scale.data_ptr<float>();
+    }
+    cudaStream_t st = stream_of(c);
+    int e;
+    {
+      NoGil ng;
+      e = lq_gated_rms_norm(&p, st);
+      if (e == LQ_OK && two)
+        e = lq_quantize_rows(p.y, LQ_F32, p.rows, p.D, D, codes.data_ptr<int8_t>(), pitch, scale.data_ptr<float>(), st);
+    }
+    if (e != LQ_OK) return PyLong_FromLong(e);
+    if (!quantize) return THPVariable_Wrap(y);
+    return pair(THPVariable_Wrap(rows_view(codes, lead_of(x), D, pitch)), THPVariable_Wrap(scale));
+  } catch (const NotPlain&) {
+    Py_RETURN_NONE;
+  }
+  END_HANDLE_TH_ERRORS
+}
+
 PyMethodDef methods[] = {
     {"zoo_fwd", (PyCFunction)(void*)zoo_fwd, METH_FASTCALL, "one chunk call of a zoo cell"},
     {"split_rotate", (PyCFunction)(void*)split_rotate, METH_FASTCALL, "Mamba-2 prologue on xBC"},
     {"hadamard", (PyCFunction)(void*)hadamard, METH_FASTCALL, "Kronecker Hadamard rotation"},
     {"ssd_fwd", (PyCFunction)(void*)ssd_fwd, METH_FASTCALL, "Mamba-2 SSD combined forward"},
+    {"short_conv", (PyCFunction)(void*)short_conv, METH_FASTCALL, "short causal convolution of prompts"},
+    {"short_conv_step", (PyCFunction)(void*)short_conv_step, METH_FASTCALL, "short causal convolution, one token"},
+    {"selective_scan", (PyCFunction)(void*)selective_scan, METH_FASTCALL, "selective scan of prompts"},
+    {"selective_scan_step", (PyCFunction)(void*)selective_scan_step, METH_FASTCALL, "selective scan, one token"},
+    {"quantize_rows", (PyCFunction)(void*)quantize_rows, METH_FASTCALL, "symmetric INT8 codes of rows"},
+    {"int8_linear", (PyCFunction)(void*)int8_linear, METH_FASTCALL, "INT8 product with token and channel scales"},
+    {"rms_norm", (PyCFunction)(void*)rms_norm, METH_FASTCALL, "residual add and norms"},
+    {"gated_rms_norm", (PyCFunction)(void*)gated_rms_norm, METH_FASTCALL, "norm with a gate"},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

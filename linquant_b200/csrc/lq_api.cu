@@ -101,7 +101,9 @@ int run_diag_stage(const lq_zoo_problem* p, const lq_zoo_workspace* ws, bool del
 
 extern "C" int lq_version(void) { return 100; }
 extern "C" unsigned long long lq_struct_bytes(int which) {
-  return which == 0 ? sizeof(lq_zoo_problem) : which == 1 ? sizeof(lq_ssd_problem) : which == 2 ? sizeof(lq_zoo_workspace) : 0;
+  return which == 0 ? sizeof(lq_zoo_problem) : which == 1 ? sizeof(lq_ssd_problem) : which == 2 ? sizeof(lq_zoo_workspace)
+         : which == 3 ? sizeof(lq_conv_problem) : which == 4 ? sizeof(lq_scan_problem) : which == 5 ? sizeof(lq_linear_problem)
+         : which == 6 ? sizeof(lq_norm_problem) : 0;
 }
 extern "C" const char* lq_last_error_string(void) { return lq::g_err; }
 

@@ -1,0 +1,114 @@
+// Helpers of the operators around the recurrence (convolution, scan, product, norms): vectors of any activation type as
+// fp32, the activation functions, and the order-independent row maximum.
+#pragma once
+#include <type_traits>
+
+#include "lq_common.cuh"
+
+namespace lq {
+
+__device__ __forceinline__ float to_f32(float x) { return x; }
+__device__ __forceinline__ float to_f32(__half x) { return __half2float(x); }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
+template <typename T>
+__device__ __forceinline__ T from_f32(float x) {
+  if constexpr (std::is_same_v<T, float>) return x;
+  else return Act<T>::from(x);
+}
+
+// VEC consecutive values on a VEC * sizeof(T) boundary (16 bytes at most in one access)
+template <typename T, int VEC>
+struct alignas(VEC * sizeof(T) > 16 ? 16 : VEC * sizeof(T)) Pack {
+  T v[VEC];
+  __device__ __forceinline__ void get(float (&x)[VEC]) const {
+    if constexpr (VEC == 8 && sizeof(T) == 2) {
+      Act<T>::unpack8(*reinterpret_cast<const uint4*>(this), x);
+    } else {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) x[i] = to_f32(v[i]);
+    }
+  }
+  __device__ __forceinline__ void set(const float (&x)[VEC]) {
+    if constexpr (sizeof(T) == 2 && VEC % 2 == 0) {
+      uint32_t* w = reinterpret_cast<uint32_t*>(this);
+#pragma unroll
+      for (int i = 0; i < VEC / 2; ++i) w[i] = Act<T>::pack2(x[2 * i], x[2 * i + 1]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) v[i] = from_f32<T>(x[i]);
+    }
+  }
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) v[i] = from_f32<T>(0.f);
+  }
+};
+template <typename T, int VEC>
+__device__ __forceinline__ Pack<T, VEC> load_pack(const T* p) { return *reinterpret_cast<const Pack<T, VEC>*>(p); }
+template <typename T, int VEC>
+__device__ __forceinline__ void store_pack(T* p, const Pack<T, VEC>& v) { *reinterpret_cast<Pack<T, VEC>*>(p) = v; }
+
+// x / (1 + e^-x); e^-x = inf gives -0
+__device__ __forceinline__ float silu(float x) { return __fdividef(x, 1.0f + __expf(-x)); }
+
+// log(1 + e^x) = max(x, 0) + log1p(w), w = e^-|x| in (0, 1]; log1p(w) = 2 atanh(s), s = w / (2 + w) <= 1/3, by the Taylor
+// series of atanh (the first term left out is below 2e-8 of the sum): accurate where the result is small, where log(1 + w)
+// would lose w's low bits, and without a branch
+__device__ __forceinline__ float softplus(float x) {
+  const float w = __expf(-fabsf(x));
+  const float s = __fdividef(w, 2.0f + w), q = s * s;
+  float t = 1.0f / 15.0f;
+  t = fmaf(t, q, 1.0f / 13.0f);
+  t = fmaf(t, q, 1.0f / 11.0f);
+  t = fmaf(t, q, 1.0f / 9.0f);
+  t = fmaf(t, q, 1.0f / 7.0f);
+  t = fmaf(t, q, 1.0f / 5.0f);
+  t = fmaf(t, q, 1.0f / 3.0f);
+  t = fmaf(t, q, 1.0f);
+  return fmaxf(x, 0.0f) + 2.0f * s * t;  // NaN stays: w is NaN
+}
+// 2^x, one hardware exponential; results below 2^-126 are zero
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {  // NaN if either is
+  float y;
+  asm("max.NaN.f32 %0, %1, %2;\n" : "=f"(y) : "f"(a), "f"(b));
+  return y;
+}
+__device__ __forceinline__ float clamp_nan(float x, float lo, float hi) {  // NaN stays
+  float y;
+  asm("min.NaN.f32 %0, %1, %2;\n" : "=f"(y) : "f"(max_nan(x, lo)), "f"(hi));
+  return y;
+}
+constexpr float kLog2e = 1.4426950408889634f;
+
+// Row scale and its inverse. Rows whose largest value is below 1.3e-36 (zeros among them) have codes 0.
+__device__ __forceinline__ float row_scale(float amax, float& inv) {
+  const float scale = __fdiv_rn(amax, 127.0f);
+  inv = scale < 1e-38f ? 0.0f : __fdiv_rn(1.0f, scale);
+  return scale;
+}
+
+// ---- host side
+template <typename F>
+static inline int with_dtype(int dtype, const char* what, F&& f) {
+  switch (dtype) {
+    case LQ_F16: return f(__half());
+    case LQ_BF16: return f(__nv_bfloat16());
+    case LQ_F32: return f(float());
+  }
+  return fail(LQ_ERR_UNSUPPORTED, "%s: dtype %d", what, dtype);
+}
+static inline int dtype_bytes(int dtype) { return dtype == LQ_F32 ? 4 : 2; }
+// largest power of two (16 at most) that divides every address and byte pitch it is shown
+struct Alignment {
+  uintptr_t bits = 16;
+  Alignment& at(const void* p) { bits |= reinterpret_cast<uintptr_t>(p); return *this; }
+  Alignment& pitch(long long elements, int size) { bits |= (uintptr_t)(elements * size); return *this; }
+  int bytes() const { return (int)(bits & (~bits + 1)); }
+};
+
+}  // namespace lq
