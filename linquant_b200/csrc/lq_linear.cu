@@ -89,6 +89,9 @@ static int launch_warp(const lq_linear_problem* p, cudaStream_t st) {
 }
 
 }  // namespace linear
+
+int run_linear_tc(const lq_linear_problem* p, cudaStream_t st);  // lq_linear_tc.cu
+
 }  // namespace lq
 
 extern "C" int lq_int8_linear(const lq_linear_problem* p, lq_stream stream) {
@@ -101,9 +104,10 @@ extern "C" int lq_int8_linear(const lq_linear_problem* p, lq_stream stream) {
   Alignment a;
   if (a.at(p->x).at(p->w).pitch(p->x_stride, 1).pitch(p->w_stride, 1).bytes() != 16)
     return fail(LQ_ERR_ALIGN, "int8_linear: rows of codes start on 16-byte boundaries (pitches %lld, %lld)", p->x_stride, p->w_stride);
+  cudaStream_t st = (cudaStream_t)stream;
+  if (p->M > 64) return run_linear_tc(p, st);
   return with_dtype(p->out_dtype, "int8_linear", [&](auto t) {
     using TO = decltype(t);
-    cudaStream_t st = (cudaStream_t)stream;
     return p->M <= 8 ? linear::launch_warp<1, TO>(p, st) : p->M <= 16 ? linear::launch_warp<2, TO>(p, st) : linear::launch_warp<4, TO>(p, st);
   });
 }
