@@ -326,6 +326,7 @@ typedef struct {
   void* state;                 /* step: [n_slots,D,N] */
   const int* slots;            /* step: as above */
   int n_slots;
+  int* status;                 /* as in lq_ssd_problem */
 } lq_scan_problem;
 /* h_t = exp(dt_t A) h_{t-1} + dt_t u_t B_t;  y_t = C_t . h_t + skip u_t;  states in fp32 */
 int lq_selective_scan_fwd(const lq_scan_problem* p, lq_stream stream);

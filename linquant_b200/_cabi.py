@@ -51,7 +51,7 @@ class ScanProblem(C.Structure):
                        longlong="u_stride_b u_stride_t dt_stride_b dt_stride_t z_stride_b z_stride_t B_stride_b B_stride_t B_stride_g "
                                 "C_stride_b C_stride_t C_stride_g",
                        void_p="u dt z Bm Cm A skip dt_bias", int_2="skip_has_hdim",
-                       void_p_2="initial_state lengths y final_state state slots", int_3="n_slots")
+                       void_p_2="initial_state lengths y final_state state slots", int_3="n_slots", void_p_3="status")
 
 
 class LinearProblem(C.Structure):

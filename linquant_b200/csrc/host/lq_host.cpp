@@ -566,6 +566,7 @@ PyObject* selective_scan(PyObject*, PyObject* const* a, Py_ssize_t n) {
       state = empty({B, D, N}, at::kFloat, c.dev);
       p.final_state = state.data_ptr<float>();
     }
+    p.status = status_word(c.dev);
     cudaStream_t st = stream_of(c);
     int e;
     {

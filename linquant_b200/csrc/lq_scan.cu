@@ -2,132 +2,500 @@
 //
 //   h_t[n] = exp(dt_t A[n]) h_{t-1}[n] + dt_t u_t B_t[n],   y_t = sum_n C_t[n] h_t[n] + skip u_t,   y_t *= silu(z_t)
 //
-// Bound by the exponentials: one per token, channel and state at 16 a clock and SM. A channel's states are spread over LP
-// lanes with SPT states in the registers of each, so every exponential is computed once and no lane recomputes another's
-// part; tokens go one after the other, a tile of them at a time through shared memory (dt and dt u of the tile's channels,
-// B and C shared by the channels of a group), and a lane's part of y_t is summed over the LP lanes when the tile is stored.
+// Two resources bound it: the exponentials (one per token, channel and state, 16 a clock and SM) and what shared memory
+// delivers to registers (128 bytes a clock and SM, broadcasts included). A thread of the recurrence holds SPT states of a
+// channel, LP threads share the channel; tokens go one after the other, four at a time: dt and dt u (16 bytes each), B and C
+// of its states (in the activation's type) and its part of y lie with the token index contiguous, so that one access covers
+// the four, and the products around the recurrence take two tokens an instruction. Per token a warp takes 3 + SPT size / 2
+// clocks of shared memory and 2 SPT of exponentials.
+// A tile of TT tokens passes three jobs, each with warps of its own, so that their latencies overlap: dt and dt u are
+// prepared and B and C turned, the recurrence runs, and y is stored (the sum of the threads' parts, skip and gate). Buffers of
+// two, one barrier a tile. Inputs come as TMA tiles into a ring of ST tiles, requested ST - 2 tiles ahead of their use. Where
+// rows do not lie on 16-byte boundaries the storing warps copy them in words of four bytes, the words that hold a row's ends
+// included.
+// At 1 x 16384 x 2048 with 16 states (bf16, gate): 375 us; 115 us of exponentials, 41 us of bytes. All jobs in every warp took
+// 1 139 us, two jobs and plain loads 937 us, three jobs with the state index contiguous 462 us. The recurrence alone takes 323
+// us: its one warp a quadrant issues in 57 % of the clocks.
 #include "lq_layer.cuh"
+#include "lq_tc.cuh"
 
 namespace lq {
 
 namespace scan {
 
-template <typename T, int SPT, int LP, int THREADS, int TT>
+// RT threads of the recurrence
+template <typename T, int RT_, int SPT, int LP, int ST_, int TT_>
 struct Shape {
-  static constexpr int NP = SPT * LP, CH = THREADS / LP, EPT = TT > LP ? TT / LP : 1;  // EPT: elements of a tile a thread loads and stores
-  struct Smem {
-    float2 step[TT][CH];  // dt, dt u
-    float y[TT][THREADS];
-    float B[TT][NP], C[TT][NP];
+  static constexpr int RT = RT_, ST = ST_, TT = TT_, JOB = 256, THREADS = RT + 2 * JOB;  // JOB: threads of the preparing and of the storing job
+  static constexpr int NP = SPT * LP, CH = RT / LP, PT = TT + 4;        // PT: pitch of a row of tokens, no two rows of an access on one bank
+  static constexpr int GSTEP = JOB / CH, GROUPS = TT / 4;               // a job's thread has one channel, every GSTEP-th group of four tokens
+  static constexpr int E = sizeof(T), CB = CH * E, NB = NP * E;         // bytes of a row of channels, of states
+  static constexpr int CROW = (CB + 31) / 16 * 16, NROW = (NB + 31) / 16 * 16;  // pitch of rows that are copied by words
+  static constexpr int STAGE = TT * (3 * CROW + 2 * NROW);
+  static constexpr int YC = LP * PT + 4;                                // parts of y of a channel: again on banks of their own
+  static_assert(JOB % CH == 0 && CH % 8 == 0, "");
+  struct alignas(128) Smem {
+    uint8_t raw[ST][STAGE];  // rows of u, dt, z, B, C
+    float dt[2][CH * PT], du[2][CH * PT], y[2][CH * YC];
+    T B[2][NP * PT], C[2][NP * PT];
+    uint64_t full[ST];
+    float behind[16];        // the recurrence requests up to 16 tokens behind a row
   };
 };
 
-template <typename T, int SPT, int LP, int THREADS, int TT>
-__global__ void __launch_bounds__(THREADS) selective_scan_kernel(const lq_scan_problem p) {
-  pdl_enter();
-  using S = Shape<T, SPT, LP, THREADS, TT>;
-  constexpr int NP = S::NP, CH = S::CH, EPT = S::EPT;
-  extern __shared__ __align__(16) uint8_t smem_raw[];
-  typename S::Smem& sm = *reinterpret_cast<typename S::Smem*>(smem_raw);
-  const int tid = threadIdx.x, b = blockIdx.z, grp = blockIdx.y, Dg = p.D / p.G;
-  const int ch0 = blockIdx.x * CH;                    // within the group
-  const int ch = tid / LP, ln = tid % LP;             // recurrence: channel and first state / SPT of this thread
-  const int ech = tid % CH, et = tid / CH;            // loads and stores: channel and first token
-  const bool on = ch0 + ch < Dg, eon = ch0 + ech < Dg;
-  const int d = grp * Dg + ch0 + ch, ed = grp * Dg + ch0 + ech;
-  const int len = p.lengths ? min(max(p.lengths[b], 0), p.T) : p.T;
+struct Maps {
+  CUtensorMap u, dt, z, B, C;
+};
 
-  float a2[SPT], h[SPT];
-#pragma unroll
-  for (int j = 0; j < SPT; ++j) {
-    const int n = ln * SPT + j;
-    const bool live = on && n < p.N;
-    a2[j] = live ? p.A[(size_t)d * p.N + n] * kLog2e : 0.f;
-    h[j] = live && p.initial_state ? p.initial_state[((size_t)b * p.D + d) * p.N + n] : 0.f;
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, uint32_t bar) {
+  asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];\n" ::"r"(dst),
+               "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(bar)
+               : "memory");
+}
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, int c3, uint32_t bar) {
+  asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];\n" ::"r"(dst),
+               "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(bar)
+               : "memory");
+}
+
+// One input of the CTA in global memory
+struct Rows {
+  const uint8_t* from;  // row 0 of the sequence
+  long long pitch;      // bytes
+  // element 0 of a row that was copied by words lies this many bytes behind the copy's start
+  __device__ __forceinline__ int shift(int t) const { return ((uint32_t)reinterpret_cast<uintptr_t>(from) + (uint32_t)t * (uint32_t)pitch) & 3; }
+  template <int JOB>
+  __device__ __forceinline__ void copy(uint32_t to, int row_pitch, int bytes, int rows, int t0, int len, int tid) const {
+    if (from == nullptr) return;
+    for (int row = tid >> 3; row < rows && t0 + row < len; row += JOB / 8) {
+      const uint8_t* at = from + (t0 + row) * pitch;
+      const int sh = shift(t0 + row), words = (bytes + sh + 3) >> 2;
+      for (int w = tid & 7; w < words; w += 8)
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 4;\n" ::"r"(to + row * row_pitch + 4 * w), "l"(at - sh + 4 * w) : "memory");
+    }
   }
-  const float bias = eon && p.dt_bias ? p.dt_bias[ed] : 0.f, skip = eon && p.skip ? p.skip[ed] : 0.f;
-  const T* u = reinterpret_cast<const T*>(p.u) + b * p.u_stride_b + ed;
-  const T* dt = reinterpret_cast<const T*>(p.dt) + b * p.dt_stride_b + ed;
-  const T* z = p.z ? reinterpret_cast<const T*>(p.z) + b * p.z_stride_b + ed : nullptr;
-  const T* Bm = reinterpret_cast<const T*>(p.Bm) + b * p.B_stride_b + grp * p.B_stride_g;
-  const T* Cm = reinterpret_cast<const T*>(p.Cm) + b * p.C_stride_b + grp * p.C_stride_g;
-  T* y = reinterpret_cast<T*>(p.y) + (size_t)b * p.T * p.D + ed;
-  constexpr int ESTEP = LP;  // tokens between a thread's elements
-  const bool ein = et < TT;
+};
 
-  for (int t0 = 0; t0 < len; t0 += TT) {
-    float uu[EPT], zz[EPT];
+// ---- what the preparing and the storing job share
+// WIDE: rows on 16-byte boundaries, TMA tiles
+template <typename T, typename S, bool WIDE>
+struct Job {
+  const lq_scan_problem& p;
+  const Maps& maps;
+  typename S::Smem& sm;
+  const int tid, b, grp, ch0, len, tiles, ch, g0;
+  const bool on;  // the thread's channel is one of the group's
+  Rows u, dt, z, B, C;
+
+  __device__ __forceinline__ Job(const lq_scan_problem& p, const Maps& maps, typename S::Smem& sm, int tid, int b, int grp, int ch0, int len)
+      : p(p), maps(maps), sm(sm), tid(tid), b(b), grp(grp), ch0(ch0), len(len), tiles((len + S::TT - 1) / S::TT), ch(tid % S::CH), g0(tid / S::CH),
+        on(ch0 + tid % S::CH < p.D / p.G) {
+    const int d = grp * (p.D / p.G) + ch0;
+    auto base = [](const void* x, long long elements) { return x ? reinterpret_cast<const uint8_t*>(x) + elements * S::E : nullptr; };
+    u = {base(p.u, b * p.u_stride_b + d), p.u_stride_t * S::E};
+    dt = {base(p.dt, b * p.dt_stride_b + d), p.dt_stride_t * S::E};
+    z = {base(p.z, b * p.z_stride_b + d), p.z_stride_t * S::E};
+    B = {base(p.Bm, b * p.B_stride_b + grp * p.B_stride_g), p.B_stride_t * S::E};
+    C = {base(p.Cm, b * p.C_stride_b + grp * p.C_stride_g), p.C_stride_t * S::E};
+  }
+  __device__ __forceinline__ int channel() const { return grp * (p.D / p.G) + ch0 + ch; }
+  // where array i of a stage (u, dt, z, B, C) begins, and the pitch of its rows
+  static __device__ __forceinline__ constexpr int offset(int i) { return i < 3 ? i * S::TT * S::CROW : 3 * S::TT * S::CROW + (i - 3) * S::TT * S::NROW; }
+  static __device__ __forceinline__ constexpr int pitch(int i) { return i < 3 ? (WIDE ? S::CB : S::CROW) : (WIDE ? S::NB : S::NROW); }
+  __device__ __forceinline__ const uint8_t* stage(int tile) const { return sm.raw[tile % S::ST]; }
+  // element c of row r of array i
+  template <int I>
+  __device__ __forceinline__ T at(const uint8_t* stage, const Rows& src, int tile, int r, int c) const {
+    int o = offset(I) + r * pitch(I) + c * S::E;
+    if constexpr (!WIDE) o += src.shift(tile * S::TT + r);
+    return *reinterpret_cast<const T*>(stage + o);
+  }
+};
+
+// ---- dt and dt u of a tile; B and C with the token index contiguous
+template <typename T, typename S, bool WIDE>
+struct Prepare : Job<T, S, WIDE> {
+  using J = Job<T, S, WIDE>;
+  using J::p, J::sm, J::tid, J::len, J::ch, J::g0, J::on, J::u, J::dt, J::B, J::C;
+  float bias;
+  bool ok = true;
+
+  template <typename... A>
+  __device__ __forceinline__ Prepare(A&&... a) : J(a...), bias(on && p.dt_bias ? p.dt_bias[J::channel()] : 0.f) {}
+  // FULL: every token of the tile counts
+  template <bool FULL, bool SOFTPLUS>
+  __device__ __forceinline__ void steps(const uint8_t* st, int tile) {
+    const int t0 = tile * S::TT, buf = tile & 1;
 #pragma unroll
-    for (int i = 0; i < EPT; ++i) {
-      const int t = t0 + et + i * ESTEP;
-      const bool live = eon && t < len;
-      uu[i] = live ? to_f32(u[t * p.u_stride_t]) : 0.f;
-      zz[i] = live && z ? to_f32(z[t * p.z_stride_t]) : 0.f;
-      float v = live ? to_f32(dt[t * p.dt_stride_t]) + bias : 0.f;
-      v = p.softplus ? softplus(v) : v;
-      v = clamp_nan(v, p.dt_min, p.dt_max);
-      if (ein) sm.step[et + i * ESTEP][ech] = live ? make_float2(v, v * uu[i]) : make_float2(0.f, 0.f);
-    }
-    for (int i = tid; i < TT * NP; i += THREADS) {
-      const int tt = i / NP, n = i % NP, t = t0 + tt;
-      const bool live = t < len && n < p.N;  // what lies behind the last token takes no part, not even as 0 x NaN
-      sm.B[tt][n] = live ? to_f32(Bm[t * p.B_stride_t + n]) : 0.f;
-      sm.C[tt][n] = live ? to_f32(Cm[t * p.C_stride_t + n]) : 0.f;
-    }
-    __syncthreads();
-#pragma unroll 4
-    for (int tt = 0; tt < TT; ++tt) {
-      const float2 s = sm.step[tt][ch];
-      float acc = 0.f;
+    for (int g = g0; g < S::GROUPS; g += S::GSTEP) {
+      float v[4], w[4];
 #pragma unroll
-      for (int j = 0; j < SPT; ++j) {
-        h[j] = fmaf(ex2(s.x * a2[j]), h[j], s.y * sm.B[tt][ln * SPT + j]);
-        acc = fmaf(h[j], sm.C[tt][ln * SPT + j], acc);
+      for (int k = 0; k < 4; ++k) {
+        v[k] = to_f32(J::template at<1>(st, dt, tile, 4 * g + k, ch)) + bias;
+        w[k] = to_f32(J::template at<0>(st, u, tile, 4 * g + k, ch));
       }
-      sm.y[tt][tid] = acc;
-    }
-    __syncthreads();
 #pragma unroll
-    for (int i = 0; i < EPT; ++i) {
-      const int tt = et + i * ESTEP, t = t0 + tt;
-      if (!ein) break;
-      float v = skip * uu[i];
-#pragma unroll
-      for (int l = 0; l < LP; ++l) v += sm.y[tt][ech * LP + l];
-      if (z) v *= silu(zz[i]);
-      if (eon && t < p.T) y[(size_t)t * p.D] = from_f32<T>(t < len ? v : 0.f);
+      for (int k = 0; k < 4; ++k) {
+        v[k] = clamp_nan(SOFTPLUS ? softplus(v[k]) : v[k], p.dt_min, p.dt_max);
+        w[k] *= v[k];
+        if (!FULL && t0 + 4 * g + k >= len) v[k] = w[k] = 0.f;  // a token behind the last is a step of nothing
+      }
+      *reinterpret_cast<float4*>(&sm.dt[buf][ch * S::PT + 4 * g]) = make_float4(v[0], v[1], v[2], v[3]);
+      *reinterpret_cast<float4*>(&sm.du[buf][ch * S::PT + 4 * g]) = make_float4(w[0], w[1], w[2], w[3]);
     }
   }
-  if (eon && ein)  // tiles that no token reaches
-    for (int t = (len + TT - 1) / TT * TT + et; t < p.T; t += ESTEP < TT ? ESTEP : TT) y[(size_t)t * p.D] = from_f32<T>(0.f);
-  if (p.final_state && on) {
+  template <bool FULL>
+  __device__ __forceinline__ void turn(const uint8_t* st, int tile) {
+    const int t0 = tile * S::TT, buf = tile & 1;
+    const T none = from_f32<T>(0.f);
+    constexpr int PER = S::JOB / S::NP, WORK = S::TT / 2;  // pairs of tokens, of a state in PER threads
+    const int n = tid % S::NP;
 #pragma unroll
-    for (int j = 0; j < SPT; ++j)
-      if (ln * SPT + j < p.N) p.final_state[((size_t)b * p.D + d) * p.N + ln * SPT + j] = h[j];
+    for (int i = 0; i < (WORK + PER - 1) / PER; ++i) {
+      const int r = 2 * (tid / S::NP + i * PER);
+      if (WORK % PER && r >= S::TT) break;
+      // what lies behind the last token or state takes no part, not even as 0 x NaN
+      const bool in0 = FULL || (n < p.N && t0 + r < len), in1 = FULL || (n < p.N && t0 + r + 1 < len);
+      Pack<T, 2> vB, vC;
+      vB.v[0] = in0 ? J::template at<3>(st, B, tile, r, n) : none;
+      vB.v[1] = in1 ? J::template at<3>(st, B, tile, r + 1, n) : none;
+      vC.v[0] = in0 ? J::template at<4>(st, C, tile, r, n) : none;
+      vC.v[1] = in1 ? J::template at<4>(st, C, tile, r + 1, n) : none;
+      store_pack(&sm.B[buf][n * S::PT + r], vB);
+      store_pack(&sm.C[buf][n * S::PT + r], vC);
+    }
+  }
+  __device__ __forceinline__ void run(int tile) {
+    if (WIDE && ok) ok = mbar_wait_bounded(smem_u32(&sm.full[tile % S::ST]), (uint32_t)((tile / S::ST) & 1));
+    const uint8_t* st = J::stage(tile);
+    if (WIDE && (tile + 1) * S::TT <= len) {  // TMA fills with zeros behind the last state
+      turn<true>(st, tile);
+      if (p.softplus) steps<true, true>(st, tile);
+      else steps<true, false>(st, tile);
+    } else {
+      turn<false>(st, tile);
+      if (p.softplus) steps<false, true>(st, tile);
+      else steps<false, false>(st, tile);
+    }
+  }
+};
+
+// ---- loads, and y of a tile
+template <typename T, typename S, bool WIDE>
+struct Store : Job<T, S, WIDE> {
+  using J = Job<T, S, WIDE>;
+  using J::p, J::maps, J::sm, J::tid, J::len, J::ch, J::g0, J::on, J::u, J::dt, J::z, J::B, J::C;
+  T* y;
+  float skip;
+
+  template <typename... A>
+  __device__ __forceinline__ Store(A&&... a) : J(a...), y(reinterpret_cast<T*>(p.y) + (size_t)J::b * p.T * p.D + J::channel()), skip(on && p.skip ? p.skip[J::channel()] : 0.f) {}
+  __device__ __forceinline__ void request(int tile) const {
+    const int t0 = tile * S::TT;
+    const uint32_t to = smem_u32(J::stage(tile));
+    if constexpr (WIDE) {
+      if (tid == 0 && tile < J::tiles) {
+        const uint32_t bar = smem_u32(&sm.full[tile % S::ST]);
+        const int d = J::grp * (p.D / p.G) + J::ch0;
+        asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");  // the stage has been read with plain loads
+        asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n" ::"r"(bar), "r"((uint32_t)(S::TT * ((p.z ? 3 : 2) * S::CB + 2 * S::NB)))
+                     : "memory");
+        tma_load_3d(to + J::offset(0), &maps.u, d, t0, J::b, bar);
+        tma_load_3d(to + J::offset(1), &maps.dt, d, t0, J::b, bar);
+        if (p.z) tma_load_3d(to + J::offset(2), &maps.z, d, t0, J::b, bar);
+        tma_load_4d(to + J::offset(3), &maps.B, 0, J::grp, t0, J::b, bar);
+        tma_load_4d(to + J::offset(4), &maps.C, 0, J::grp, t0, J::b, bar);
+      }
+    } else {
+      const int bytes = min(S::CH, p.D / p.G - J::ch0) * S::E;
+      u.template copy<S::JOB>(to + J::offset(0), S::CROW, bytes, S::TT, t0, len, tid);
+      dt.template copy<S::JOB>(to + J::offset(1), S::CROW, bytes, S::TT, t0, len, tid);
+      z.template copy<S::JOB>(to + J::offset(2), S::CROW, bytes, S::TT, t0, len, tid);
+      B.template copy<S::JOB>(to + J::offset(3), S::NROW, p.N * S::E, S::TT, t0, len, tid);
+      C.template copy<S::JOB>(to + J::offset(4), S::NROW, p.N * S::E, S::TT, t0, len, tid);
+      cp_async_commit();
+    }
+  }
+  // tiles up to the ST - 3 newest requests are there for everybody from the next barrier on
+  __device__ __forceinline__ void arrived() const {
+    if constexpr (!WIDE) cp_async_wait<S::ST - 3>();
+  }
+  template <int LP, bool FULL, bool GATE>
+  __device__ __forceinline__ void outputs(int tile) const {
+    const int t0 = tile * S::TT;
+    const uint8_t* st = J::stage(tile);
+#pragma unroll
+    for (int g = g0; g < S::GROUPS; g += S::GSTEP) {
+      const float* parts = &sm.y[tile & 1][ch * S::YC + 4 * g];
+      float4 q = *reinterpret_cast<const float4*>(parts);
+      F2 lo(q.x, q.y), hi(q.z, q.w);
+#pragma unroll
+      for (int l = 1; l < LP; ++l) {
+        q = *reinterpret_cast<const float4*>(parts + l * S::PT);
+        lo = add2(lo, F2(q.x, q.y));
+        hi = add2(hi, F2(q.z, q.w));
+      }
+      float s[4];
+      lo.get(s[0], s[1]);
+      hi.get(s[2], s[3]);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        s[k] = fmaf(skip, to_f32(J::template at<0>(st, u, tile, 4 * g + k, ch)), s[k]);
+        if (GATE) s[k] *= silu(to_f32(J::template at<2>(st, z, tile, 4 * g + k, ch)));
+      }
+      T* to = y + (size_t)(t0 + 4 * g) * p.D;
+#pragma unroll
+      for (int k = 0; k < 4; ++k, to += p.D)
+        if (FULL || t0 + 4 * g + k < p.T) *to = from_f32<T>(FULL || t0 + 4 * g + k < len ? s[k] : 0.f);
+    }
+  }
+  template <int LP>
+  __device__ __forceinline__ void run(int tile) const {
+    if (!on) return;
+    if ((tile + 1) * S::TT <= len) {
+      if (p.z) outputs<LP, true, true>(tile);
+      else outputs<LP, true, false>(tile);
+    } else {
+      if (p.z) outputs<LP, false, true>(tile);
+      else outputs<LP, false, false>(tile);
+    }
+  }
+  __device__ __forceinline__ void zeros(int t0) const {  // tiles that no token reaches
+    if (!on) return;
+    for (int t = t0 + g0; t < p.T; t += S::GSTEP) y[(size_t)t * p.D] = from_f32<T>(0.f);
+  }
+};
+
+// ---- the recurrence of a tile, four tokens at a time. Few warps run it, so one's own instructions have to cover latencies: the
+// exponentials of four tokens are taken while the recurrence of the four before runs, their operands requested ahead of that.
+template <typename T, typename S, int SPT, int LP>
+struct Recurrence {
+  struct Operands {
+    float4 du;
+    Pack<T, 4> B[SPT], C[SPT];
+  };
+  typename S::Smem& sm;
+  const int ch, ln;  // states ln, ln + LP, ..
+  float a2[SPT], h[SPT];
+
+  // of the tile: rows of this thread's channel and first state
+  const float *pdt, *pdu;
+  const T *pB, *pC;
+  float* py;
+
+  __device__ __forceinline__ float4 load_dt(int t) const { return *reinterpret_cast<const float4*>(pdt + t); }
+  __device__ __forceinline__ void load(Operands& o, int t) const {
+    o.du = *reinterpret_cast<const float4*>(pdu + t);
+#pragma unroll
+    for (int j = 0; j < SPT; ++j) {
+      o.B[j] = load_pack<T, 4>(pB + j * LP * S::PT + t);
+      o.C[j] = load_pack<T, 4>(pC + j * LP * S::PT + t);
+    }
+  }
+  __device__ __forceinline__ void decays(float (&a)[SPT][4], const float4& dt) const {
+#pragma unroll
+    for (int j = 0; j < SPT; ++j) {
+      a[j][0] = ex2(dt.x * a2[j]);
+      a[j][1] = ex2(dt.y * a2[j]);
+      a[j][2] = ex2(dt.z * a2[j]);
+      a[j][3] = ex2(dt.w * a2[j]);
+    }
+  }
+  __device__ __forceinline__ void run(const Operands& o, const float (&a)[SPT][4], int t) {
+    const float du[4] = {o.du.x, o.du.y, o.du.z, o.du.w};
+    float y[4];
+#pragma unroll
+    for (int j = 0; j < SPT; ++j) {
+      float b[4], c[4];
+      o.B[j].get(b);
+      o.C[j].get(c);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        h[j] = fmaf(a[j][k], h[j], du[k] * b[k]);
+        y[k] = j == 0 ? h[j] * c[k] : fmaf(h[j], c[k], y[k]);
+      }
+    }
+    *reinterpret_cast<float4*>(py + t) = make_float4(y[0], y[1], y[2], y[3]);
+  }
+  __device__ __forceinline__ void tile(int buf) {
+    pdt = &sm.dt[buf][ch * S::PT];
+    pdu = &sm.du[buf][ch * S::PT];
+    pB = &sm.B[buf][ln * S::PT];
+    pC = &sm.C[buf][ln * S::PT];
+    py = &sm.y[buf][ch * S::YC + ln * S::PT];
+    if constexpr (SPT <= 2) {
+      Operands x0, x1;
+      float a0[SPT][4], a1[SPT][4];
+      load(x0, 0);
+      float4 d0 = load_dt(0), d1 = load_dt(4);
+      decays(a0, d0);
+#pragma unroll 1
+      for (int i = 0; i < S::TT; i += 16, pdt += 16, pdu += 16, pB += 16, pC += 16, py += 16) {
+#pragma unroll
+        for (int t = 0; t < 16; t += 8) {  // behind the tile's end: what is read there is not used
+          load(x1, t + 4);
+          d0 = load_dt(t + 8);
+          decays(a1, d1);
+          run(x0, a0, t);
+          load(x0, t + 8);
+          d1 = load_dt(t + 12);
+          decays(a0, d0);
+          run(x1, a1, t + 4);
+        }
+      }
+    } else {  // no registers for a second set
+#pragma unroll 1
+      for (int i = 0; i < S::TT; i += 16, pdt += 16, pdu += 16, pB += 16, pC += 16, py += 16) {
+#pragma unroll
+        for (int t = 0; t < 16; t += 4) {
+          Operands x;
+          float a[SPT][4];
+          const float4 d = load_dt(t);
+          load(x, t);
+          decays(a, d);
+          run(x, a, t);
+        }
+      }
+    }
+  }
+};
+
+template <typename T, bool WIDE, int RT, int SPT, int LP, int ST, int TT>
+__global__ void __launch_bounds__(RT + 512, 1) selective_scan_kernel(const __grid_constant__ Maps maps, const lq_scan_problem p) {
+  using S = Shape<T, RT, SPT, LP, ST, TT>;
+  extern __shared__ __align__(128) uint8_t smem_raw[];
+  typename S::Smem& sm = *reinterpret_cast<typename S::Smem*>(smem_raw + ((128 - (smem_u32(smem_raw) & 127)) & 127));
+  const int b = blockIdx.z, grp = blockIdx.y, Dg = p.D / p.G, ch0 = blockIdx.x * S::CH;  // ch0: within the group
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < ST; ++i) asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;\n" ::"r"(smem_u32(&sm.full[i])));
+    asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+  }
+  pdl_enter();
+  const int len = p.lengths ? min(max(p.lengths[b], 0), p.T) : p.T;
+  const int tiles = (len + TT - 1) / TT;
+  __syncthreads();
+  // iteration i: the recurrence runs tile i, tile i + 1 is prepared, tile i - 1 is stored
+  if (threadIdx.x < RT) {
+    Recurrence<T, S, SPT, LP> r{sm, (int)threadIdx.x / LP, (int)threadIdx.x % LP};
+    const bool on = ch0 + r.ch < Dg;
+    const size_t at = (size_t)(grp * Dg + ch0 + r.ch) * p.N;
+#pragma unroll
+    for (int j = 0; j < SPT; ++j) {
+      const int n = r.ln + j * LP;
+      const bool live = on && n < p.N;
+      r.a2[j] = live ? p.A[at + n] * kLog2e : 0.f;
+      r.h[j] = live && p.initial_state ? p.initial_state[(size_t)b * p.D * p.N + at + n] : 0.f;
+    }
+    for (int i = -1; i <= tiles; ++i) {
+      __syncthreads();
+      if (i >= 0 && i < tiles) r.tile(i & 1);
+    }
+    if (p.final_state && on) {
+      float* to = p.final_state + (size_t)b * p.D * p.N + at;
+#pragma unroll
+      for (int j = 0; j < SPT; ++j)
+        if (r.ln + j * LP < p.N) to[r.ln + j * LP] = r.h[j];
+    }
+  } else if (threadIdx.x < RT + S::JOB) {
+    Prepare<T, S, WIDE> job(p, maps, sm, (int)threadIdx.x - RT, b, grp, ch0, len);
+    for (int i = -1; i <= tiles; ++i) {
+      __syncthreads();
+      if (i + 1 < tiles) job.run(i + 1);
+    }
+    if (!job.ok) {  // what was requested still lands
+      for (int i = max(0, tiles - ST); i < tiles; ++i) mbar_wait_bounded(smem_u32(&sm.full[i % ST]), (uint32_t)((i / ST) & 1));
+      if (p.status) atomicExch(p.status, 1);
+    }
+  } else {
+    const Store<T, S, WIDE> job(p, maps, sm, (int)threadIdx.x - RT - S::JOB, b, grp, ch0, len);
+    for (int i = 0; i < ST - 2; ++i) job.request(i);
+    job.arrived();
+    for (int i = -1; i <= tiles; ++i) {
+      __syncthreads();
+      if (i > 0) {
+        job.template run<LP>(i - 1);
+        asm volatile("bar.sync 1, %0;\n" ::"n"(S::JOB) : "memory");  // nobody reads tile i - 1 any more
+      }
+      job.request(i + ST - 1);
+      job.arrived();
+    }
+    cp_async_wait<0>();
+    job.zeros(tiles * TT);
   }
 }
 
-template <typename T, int SPT, int LP>
+static int encode(CUtensorMap* m, int dtype, int rank, const void* base, const cuuint64_t* dims, const cuuint64_t* strides, const cuuint32_t* box) {
+  EncodeTiledFn enc = encode_tiled_fn();
+  if (enc == nullptr) return fail(LQ_ERR_LAUNCH, "selective_scan: the driver does not export cuTensorMapEncodeTiled");
+  const cuuint32_t ones[4] = {1, 1, 1, 1};
+  const CUtensorMapDataType t = dtype == LQ_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : dtype == LQ_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  const CUresult r = enc(m, t, rank, const_cast<void*>(base), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE,
+                         CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? LQ_OK : fail(LQ_ERR_LAUNCH, "selective_scan: cuTensorMapEncodeTiled failed with CUresult %d", (int)r);
+}
+
+template <typename T, int RT, int SPT, int LP, int ST, int TT>
 static int launch_scan(const lq_scan_problem* p, cudaStream_t st) {
-  constexpr int THREADS = 256, TT = SPT * LP > 64 ? 16 : 32;
-  using S = Shape<T, SPT, LP, THREADS, TT>;
+  using S = Shape<T, RT, SPT, LP, ST, TT>;
   const int Dg = p->D / p->G;
+  constexpr int E = sizeof(T);
   const dim3 grid((Dg + S::CH - 1) / S::CH, p->G, p->B);
   if (grid.y > 65535 || grid.z > 65535) return fail(LQ_ERR_SHAPE, "selective_scan: B=%d G=%d", p->B, p->G);
-  const cudaError_t e = launch_opt_in(selective_scan_kernel<T, SPT, LP, THREADS, TT>, grid, dim3(THREADS), sizeof(typename S::Smem), st, *p);
+  // TMA: addresses, pitches and rows of 16 bytes; a pitch of 0 (an expanded input) is not one
+  Maps maps = {};
+  Alignment a;
+  bool wide = S::CB % 16 == 0 && S::NB % 16 == 0 && p->T > 0;
+  a.at(p->y).pitch(Dg, E).pitch(p->N, E);
+  auto pitch = [&](long long elements, long long extent) {  // bytes; of no meaning where there is one
+    if (extent == 1) return (cuuint64_t)16;
+    a.pitch(elements, E);
+    wide = wide && elements > 0;
+    return (cuuint64_t)(elements * E);
+  };
+  struct In { CUtensorMap* map; const void* x; long long sb, st, sg; };
+  const In in[5] = {{&maps.u, p->u, p->u_stride_b, p->u_stride_t, 0}, {&maps.dt, p->dt, p->dt_stride_b, p->dt_stride_t, 0},
+                    {&maps.z, p->z, p->z_stride_b, p->z_stride_t, 0}, {&maps.B, p->Bm, p->B_stride_b, p->B_stride_t, p->B_stride_g},
+                    {&maps.C, p->Cm, p->C_stride_b, p->C_stride_t, p->C_stride_g}};
+  cuuint64_t pitches[5][3];
+  for (int i = 0; i < 5; ++i) {
+    if (in[i].x == nullptr) continue;
+    a.at(in[i].x);
+    pitches[i][0] = i < 3 ? 16 : pitch(in[i].sg, p->G);
+    pitches[i][1] = pitch(in[i].st, p->T);
+    pitches[i][2] = pitch(in[i].sb, p->B);
+  }
+  wide = wide && a.bytes() == 16;
+  for (int i = 0; i < 5 && wide; ++i) {
+    if (in[i].x == nullptr) continue;
+    const cuuint64_t chans[3] = {(cuuint64_t)p->D, (cuuint64_t)p->T, (cuuint64_t)p->B};
+    const cuuint64_t states[4] = {(cuuint64_t)p->N, (cuuint64_t)p->G, (cuuint64_t)p->T, (cuuint64_t)p->B};
+    const cuuint32_t cbox[3] = {S::CH, TT, 1}, nbox[4] = {S::NP, 1, TT, 1};
+    if (int e = i < 3 ? encode(in[i].map, p->dtype, 3, in[i].x, chans, &pitches[i][1], cbox) : encode(in[i].map, p->dtype, 4, in[i].x, states, pitches[i], nbox)) return e;
+  }
+  auto go = [&](auto kern) { return launch_opt_in(kern, grid, dim3(S::THREADS), sizeof(typename S::Smem) + 128, st, maps, *p); };
+  const cudaError_t e = wide ? go(selective_scan_kernel<T, true, RT, SPT, LP, ST, TT>) : go(selective_scan_kernel<T, false, RT, SPT, LP, ST, TT>);
   if (e != cudaSuccess) return fail(LQ_ERR_LAUNCH, "selective_scan: %s", cudaGetErrorString(e));
   return check_launch("selective_scan_kernel");
 }
 
+// One CTA an SM. 16 channels a CTA leave each SM quadrant one warp of the recurrence, 64 channels two with twice the states: less
+// time a channel where there are channels enough. Measured clocks a token and CTA (16 bits, gate): 44 against 128 with 16
+// states, 42 against 94 with 8, 65 against 103 with 4; what counts is rounds of CTAs times that.
 template <typename T>
 static int run(const lq_scan_problem* p, cudaStream_t st) {
-  if (p->N <= 4) return launch_scan<T, 4, 1>(p, st);
-  if (p->N <= 8) return launch_scan<T, 4, 2>(p, st);
-  if (p->N <= 16) return launch_scan<T, 4, 4>(p, st);
-  if (p->N <= 32) return launch_scan<T, 4, 8>(p, st);
-  if (p->N <= 64) return launch_scan<T, 4, 16>(p, st);
-  if (p->N <= 128) return launch_scan<T, 4, 32>(p, st);
-  return launch_scan<T, 8, 32>(p, st);
+  constexpr int R = sizeof(T) == 2 ? 4 : 3, F = R + 1;  // tiles in the ring, as shared memory allows
+  const long long sms = sm_count(), Dg = p->D / p->G, groups = (long long)p->B * p->G;
+  auto narrow = [&](int clocks16, int clocks64) {
+    const long long r16 = (groups * ((Dg + 15) / 16) + sms - 1) / sms, r64 = (groups * ((Dg + 63) / 64) + sms - 1) / sms;
+    return r16 * clocks16 < r64 * clocks64;
+  };
+  if (p->N <= 4) return narrow(65, 103) ? launch_scan<T, 64, 1, 4, F, 64>(p, st) : launch_scan<T, 128, 2, 2, R, 32>(p, st);
+  if (p->N <= 8) return narrow(42, 94) ? launch_scan<T, 64, 2, 4, F, 64>(p, st) : launch_scan<T, 128, 4, 2, R, 32>(p, st);
+  if (p->N <= 16) return narrow(44, 128) ? launch_scan<T, 128, 2, 8, F, 64>(p, st) : launch_scan<T, 256, 4, 4, R, 32>(p, st);
+  if (p->N <= 32) return launch_scan<T, 256, 4, 8, R, 32>(p, st);
+  if (p->N <= 64) return launch_scan<T, 256, 4, 16, R, 32>(p, st);
+  if (p->N <= 128) return launch_scan<T, 128, 8, 16, 3, 16>(p, st);
+  return launch_scan<T, 128, 16, 16, 3, 16>(p, st);
 }
 
 // ------------------------------------------------------------------------------------------------ one token
