@@ -348,6 +348,9 @@ typedef struct {
 } lq_linear_problem;
 /* y[m,n] = (sum_k x[m,k] w[n,k]) x_scale[m] w_scale[n] + bias[n] */
 int lq_int8_linear(const lq_linear_problem* p, lq_stream stream);
+/* The same from values: their codes and scales as lq_quantize_rows makes them. p->x and p->x_scale name scratch for them ([M]
+ * rows at x_stride bytes, [M]), which may be written. */
+int lq_int8_linear_values(const lq_linear_problem* p, const void* values, int dtype, long long stride, lq_stream stream);
 
 typedef struct {
   int rows, D, group;          /* group: channels that are normed together (divides D; the gated form only, else D) */

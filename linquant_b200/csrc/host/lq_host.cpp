@@ -748,11 +748,10 @@ PyObject* int8_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const at::Tensor y = empty(shape, ot, c.dev);
     p.y = y.data_ptr();
     p.status = status_word(c.dev);
-    int e = LQ_OK;
+    int e;
     {
       NoGil ng;
-      if (codes) e = lq_quantize_rows(x.const_data_ptr(), dt, p.M, p.K, xr.pitch, codes, p.x_stride, scale, st);
-      if (e == LQ_OK) e = lq_int8_linear(&p, st);
+      e = codes ? lq_int8_linear_values(&p, x.const_data_ptr(), dt, xr.pitch, st) : lq_int8_linear(&p, st);
     }
     return e != LQ_OK ? PyLong_FromLong(e) : THPVariable_Wrap(y);
   } catch (const NotPlain&) {

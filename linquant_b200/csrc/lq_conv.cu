@@ -13,15 +13,25 @@ template <typename T, int W, int VEC>
 struct Taps {
   float w[VEC][W], b[VEC];
   __device__ __forceinline__ Taps(const lq_conv_problem& p, int c) {
+    // the taps of a thread's channels lie one after the other: pieces as large as the channels' alignment allows
+    constexpr int PIECE = VEC * W % 4 == 0 ? 4 : VEC * W % 2 == 0 ? 2 : 1;
+    const float* from = p.weight + (size_t)c * W;
+    if ((reinterpret_cast<uintptr_t>(from) & (4 * PIECE - 1)) == 0) {
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-      b[i] = p.bias ? __ldg(p.bias + c + i) : 0.f;
+      for (int i = 0; i < VEC * W; i += PIECE) {
+        const Pack<float, PIECE> v = load_pack<float, PIECE>(from + i);
 #pragma unroll
-      for (int k = 0; k < W; ++k) w[i][k] = __ldg(p.weight + (size_t)(c + i) * W + k);
+        for (int k = 0; k < PIECE; ++k) w[(i + k) / W][(i + k) % W] = v.v[k];
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < VEC * W; ++i) w[i / W][i % W] = __ldg(from + i);
     }
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) b[i] = p.bias ? __ldg(p.bias + c + i) : 0.f;
   }
   // line: the W inputs of a token, oldest first
-  __device__ __forceinline__ Pack<T, VEC> out(const float (&line)[W][VEC], int act) const {
+  __device__ __forceinline__ Pack<T, VEC> out(const float (&line)[W][VEC], bool act) const {
     float y[VEC];
 #pragma unroll
     for (int i = 0; i < VEC; ++i) {
@@ -36,12 +46,14 @@ struct Taps {
   }
 };
 
-// A thread walks a run of tokens of VEC channels with the last W-1 inputs in registers, eight tokens requested at a time;
+// A thread walks a run of tokens of VEC channels with the last W-1 inputs in registers;
 // the threads behind the last run write the final state.
-template <typename T, int W, int VEC>
+template <typename T, int W, int VEC, bool ACT>
 __global__ void __launch_bounds__(128) short_conv_kernel(const lq_conv_problem p, int run, int runs) {
   pdl_enter();
-  constexpr int U = 8;
+  constexpr bool WIDE = VEC * sizeof(T) == 16;
+  constexpr int U = WIDE ? 4 : 8, RING = 16;
+  __shared__ Pack<T, VEC> ring[WIDE ? RING : 1][WIDE ? 128 : 1];
   const int nvec = p.D / VEC, per_b = runs + (p.final_state != nullptr);
   const long long idx = (long long)blockIdx.x * 128 + threadIdx.x;
   const long long rest = idx / nvec;
@@ -70,21 +82,49 @@ __global__ void __launch_bounds__(128) short_conv_kernel(const lq_conv_problem p
     float line[W][VEC];
 #pragma unroll
     for (int k = 1; k < W; ++k) input(t0 - W + k).get(line[k]);
-    for (int t = t0; t < live; t += U) {
-      Pack<T, VEC> raw[U];
+    auto next = [&](const Pack<T, VEC>& raw, int t) {
 #pragma unroll
-      for (int u = 0; u < U; ++u)
-        if (t + u < live) raw[u] = load_pack<T, VEC>(x + (t + u) * p.x_stride_t);
+      for (int k = 0; k + 1 < W; ++k)
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        if (t + u >= live) break;
+        for (int i = 0; i < VEC; ++i) line[k][i] = line[k + 1][i];
+      raw.get(line[W - 1]);
+      store_pack(y + (size_t)t * p.D, taps.out(line, ACT));
+    };
+    if constexpr (VEC * sizeof(T) == 16) {  // tokens arrive in a ring of the thread's own: AHEAD of them on their way without registers
+      auto issue = [&](int g) {
+        if (t0 + g * U < live) {
 #pragma unroll
-        for (int k = 0; k + 1 < W; ++k)
+          for (int u = 0; u < U; ++u) {
+            const int t = t0 + g * U + u;
+            if (t < live) cp_async16(&ring[(g * U + u) % RING][threadIdx.x], x + t * p.x_stride_t);
+          }
+        }
+        cp_async_commit();
+      };
 #pragma unroll
-          for (int i = 0; i < VEC; ++i) line[k][i] = line[k + 1][i];
-        raw[u].get(line[W - 1]);
-        store_pack(y + (size_t)(t + u) * p.D, taps.out(line, p.silu));
+      for (int g = 0; g < RING / U - 1; ++g) issue(g);
+      for (int g = 0, t = t0; t < live; ++g, t += U) {
+        issue(g + RING / U - 1);
+        cp_async_wait<RING / U - 1>();
+        if (t + U <= live) {
+#pragma unroll
+          for (int u = 0; u < U; ++u) next(ring[(g * U + u) % RING][threadIdx.x], t + u);
+        } else {
+          for (int u = 0; t + u < live; ++u) next(ring[(g * U + u) % RING][threadIdx.x], t + u);
+        }
       }
+      cp_async_wait<0>();
+    } else {
+      int t = t0;
+      for (; t + U <= live; t += U) {
+        Pack<T, VEC> raw[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) raw[u] = load_pack<T, VEC>(x + (t + u) * p.x_stride_t);
+#pragma unroll
+        for (int u = 0; u < U; ++u) next(raw[u], t + u);
+      }
+#pragma unroll 1
+      for (; t < live; ++t) next(load_pack<T, VEC>(x + t * p.x_stride_t), t);
     }
   }
   Pack<T, VEC> none;
@@ -100,6 +140,9 @@ __global__ void __launch_bounds__(128) short_conv_step_kernel(const lq_conv_prob
   const int b = (int)(idx / nvec), c = (int)(idx - (long long)b * nvec) * VEC;
   if (b >= p.B) return;
   const int slot = p.slots ? p.slots[b] : b;
+  const Taps<T, W, VEC> taps(p, c);
+  Pack<T, VEC> raw[W];
+  raw[W - 1] = load_pack<T, VEC>(reinterpret_cast<const T*>(p.x) + b * p.x_stride_b + c);
   T* y = reinterpret_cast<T*>(p.y) + (size_t)b * p.D + c;
   if (slot < 0 || slot >= p.n_slots) {
     Pack<T, VEC> none;
@@ -108,11 +151,8 @@ __global__ void __launch_bounds__(128) short_conv_step_kernel(const lq_conv_prob
     return;
   }
   T* state = reinterpret_cast<T*>(p.state) + (size_t)slot * (W - 1) * p.D + c;
-  Pack<T, VEC> raw[W];
 #pragma unroll
   for (int k = 0; k + 1 < W; ++k) raw[k] = load_pack<T, VEC>(state + (size_t)k * p.D);
-  raw[W - 1] = load_pack<T, VEC>(reinterpret_cast<const T*>(p.x) + b * p.x_stride_b + c);
-  const Taps<T, W, VEC> taps(p, c);
   float line[W][VEC];
 #pragma unroll
   for (int k = 0; k < W; ++k) raw[k].get(line[k]);
@@ -139,15 +179,17 @@ static int with_taps(int W, F&& f) {
 
 template <typename T, int VEC>
 static int run_fwd(const lq_conv_problem* p, cudaStream_t st) {
-  // Long runs read fewer inputs twice (W - 1 per run), short ones fill the GPU
-  const long long lanes = (long long)p->B * (p->D / VEC);
-  const int run = lanes * (p->T / 32) >= (long long)sm_count() * 1024 ? 32 : 8;
+  // Long runs load the taps and the inputs ahead of a run (W - 1) less often, short ones fill the GPU
+  const long long lanes = (long long)p->B * (p->D / VEC), fill = (long long)sm_count() * 512;
+  const int run = lanes * (p->T / 128) >= 3 * fill ? 128 : lanes * (p->T / 32) >= fill ? 32 : 8;
   const int runs = (p->T + run - 1) / run;
   const long long threads = lanes * (runs + (p->final_state != nullptr));
   if (threads == 0) return LQ_OK;
   if (threads / 128 >= (1ll << 31) - 1) return fail(LQ_ERR_SHAPE, "short_conv: B=%d T=%d D=%d", p->B, p->T, p->D);
   return with_taps(p->W, [&](auto w) {
-    launch(short_conv_kernel<T, decltype(w)::value, VEC>, dim3((unsigned)((threads + 127) / 128)), dim3(128), 0, st, *p, run, runs);
+    auto go = [&](auto kern) { launch(kern, dim3((unsigned)((threads + 127) / 128)), dim3(128), 0, st, *p, run, runs); };
+    if (p->silu) go(short_conv_kernel<T, decltype(w)::value, VEC, true>);
+    else go(short_conv_kernel<T, decltype(w)::value, VEC, false>);
     return check_launch("short_conv_kernel");
   });
 }
@@ -181,9 +223,8 @@ extern "C" int lq_short_conv_step(const lq_conv_problem* p, lq_stream stream) {
   if (int e = conv::check(p, true, "short_conv_step")) return e;
   return with_dtype(p->dtype, "short_conv_step", [&](auto t) {
     using T = decltype(t);
-    constexpr int FULL = 16 / sizeof(T);
-    Alignment a;
+    Alignment a;  // two channels a thread: more of them share the latency of the loads
     a.at(p->x).at(p->y).at(p->state).pitch(p->x_stride_b, sizeof(T)).pitch(p->D, sizeof(T));
-    return a.bytes() == 16 ? conv::run_step<T, FULL>(p, (cudaStream_t)stream) : conv::run_step<T, 1>(p, (cudaStream_t)stream);
+    return a.bytes() >= 2 * (int)sizeof(T) ? conv::run_step<T, 2>(p, (cudaStream_t)stream) : conv::run_step<T, 1>(p, (cudaStream_t)stream);
   });
 }

@@ -55,8 +55,13 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
   return y;
 }
+__device__ __forceinline__ float rcp(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
+  return y;
+}
 // x / (1 + e^-x); e^-x = inf gives -0
-__device__ __forceinline__ float silu(float x) { return __fdividef(x, 1.0f + __expf(-x)); }
+__device__ __forceinline__ float silu(float x) { return x * rcp(1.0f + ex2(-kLog2e * x)); }
 
 // log(1 + e^x) = max(x, 0) + log1p(w), w = e^-|x| in (0, 1]; log1p(w) = 2 atanh(s), s = w / (2 + w) <= 1/3: accurate where the
 // result is small, where log(1 + w) would lose w's low bits, and without a branch. atanh(s) / s is a polynomial in s^2 fitted at
@@ -64,7 +69,7 @@ __device__ __forceinline__ float silu(float x) { return __fdividef(x, 1.0f + __e
 __device__ __forceinline__ float softplus(float x) {
   const float a = -fabsf(x), e = a * kLog2e;
   // what e lost to rounding, with the part of log2(e) that a float does not hold: w is dt's relative error where x is negative
-  const float w = ex2(e), low = fmaf(a, kLog2e, -e) + a * 1.92596299e-8f, ww = fmaf(w, low * 0.6931471805599453f, w);
+  const float w = ex2(e), low = fmaf(a, kLog2e, -e) + a * 1.92596299e-8f, ww = w > 0.0f ? fmaf(w, low * 0.6931471805599453f, w) : w;
   const float s = __fdividef(ww, 2.0f + ww), q = s * s;
   float t = 0.14087328631750926f;
   t = fmaf(t, q, 0.13980709417397671f);

@@ -14,22 +14,23 @@ namespace lq {
 
 namespace norm {
 
-enum Kind { ADD, GATED, PLAIN };
+enum Kind { PLAIN, ADD, ADD32, GATED };  // ADD32: the residual stream in fp32
 
 // A team holds one row (or group): a power of two up to 32 lanes of a warp, or all warps of the CTA.
 struct Team {
-  int size, rank;
-  float* sm;  // 32 floats per reduction, each reduction its own
+  int size;
+  float* sm;  // 32 floats; reductions take turns between two of them, so one barrier each is enough
+  int turn = 0;
   template <typename Op>
   __device__ __forceinline__ float reduce(float v, Op op) {
     for (int m = min(size, 32) >> 1; m; m >>= 1) v = op(v, __shfl_xor_sync(0xffffffffu, v, m));
     if (size > 32) {
-      const int warp = threadIdx.x >> 5, nwarps = size >> 5;
-      if ((threadIdx.x & 31) == 0) sm[warp] = v;
+      float* part = sm + 32 * turn;
+      turn ^= 1;
+      if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
       __syncthreads();
-      v = sm[0];
-      for (int w = 1; w < nwarps; ++w) v = op(v, sm[w]);
-      sm += 32;
+      v = part[0];
+      for (int w = 1; w < size >> 5; ++w) v = op(v, part[w]);
     }
     return v;
   }
@@ -37,155 +38,230 @@ struct Team {
   __device__ __forceinline__ float max(float v) { return reduce(v, [](float a, float b) { return max_nan(a, b); }); }
 };
 
-template <int VEC>
-__device__ __forceinline__ void load_f32(const float* p, int c, float (&x)[VEC]) {  // parameters: dense, 16-byte aligned where VEC > 1
-  if constexpr (VEC % 4 == 0) {
+// The code rule for a row whose scale is its own: |x inv| exceeds 127 by roundings at most, so nothing has to be clamped
+__device__ __forceinline__ int code(float x, float inv) {
+  const float y = __fmul_rn(x, inv);
+  return __float2int_rz(__fadd_rn(y, copysignf(0.5f, y)));
+}
+
+// A thread has NV packs of VEC channels. OFF: the rows do not start on a pack's boundary, but those of all tensors at the same
+// distance behind one; packs lie on the boundaries, the first and the last of a row hold channels that are not the row's.
+template <int VEC, bool OFF>
+struct Place {
+  int c, n;  // first channel, channels of the row
+  __device__ __forceinline__ bool any() const { return OFF ? c > -VEC && c < n : c < n; }
+  __device__ __forceinline__ bool all() const { return !OFF || (c >= 0 && c + VEC <= n); }
+  __device__ __forceinline__ bool has(int i) const { return !OFF || ((unsigned)(c + i) < (unsigned)n); }
+};
+
+template <int VEC, bool OFF>
+__device__ __forceinline__ void load_f32(const float* p, const Place<VEC, OFF>& at, float (&x)[VEC]) {  // parameters: dense
+  if constexpr (VEC % 4 == 0 && !OFF) {
 #pragma unroll
     for (int i = 0; i < VEC; i += 4) {
-      const float4 v = __ldg(reinterpret_cast<const float4*>(p + c + i));
+      const float4 v = __ldg(reinterpret_cast<const float4*>(p + at.c + i));
       x[i] = v.x; x[i + 1] = v.y; x[i + 2] = v.z; x[i + 3] = v.w;
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) x[i] = __ldg(p + c + i);
+    for (int i = 0; i < VEC; ++i) x[i] = at.all() || at.has(i) ? __ldg(p + at.c + i) : 0.f;
   }
 }
-template <int VEC>
-__device__ __forceinline__ void store_as(void* base, size_t at, int dtype, const float (&y)[VEC]) {
-  if (dtype == LQ_F32) {
-    if constexpr (VEC % 4 == 0) {
+template <typename TO, int VEC, bool OFF>
+__device__ __forceinline__ void store_row(TO* row, const Place<VEC, OFF>& at, const float (&y)[VEC]) {
+  if (at.all()) {
+    constexpr int PV = VEC * sizeof(TO) > 16 ? 16 / sizeof(TO) : VEC;
 #pragma unroll
-      for (int i = 0; i < VEC; i += 4)
-        *reinterpret_cast<float4*>(reinterpret_cast<float*>(base) + at + i) = make_float4(y[i], y[i + 1], y[i + 2], y[i + 3]);
-    } else {
+    for (int k = 0; k < VEC; k += PV) {
+      float f[PV];
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) reinterpret_cast<float*>(base)[at + i] = y[i];
+      for (int i = 0; i < PV; ++i) f[i] = y[k + i];
+      Pack<TO, PV> v;
+      v.set(f);
+      store_pack(row + at.c + k, v);
     }
-  } else if (dtype == LQ_F16) {
-    Pack<__half, VEC> v;
-    v.set(y);
-    store_pack(reinterpret_cast<__half*>(base) + at, v);
   } else {
-    Pack<__nv_bfloat16, VEC> v;
-    v.set(y);
-    store_pack(reinterpret_cast<__nv_bfloat16*>(base) + at, v);
+#pragma unroll
+    for (int i = 0; i < VEC; ++i)
+      if (at.has(i)) row[at.c + i] = from_f32<TO>(y[i]);
   }
 }
+template <int VEC, bool OFF>
+__device__ __forceinline__ void store_as(void* base, size_t at_row, int dtype, const Place<VEC, OFF>& at, const float (&y)[VEC]) {
+  if (dtype == LQ_F32) store_row(reinterpret_cast<float*>(base) + at_row, at, y);
+  else if (dtype == LQ_F16) store_row(reinterpret_cast<__half*>(base) + at_row, at, y);
+  else store_row(reinterpret_cast<__nv_bfloat16*>(base) + at_row, at, y);
+}
 
-template <typename T, int VEC, int NV, Kind KIND>
-__global__ void __launch_bounds__(NV * VEC > 16 ? 512 : 1024) norm_kernel(const lq_norm_problem p, int team_size, long long units) {
+// CTAs walk over the rows; a row's loads are requested while the one before is summed and stored.
+template <typename T, int VEC, int NV, Kind KIND, bool OFF>
+__global__ void __launch_bounds__(NV == 1 || NV * VEC == 4 ? 1024 : 512) norm_kernel(const lq_norm_problem p, int team_size, long long units) {
   pdl_enter();
-  __shared__ float sm[3 * 32];
-  const int rank = threadIdx.x % team_size;
-  const long long unit = (long long)blockIdx.x * (blockDim.x / team_size) + threadIdx.x / team_size;
-  const bool live = unit < units;  // lanes of a team that has no row still take part in the shuffles
-  const int per_row = p.D / p.group;
-  const long long row = live ? unit / per_row : 0;
-  const int c0 = (int)(live ? unit - row * per_row : 0) * p.group;
-  const T* x = reinterpret_cast<const T*>(p.x) + row * p.x_stride + c0;
-  Team team{team_size, rank, sm};
+  constexpr bool SECOND = KIND != PLAIN;
+  using R = std::conditional_t<KIND == ADD32, float, T>;  // of the second input: the residual or the gate
+  __shared__ float sm[2 * 32];
+  const int rank = threadIdx.x % team_size, per_row = p.D / p.group;
+  const long long step = (long long)gridDim.x * (blockDim.x / team_size);
+  Team team{team_size, sm};
   const float inv_n = 1.0f / (float)p.group;
+  const bool has_second = KIND == GATED || p.residual != nullptr;
 
-  float v[NV][VEC], g[KIND == GATED ? NV : 1][VEC];
-  bool on[NV];
-  {
-    Pack<T, VEC> raw[NV], rawg[KIND == GATED ? NV : 1];
+  Pack<T, VEC> raw[NV];
+  constexpr int RV = VEC * sizeof(R) > 16 ? 16 / sizeof(R) : VEC;
+  Pack<R, RV> raw2[SECOND ? NV : 1][SECOND ? VEC / RV : 1];
+  auto place = [&](const T* x, int j) {
+    const int off = OFF ? (int)((reinterpret_cast<uintptr_t>(x) / sizeof(T)) & (VEC - 1)) : 0;
+    return Place<VEC, OFF>{(j * team_size + rank) * VEC - off, p.group};
+  };
+  auto row_of = [&](long long unit, long long& row, int& c0) {
+    row = per_row == 1 ? unit : unit / per_row;
+    c0 = per_row == 1 ? 0 : (int)(unit - row * per_row) * p.group;
+  };
+  auto request = [&](long long unit) {
+    if (unit >= units) return;
+    long long row;
+    int c0;
+    row_of(unit, row, c0);
+    const T* x = reinterpret_cast<const T*>(p.x) + row * p.x_stride + c0;
+    const R* r = nullptr;
+    if constexpr (KIND == GATED) r = reinterpret_cast<const R*>(p.gate) + row * p.gate_stride + c0;
+    else if constexpr (SECOND) r = reinterpret_cast<const R*>(p.residual) + row * p.residual_stride;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      const int c = (j * team_size + rank) * VEC;
-      on[j] = live && c < p.group;
-      raw[j].zero();
-      if (on[j]) raw[j] = load_pack<T, VEC>(x + c);
-      if constexpr (KIND == GATED) {
-        rawg[j].zero();
-        if (on[j]) rawg[j] = load_pack<T, VEC>(reinterpret_cast<const T*>(p.gate) + row * p.gate_stride + c0 + c);
+      const Place<VEC, OFF> at = place(x, j);
+      if (!at.any()) continue;
+      raw[j] = load_pack<T, VEC>(x + at.c);
+      if constexpr (SECOND) {
+        if (has_second) {
+#pragma unroll
+          for (int k = 0; k < VEC / RV; ++k) raw2[j][k] = load_pack<R, RV>(r + at.c + k * RV);
+        }
       }
     }
+  };
+
+  long long unit = (long long)blockIdx.x * (blockDim.x / team_size) + threadIdx.x / team_size;
+  const long long rounds = (units - (long long)blockIdx.x * (blockDim.x / team_size) + step - 1) / step;  // the same for all teams: lanes without a row take part
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      raw[j].get(v[j]);
-      if constexpr (KIND == GATED) rawg[j].get(g[j]);
+  for (int j = 0; j < NV; ++j) {  // packs behind the last stay zero
+    raw[j].zero();
+    if constexpr (SECOND) {
+#pragma unroll
+      for (int k = 0; k < VEC / RV; ++k) raw2[j][k].zero();
     }
   }
-  auto rms = [&]() {
-    float s = 0.f;
-#pragma unroll
-    for (int j = 0; j < NV; ++j)
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) s = fmaf(v[j][i], v[j][i], s);
-    return rsqrtf(fmaf(team.sum(s), inv_n, p.eps));
-  };
-  auto times = [&](float f, const float* w) {  // v f w
+  request(unit);
+  for (long long round = 0; round < rounds; ++round, unit += step) {
+    const bool live = unit < units;
+    long long row;
+    int c0;
+    row_of(live ? unit : 0, row, c0);
+    const T* x = reinterpret_cast<const T*>(p.x) + row * p.x_stride + c0;
+    float v[NV][VEC], g[SECOND ? NV : 1][VEC];
+    Place<VEC, OFF> at[NV];
+    bool on[NV];
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      if (!on[j]) continue;
-      float ww[VEC];
-      load_f32<VEC>(w, c0 + (j * team_size + rank) * VEC, ww);
+      at[j] = place(x, j);
+      on[j] = live && at[j].any();
+      raw[j].get(v[j]);
+      if constexpr (SECOND) {
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) v[j][i] = v[j][i] * f * ww[i];
-    }
-  };
-
-  if constexpr (KIND == ADD) {
-    if (p.post_weight) times(rms(), p.post_weight);
-    if (p.residual) {
+        for (int k = 0; k < VEC / RV; ++k) {
+          float f[RV];
+          raw2[j][k].get(f);
 #pragma unroll
-      for (int j = 0; j < NV; ++j) {
-        if (!on[j]) continue;
-        const int c = (j * team_size + rank) * VEC;
-        float r[VEC], s[VEC];
-        if (p.residual_f32) load_f32<VEC>(reinterpret_cast<const float*>(p.residual) + row * p.residual_stride, c, r);
-        else load_pack<T, VEC>(reinterpret_cast<const T*>(p.residual) + row * p.residual_stride + c).get(r);
-        if (p.scale_vec) load_f32<VEC>(p.scale_vec, c, s);
+          for (int i = 0; i < RV; ++i) g[j][k * RV + i] = f[i];
+        }
+      }
+      if (OFF && !at[j].all()) {  // channels of the rows next to this one
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) v[j][i] = fmaf(p.scale_vec ? s[i] * p.residual_scale : p.residual_scale, v[j][i], r[i]);
-        if (p.residual_f32) store_as<VEC>(p.residual_out, (size_t)row * p.D + c, LQ_F32, v[j]);
-        else store_as<VEC>(p.residual_out, (size_t)row * p.D + c, std::is_same_v<T, float> ? LQ_F32 : std::is_same_v<T, __half> ? LQ_F16 : LQ_BF16, v[j]);
+        for (int i = 0; i < VEC; ++i)
+          if (!at[j].has(i)) {
+            v[j][i] = 0.f;
+            if constexpr (SECOND) g[j][i] = 0.f;
+          }
       }
     }
-    if (p.weight) times(rms(), p.weight);
-  } else if constexpr (KIND == GATED) {
-    auto gate = [&]() {
+    request(unit + step);
+    auto rms = [&]() {
+      float s = 0.f;
 #pragma unroll
       for (int j = 0; j < NV; ++j)
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) v[j][i] *= silu(g[j][i]);
+        for (int i = 0; i < VEC; ++i) s = fmaf(v[j][i], v[j][i], s);
+      return rsqrtf(fmaf(team.sum(s), inv_n, p.eps));
     };
-    if (p.gate_first) gate();
-    times(rms(), p.weight);
-    if (!p.gate_first) gate();
-  }
-  if (p.codes) {
-    float amax = 0.f, inv;
+    auto times = [&](float f, const float* w) {  // v f w
 #pragma unroll
-    for (int j = 0; j < NV; ++j)
-      if (on[j])
+      for (int j = 0; j < NV; ++j) {
+        if (!on[j]) continue;
+        float ww[VEC];
+        load_f32(w + c0, at[j], ww);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) v[j][i] = v[j][i] * f * ww[i];
+      }
+    };
+
+    if constexpr (KIND == ADD || KIND == ADD32) {
+      if (p.post_weight) times(rms(), p.post_weight);
+      if (has_second) {
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+          if (!on[j]) continue;
+          float s[VEC];
+          if (p.scale_vec) load_f32(p.scale_vec, at[j], s);
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) v[j][i] = fmaf(p.scale_vec ? s[i] * p.residual_scale : p.residual_scale, v[j][i], g[j][i]);
+          store_row(reinterpret_cast<R*>(p.residual_out) + (size_t)row * p.D, at[j], v[j]);
+        }
+      }
+      if (p.weight) times(rms(), p.weight);
+    } else if constexpr (KIND == GATED) {
+      auto gate = [&]() {
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) v[j][i] *= silu(g[j][i]);
+      };
+      if (p.gate_first) gate();
+      times(rms(), p.weight);
+      if (!p.gate_first) gate();
+    }
+    if (p.codes) {
+      float amax = 0.f, inv;
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
 #pragma unroll
         for (int i = 0; i < VEC; ++i) amax = max_nan(amax, fabsf(v[j][i]));
-    const float scale = row_scale(team.max(amax), inv);
-    if (live && rank == 0) p.scale[row] = scale;
+      const float scale = row_scale(team.max(amax), inv);
+      if (live && rank == 0) p.scale[row] = scale;
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      if (!on[j]) continue;
-      int8_t* out = p.codes + row * p.codes_stride + (j * team_size + rank) * VEC;
-      if constexpr (VEC == 1) {
-        out[0] = (int8_t)q8(v[j][0], inv, 127.f);
-      } else {
+      for (int j = 0; j < NV; ++j) {
+        if (!on[j]) continue;
+        int8_t* out = p.codes + row * p.codes_stride + at[j].c;
+        if constexpr (VEC == 1 || OFF) {
 #pragma unroll
-        for (int i = 0; i < VEC; i += 4)
-          reinterpret_cast<uint32_t*>(out)[i / 4] = q8x4_127(v[j][i], v[j][i + 1], v[j][i + 2], v[j][i + 3], inv);
+          for (int i = 0; i < VEC; ++i)
+            if (at[j].has(i)) out[i] = (int8_t)code(v[j][i], inv);
+        } else {
+          uint32_t w[VEC / 4];
+#pragma unroll
+          for (int i = 0; i < VEC; i += 4)
+            w[i / 4] = pack_sat_s8x2(code(v[j][i + 1], inv), code(v[j][i], inv), pack_sat_s8x2(code(v[j][i + 3], inv), code(v[j][i + 2], inv), 0u));
+          if constexpr (VEC == 8) *reinterpret_cast<uint2*>(out) = make_uint2(w[0], w[1]);
+          else *reinterpret_cast<uint32_t*>(out) = w[0];
+        }
       }
-    }
-  } else if (p.y) {
+    } else if (p.y) {
 #pragma unroll
-    for (int j = 0; j < NV; ++j)
-      if (on[j]) store_as<VEC>(p.y, (size_t)row * p.D + c0 + (j * team_size + rank) * VEC, p.out_dtype, v[j]);
+      for (int j = 0; j < NV; ++j)
+        if (on[j]) store_as(p.y, (size_t)row * p.D + c0, p.out_dtype, at[j], v[j]);
+    }
   }
 }
 
-// Registers hold the row: the fewest loads a thread that leave a team of at most 256 threads (a row is then in flight from
-// many small CTAs), more where the row is longer.
-template <typename T, Kind KIND, int VEC, int NV>
+template <typename T, Kind KIND, int VEC, int NV, bool OFF>
 static int launch_as(const lq_norm_problem* p, int packs, cudaStream_t st) {
   const int need = (packs + NV - 1) / NV;
   int team = 1;
@@ -194,37 +270,65 @@ static int launch_as(const lq_norm_problem* p, int packs, cudaStream_t st) {
   const int threads = team > 32 ? team : 128;  // teams of several warps have the CTA's barrier and its sums to themselves
   const long long units = (long long)p->rows * (p->D / p->group), per_cta = threads / team;
   const long long ctas = (units + per_cta - 1) / per_cta;
-  if (ctas >= (1ll << 31)) return fail(LQ_ERR_SHAPE, "norm: rows=%d D=%d group=%d", p->rows, p->D, p->group);
-  launch(norm_kernel<T, VEC, NV, KIND>, dim3((unsigned)ctas), dim3(threads), 0, st, *p, team, units);
+  int per_sm = 0;
+  auto kern = norm_kernel<T, VEC, NV, KIND, OFF>;
+  const cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, threads, 0);
+  if (e != cudaSuccess) return fail(LQ_ERR_LAUNCH, "norm: %s", cudaGetErrorString(e));
+  const long long most = (long long)sm_count() * per_sm;
+  launch(kern, dim3((unsigned)(ctas < most ? ctas : most)), dim3(threads), 0, st, *p, team, units);
   return check_launch("norm_kernel");
 }
-template <typename T, Kind KIND, int VEC>
+// Registers hold the row, the next one on its way. Few loads a thread where rows are short of threads for the GPU (their
+// latency is what such a call costs); else two, which leaves the most rows in flight: at 32768 x 5120 (gated, bf16) NV = 1, 2,
+// 4 take 336, 242, 252 us, at 64 x 2560 2.4, 2.8, 4.1.
+template <typename T, Kind KIND, int VEC, bool OFF>
 static int launch_vec(const lq_norm_problem* p, cudaStream_t st) {
-  const int packs = (p->group + VEC - 1) / VEC;
-  constexpr int MOST = VEC == 1 ? 32 : 32 / VEC;  // 32 values a thread
-  if (packs <= 256) return launch_as<T, KIND, VEC, 1>(p, packs, st);
-  if (packs <= 1024) return launch_as<T, KIND, VEC, MOST < 4 ? MOST : 4>(p, packs, st);
-  if (packs <= 512 * MOST) return launch_as<T, KIND, VEC, MOST>(p, packs, st);
-  return fail(LQ_ERR_UNSUPPORTED, "norm over %d channels (at most %d)", p->group, 16384);
+  const int packs = (p->group + VEC - 1) / VEC + OFF;
+  const bool few = (long long)p->rows * (p->D / p->group) <= sm_count();
+  if constexpr (VEC == 1) {
+    if (packs <= 1024) return launch_as<T, KIND, 1, 4, OFF>(p, packs, st);
+    if (packs <= 16384) return launch_as<T, KIND, 1, 32, OFF>(p, packs, st);
+  } else {
+    if (packs <= 32 || (few && packs <= 1024)) return launch_as<T, KIND, VEC, 1, OFF>(p, packs, st);
+    if (packs <= 1024) return launch_as<T, KIND, VEC, 2, OFF>(p, packs, st);
+    if (packs <= 512 * 32 / VEC + OFF) return launch_as<T, KIND, VEC, 32 / VEC, OFF>(p, packs, st);
+  }
+  return fail(LQ_ERR_UNSUPPORTED, "norm over %d channels (at most 16384)", p->group);
 }
-template <Kind KIND>
-static int run(const lq_norm_problem* p, const char* what, cudaStream_t st) {
+template <typename T, Kind KIND>
+static int run_kind(const lq_norm_problem* p, cudaStream_t st) {
+  constexpr int FULL = 16 / sizeof(T), S = sizeof(T);
+  // every row of every tensor on a pack's boundary, the codes' on FULL bytes
+  Alignment in, params, y;
+  in.at(p->x).pitch(p->x_stride, S).pitch(p->group, S);
+  if (p->gate) in.at(p->gate).pitch(p->gate_stride, S);
+  params.at(p->weight).at(p->post_weight).at(p->scale_vec);
+  if (KIND == ADD32) params.at(p->residual).pitch(p->residual_stride, 4).at(p->residual_out).pitch(p->D, 4);
+  else if (p->residual) in.at(p->residual).pitch(p->residual_stride, S).at(p->residual_out);
+  const int so = dtype_bytes(p->out_dtype), out = so * FULL;
+  y.at(p->y).pitch(p->D, so).pitch(p->group, so);
+  if (in.bytes() == 16 && params.bytes() == 16 && (p->y == nullptr || y.bytes() >= (out < 16 ? out : 16))) return launch_vec<T, KIND, FULL, false>(p, st);
+  // rows off the boundary, all tensors' alike: one type, one pitch and one distance
+  if constexpr (KIND != ADD32) {
+    auto alike = [&](const void* t, long long pitch, int size) {
+      return t == nullptr || (size == S && pitch == p->x_stride && ((reinterpret_cast<uintptr_t>(t) ^ reinterpret_cast<uintptr_t>(p->x)) & 15) == 0);
+    };
+    if (p->group == p->D && alike(p->gate, p->gate_stride, S) && alike(p->residual, p->residual_stride, S) && alike(p->residual_out, p->D, S) &&
+        alike(p->y, p->D, so))
+      return launch_vec<T, KIND, FULL, true>(p, st);
+  }
+  return launch_vec<T, KIND, 1, false>(p, st);
+}
+enum Form { NORM, GATE, CODES };
+static int run(const lq_norm_problem* p, Form form, const char* what, cudaStream_t st) {
   return with_dtype(p->dtype, what, [&](auto t) {
     using T = decltype(t);
-    constexpr int FULL = 16 / sizeof(T), S = sizeof(T);
-    const int out = dtype_bytes(p->out_dtype) * FULL, res = p->residual_f32 ? 4 : S;
-    Alignment in, params;
-    in.at(p->x).pitch(p->x_stride, S).pitch(p->group, S);
-    if (p->gate) in.at(p->gate).pitch(p->gate_stride, S);
-    params.at(p->weight).at(p->post_weight).at(p->scale_vec);
-    if (p->residual_f32) params.at(p->residual).pitch(p->residual_stride, 4).at(p->residual_out).pitch(p->D, 4);
-    else if (p->residual) in.at(p->residual).pitch(p->residual_stride, res).at(p->residual_out);
-    Alignment y;
-    y.at(p->y).pitch(p->D, dtype_bytes(p->out_dtype)).pitch(p->group, dtype_bytes(p->out_dtype));
-    Alignment codes;
-    codes.at(p->codes).pitch(p->codes_stride, 1);
-    const bool wide = in.bytes() == 16 && params.bytes() == 16 && (p->y == nullptr || y.bytes() >= (out < 16 ? out : 16)) && codes.bytes() == 16;
-    return wide ? launch_vec<T, KIND, FULL>(p, st) : launch_vec<T, KIND, 1>(p, st);
+    if (form == GATE) return run_kind<T, GATED>(p, st);
+    if (form == CODES) return run_kind<T, PLAIN>(p, st);
+    if constexpr (!std::is_same_v<T, float>) {
+      if (p->residual && p->residual_f32) return run_kind<T, ADD32>(p, st);
+    }
+    return run_kind<T, ADD>(p, st);
   });
 }
 
@@ -255,7 +359,7 @@ extern "C" int lq_rms_norm(const lq_norm_problem* p, lq_stream stream) {
   if ((p->y || p->codes) != (p->weight != nullptr)) return fail(LQ_ERR_NULL, "rms_norm: an output and its weight go together");
   if (!p->weight && !p->residual) return fail(LQ_ERR_NULL, "rms_norm: nothing to compute");
   if (p->post_weight && !p->residual) return fail(LQ_ERR_NULL, "rms_norm: post_weight without a residual");
-  return norm::run<norm::ADD>(p, "rms_norm", (cudaStream_t)stream);
+  return norm::run(p, norm::NORM, "rms_norm", (cudaStream_t)stream);
 }
 
 extern "C" int lq_gated_rms_norm(const lq_norm_problem* p, lq_stream stream) {
@@ -264,7 +368,7 @@ extern "C" int lq_gated_rms_norm(const lq_norm_problem* p, lq_stream stream) {
   if (p->rows == 0) return LQ_OK;
   if (!p->gate || !p->weight || !(p->y || p->codes)) return fail(LQ_ERR_NULL, "gated_rms_norm: gate, weight and an output must be non-null");
   if (p->residual || p->post_weight) return fail(LQ_ERR_UNSUPPORTED, "gated_rms_norm takes no residual");
-  return norm::run<norm::GATED>(p, "gated_rms_norm", (cudaStream_t)stream);
+  return norm::run(p, norm::GATE, "gated_rms_norm", (cudaStream_t)stream);
 }
 
 extern "C" int lq_quantize_rows(const void* x, int dtype, int rows, int D, long long x_stride, int8_t* codes, long long codes_stride, float* scale,
@@ -277,5 +381,5 @@ extern "C" int lq_quantize_rows(const void* x, int dtype, int rows, int D, long 
   if (int e = norm::check(&p, "quantize_rows")) return e;
   if (rows == 0) return LQ_OK;
   if (!codes) return fail(LQ_ERR_NULL, "quantize_rows: codes is null");
-  return norm::run<norm::PLAIN>(&p, "quantize_rows", (cudaStream_t)stream);
+  return norm::run(&p, norm::CODES, "quantize_rows", (cudaStream_t)stream);
 }

@@ -502,7 +502,7 @@ static int run(const lq_scan_problem* p, cudaStream_t st) {
 // A row is the N states of one channel. LPR lanes hold it, VEC states each per step over N; a thread group takes R rows of
 // one head (HEADS: they share the decay, B and C) or one row with a decay rate per state.
 template <typename T, typename TS, int VEC, int R, bool HEADS>
-__global__ void __launch_bounds__(128) selective_scan_step_kernel(const lq_scan_problem p, int lpr) {
+__global__ void __launch_bounds__(128) selective_scan_step_kernel(const lq_scan_problem p, int lpr, bool wide_bc) {
   pdl_enter();
   const long long idx = (long long)blockIdx.x * 128 + threadIdx.x;
   const int ln = (int)(idx % lpr), per_b = p.D / R;
@@ -513,34 +513,58 @@ __global__ void __launch_bounds__(128) selective_scan_step_kernel(const lq_scan_
   const bool on = live && slot >= 0 && slot < p.n_slots;
   const int head = HEADS ? d0 / p.P : d0;
   const int grp = HEADS ? head / (p.H / p.G) : d0 / (p.D / p.G);
-  float dt = 0.f;
+  const T* Bm = reinterpret_cast<const T*>(p.Bm) + b * p.B_stride_b + grp * p.B_stride_g;
+  const T* Cm = reinterpret_cast<const T*>(p.Cm) + b * p.C_stride_b + grp * p.C_stride_g;
+  TS* state = reinterpret_cast<TS*>(p.state) + ((size_t)(on ? slot : 0) * p.D + d0) * p.N;
+  Pack<TS, VEC> raw[R];
+  Pack<T, VEC> rB, rC;
+  float A[HEADS ? 1 : VEC];
+  auto request = [&](int n) {
+    const bool in = on && n < p.N;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      raw[r].zero();
+      if (in) raw[r] = load_pack<TS, VEC>(state + (size_t)r * p.N + n);
+    }
+    rB.zero();
+    rC.zero();
+    if (in) {
+      if (wide_bc) {
+        rB = load_pack<T, VEC>(Bm + n);
+        rC = load_pack<T, VEC>(Cm + n);
+      } else {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+          rB.v[i] = Bm[n + i];
+          rC.v[i] = Cm[n + i];
+        }
+      }
+      if constexpr (!HEADS) {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) A[i] = p.A[(size_t)d0 * p.N + n + i];
+      }
+    }
+  };
+  request(ln * VEC);  // the state first: everything else is small and comes out of the caches
+  float dt = 0.f, u[R], acc[R];
   if (on) {
     dt = to_f32(reinterpret_cast<const T*>(p.dt)[b * p.dt_stride_b + head]) + (p.dt_bias ? p.dt_bias[head] : 0.f);
+    if constexpr (HEADS) A[0] = p.A[head];
+#pragma unroll
+    for (int r = 0; r < R; ++r) u[r] = to_f32(reinterpret_cast<const T*>(p.u)[b * p.u_stride_b + d0 + r]);
     dt = p.softplus ? softplus(dt) : dt;
     dt = clamp_nan(dt, p.dt_min, p.dt_max);
   }
-  const T* Bm = reinterpret_cast<const T*>(p.Bm) + b * p.B_stride_b + grp * p.B_stride_g;
-  const T* Cm = reinterpret_cast<const T*>(p.Cm) + b * p.C_stride_b + grp * p.C_stride_g;
-  float u[R], acc[R];
 #pragma unroll
-  for (int r = 0; r < R; ++r) {
-    u[r] = on ? to_f32(reinterpret_cast<const T*>(p.u)[b * p.u_stride_b + d0 + r]) : 0.f;
-    acc[r] = 0.f;
-  }
-  const float head_decay = HEADS && on ? ex2(dt * (p.A[head] * kLog2e)) : 0.f;
+  for (int r = 0; r < R; ++r) acc[r] = 0.f;
   if (on) {
-    TS* state = reinterpret_cast<TS*>(p.state) + ((size_t)slot * p.D + d0) * p.N;
-    for (int n = ln * VEC; n < p.N; n += lpr * VEC) {
-      Pack<TS, VEC> raw[R];
-#pragma unroll
-      for (int r = 0; r < R; ++r) raw[r] = load_pack<TS, VEC>(state + (size_t)r * p.N + n);
+    const float head_decay = HEADS ? ex2(dt * (A[0] * kLog2e)) : 0.f;
+    for (int n = ln * VEC; n < p.N;) {
       float Bv[VEC], Cv[VEC], a[VEC];
+      rB.get(Bv);
+      rC.get(Cv);
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        Bv[i] = to_f32(Bm[n + i]);
-        Cv[i] = to_f32(Cm[n + i]);
-        a[i] = HEADS ? head_decay : ex2(dt * (p.A[(size_t)d0 * p.N + n + i] * kLog2e));
-      }
+      for (int i = 0; i < VEC; ++i) a[i] = HEADS ? head_decay : ex2(dt * (A[HEADS ? 0 : i] * kLog2e));
 #pragma unroll
       for (int r = 0; r < R; ++r) {
         float h[VEC];
@@ -554,6 +578,8 @@ __global__ void __launch_bounds__(128) selective_scan_step_kernel(const lq_scan_
         raw[r].set(h);
         store_pack(state + (size_t)r * p.N + n, raw[r]);
       }
+      n += lpr * VEC;
+      if (n < p.N) request(n);
     }
   }
 #pragma unroll
@@ -570,6 +596,128 @@ __global__ void __launch_bounds__(128) selective_scan_step_kernel(const lq_scan_
   }
 }
 
+// One decay a head and N states in one access of LPR lanes: a team walks over the channels of a head, R = 4 rows at a time, the
+// next four requested while those at hand are stored (a load, its sum and its store one after the other reach 4.0 TB/s).
+template <typename T, typename TS, int VEC>
+__global__ void __launch_bounds__(128) heads_step_kernel(const lq_scan_problem p, int lpr, int groups, bool wide_bc) {
+  pdl_enter();
+  constexpr int R = 4;
+  const long long idx = (long long)blockIdx.x * 128 + threadIdx.x;
+  const int ln = (int)(idx % lpr), per_head = p.P / (R * groups);
+  const long long unit = idx / lpr;
+  const bool live = unit < (long long)p.B * p.H * per_head;  // idle lanes still take part in the shuffles
+  const int b = live ? (int)(unit / (p.H * per_head)) : 0, in_b = live ? (int)(unit - (long long)b * p.H * per_head) : 0;
+  const int head = in_b / per_head, d0 = head * p.P + (in_b - head * per_head) * R * groups, grp = head / (p.H / p.G), n = ln * VEC;
+  const int slot = p.slots ? p.slots[b] : b;
+  const bool on = live && slot >= 0 && slot < p.n_slots, in = on && n < p.N;
+  TS* state = reinterpret_cast<TS*>(p.state) + ((size_t)(on ? slot : 0) * p.D + d0) * p.N + n;
+  const T* u = reinterpret_cast<const T*>(p.u) + b * p.u_stride_b + d0;
+  Pack<TS, VEC> next[R];
+  T nu[R];
+  auto request = [&](int g) {
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      if (in) next[r] = load_pack<TS, VEC>(state + (size_t)(g * R + r) * p.N);
+      else next[r].zero();
+      nu[r] = on ? u[g * R + r] : from_f32<T>(0.f);
+    }
+  };
+  request(0);
+  float Bv[VEC], Cv[VEC];
+  {
+    Pack<T, VEC> rB, rC;
+    rB.zero();
+    rC.zero();
+    const T* Bm = reinterpret_cast<const T*>(p.Bm) + b * p.B_stride_b + grp * p.B_stride_g + n;
+    const T* Cm = reinterpret_cast<const T*>(p.Cm) + b * p.C_stride_b + grp * p.C_stride_g + n;
+    if (in && wide_bc) {
+      rB = load_pack<T, VEC>(Bm);
+      rC = load_pack<T, VEC>(Cm);
+    } else if (in) {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        rB.v[i] = Bm[i];
+        rC.v[i] = Cm[i];
+      }
+    }
+    rB.get(Bv);
+    rC.get(Cv);
+  }
+  float decay = 0.f;
+  if (on) {
+    float dt = to_f32(reinterpret_cast<const T*>(p.dt)[b * p.dt_stride_b + head]) + (p.dt_bias ? p.dt_bias[head] : 0.f);
+    dt = clamp_nan(p.softplus ? softplus(dt) : dt, p.dt_min, p.dt_max);
+    decay = ex2(dt * (p.A[head] * kLog2e));
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) Bv[i] *= dt;
+  }
+  for (int g = 0; g < groups; ++g) {
+    Pack<TS, VEC> raw[R];
+    float uu[R], acc[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      raw[r] = next[r];
+      uu[r] = to_f32(nu[r]);
+    }
+    if (g + 1 < groups) request(g + 1);
+    const int d = d0 + g * R;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      float h[VEC];
+      raw[r].get(h);
+      acc[r] = 0.f;
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        h[i] = fmaf(decay, h[i], uu[r] * Bv[i]);
+        acc[r] = fmaf(h[i], Cv[i], acc[r]);
+      }
+      raw[r].set(h);
+      if (in) store_pack(state + (size_t)(g * R + r) * p.N, raw[r]);
+    }
+    int row;
+    if (lpr >= 4) {  // rows are handed out over the lanes while they are summed: each lane ends with one row
+      const bool hi = ln & (lpr >> 1), hi2 = ln & (lpr >> 2);
+      float a0 = hi ? acc[2] : acc[0], a1 = hi ? acc[3] : acc[1];
+      a0 += __shfl_xor_sync(0xffffffffu, hi ? acc[0] : acc[2], lpr >> 1);
+      a1 += __shfl_xor_sync(0xffffffffu, hi ? acc[1] : acc[3], lpr >> 1);
+      float v = hi2 ? a1 : a0;
+      v += __shfl_xor_sync(0xffffffffu, hi2 ? a0 : a1, lpr >> 2);
+      for (int m = lpr >> 3; m; m >>= 1) v += __shfl_xor_sync(0xffffffffu, v, m);
+      acc[0] = v;
+      row = 2 * hi + hi2;
+      if (ln & ((lpr >> 2) - 1)) row = R;  // one lane of each row's writes it
+    } else {
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+        for (int m = lpr >> 1; m; m >>= 1) acc[r] += __shfl_xor_sync(0xffffffffu, acc[r], m);
+      row = -1;  // lane 0 writes all
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      if (!live || !(row == r || (row == -1 && ln == 0))) continue;
+      float v = row < 0 ? acc[r] : acc[0];
+      if (p.skip) v = fmaf(p.skip[p.skip_has_hdim ? d + r : head], uu[r], v);
+      if (p.z && on) v *= silu(to_f32(reinterpret_cast<const T*>(p.z)[b * p.z_stride_b + d + r]));
+      reinterpret_cast<T*>(p.y)[(size_t)b * p.D + d + r] = from_f32<T>(on ? v : 0.f);
+    }
+  }
+}
+template <typename T, typename TS, int VEC>
+static int launch_heads(const lq_scan_problem* p, cudaStream_t st) {
+  int lpr = 1, groups = p->P / 4;
+  while (lpr * VEC < p->N) lpr *= 2;
+  // as many channels a team as leave threads for the GPU
+  auto threads = [&] { return (long long)p->B * p->H * (p->P / (4 * groups)) * lpr; };
+  while (groups > 1 && groups % 2 == 0 && threads() < (long long)sm_count() * 1024) groups /= 2;
+  if (threads() == 0) return LQ_OK;
+  if (threads() / 128 >= (1ll << 31) - 1) return fail(LQ_ERR_SHAPE, "selective_scan_step: B=%d D=%d N=%d", p->B, p->D, p->N);
+  constexpr int E = sizeof(T), BYTES = VEC * E < 16 ? VEC * E : 16;
+  Alignment a;
+  a.at(p->Bm).at(p->Cm).pitch(p->B_stride_b, E).pitch(p->B_stride_g, E).pitch(p->C_stride_b, E).pitch(p->C_stride_g, E);
+  launch(heads_step_kernel<T, TS, VEC>, dim3((unsigned)((threads() + 127) / 128)), dim3(128), 0, st, *p, lpr, groups, a.bytes() >= BYTES);
+  return check_launch("heads_step_kernel");
+}
+
 template <typename T, typename TS, int VEC, int R, bool HEADS>
 static int launch_step(const lq_scan_problem* p, cudaStream_t st) {
   int lpr = 1;
@@ -577,7 +725,10 @@ static int launch_step(const lq_scan_problem* p, cudaStream_t st) {
   const long long threads = (long long)p->B * (p->D / R) * lpr;
   if (threads == 0) return LQ_OK;
   if (threads / 128 >= (1ll << 31) - 1) return fail(LQ_ERR_SHAPE, "selective_scan_step: B=%d D=%d N=%d", p->B, p->D, p->N);
-  launch(selective_scan_step_kernel<T, TS, VEC, R, HEADS>, dim3((unsigned)((threads + 127) / 128)), dim3(128), 0, st, *p, lpr);
+  constexpr int E = sizeof(T), BYTES = VEC * E < 16 ? VEC * E : 16;
+  Alignment a;
+  a.at(p->Bm).at(p->Cm).pitch(p->B_stride_b, E).pitch(p->B_stride_g, E).pitch(p->C_stride_b, E).pitch(p->C_stride_g, E);
+  launch(selective_scan_step_kernel<T, TS, VEC, R, HEADS>, dim3((unsigned)((threads + 127) / 128)), dim3(128), 0, st, *p, lpr, a.bytes() >= BYTES);
   return check_launch("selective_scan_step_kernel");
 }
 template <typename T, typename TS>
@@ -586,7 +737,7 @@ static int run_step(const lq_scan_problem* p, cudaStream_t st) {
   Alignment a;
   const bool wide = a.at(p->state).pitch(p->N, sizeof(TS)).bytes() == 16;
   if (p->H == 0) return wide ? launch_step<T, TS, FULL, 1, false>(p, st) : launch_step<T, TS, 1, 1, false>(p, st);
-  if (p->P % 4 == 0) return wide ? launch_step<T, TS, FULL, 4, true>(p, st) : launch_step<T, TS, 1, 4, true>(p, st);
+  if (p->P % 4 == 0 && wide && p->N <= 32 * FULL) return launch_heads<T, TS, FULL>(p, st);
   return wide ? launch_step<T, TS, FULL, 1, true>(p, st) : launch_step<T, TS, 1, 1, true>(p, st);
 }
 
