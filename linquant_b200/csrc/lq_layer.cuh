@@ -94,6 +94,11 @@ __device__ __forceinline__ float row_scale(float amax, float& inv) {
   inv = scale < 1e-38f ? 0.0f : __fdiv_rn(1.0f, scale);
   return scale;
 }
+// The code rule for a row whose scale is its own: |x inv| exceeds 127 by roundings at most, so nothing has to be clamped
+__device__ __forceinline__ int row_code(float x, float inv) {
+  const float y = __fmul_rn(x, inv);
+  return __float2int_rz(__fadd_rn(y, copysignf(0.5f, y)));
+}
 
 // ---- host side
 template <typename F>

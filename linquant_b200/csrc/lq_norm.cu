@@ -22,15 +22,25 @@ struct Team {
   float* sm;  // 32 floats; reductions take turns between two of them, so one barrier each is enough
   int turn = 0;
   template <typename Op>
-  __device__ __forceinline__ float reduce(float v, Op op) {
-    for (int m = min(size, 32) >> 1; m; m >>= 1) v = op(v, __shfl_xor_sync(0xffffffffu, v, m));
+  static __device__ __forceinline__ float over_warp(float v, Op op) {
+#pragma unroll
+    for (int m = 16; m; m >>= 1) v = op(v, __shfl_xor_sync(0xffffffffu, v, m));
+    return v;
+  }
+  template <typename Op>
+  __device__ __forceinline__ float reduce(float v, Op op) {  // of values that are not negative, so that 0 adds nothing
+    if (size < 32) {
+      for (int m = size >> 1; m; m >>= 1) v = op(v, __shfl_xor_sync(0xffffffffu, v, m));
+      return v;
+    }
+    v = over_warp(v, op);
     if (size > 32) {
       float* part = sm + 32 * turn;
       turn ^= 1;
-      if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
+      const int lane = threadIdx.x & 31;
+      if (lane == 0) part[threadIdx.x >> 5] = v;
       __syncthreads();
-      v = part[0];
-      for (int w = 1; w < size >> 5; ++w) v = op(v, part[w]);
+      v = over_warp(lane < size >> 5 ? part[lane] : 0.f, op);
     }
     return v;
   }
@@ -38,14 +48,8 @@ struct Team {
   __device__ __forceinline__ float max(float v) { return reduce(v, [](float a, float b) { return max_nan(a, b); }); }
 };
 
-// The code rule for a row whose scale is its own: |x inv| exceeds 127 by roundings at most, so nothing has to be clamped
-__device__ __forceinline__ int code(float x, float inv) {
-  const float y = __fmul_rn(x, inv);
-  return __float2int_rz(__fadd_rn(y, copysignf(0.5f, y)));
-}
-
-// A thread has NV packs of VEC channels. OFF: the rows do not start on a pack's boundary, but those of all tensors at the same
-// distance behind one; packs lie on the boundaries, the first and the last of a row hold channels that are not the row's.
+// A thread has NV packs of VEC channels. OFF: a row may start inside a pack, the rows of all tensors at the same distance
+// behind its boundary; the first and the last pack of a row then hold channels that are not the row's.
 template <int VEC, bool OFF>
 struct Place {
   int c, n;  // first channel, channels of the row
@@ -62,9 +66,12 @@ __device__ __forceinline__ void load_f32(const float* p, const Place<VEC, OFF>& 
       const float4 v = __ldg(reinterpret_cast<const float4*>(p + at.c + i));
       x[i] = v.x; x[i + 1] = v.y; x[i + 2] = v.z; x[i + 3] = v.w;
     }
+  } else if (at.all()) {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) x[i] = __ldg(p + at.c + i);
   } else {
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) x[i] = at.all() || at.has(i) ? __ldg(p + at.c + i) : 0.f;
+    for (int i = 0; i < VEC; ++i) x[i] = at.has(i) ? __ldg(p + at.c + i) : 0.f;
   }
 }
 template <typename TO, int VEC, bool OFF>
@@ -86,16 +93,17 @@ __device__ __forceinline__ void store_row(TO* row, const Place<VEC, OFF>& at, co
       if (at.has(i)) row[at.c + i] = from_f32<TO>(y[i]);
   }
 }
-template <int VEC, bool OFF>
+template <typename T, int VEC, bool OFF>
 __device__ __forceinline__ void store_as(void* base, size_t at_row, int dtype, const Place<VEC, OFF>& at, const float (&y)[VEC]) {
-  if (dtype == LQ_F32) store_row(reinterpret_cast<float*>(base) + at_row, at, y);
+  if (dtype == (std::is_same_v<T, float> ? LQ_F32 : std::is_same_v<T, __half> ? LQ_F16 : LQ_BF16)) store_row(reinterpret_cast<T*>(base) + at_row, at, y);
+  else if (dtype == LQ_F32) store_row(reinterpret_cast<float*>(base) + at_row, at, y);
   else if (dtype == LQ_F16) store_row(reinterpret_cast<__half*>(base) + at_row, at, y);
   else store_row(reinterpret_cast<__nv_bfloat16*>(base) + at_row, at, y);
 }
 
 // CTAs walk over the rows; a row's loads are requested while the one before is summed and stored.
 template <typename T, int VEC, int NV, Kind KIND, bool OFF>
-__global__ void __launch_bounds__(NV == 1 || NV * VEC == 4 ? 1024 : 512) norm_kernel(const lq_norm_problem p, int team_size, long long units) {
+__global__ void __launch_bounds__(NV == 1 && !OFF || NV * VEC == 4 ? 1024 : 512) norm_kernel(const lq_norm_problem p, int team_size, long long units) {
   pdl_enter();
   constexpr bool SECOND = KIND != PLAIN;
   using R = std::conditional_t<KIND == ADD32, float, T>;  // of the second input: the residual or the gate
@@ -243,12 +251,12 @@ __global__ void __launch_bounds__(NV == 1 || NV * VEC == 4 ? 1024 : 512) norm_ke
         if constexpr (VEC == 1 || OFF) {
 #pragma unroll
           for (int i = 0; i < VEC; ++i)
-            if (at[j].has(i)) out[i] = (int8_t)code(v[j][i], inv);
+            if (at[j].has(i)) out[i] = (int8_t)row_code(v[j][i], inv);
         } else {
           uint32_t w[VEC / 4];
 #pragma unroll
           for (int i = 0; i < VEC; i += 4)
-            w[i / 4] = pack_sat_s8x2(code(v[j][i + 1], inv), code(v[j][i], inv), pack_sat_s8x2(code(v[j][i + 3], inv), code(v[j][i + 2], inv), 0u));
+            w[i / 4] = pack_sat_s8x2(row_code(v[j][i + 1], inv), row_code(v[j][i], inv), pack_sat_s8x2(row_code(v[j][i + 3], inv), row_code(v[j][i + 2], inv), 0u));
           if constexpr (VEC == 8) *reinterpret_cast<uint2*>(out) = make_uint2(w[0], w[1]);
           else *reinterpret_cast<uint32_t*>(out) = w[0];
         }
@@ -256,7 +264,7 @@ __global__ void __launch_bounds__(NV == 1 || NV * VEC == 4 ? 1024 : 512) norm_ke
     } else if (p.y) {
 #pragma unroll
       for (int j = 0; j < NV; ++j)
-        if (on[j]) store_as(p.y, (size_t)row * p.D + c0, p.out_dtype, at[j], v[j]);
+        if (on[j]) store_as<T>(p.y, (size_t)row * p.D + c0, p.out_dtype, at[j], v[j]);
     }
   }
 }
@@ -288,10 +296,14 @@ static int launch_vec(const lq_norm_problem* p, cudaStream_t st) {
   if constexpr (VEC == 1) {
     if (packs <= 1024) return launch_as<T, KIND, 1, 4, OFF>(p, packs, st);
     if (packs <= 16384) return launch_as<T, KIND, 1, 32, OFF>(p, packs, st);
+  } else if constexpr (OFF) {
+    if (packs <= 512) return launch_as<T, KIND, VEC, 1, OFF>(p, packs, st);
+    if (packs <= 1024) return launch_as<T, KIND, VEC, 2, OFF>(p, packs, st);
+    return launch_as<T, KIND, VEC, 32 / VEC, OFF>(p, packs, st);
   } else {
     if (packs <= 32 || (few && packs <= 1024)) return launch_as<T, KIND, VEC, 1, OFF>(p, packs, st);
     if (packs <= 1024) return launch_as<T, KIND, VEC, 2, OFF>(p, packs, st);
-    if (packs <= 512 * 32 / VEC + OFF) return launch_as<T, KIND, VEC, 32 / VEC, OFF>(p, packs, st);
+    if (packs <= 512 * 32 / VEC) return launch_as<T, KIND, VEC, 32 / VEC, OFF>(p, packs, st);
   }
   return fail(LQ_ERR_UNSUPPORTED, "norm over %d channels (at most 16384)", p->group);
 }
@@ -308,13 +320,13 @@ static int run_kind(const lq_norm_problem* p, cudaStream_t st) {
   const int so = dtype_bytes(p->out_dtype), out = so * FULL;
   y.at(p->y).pitch(p->D, so).pitch(p->group, so);
   if (in.bytes() == 16 && params.bytes() == 16 && (p->y == nullptr || y.bytes() >= (out < 16 ? out : 16))) return launch_vec<T, KIND, FULL, false>(p, st);
-  // rows off the boundary, all tensors' alike: one type, one pitch and one distance
+  // rows of a length that is no multiple of a pack: the tensors' rows all at the same distance behind a boundary
   if constexpr (KIND != ADD32) {
     auto alike = [&](const void* t, long long pitch, int size) {
-      return t == nullptr || (size == S && pitch == p->x_stride && ((reinterpret_cast<uintptr_t>(t) ^ reinterpret_cast<uintptr_t>(p->x)) & 15) == 0);
+      return t == nullptr || (size == S && ((pitch - p->x_stride) * S & 15) == 0 && ((reinterpret_cast<uintptr_t>(t) ^ reinterpret_cast<uintptr_t>(p->x)) & 15) == 0);
     };
-    if (p->group == p->D && alike(p->gate, p->gate_stride, S) && alike(p->residual, p->residual_stride, S) && alike(p->residual_out, p->D, S) &&
-        alike(p->y, p->D, so))
+    if (p->group == p->D && p->D <= 16384 - FULL && alike(p->gate, p->gate_stride, S) && alike(p->residual, p->residual_stride, S) &&
+        alike(p->residual_out, p->D, S) && alike(p->y, p->D, so))
       return launch_vec<T, KIND, FULL, true>(p, st);
   }
   return launch_vec<T, KIND, 1, false>(p, st);
