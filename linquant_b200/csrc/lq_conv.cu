@@ -82,23 +82,22 @@ __global__ void __launch_bounds__(128) short_conv_kernel(const lq_conv_problem p
     float line[W][VEC];
 #pragma unroll
     for (int k = 1; k < W; ++k) input(t0 - W + k).get(line[k]);
-    auto next = [&](const Pack<T, VEC>& raw, int t) {
+    T* to = y + (size_t)t0 * p.D;
+    auto next = [&](const Pack<T, VEC>& raw) {
 #pragma unroll
       for (int k = 0; k + 1 < W; ++k)
 #pragma unroll
         for (int i = 0; i < VEC; ++i) line[k][i] = line[k + 1][i];
       raw.get(line[W - 1]);
-      store_pack(y + (size_t)t * p.D, taps.out(line, ACT));
+      store_pack(to, taps.out(line, ACT));
+      to += p.D;
     };
+    const T* from = x + t0 * p.x_stride_t;
     if constexpr (VEC * sizeof(T) == 16) {  // tokens arrive in a ring of the thread's own: AHEAD of them on their way without registers
       auto issue = [&](int g) {
-        if (t0 + g * U < live) {
 #pragma unroll
-          for (int u = 0; u < U; ++u) {
-            const int t = t0 + g * U + u;
-            if (t < live) cp_async16(&ring[(g * U + u) % RING][threadIdx.x], x + t * p.x_stride_t);
-          }
-        }
+        for (int u = 0; u < U; ++u, from += p.x_stride_t)
+          if (t0 + g * U + u < live) cp_async16(&ring[(g * U + u) % RING][threadIdx.x], from);
         cp_async_commit();
       };
 #pragma unroll
@@ -108,9 +107,9 @@ __global__ void __launch_bounds__(128) short_conv_kernel(const lq_conv_problem p
         cp_async_wait<RING / U - 1>();
         if (t + U <= live) {
 #pragma unroll
-          for (int u = 0; u < U; ++u) next(ring[(g * U + u) % RING][threadIdx.x], t + u);
+          for (int u = 0; u < U; ++u) next(ring[(g * U + u) % RING][threadIdx.x]);
         } else {
-          for (int u = 0; t + u < live; ++u) next(ring[(g * U + u) % RING][threadIdx.x], t + u);
+          for (int u = 0; t + u < live; ++u) next(ring[(g * U + u) % RING][threadIdx.x]);
         }
       }
       cp_async_wait<0>();
@@ -119,12 +118,12 @@ __global__ void __launch_bounds__(128) short_conv_kernel(const lq_conv_problem p
       for (; t + U <= live; t += U) {
         Pack<T, VEC> raw[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u) raw[u] = load_pack<T, VEC>(x + (t + u) * p.x_stride_t);
+        for (int u = 0; u < U; ++u, from += p.x_stride_t) raw[u] = load_pack<T, VEC>(from);
 #pragma unroll
-        for (int u = 0; u < U; ++u) next(raw[u], t + u);
+        for (int u = 0; u < U; ++u) next(raw[u]);
       }
 #pragma unroll 1
-      for (; t < live; ++t) next(load_pack<T, VEC>(x + t * p.x_stride_t), t);
+      for (; t < live; ++t, from += p.x_stride_t) next(load_pack<T, VEC>(from));
     }
   }
   Pack<T, VEC> none;

@@ -3,8 +3,8 @@
 // Persistent kernel, one CTA per SM, tiles of 128 tokens x BN output channels. Both operands are codes with the reduction
 // index contiguous: TMA brings blocks of 128 bytes of K (128-byte swizzle, zero-filled behind the last row and the last byte
 // of K) into a ring of stages, one thread issues tcgen05.mma.kind::i8 (M = 128, N = BN, four steps of 32 per stage) into one
-// of two accumulators in tensor memory, and four warps turn the other one into outputs meanwhile: INT32 to fp32, both scales
-// and the bias, through a swizzled 128-byte row per lane in shared memory, stored as whole rows of 128 bytes.
+// of two accumulators in tensor memory, and eight warps turn the other one into outputs meanwhile: INT32 to fp32, both scales
+// and the bias, through a swizzled 64-byte row per lane in shared memory, stored as pieces of 64 bytes a row.
 // Every wait is bounded; on expiry the CTA raises the status word, lets its copies and products land, frees its tensor
 // memory and returns.
 #include "lq_layer.cuh"
@@ -14,12 +14,13 @@ namespace lq {
 
 namespace lineartc {
 
-constexpr int BM = 128, BK = 128, THREADS = 192, STAGE_BYTES = 192 * 1024;
+constexpr int BM = 128, BK = 128, OUT_WARPS = 8, THREADS = 32 * (OUT_WARPS + 2), STAGE_BYTES = 192 * 1024;
 
 template <int BN>
 struct Shape {
   static constexpr int STAGE = (BM + BN) * BK, STAGES = STAGE_BYTES / STAGE;
-  static constexpr int OUT = 4 * 32 * 128, COLS = 4 * 2 * BN * 4;  // per epilogue warp: 32 rows of 128 bytes; w_scale and bias of the tile
+  static constexpr int HALF = BN / 2;                                     // columns of a storing warp: two share 32 rows
+  static constexpr int OUT = OUT_WARPS * 32 * 64, COLS = OUT_WARPS * 2 * HALF * 4;  // per storing warp: 32 rows of 64 bytes; w_scale and bias of its columns
   static constexpr int BARS = (2 * STAGES + 4) * 8;
   static constexpr size_t SMEM = 1024 + (size_t)STAGES * STAGE + OUT + COLS + BARS + 16;
 };
@@ -43,6 +44,14 @@ __device__ __forceinline__ uint4 lds_u4(uint32_t addr) {
 }
 __device__ __forceinline__ void sts_u4(uint32_t addr, const uint4& v) {
   asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};\n" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+
+__device__ __forceinline__ void tmem_ld_32x32b_x16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+        "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
 }
 
 // Tiles of up to 16 row blocks share the weights of a column block before the next column block is taken
@@ -71,11 +80,11 @@ __global__ void __launch_bounds__(THREADS, 1) int8_linear_tc_kernel(const __grid
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(s_acc + 8 * i, 1);
-      mbar_init(s_free + 8 * i, 4);
+      mbar_init(s_free + 8 * i, OUT_WARPS);
     }
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
   }
-  if (warp == 5) {
+  if (warp == OUT_WARPS + 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(s_tbase), "r"((uint32_t)(2 * BN)) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
   }
@@ -85,7 +94,7 @@ __global__ void __launch_bounds__(THREADS, 1) int8_linear_tc_kernel(const __grid
   const uint32_t tbase = lds_u32(s_tbase);
   bool ok = true;
 
-  if (warp == 4) {  // loads
+  if (warp == OUT_WARPS) {  // loads
     if (lane == 0) {
       long long fill = 0;
       for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
@@ -102,7 +111,7 @@ __global__ void __launch_bounds__(THREADS, 1) int8_linear_tc_kernel(const __grid
       for (long long f = fill > S::STAGES ? fill - S::STAGES : 0; f < fill; ++f)  // nothing may land after the CTA has gone
         ok &= mbar_wait_bounded(s_full + 8 * (int)(f % S::STAGES), (uint32_t)((f / S::STAGES) & 1));
     }
-  } else if (warp == 5) {  // products
+  } else if (warp == OUT_WARPS + 1) {  // products
     if (lane == 0) {
       const uint32_t idesc = idesc_i8(BM, BN);
       long long fill = 0;
@@ -127,82 +136,81 @@ __global__ void __launch_bounds__(THREADS, 1) int8_linear_tc_kernel(const __grid
         for (long long f = fill > S::STAGES ? fill - S::STAGES : 0; f < fill; ++f)
           mbar_wait_bounded(s_empty + 8 * (int)(f % S::STAGES), (uint32_t)((f / S::STAGES) & 1));
     }
-  } else {  // outputs: warp w holds the accumulator rows 32 w ..
-    constexpr int CHUNK = 128 / sizeof(TO);  // columns of a 128-byte piece of a row
-    const uint32_t out = s_out + warp * 32 * 128, cols = s_cols + warp * 2 * BN * 4;
+  } else {  // outputs: warp w has the accumulator rows 32 (w & 3) .. and half of the columns
+    constexpr int CHUNK = 64 / sizeof(TO), PER = 16 / sizeof(TO);  // columns of a 64-byte piece of a row, of 16 bytes
+    const int quad = warp & 3, half = (warp >> 2) * S::HALF;
+    const uint32_t out = s_out + warp * 32 * 64, cols = s_cols + warp * 2 * S::HALF * 4;
     const bool wide = ((size_t)p.N * sizeof(TO)) % 16 == 0 && (reinterpret_cast<uintptr_t>(p.y) & 15u) == 0;
     int i = 0;
     for (int t = blockIdx.x; t < tiles; t += gridDim.x, ++i) {
       int m, n;
       tile_at(t, mt, nt, m, n);
-      const int acc = i & 1, row0 = m * BM + 32 * warp, n0 = n * BN;
+      const int acc = i & 1, row0 = m * BM + 32 * quad, n0 = n * BN + half;
       const float xs = row0 + lane < p.M ? __ldg(p.x_scale + row0 + lane) : 0.f;
       __syncwarp();
 #pragma unroll
-      for (int c = lane; c < BN; c += 32) {
+      for (int c = lane; c < S::HALF; c += 32) {
         const bool in = n0 + c < p.N;
         sts_u32(cols + 4 * c, __float_as_uint(in ? __ldg(p.w_scale + n0 + c) : 0.f));
-        sts_u32(cols + 4 * (BN + c), __float_as_uint(in && p.bias ? __ldg(p.bias + n0 + c) : 0.f));
+        sts_u32(cols + 4 * (S::HALF + c), __float_as_uint(in && p.bias ? __ldg(p.bias + n0 + c) : 0.f));
       }
       __syncwarp();
       if (!(ok = __all_sync(0xffffffffu, mbar_wait_bounded(s_acc + 8 * acc, (uint32_t)((i / 2) & 1))))) break;
       asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
 #pragma unroll 1
-      for (int c0 = 0; c0 < BN; c0 += CHUNK) {
+      for (int c0 = 0; c0 < S::HALF; c0 += CHUNK) {
         if (n0 + c0 >= p.N) break;
+        uint32_t r[CHUNK];
+        const uint32_t from = tbase + ((uint32_t)(32 * quad) << 16) + acc * BN + half + c0;
+        if constexpr (CHUNK == 32) tmem_ld_32x32b_x32(from, r);
+        else tmem_ld_32x32b_x16(from, r);
+        asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
+        float v[CHUNK];
+#pragma unroll
+        for (int j = 0; j < CHUNK; j += 4) {
+          const float4 ws = lds_f4(cols + 4 * (c0 + j)), b = lds_f4(cols + 4 * (S::HALF + c0 + j));
+          v[j] = fmaf((float)(int)r[j] * xs, ws.x, b.x);
+          v[j + 1] = fmaf((float)(int)r[j + 1] * xs, ws.y, b.y);
+          v[j + 2] = fmaf((float)(int)r[j + 2] * xs, ws.z, b.z);
+          v[j + 3] = fmaf((float)(int)r[j + 3] * xs, ws.w, b.w);
+        }
         __syncwarp();  // the chunk before has been read
+        // rows of 64 bytes, pairs of them on the same banks: a piece at its place exclusive-or half the row's number
+        auto place = [](int row, int piece) { return row * 64 + ((piece ^ ((row >> 1) & 3)) << 4); };
 #pragma unroll
-        for (int h = 0; h < CHUNK; h += 32) {
-          uint32_t r[32];
-          tmem_ld_32x32b_x32(tbase + ((uint32_t)(32 * warp) << 16) + acc * BN + c0 + h, r);
-          asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
-          float v[32];
-#pragma unroll
-          for (int j = 0; j < 32; j += 4) {
-            const float4 ws = lds_f4(cols + 4 * (c0 + h + j)), b = lds_f4(cols + 4 * (BN + c0 + h + j));
-            v[j] = fmaf((float)(int)r[j] * xs, ws.x, b.x);
-            v[j + 1] = fmaf((float)(int)r[j + 1] * xs, ws.y, b.y);
-            v[j + 2] = fmaf((float)(int)r[j + 2] * xs, ws.z, b.z);
-            v[j + 3] = fmaf((float)(int)r[j + 3] * xs, ws.w, b.w);
+        for (int j = 0; j < CHUNK; j += PER) {
+          uint4 w;
+          if constexpr (sizeof(TO) == 4) {
+            w = make_uint4(__float_as_uint(v[j]), __float_as_uint(v[j + 1]), __float_as_uint(v[j + 2]), __float_as_uint(v[j + 3]));
+          } else {
+            w = make_uint4(Act<TO>::pack2(v[j], v[j + 1]), Act<TO>::pack2(v[j + 2], v[j + 3]), Act<TO>::pack2(v[j + 4], v[j + 5]),
+                           Act<TO>::pack2(v[j + 6], v[j + 7]));
           }
-          constexpr int PER = 16 / sizeof(TO);
-#pragma unroll
-          for (int j = 0; j < 32; j += PER) {
-            uint4 w;
-            if constexpr (sizeof(TO) == 4) {
-              w = make_uint4(__float_as_uint(v[j]), __float_as_uint(v[j + 1]), __float_as_uint(v[j + 2]), __float_as_uint(v[j + 3]));
-            } else {
-              w = make_uint4(Act<TO>::pack2(v[j], v[j + 1]), Act<TO>::pack2(v[j + 2], v[j + 3]), Act<TO>::pack2(v[j + 4], v[j + 5]),
-                             Act<TO>::pack2(v[j + 6], v[j + 7]));
-            }
-            sts_u4(out + lane * 128 + ((((h + j) / PER) ^ (lane & 7)) << 4), w);
-          }
+          sts_u4(out + place(lane, j / PER), w);
         }
         __syncwarp();
         TO* y = reinterpret_cast<TO*>(p.y);
         if (wide) {
-          constexpr int PER = 16 / sizeof(TO);
-          const int piece = lane & 7, c = n0 + c0 + piece * PER;
+          const int piece = lane & 3, c = n0 + c0 + piece * PER;
 #pragma unroll
-          for (int q = 0; q < 8; ++q) {
-            const int row = 4 * q + (lane >> 3);
-            const uint4 w = lds_u4(out + row * 128 + ((piece ^ (row & 7)) << 4));
+          for (int q = 0; q < 4; ++q) {
+            const int row = 8 * q + (lane >> 2);
+            const uint4 w = lds_u4(out + place(row, piece));
             if (row0 + row < p.M && c < p.N) *reinterpret_cast<uint4*>(y + (size_t)(row0 + row) * p.N + c) = w;
           }
-        } else {  // rows off 16-byte boundaries: 32 consecutive values a store
-          for (int row = 0; row < 32 && row0 + row < p.M; ++row) {
-#pragma unroll
-            for (int h = 0; h < CHUNK; h += 32) {
-              const int e = h + lane, byte = e * (int)sizeof(TO);
-              const uint32_t a = out + row * 128 + (((byte >> 4) ^ (row & 7)) << 4) + (byte & 15);
-              if (n0 + c0 + e < p.N) {
-                if constexpr (sizeof(TO) == 4) {
-                  y[(size_t)(row0 + row) * p.N + n0 + c0 + e] = __uint_as_float(lds_u32(a));
-                } else {
-                  uint16_t v;
-                  asm volatile("ld.shared.u16 %0, [%1];\n" : "=h"(v) : "r"(a));
-                  reinterpret_cast<uint16_t*>(y)[(size_t)(row0 + row) * p.N + n0 + c0 + e] = v;
-                }
+        } else {  // rows off 16-byte boundaries: consecutive values a store
+          constexpr int ROWS = 32 / CHUNK;
+          const int e = lane % CHUNK, byte = e * (int)sizeof(TO);
+          for (int q = 0; q < 32; q += ROWS) {
+            const int row = q + lane / CHUNK;
+            const uint32_t a = out + place(row, byte >> 4) + (byte & 15);
+            if (row0 + row < p.M && n0 + c0 + e < p.N) {
+              if constexpr (sizeof(TO) == 4) {
+                y[(size_t)(row0 + row) * p.N + n0 + c0 + e] = __uint_as_float(lds_u32(a));
+              } else {
+                uint16_t w;
+                asm volatile("ld.shared.u16 %0, [%1];\n" : "=h"(w) : "r"(a));
+                reinterpret_cast<uint16_t*>(y)[(size_t)(row0 + row) * p.N + n0 + c0 + e] = w;
               }
             }
           }
@@ -217,7 +225,7 @@ __global__ void __launch_bounds__(THREADS, 1) int8_linear_tc_kernel(const __grid
   __syncwarp();
   asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
   __syncthreads();
-  if (warp == 5) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tbase), "r"((uint32_t)(2 * BN)) : "memory");
+  if (warp == OUT_WARPS + 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tbase), "r"((uint32_t)(2 * BN)) : "memory");
 }
 
 static int encode(CUtensorMap* m, const void* base, long long row_bytes, long long pitch, long long rows, int box_rows) {

@@ -5,17 +5,17 @@
 // Two resources bound it: the exponentials (one per token, channel and state, 16 a clock and SM) and what shared memory
 // delivers to registers (128 bytes a clock and SM, broadcasts included). A thread of the recurrence holds SPT states of a
 // channel, LP threads share the channel; tokens go one after the other, four at a time: dt and dt u (16 bytes each), B and C
-// of its states (in the activation's type) and its part of y lie with the token index contiguous, so that one access covers
-// the four, and the products around the recurrence take two tokens an instruction. Per token a warp takes 3 + SPT size / 2
-// clocks of shared memory and 2 SPT of exponentials.
+// of its states (in fp32 up to four states: unpacking costs more issue slots than the bytes cost clocks) and its part of y lie
+// with the token index contiguous, so that one access covers the four. Per token a warp takes 3 + 2 SPT clocks of shared memory
+// and 2 SPT of exponentials.
 // A tile of TT tokens passes three jobs, each with warps of its own, so that their latencies overlap: dt and dt u are
 // prepared and B and C turned, the recurrence runs, and y is stored (the sum of the threads' parts, skip and gate). Buffers of
 // two, one barrier a tile. Inputs come as TMA tiles into a ring of ST tiles, requested ST - 2 tiles ahead of their use. Where
 // rows do not lie on 16-byte boundaries the storing warps copy them in words of four bytes, the words that hold a row's ends
 // included.
-// At 1 x 16384 x 2048 with 16 states (bf16, gate): 375 us; 115 us of exponentials, 41 us of bytes. All jobs in every warp took
-// 1 139 us, two jobs and plain loads 937 us, three jobs with the state index contiguous 462 us. The recurrence alone takes 323
-// us: its one warp a quadrant issues in 57 % of the clocks.
+// At 1 x 16384 x 2048 with 16 states (bf16, gate): 372 us; 115 us of exponentials, 41 us of bytes. All jobs in every warp took
+// 1 139 us, two jobs and plain loads 937 us, three jobs with the state index contiguous 462 us. The recurrence alone takes 259
+// us, the other two jobs alone 211 us; together shared memory is busy in 75 % of the clocks.
 #include "lq_layer.cuh"
 #include "lq_tc.cuh"
 
@@ -26,6 +26,7 @@ namespace scan {
 // RT threads of the recurrence
 template <typename T, int RT_, int SPT, int LP, int ST_, int TT_>
 struct Shape {
+  using BT = std::conditional_t<SPT <= 4 || sizeof(T) == 4, float, T>;  // B and C of the recurrence
   static constexpr int RT = RT_, ST = ST_, TT = TT_, JOB = 256, THREADS = RT + 2 * JOB;  // JOB: threads of the preparing and of the storing job
   static constexpr int NP = SPT * LP, CH = RT / LP, PT = TT + 4;        // PT: pitch of a row of tokens, no two rows of an access on one bank
   static constexpr int GSTEP = JOB / CH, GROUPS = TT / 4;               // a job's thread has one channel, every GSTEP-th group of four tokens
@@ -37,7 +38,7 @@ struct Shape {
   struct alignas(128) Smem {
     uint8_t raw[ST][STAGE];  // rows of u, dt, z, B, C
     float dt[2][CH * PT], du[2][CH * PT], y[2][CH * YC];
-    T B[2][NP * PT], C[2][NP * PT];
+    BT B[2][NP * PT], C[2][NP * PT];
     uint64_t full[ST];
     float behind[16];        // the recurrence requests up to 16 tokens behind a row
   };
@@ -156,11 +157,11 @@ struct Prepare : Job<T, S, WIDE> {
       if (WORK % PER && r >= S::TT) break;
       // what lies behind the last token or state takes no part, not even as 0 x NaN
       const bool in0 = FULL || (n < p.N && t0 + r < len), in1 = FULL || (n < p.N && t0 + r + 1 < len);
-      Pack<T, 2> vB, vC;
-      vB.v[0] = in0 ? J::template at<3>(st, B, tile, r, n) : none;
-      vB.v[1] = in1 ? J::template at<3>(st, B, tile, r + 1, n) : none;
-      vC.v[0] = in0 ? J::template at<4>(st, C, tile, r, n) : none;
-      vC.v[1] = in1 ? J::template at<4>(st, C, tile, r + 1, n) : none;
+      Pack<typename S::BT, 2> vB, vC;
+      vB.v[0] = from_f32<typename S::BT>(to_f32(in0 ? J::template at<3>(st, B, tile, r, n) : none));
+      vB.v[1] = from_f32<typename S::BT>(to_f32(in1 ? J::template at<3>(st, B, tile, r + 1, n) : none));
+      vC.v[0] = from_f32<typename S::BT>(to_f32(in0 ? J::template at<4>(st, C, tile, r, n) : none));
+      vC.v[1] = from_f32<typename S::BT>(to_f32(in1 ? J::template at<4>(st, C, tile, r + 1, n) : none));
       store_pack(&sm.B[buf][n * S::PT + r], vB);
       store_pack(&sm.C[buf][n * S::PT + r], vC);
     }
@@ -272,7 +273,7 @@ template <typename T, typename S, int SPT, int LP>
 struct Recurrence {
   struct Operands {
     float4 du;
-    Pack<T, 4> B[SPT], C[SPT];
+    Pack<typename S::BT, 4> B[SPT], C[SPT];
   };
   typename S::Smem& sm;
   const int ch, ln;  // states ln, ln + LP, ..
@@ -280,7 +281,7 @@ struct Recurrence {
 
   // of the tile: rows of this thread's channel and first state
   const float *pdt, *pdu;
-  const T *pB, *pC;
+  const typename S::BT *pB, *pC;
   float* py;
 
   __device__ __forceinline__ float4 load_dt(int t) const { return *reinterpret_cast<const float4*>(pdt + t); }
@@ -288,8 +289,8 @@ struct Recurrence {
     o.du = *reinterpret_cast<const float4*>(pdu + t);
 #pragma unroll
     for (int j = 0; j < SPT; ++j) {
-      o.B[j] = load_pack<T, 4>(pB + j * LP * S::PT + t);
-      o.C[j] = load_pack<T, 4>(pC + j * LP * S::PT + t);
+      o.B[j] = load_pack<typename S::BT, 4>(pB + j * LP * S::PT + t);
+      o.C[j] = load_pack<typename S::BT, 4>(pC + j * LP * S::PT + t);
     }
   }
   __device__ __forceinline__ void decays(float (&a)[SPT][4], const float4& dt) const {
