@@ -11,8 +11,8 @@
 // A tile of TT tokens passes three jobs, each with warps of its own, so that their latencies overlap: dt and dt u are
 // prepared and B and C turned, the recurrence runs, and y is stored (the sum of the threads' parts, skip and gate). Buffers of
 // two, one barrier a tile. Inputs come as TMA tiles into a ring of ST tiles, requested ST - 2 tiles ahead of their use. Where
-// rows do not lie on 16-byte boundaries the storing warps copy them in words of four bytes, the words that hold a row's ends
-// included.
+// rows do not lie on 16-byte boundaries the storing warps copy them in pieces of eight or four bytes, the pieces that hold a
+// row's ends included.
 // At 1 x 16384 x 2048 with 16 states (bf16, gate): 372 us; 115 us of exponentials, 41 us of bytes. All jobs in every warp took
 // 1 139 us, two jobs and plain loads 937 us, three jobs with the state index contiguous 462 us. The recurrence alone takes 259
 // us, the other two jobs alone 211 us; together shared memory is busy in 75 % of the clocks.
@@ -26,6 +26,9 @@ namespace scan {
 // RT threads of the recurrence
 template <typename T, int RT_, int SPT, int LP, int ST_, int TT_>
 struct Shape {
+  // The exponent's rounding costs a decay up to |dt A| 2^-24, which a state that only decays collects: 1e-6 of it over 100 tokens
+  // of dt A = -0.1. With fp32 inputs expf carries what the product with log2(e) loses; it takes a fifth more time.
+  static constexpr bool ACCURATE = sizeof(T) == 4;
   using BT = std::conditional_t<SPT <= 4 || sizeof(T) == 4, float, T>;  // B and C of the recurrence
   static constexpr int RT = RT_, ST = ST_, TT = TT_, JOB = 256, THREADS = RT + 2 * JOB;  // JOB: threads of the preparing and of the storing job
   static constexpr int NP = SPT * LP, CH = RT / LP, PT = TT + 4;        // PT: pitch of a row of tokens, no two rows of an access on one bank
@@ -37,7 +40,7 @@ struct Shape {
   static_assert(JOB % CH == 0 && CH % 8 == 0, "");
   struct alignas(128) Smem {
     uint8_t raw[ST][STAGE];  // rows of u, dt, z, B, C
-    float dt[2][CH * PT], du[2][CH * PT], y[2][CH * YC];
+    float dt[2][CH * PT], du[2][CH * PT], y[2][CH * YC];  // dt (times log2(e) unless ACCURATE), dt u, parts of y
     BT B[2][NP * PT], C[2][NP * PT];
     uint64_t full[ST];
     float behind[16];        // the recurrence requests up to 16 tokens behind a row
@@ -63,17 +66,30 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map
 struct Rows {
   const uint8_t* from;  // row 0 of the sequence
   long long pitch;      // bytes
-  // element 0 of a row that was copied by words lies this many bytes behind the copy's start
+  // element 0 of a row that was copied by pieces lies this many bytes behind the copy's start
   __device__ __forceinline__ int shift(int t) const { return ((uint32_t)reinterpret_cast<uintptr_t>(from) + (uint32_t)t * (uint32_t)pitch) & 3; }
-  template <int JOB>
-  __device__ __forceinline__ void copy(uint32_t to, int row_pitch, int bytes, int rows, int t0, int len, int tid) const {
-    if (from == nullptr) return;
-    for (int row = tid >> 3; row < rows && t0 + row < len; row += JOB / 8) {
-      const uint8_t* at = from + (t0 + row) * pitch;
-      const int sh = shift(t0 + row), words = (bytes + sh + 3) >> 2;
-      for (int w = tid & 7; w < words; w += 8)
-        asm volatile("cp.async.ca.shared.global [%0], [%1], 4;\n" ::"r"(to + row * row_pitch + 4 * w), "l"(at - sh + 4 * w) : "memory");
+  // rows of at most MOST bytes at ROW bytes in shared memory, TT of them; eight threads a row. UNIT: bytes of a copy
+  template <int JOB, int TT, int ROW, int MOST, int UNIT>
+  __device__ __forceinline__ void copy_by(uint32_t to, int bytes, int t0, int len, int tid) const {
+    const uint8_t* at = from + (t0 + (tid >> 3)) * pitch;
+    to += (tid >> 3) * ROW + (tid & 7) * UNIT;
+#pragma unroll
+    for (int i = 0; i < (TT + JOB / 8 - 1) / (JOB / 8); ++i, at += JOB / 8 * pitch, to += JOB / 8 * ROW) {
+      const int row = (tid >> 3) + i * (JOB / 8);
+      if (row >= TT || t0 + row >= len) break;
+      const int sh = UNIT == 4 ? (int)((uint32_t)reinterpret_cast<uintptr_t>(at) & 3) : 0, units = (bytes + sh + UNIT - 1) / UNIT;
+      const uint8_t* piece = at - sh + (tid & 7) * UNIT;
+#pragma unroll
+      for (int j = 0; j < (MOST + 3 + UNIT - 1) / UNIT; j += 8)
+        if ((tid & 7) + j < units)
+          asm volatile("cp.async.ca.shared.global [%0], [%1], %2;\n" ::"r"(to + j * UNIT), "l"(piece + j * UNIT), "n"(UNIT) : "memory");
     }
+  }
+  template <int JOB, int TT, int ROW, int MOST>
+  __device__ __forceinline__ void copy(uint32_t to, int bytes, int t0, int len, int tid, bool by8) const {
+    if (from == nullptr) return;
+    if (by8) copy_by<JOB, TT, ROW, MOST, 8>(to, bytes, t0, len, tid);
+    else copy_by<JOB, TT, ROW, MOST, 4>(to, bytes, t0, len, tid);
   }
 };
 
@@ -139,6 +155,8 @@ struct Prepare : Job<T, S, WIDE> {
       for (int k = 0; k < 4; ++k) {
         v[k] = clamp_nan(SOFTPLUS ? softplus(v[k]) : v[k], p.dt_min, p.dt_max);
         w[k] *= v[k];
+        // here and not on A: the rounding of a factor that all tokens share would add up over them
+        if constexpr (!S::ACCURATE) v[k] *= kLog2e;
         if (!FULL && t0 + 4 * g + k >= len) v[k] = w[k] = 0.f;  // a token behind the last is a step of nothing
       }
       *reinterpret_cast<float4*>(&sm.dt[buf][ch * S::PT + 4 * g]) = make_float4(v[0], v[1], v[2], v[3]);
@@ -186,11 +204,12 @@ template <typename T, typename S, bool WIDE>
 struct Store : Job<T, S, WIDE> {
   using J = Job<T, S, WIDE>;
   using J::p, J::maps, J::sm, J::tid, J::len, J::ch, J::g0, J::on, J::u, J::dt, J::z, J::B, J::C;
+  const bool by8;  // rows on 8-byte boundaries
   T* y;
   float skip;
 
   template <typename... A>
-  __device__ __forceinline__ Store(A&&... a) : J(a...), y(reinterpret_cast<T*>(p.y) + (size_t)J::b * p.T * p.D + J::channel()), skip(on && p.skip ? p.skip[J::channel()] : 0.f) {}
+  __device__ __forceinline__ Store(bool by8, A&&... a) : J(a...), by8(by8), y(reinterpret_cast<T*>(p.y) + (size_t)J::b * p.T * p.D + J::channel()), skip(on && p.skip ? p.skip[J::channel()] : 0.f) {}
   __device__ __forceinline__ void request(int tile) const {
     const int t0 = tile * S::TT;
     const uint32_t to = smem_u32(J::stage(tile));
@@ -209,11 +228,11 @@ struct Store : Job<T, S, WIDE> {
       }
     } else {
       const int bytes = min(S::CH, p.D / p.G - J::ch0) * S::E;
-      u.template copy<S::JOB>(to + J::offset(0), S::CROW, bytes, S::TT, t0, len, tid);
-      dt.template copy<S::JOB>(to + J::offset(1), S::CROW, bytes, S::TT, t0, len, tid);
-      z.template copy<S::JOB>(to + J::offset(2), S::CROW, bytes, S::TT, t0, len, tid);
-      B.template copy<S::JOB>(to + J::offset(3), S::NROW, p.N * S::E, S::TT, t0, len, tid);
-      C.template copy<S::JOB>(to + J::offset(4), S::NROW, p.N * S::E, S::TT, t0, len, tid);
+      u.template copy<S::JOB, S::TT, S::CROW, S::CB>(to + J::offset(0), bytes, t0, len, tid, by8);
+      dt.template copy<S::JOB, S::TT, S::CROW, S::CB>(to + J::offset(1), bytes, t0, len, tid, by8);
+      z.template copy<S::JOB, S::TT, S::CROW, S::CB>(to + J::offset(2), bytes, t0, len, tid, by8);
+      B.template copy<S::JOB, S::TT, S::NROW, S::NB>(to + J::offset(3), p.N * S::E, t0, len, tid, by8);
+      C.template copy<S::JOB, S::TT, S::NROW, S::NB>(to + J::offset(4), p.N * S::E, t0, len, tid, by8);
       cp_async_commit();
     }
   }
@@ -277,7 +296,7 @@ struct Recurrence {
   };
   typename S::Smem& sm;
   const int ch, ln;  // states ln, ln + LP, ..
-  float a2[SPT], h[SPT];
+  float A[SPT], h[SPT];
 
   // of the tile: rows of this thread's channel and first state
   const float *pdt, *pdu;
@@ -294,13 +313,11 @@ struct Recurrence {
     }
   }
   __device__ __forceinline__ void decays(float (&a)[SPT][4], const float4& dt) const {
+    const float t[4] = {dt.x, dt.y, dt.z, dt.w};
 #pragma unroll
-    for (int j = 0; j < SPT; ++j) {
-      a[j][0] = ex2(dt.x * a2[j]);
-      a[j][1] = ex2(dt.y * a2[j]);
-      a[j][2] = ex2(dt.z * a2[j]);
-      a[j][3] = ex2(dt.w * a2[j]);
-    }
+    for (int j = 0; j < SPT; ++j)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) a[j][k] = S::ACCURATE ? expf(t[k] * A[j]) : ex2(t[k] * A[j]);
   }
   __device__ __forceinline__ void run(const Operands& o, const float (&a)[SPT][4], int t) {
     const float du[4] = {o.du.x, o.du.y, o.du.z, o.du.w};
@@ -362,7 +379,7 @@ struct Recurrence {
 };
 
 template <typename T, bool WIDE, int RT, int SPT, int LP, int ST, int TT>
-__global__ void __launch_bounds__(RT + 512, 1) selective_scan_kernel(const __grid_constant__ Maps maps, const lq_scan_problem p) {
+__global__ void __launch_bounds__(RT + 512, 1) selective_scan_kernel(const __grid_constant__ Maps maps, const lq_scan_problem p, bool by8) {
   using S = Shape<T, RT, SPT, LP, ST, TT>;
   extern __shared__ __align__(128) uint8_t smem_raw[];
   typename S::Smem& sm = *reinterpret_cast<typename S::Smem*>(smem_raw + ((128 - (smem_u32(smem_raw) & 127)) & 127));
@@ -384,7 +401,7 @@ __global__ void __launch_bounds__(RT + 512, 1) selective_scan_kernel(const __gri
     for (int j = 0; j < SPT; ++j) {
       const int n = r.ln + j * LP;
       const bool live = on && n < p.N;
-      r.a2[j] = live ? p.A[at + n] * kLog2e : 0.f;
+      r.A[j] = live ? p.A[at + n] : 0.f;
       r.h[j] = live && p.initial_state ? p.initial_state[(size_t)b * p.D * p.N + at + n] : 0.f;
     }
     for (int i = -1; i <= tiles; ++i) {
@@ -408,7 +425,7 @@ __global__ void __launch_bounds__(RT + 512, 1) selective_scan_kernel(const __gri
       if (p.status) atomicExch(p.status, 1);
     }
   } else {
-    const Store<T, S, WIDE> job(p, maps, sm, (int)threadIdx.x - RT - S::JOB, b, grp, ch0, len);
+    const Store<T, S, WIDE> job(by8, p, maps, sm, (int)threadIdx.x - RT - S::JOB, b, grp, ch0, len);
     for (int i = 0; i < ST - 2; ++i) job.request(i);
     job.arrived();
     for (int i = -1; i <= tiles; ++i) {
@@ -446,7 +463,6 @@ static int launch_scan(const lq_scan_problem* p, cudaStream_t st) {
   Maps maps = {};
   Alignment a;
   bool wide = S::CB % 16 == 0 && S::NB % 16 == 0 && p->T > 0;
-  a.at(p->y).pitch(Dg, E).pitch(p->N, E);
   auto pitch = [&](long long elements, long long extent) {  // bytes; of no meaning where there is one
     if (extent == 1) return (cuuint64_t)16;
     a.pitch(elements, E);
@@ -465,7 +481,8 @@ static int launch_scan(const lq_scan_problem* p, cudaStream_t st) {
     pitches[i][1] = pitch(in[i].st, p->T);
     pitches[i][2] = pitch(in[i].sb, p->B);
   }
-  wide = wide && a.bytes() == 16;
+  const bool by8 = Alignment(a).pitch(p->G > 1 ? Dg : 0, E).bytes() >= 8;
+  wide = wide && a.at(p->y).pitch(Dg, E).pitch(p->N, E).bytes() == 16;
   for (int i = 0; i < 5 && wide; ++i) {
     if (in[i].x == nullptr) continue;
     const cuuint64_t chans[3] = {(cuuint64_t)p->D, (cuuint64_t)p->T, (cuuint64_t)p->B};
@@ -473,7 +490,7 @@ static int launch_scan(const lq_scan_problem* p, cudaStream_t st) {
     const cuuint32_t cbox[3] = {S::CH, TT, 1}, nbox[4] = {S::NP, 1, TT, 1};
     if (int e = i < 3 ? encode(in[i].map, p->dtype, 3, in[i].x, chans, &pitches[i][1], cbox) : encode(in[i].map, p->dtype, 4, in[i].x, states, pitches[i], nbox)) return e;
   }
-  auto go = [&](auto kern) { return launch_opt_in(kern, grid, dim3(S::THREADS), sizeof(typename S::Smem) + 128, st, maps, *p); };
+  auto go = [&](auto kern) { return launch_opt_in(kern, grid, dim3(S::THREADS), sizeof(typename S::Smem) + 128, st, maps, *p, by8); };
   const cudaError_t e = wide ? go(selective_scan_kernel<T, true, RT, SPT, LP, ST, TT>) : go(selective_scan_kernel<T, false, RT, SPT, LP, ST, TT>);
   if (e != cudaSuccess) return fail(LQ_ERR_LAUNCH, "selective_scan: %s", cudaGetErrorString(e));
   return check_launch("selective_scan_kernel");
@@ -559,13 +576,13 @@ __global__ void __launch_bounds__(128) selective_scan_step_kernel(const lq_scan_
 #pragma unroll
   for (int r = 0; r < R; ++r) acc[r] = 0.f;
   if (on) {
-    const float head_decay = HEADS ? ex2(dt * (A[0] * kLog2e)) : 0.f;
+    const float head_decay = HEADS ? ex2(dt * kLog2e * A[0]) : 0.f;
     for (int n = ln * VEC; n < p.N;) {
       float Bv[VEC], Cv[VEC], a[VEC];
       rB.get(Bv);
       rC.get(Cv);
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) a[i] = HEADS ? head_decay : ex2(dt * (A[HEADS ? 0 : i] * kLog2e));
+      for (int i = 0; i < VEC; ++i) a[i] = HEADS ? head_decay : ex2(dt * kLog2e * A[HEADS ? 0 : i]);
 #pragma unroll
       for (int r = 0; r < R; ++r) {
         float h[VEC];
@@ -648,7 +665,7 @@ __global__ void __launch_bounds__(128) heads_step_kernel(const lq_scan_problem p
   if (on) {
     float dt = to_f32(reinterpret_cast<const T*>(p.dt)[b * p.dt_stride_b + head]) + (p.dt_bias ? p.dt_bias[head] : 0.f);
     dt = clamp_nan(p.softplus ? softplus(dt) : dt, p.dt_min, p.dt_max);
-    decay = ex2(dt * (p.A[head] * kLog2e));
+    decay = ex2(dt * kLog2e * p.A[head]);
 #pragma unroll
     for (int i = 0; i < VEC; ++i) Bv[i] *= dt;
   }
