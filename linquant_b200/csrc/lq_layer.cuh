@@ -66,11 +66,15 @@ __device__ __forceinline__ float silu(float x) { return x * rcp(1.0f + ex2(-kLog
 // log(1 + e^x) = max(x, 0) + log1p(w), w = e^-|x| in (0, 1]; log1p(w) = 2 atanh(s), s = w / (2 + w) <= 1/3: accurate where the
 // result is small, where log(1 + w) would lose w's low bits, and without a branch. atanh(s) / s is a polynomial in s^2 fitted at
 // Chebyshev nodes of [0, 1/9] (degree 4: within 8e-9 with these fp32 coefficients).
+template <bool EXACT = true>
 __device__ __forceinline__ float softplus(float x) {
   const float a = -fabsf(x), e = a * kLog2e;
-  // what e lost to rounding, with the part of log2(e) that a float does not hold: w is dt's relative error where x is negative
-  const float w = ex2(e), low = fmaf(a, kLog2e, -e) + a * 1.92596299e-8f, ww = w > 0.0f ? fmaf(w, low * 0.6931471805599453f, w) : w;
-  const float s = __fdividef(ww, 2.0f + ww), q = s * s;
+  float w = ex2(e);
+  if constexpr (EXACT) {  // what e lost to rounding, with the part of log2(e) that a float does not hold: w is dt's relative error where x is negative
+    const float low = fmaf(a, kLog2e, -e) + a * 1.92596299e-8f;
+    w = w > 0.0f ? fmaf(w, low * 0.6931471805599453f, w) : w;
+  }
+  const float s = w * rcp(2.0f + w), q = s * s;
   float t = 0.14087328631750926f;
   t = fmaf(t, q, 0.13980709417397671f);
   t = fmaf(t, q, 0.20012426861730928f);

@@ -1,10 +1,13 @@
 // INT8 matrix product on the Blackwell tensor cores: y[m,n] = (sum_k x[m,k] w[n,k]) x_scale[m] w_scale[n] + bias[n].
 //
-// Persistent kernel, one CTA per SM, tiles of 128 tokens x BN output channels. Both operands are codes with the reduction
-// index contiguous: TMA brings blocks of 128 bytes of K (128-byte swizzle, zero-filled behind the last row and the last byte
-// of K) into a ring of stages, one thread issues tcgen05.mma.kind::i8 (M = 128, N = BN, four steps of 32 per stage) into one
-// of two accumulators in tensor memory, and eight warps turn the other one into outputs meanwhile: INT32 to fp32, both scales
-// and the bias, through a swizzled 64-byte row per lane in shared memory, stored as pieces of 64 bytes a row.
+// Persistent kernel, one CTA per SM, tiles of 128 tokens x BN output channels; for many tiles two CTAs of a cluster share one of
+// 256 x 256 (tcgen05 cta_group::2: each brings its tokens and half of the weights, the first issues the products of both). Both
+// operands are codes with the reduction index contiguous: TMA brings blocks of 128 bytes of K (128-byte swizzle, zero-filled
+// behind the last row and the last byte of K) into a ring of stages, one thread issues tcgen05.mma.kind::i8 (four steps of 32 per
+// stage) into one of two accumulators in tensor memory, and eight warps turn the other one into outputs meanwhile: INT32 to fp32,
+// both scales and the bias, through a swizzled 64-byte row per lane in shared memory, stored as pieces of 64 bytes a row.
+// Bound by the tensor pipe: 8192^3 339 us (3.24 POP/s; 366 us without pairs), 32768 x 2560 -> 10576 688 us (2.58), where what
+// torch's INT8 product reaches is 2.94 with INT32 outputs and no scales.
 // Every wait is bounded; on expiry the CTA raises the status word, lets its copies and products land, frees its tensor
 // memory and returns.
 #include "lq_layer.cuh"
@@ -16,9 +19,10 @@ namespace lineartc {
 
 constexpr int BM = 128, BK = 128, OUT_WARPS = 8, THREADS = 32 * (OUT_WARPS + 2), STAGE_BYTES = 192 * 1024;
 
-template <int BN>
+// PAIR: two CTAs of a cluster on one tile of 256 tokens, each with 128 of them and half of the weights' rows
+template <int BN, bool PAIR>
 struct Shape {
-  static constexpr int STAGE = (BM + BN) * BK, STAGES = STAGE_BYTES / STAGE;
+  static constexpr int WROWS = PAIR ? BN / 2 : BN, STAGE = (BM + WROWS) * BK, STAGES = STAGE_BYTES / STAGE;
   static constexpr int HALF = BN / 2;                                     // columns of a storing warp: two share 32 rows
   static constexpr int OUT = OUT_WARPS * 32 * 64, COLS = OUT_WARPS * 2 * HALF * 4;  // per storing warp: 32 rows of 64 bytes; w_scale and bias of its columns
   static constexpr int BARS = (2 * STAGES + 4) * 8;
@@ -46,6 +50,70 @@ __device__ __forceinline__ void sts_u4(uint32_t addr, const uint4& v) {
   asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};\n" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
 
+// ---- one CTA, or a pair of a cluster
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;\n" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+}
+__device__ __forceinline__ uint32_t in_first(uint32_t addr) {  // the same place in the pair's first CTA
+  uint32_t a;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, 0;\n" : "=r"(a) : "r"(addr));
+  return a;
+}
+__device__ __forceinline__ void mbar_arrive_first(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];\n" ::"r"(in_first(bar)) : "memory");
+}
+__device__ __forceinline__ bool mbar_wait_cluster(uint32_t bar, uint32_t parity) {  // what the other CTA did before it arrived is visible
+  for (int it = 0; it < (1 << 20); ++it) {
+    uint32_t done;
+    asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}\n"
+                 : "=r"(done) : "r"(bar), "r"(parity) : "memory");
+    if (done) return true;
+  }
+  return false;
+}
+template <bool PAIR>
+__device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, int c0, int c1, uint32_t bar) {
+  if constexpr (PAIR)
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3}], [%4];\n" ::"r"(dst),
+                 "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(in_first(bar))
+                 : "memory");
+  else tma_load_2d(dst, map, c0, c1, bar);
+}
+template <bool PAIR>
+__device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  if constexpr (PAIR)
+    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n}\n" ::"r"(d), "l"(a), "l"(b), "r"(idesc),
+                 "r"(accumulate)
+                 : "memory");
+  else umma_i8(d, a, b, idesc, accumulate);
+}
+template <bool PAIR>
+__device__ __forceinline__ void commit(uint32_t bar) {  // of a pair: the barriers of both
+  if constexpr (PAIR)
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n" ::"r"(bar), "h"((uint16_t)3) : "memory");
+  else umma_commit(bar);
+}
+template <bool PAIR>
+__device__ __forceinline__ void tmem_alloc(uint32_t to, uint32_t columns) {
+  if constexpr (PAIR) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(to), "r"(columns) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;\n" ::: "memory");
+  } else {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(to), "r"(columns) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
+  }
+}
+template <bool PAIR>
+__device__ __forceinline__ void tmem_free(uint32_t from, uint32_t columns) {
+  if constexpr (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;\n" ::"r"(from), "r"(columns) : "memory");
+  else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(from), "r"(columns) : "memory");
+}
+
 __device__ __forceinline__ void tmem_ld_32x32b_x16(uint32_t taddr, uint32_t (&r)[16]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n"
@@ -62,15 +130,17 @@ __device__ __forceinline__ void tile_at(int t, int mt, int nt, int& m, int& n) {
   m = g * GROUP + in - n * rows;
 }
 
-template <int BN, typename TO>
+template <int BN, bool PAIR, typename TO>
 __global__ void __launch_bounds__(THREADS, 1) int8_linear_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
                                                                     const lq_linear_problem p) {
-  using S = Shape<BN>;
+  using S = Shape<BN, PAIR>;
+  constexpr int CTAS = PAIR ? 2 : 1;
   extern __shared__ uint8_t smem_dyn[];
   const uint32_t s_stage = (smem_u32(smem_dyn) + 1023u) & ~1023u, s_out = s_stage + S::STAGES * S::STAGE, s_cols = s_out + S::OUT;
   const uint32_t s_full = s_cols + S::COLS, s_empty = s_full + 8 * S::STAGES, s_acc = s_empty + 8 * S::STAGES, s_free = s_acc + 16, s_tbase = s_free + 16;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int mt = (p.M + BM - 1) / BM, nt = (p.N + BN - 1) / BN, tiles = mt * nt, kblocks = (p.K + BK - 1) / BK;
+  const int rank = PAIR ? (int)cluster_rank() : 0, first = blockIdx.x / CTAS, step = gridDim.x / CTAS;
+  const int mt = (p.M + CTAS * BM - 1) / (CTAS * BM), nt = (p.N + BN - 1) / BN, tiles = mt * nt, kblocks = (p.K + BK - 1) / BK;
 
   pdl_enter();
   if (tid == 0) {
@@ -80,61 +150,68 @@ __global__ void __launch_bounds__(THREADS, 1) int8_linear_tc_kernel(const __grid
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(s_acc + 8 * i, 1);
-      mbar_init(s_free + 8 * i, OUT_WARPS);
+      mbar_init(s_free + 8 * i, CTAS * OUT_WARPS);
     }
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
   }
-  if (warp == OUT_WARPS + 1) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(s_tbase), "r"((uint32_t)(2 * BN)) : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
-  }
+  if (warp == OUT_WARPS + 1) tmem_alloc<PAIR>(s_tbase, 2 * BN);
   asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
   __syncthreads();
+  if constexpr (PAIR) cluster_sync();  // the other CTA's barriers are there
   asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
   const uint32_t tbase = lds_u32(s_tbase);
   bool ok = true;
 
-  if (warp == OUT_WARPS) {  // loads
+  // a stage and how often it has been filled before, without a division per block
+  struct Ring {
+    int s = 0;
+    uint32_t lap = 0;
+    __device__ __forceinline__ void next() {
+      if (++s == S::STAGES) s = 0, ++lap;
+    }
+  };
+  auto wait = [&](uint32_t bar, uint32_t parity) { return PAIR ? mbar_wait_cluster(bar, parity) : mbar_wait_bounded(bar, parity); };
+  if (warp == OUT_WARPS) {  // loads; of a pair, all arrive at the first CTA's barriers
     if (lane == 0) {
-      long long fill = 0;
-      for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+      Ring r;
+      for (int t = first; t < tiles && ok; t += step) {
         int m, n;
         tile_at(t, mt, nt, m, n);
-        for (int kb = 0; kb < kblocks; ++kb, ++fill) {
-          const int s = (int)(fill % S::STAGES);
-          if (fill >= S::STAGES && !(ok = mbar_wait_bounded(s_empty + 8 * s, (uint32_t)((fill / S::STAGES + 1) & 1)))) break;
-          mbar_expect(s_full + 8 * s, S::STAGE);
-          tma_load_2d(s_stage + s * S::STAGE, &map_x, kb * BK, m * BM, s_full + 8 * s);
-          tma_load_2d(s_stage + s * S::STAGE + BM * BK, &map_w, kb * BK, n * BN, s_full + 8 * s);
+        const int row = (m * CTAS + rank) * BM, col = n * BN + rank * S::WROWS;
+        for (int kb = 0; kb < kblocks; ++kb, r.next()) {
+          if (r.lap > 0 && !(ok = wait(s_empty + 8 * r.s, (r.lap + 1) & 1))) break;
+          if (rank == 0) mbar_expect(s_full + 8 * r.s, CTAS * S::STAGE);
+          tma_load<PAIR>(s_stage + r.s * S::STAGE, &map_x, kb * BK, row, s_full + 8 * r.s);
+          tma_load<PAIR>(s_stage + r.s * S::STAGE + BM * BK, &map_w, kb * BK, col, s_full + 8 * r.s);
         }
       }
-      for (long long f = fill > S::STAGES ? fill - S::STAGES : 0; f < fill; ++f)  // nothing may land after the CTA has gone
-        ok &= mbar_wait_bounded(s_full + 8 * (int)(f % S::STAGES), (uint32_t)((f / S::STAGES) & 1));
+      if (rank == 0)
+        for (int i = 0; i < S::STAGES; ++i, r.next())  // nothing may land after the CTA has gone: the last fill of each stage
+          if (r.lap > 0) ok &= wait(s_full + 8 * r.s, (r.lap + 1) & 1);
     }
   } else if (warp == OUT_WARPS + 1) {  // products
-    if (lane == 0) {
-      const uint32_t idesc = idesc_i8(BM, BN);
-      long long fill = 0;
+    if (lane == 0 && rank == 0) {
+      const uint32_t idesc = idesc_i8(CTAS * BM, BN);
+      Ring r;
       int i = 0;
-      for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x, ++i) {
+      for (int t = first; t < tiles && ok; t += step, ++i) {
         const int acc = i & 1;
-        if (i >= 2 && !(ok = mbar_wait_bounded(s_free + 8 * acc, (uint32_t)((i / 2 + 1) & 1)))) break;
+        if (i >= 2 && !(ok = wait(s_free + 8 * acc, (uint32_t)((i / 2 + 1) & 1)))) break;
         asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
-        for (int kb = 0; kb < kblocks; ++kb, ++fill) {
-          const int s = (int)(fill % S::STAGES);
-          if (!(ok = mbar_wait_bounded(s_full + 8 * s, (uint32_t)((fill / S::STAGES) & 1)))) break;
+        for (int kb = 0; kb < kblocks; ++kb, r.next()) {
+          if (!(ok = wait(s_full + 8 * r.s, r.lap & 1))) break;
           asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
-          const uint64_t da = desc_kmajor_sw128(s_stage + s * S::STAGE), db = desc_kmajor_sw128(s_stage + s * S::STAGE + BM * BK);
+          const uint64_t da = desc_kmajor_sw128(s_stage + r.s * S::STAGE), db = desc_kmajor_sw128(s_stage + r.s * S::STAGE + BM * BK);
 #pragma unroll
-          for (int ks = 0; ks < BK / 32; ++ks) umma_i8(tbase + acc * BN, da + 2 * ks, db + 2 * ks, idesc, (kb | ks) > 0);
-          umma_commit(s_empty + 8 * s);
+          for (int ks = 0; ks < BK / 32; ++ks) mma<PAIR>(tbase + acc * BN, da + 2 * ks, db + 2 * ks, idesc, (kb | ks) > 0);
+          commit<PAIR>(s_empty + 8 * r.s);
         }
         if (!ok) break;
-        umma_commit(s_acc + 8 * acc);
+        commit<PAIR>(s_acc + 8 * acc);
       }
-      if (!ok && fill > 0)  // the products that were issued: each stage's commit
-        for (long long f = fill > S::STAGES ? fill - S::STAGES : 0; f < fill; ++f)
-          mbar_wait_bounded(s_empty + 8 * (int)(f % S::STAGES), (uint32_t)((f / S::STAGES) & 1));
+      if (!ok)  // the products that were issued: each stage's commit
+        for (int k = 0; k < S::STAGES; ++k, r.next())
+          if (r.lap > 0) wait(s_empty + 8 * r.s, (r.lap + 1) & 1);
     }
   } else {  // outputs: warp w has the accumulator rows 32 (w & 3) .. and half of the columns
     constexpr int CHUNK = 64 / sizeof(TO), PER = 16 / sizeof(TO);  // columns of a 64-byte piece of a row, of 16 bytes
@@ -142,10 +219,10 @@ __global__ void __launch_bounds__(THREADS, 1) int8_linear_tc_kernel(const __grid
     const uint32_t out = s_out + warp * 32 * 64, cols = s_cols + warp * 2 * S::HALF * 4;
     const bool wide = ((size_t)p.N * sizeof(TO)) % 16 == 0 && (reinterpret_cast<uintptr_t>(p.y) & 15u) == 0;
     int i = 0;
-    for (int t = blockIdx.x; t < tiles; t += gridDim.x, ++i) {
+    for (int t = first; t < tiles; t += step, ++i) {
       int m, n;
       tile_at(t, mt, nt, m, n);
-      const int acc = i & 1, row0 = m * BM + 32 * quad, n0 = n * BN + half;
+      const int acc = i & 1, row0 = (m * CTAS + rank) * BM + 32 * quad, n0 = n * BN + half;
       const float xs = row0 + lane < p.M ? __ldg(p.x_scale + row0 + lane) : 0.f;
       __syncwarp();
 #pragma unroll
@@ -155,7 +232,7 @@ __global__ void __launch_bounds__(THREADS, 1) int8_linear_tc_kernel(const __grid
         sts_u32(cols + 4 * (S::HALF + c), __float_as_uint(in && p.bias ? __ldg(p.bias + n0 + c) : 0.f));
       }
       __syncwarp();
-      if (!(ok = __all_sync(0xffffffffu, mbar_wait_bounded(s_acc + 8 * acc, (uint32_t)((i / 2) & 1))))) break;
+      if (!(ok = __all_sync(0xffffffffu, wait(s_acc + 8 * acc, (uint32_t)((i / 2) & 1))))) break;
       asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
 #pragma unroll 1
       for (int c0 = 0; c0 < S::HALF; c0 += CHUNK) {
@@ -218,14 +295,18 @@ __global__ void __launch_bounds__(THREADS, 1) int8_linear_tc_kernel(const __grid
       }
       asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
       __syncwarp();
-      if (lane == 0) mbar_arrive(s_free + 8 * acc);
+      if (lane == 0) {
+        if constexpr (PAIR) mbar_arrive_first(s_free + 8 * acc);
+        else mbar_arrive(s_free + 8 * acc);
+      }
     }
   }
   if (!ok && p.status != nullptr) atomicExch(p.status, 1);
   __syncwarp();
   asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
   __syncthreads();
-  if (warp == OUT_WARPS + 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tbase), "r"((uint32_t)(2 * BN)) : "memory");
+  if constexpr (PAIR) cluster_sync();  // neither CTA's memory is used by the other any more
+  if (warp == OUT_WARPS + 1) tmem_free<PAIR>(tbase, 2 * BN);
 }
 
 static int encode(CUtensorMap* m, const void* base, long long row_bytes, long long pitch, long long rows, int box_rows) {
@@ -240,15 +321,34 @@ static int encode(CUtensorMap* m, const void* base, long long row_bytes, long lo
   return r == CUDA_SUCCESS ? LQ_OK : fail(LQ_ERR_LAUNCH, "int8_linear: cuTensorMapEncodeTiled failed with CUresult %d", (int)r);
 }
 
-template <int BN, typename TO>
+template <int BN, bool PAIR, typename TO>
 static int launch_tc(const lq_linear_problem* p, cudaStream_t st) {
+  using S = Shape<BN, PAIR>;
+  constexpr int CTAS = PAIR ? 2 : 1;
   CUtensorMap mx, mw;
   if (int e = encode(&mx, p->x, p->K, p->x_stride, p->M, BM)) return e;
-  if (int e = encode(&mw, p->w, p->K, p->w_stride, p->N, BN)) return e;
-  const long long tiles = (long long)((p->M + BM - 1) / BM) * ((p->N + BN - 1) / BN);
-  if (tiles >= 1ll << 30) return fail(LQ_ERR_SHAPE, "int8_linear: M=%d N=%d", p->M, p->N);
-  const int sms = sm_count();
-  const cudaError_t e = launch_opt_in(int8_linear_tc_kernel<BN, TO>, dim3((unsigned)(tiles < sms ? tiles : sms)), dim3(THREADS), Shape<BN>::SMEM, st, mx, mw, *p);
+  if (int e = encode(&mw, p->w, p->K, p->w_stride, p->N, S::WROWS)) return e;
+  const long long tiles = (long long)((p->M + CTAS * BM - 1) / (CTAS * BM)) * ((p->N + BN - 1) / BN);
+  if (tiles >= 1ll << 29) return fail(LQ_ERR_SHAPE, "int8_linear: M=%d N=%d", p->M, p->N);
+  const int units = sm_count() / CTAS;
+  auto kern = int8_linear_tc_kernel<BN, PAIR, TO>;
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::SMEM);
+  if (e == cudaSuccess) {
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = CTAS;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(CTAS * (tiles < units ? tiles : units)));
+    cfg.blockDim = dim3(THREADS);
+    cfg.dynamicSmemBytes = S::SMEM;
+    cfg.stream = st;
+    cfg.attrs = attr;
+    cfg.numAttrs = PAIR ? 2 : 1;
+    e = cudaLaunchKernelEx(&cfg, kern, mx, mw, *p);
+  }
   if (e != cudaSuccess) return fail(LQ_ERR_LAUNCH, "int8_linear: %s", cudaGetErrorString(e));
   return check_launch("int8_linear_tc_kernel");
 }
@@ -265,9 +365,13 @@ int run_linear_tc(const lq_linear_problem* p, cudaStream_t st) {
     const long long rounds = (mt * ((p->N + bn - 1) / bn) + sms - 1) / sms, cost = rounds * (bn + 64);
     if (least == 0 || cost < least) best = bn, least = cost;
   }
+  // Pairs of CTAs read the weights half as often from shared memory; over a few rounds their larger tiles cost more than that:
+  // 8192 x 2560 -> 2560 (4.3 rounds) 54 us against 53, 4096 x 2560 -> 10576 (9) 91 against 102, 32768 x 2560 -> 10576 (73) 688 against 743
+  const bool pair = mt * ((p->N + 255) / 256) >= 6 * sms;
   return with_dtype(p->out_dtype, "int8_linear", [&](auto t) {
     using TO = decltype(t);
-    return best == 256 ? lineartc::launch_tc<256, TO>(p, st) : best == 128 ? lineartc::launch_tc<128, TO>(p, st) : lineartc::launch_tc<64, TO>(p, st);
+    if (pair) return lineartc::launch_tc<256, true, TO>(p, st);
+    return best == 256 ? lineartc::launch_tc<256, false, TO>(p, st) : best == 128 ? lineartc::launch_tc<128, false, TO>(p, st) : lineartc::launch_tc<64, false, TO>(p, st);
   });
 }
 

@@ -103,7 +103,7 @@ __device__ __forceinline__ void store_as(void* base, size_t at_row, int dtype, c
 
 // CTAs walk over the rows; a row's loads are requested while the one before is summed and stored.
 template <typename T, int VEC, int NV, Kind KIND, bool OFF>
-__global__ void __launch_bounds__(NV == 1 && !OFF || NV * VEC == 4 ? 1024 : 512) norm_kernel(const lq_norm_problem p, int team_size, long long units) {
+__global__ void __launch_bounds__(NV == 1 && !OFF || NV * VEC == 4 ? 1024 : NV == 1 ? 384 : 512) norm_kernel(const lq_norm_problem p, int team_size, long long units) {
   pdl_enter();
   constexpr bool SECOND = KIND != PLAIN;
   using R = std::conditional_t<KIND == ADD32, float, T>;  // of the second input: the residual or the gate
@@ -297,7 +297,7 @@ static int launch_vec(const lq_norm_problem* p, cudaStream_t st) {
     if (packs <= 1024) return launch_as<T, KIND, 1, 4, OFF>(p, packs, st);
     if (packs <= 16384) return launch_as<T, KIND, 1, 32, OFF>(p, packs, st);
   } else if constexpr (OFF) {
-    if (packs <= 512) return launch_as<T, KIND, VEC, 1, OFF>(p, packs, st);
+    if (packs <= 384) return launch_as<T, KIND, VEC, 1, OFF>(p, packs, st);
     if (packs <= 1024) return launch_as<T, KIND, VEC, 2, OFF>(p, packs, st);
     return launch_as<T, KIND, VEC, 32 / VEC, OFF>(p, packs, st);
   } else {

@@ -153,7 +153,7 @@ struct Prepare : Job<T, S, WIDE> {
       }
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        v[k] = clamp_nan(SOFTPLUS ? softplus(v[k]) : v[k], p.dt_min, p.dt_max);
+        v[k] = clamp_nan(SOFTPLUS ? softplus<S::ACCURATE>(v[k]) : v[k], p.dt_min, p.dt_max);
         w[k] *= v[k];
         // here and not on A: the rounding of a factor that all tokens share would add up over them
         if constexpr (!S::ACCURATE) v[k] *= kLog2e;
