@@ -309,6 +309,128 @@ __global__ void __launch_bounds__(THREADS, 1) int8_linear_tc_kernel(const __grid
   if (warp == OUT_WARPS + 1) tmem_free<PAIR>(tbase, 2 * BN);
 }
 
+// ---- few tiles: the CTAs of a cluster take parts of K
+// Their INT32 sums meet in shared memory, each CTA adds and scales a share of the tile's rows: the sum of integers is the same
+// in any order, and no workspace is needed. A ring of 96 KB leaves room for two CTAs on an SM.
+struct Split {
+  static constexpr int BN = 64, STAGE = (BM + BN) * BK, STAGES = 4, PITCH = BN * 4 + 16;  // rows of the sums on odd multiples of 16 bytes
+  static constexpr size_t SMEM = 1024 + (size_t)STAGES * STAGE + (2 * STAGES + 1) * 8 + 8;
+  static_assert(BM * PITCH <= STAGES * STAGE);
+};
+
+__device__ __forceinline__ uint32_t in_cta(uint32_t addr, uint32_t rank) {
+  uint32_t a;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(a) : "r"(addr), "r"(rank));
+  return a;
+}
+__device__ __forceinline__ int4 ld_cluster(uint32_t addr) {
+  int4 v;
+  asm volatile("ld.shared::cluster.v4.s32 {%0,%1,%2,%3}, [%4];\n" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+
+template <typename TO>
+__global__ void __launch_bounds__(THREADS, 2) int8_linear_split_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
+                                                                       const lq_linear_problem p, int parts) {
+  using S = Split;
+  extern __shared__ uint8_t smem_dyn[];
+  const uint32_t s_stage = (smem_u32(smem_dyn) + 1023u) & ~1023u, s_full = s_stage + S::STAGES * S::STAGE, s_empty = s_full + 8 * S::STAGES;
+  const uint32_t s_acc = s_empty + 8 * S::STAGES, s_tbase = s_acc + 8;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, rank = (int)cluster_rank(), tile = blockIdx.x / parts;
+  const int nt = (p.N + S::BN - 1) / S::BN, m0 = tile / nt * BM, n0 = tile % nt * S::BN, rows = min(BM, p.M - m0);
+  const int kblocks = (p.K + BK - 1) / BK, kb0 = kblocks * rank / parts, count = kblocks * (rank + 1) / parts - kb0;
+
+  pdl_enter();
+  if (tid == 0) {
+    for (int i = 0; i < 2 * S::STAGES + 1; ++i) mbar_init(s_full + 8 * i, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+  }
+  if (warp == OUT_WARPS + 1) tmem_alloc<false>(s_tbase, S::BN);
+  asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
+  __syncthreads();
+  asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+  const uint32_t tbase = lds_u32(s_tbase);
+  bool ok = true;
+
+  if (warp == OUT_WARPS) {
+    if (lane == 0) {
+      int k = 0;
+      for (; k < count; ++k) {
+        const int s = k % S::STAGES, lap = k / S::STAGES;
+        if (lap > 0 && !(ok = mbar_wait_bounded(s_empty + 8 * s, (lap + 1) & 1))) break;
+        mbar_expect(s_full + 8 * s, S::STAGE);
+        tma_load_2d(s_stage + s * S::STAGE, &map_x, (kb0 + k) * BK, m0, s_full + 8 * s);
+        tma_load_2d(s_stage + s * S::STAGE + BM * BK, &map_w, (kb0 + k) * BK, n0, s_full + 8 * s);
+      }
+      for (int s = 0; s < min(k, S::STAGES); ++s)  // nothing may land after the CTA has gone: the last fill of each stage
+        ok &= mbar_wait_bounded(s_full + 8 * s, (k - 1 - s) / S::STAGES & 1);
+    }
+  } else if (warp == OUT_WARPS + 1) {
+    if (lane == 0) {
+      const uint32_t idesc = idesc_i8(BM, S::BN);
+      for (int k = 0; k < count; ++k) {
+        const int s = k % S::STAGES, lap = k / S::STAGES;
+        if (!(ok = mbar_wait_bounded(s_full + 8 * s, lap & 1))) break;
+        asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+        const uint64_t da = desc_kmajor_sw128(s_stage + s * S::STAGE), db = desc_kmajor_sw128(s_stage + s * S::STAGE + BM * BK);
+#pragma unroll
+        for (int ks = 0; ks < BK / 32; ++ks) umma_i8(tbase, da + 2 * ks, db + 2 * ks, idesc, (k | ks) > 0);
+        umma_commit(s_empty + 8 * s);
+      }
+      umma_commit(s_acc);
+    }
+  } else {  // sums to shared memory: the stages are free once the last product is done
+    const int quad = warp & 3, c0 = (warp >> 2) * 32;
+    ok = __all_sync(0xffffffffu, mbar_wait_bounded(s_acc, 0));
+    asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+    if (ok && 32 * quad < rows) {
+      uint32_t r[32];
+      tmem_ld_32x32b_x32(tbase + ((uint32_t)(32 * quad) << 16) + c0, r);
+      asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
+#pragma unroll
+      for (int j = 0; j < 32; j += 4) sts_u4(s_stage + (32 * quad + lane) * S::PITCH + 4 * (c0 + j), make_uint4(r[j], r[j + 1], r[j + 2], r[j + 3]));
+    }
+  }
+  if (!ok && p.status != nullptr) atomicExch(p.status, 1);
+  __syncwarp();
+  asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
+  __syncthreads();
+  cluster_sync();  // the sums of all are there
+  if (warp == OUT_WARPS + 1) tmem_free<false>(tbase, S::BN);
+  else if (warp < OUT_WARPS) {
+    constexpr int PIECES = S::BN / 4;
+    TO* y = reinterpret_cast<TO*>(p.y);
+    const bool wide = p.N % 4 == 0 && (reinterpret_cast<uintptr_t>(p.y) & (4 * sizeof(TO) - 1)) == 0;
+    for (int i = rank * 32 * OUT_WARPS + tid; i < rows * PIECES; i += parts * 32 * OUT_WARPS) {
+      const int row = i / PIECES, c = i % PIECES * 4, n = n0 + c;
+      if (n >= p.N) continue;
+      int4 sum = make_int4(0, 0, 0, 0);
+      for (int q = 0; q < parts; ++q) {
+        const int4 v = ld_cluster(in_cta(s_stage + row * S::PITCH + 4 * c, q));
+        sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
+      }
+      const float xs = __ldg(p.x_scale + m0 + row);
+      const int v[4] = {sum.x, sum.y, sum.z, sum.w};
+      float f[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        f[j] = n + j < p.N ? fmaf((float)v[j] * xs, __ldg(p.w_scale + n + j), p.bias ? __ldg(p.bias + n + j) : 0.f) : 0.f;
+      TO* to = y + (size_t)(m0 + row) * p.N + n;
+      if (wide) {
+        Pack<TO, 4> out;
+        out.set(f);
+        store_pack(to, out);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (n + j < p.N) to[j] = from_f32<TO>(f[j]);
+      }
+    }
+  }
+  __syncwarp();
+  cluster_sync();  // no CTA reads another's sums any more
+}
+
 static int encode(CUtensorMap* m, const void* base, long long row_bytes, long long pitch, long long rows, int box_rows) {
   EncodeTiledFn enc = encode_tiled_fn();
   if (enc == nullptr) return fail(LQ_ERR_LAUNCH, "int8_linear: the driver does not export cuTensorMapEncodeTiled");
@@ -321,6 +443,29 @@ static int encode(CUtensorMap* m, const void* base, long long row_bytes, long lo
   return r == CUDA_SUCCESS ? LQ_OK : fail(LQ_ERR_LAUNCH, "int8_linear: cuTensorMapEncodeTiled failed with CUresult %d", (int)r);
 }
 
+template <typename... KArgs, typename... Args>
+static int launch_clusters(void (*kern)(KArgs...), int ctas, int cluster, size_t smem, cudaStream_t st, Args&&... args) {
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (e == cudaSuccess) {
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = cluster;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)ctas);
+    cfg.blockDim = dim3(THREADS);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cfg.attrs = attr;
+    cfg.numAttrs = cluster > 1 ? 2 : 1;
+    e = cudaLaunchKernelEx(&cfg, kern, args...);
+  }
+  if (e != cudaSuccess) return fail(LQ_ERR_LAUNCH, "int8_linear: %s", cudaGetErrorString(e));
+  return check_launch("int8_linear");
+}
+
 template <int BN, bool PAIR, typename TO>
 static int launch_tc(const lq_linear_problem* p, cudaStream_t st) {
   using S = Shape<BN, PAIR>;
@@ -331,26 +476,15 @@ static int launch_tc(const lq_linear_problem* p, cudaStream_t st) {
   const long long tiles = (long long)((p->M + CTAS * BM - 1) / (CTAS * BM)) * ((p->N + BN - 1) / BN);
   if (tiles >= 1ll << 29) return fail(LQ_ERR_SHAPE, "int8_linear: M=%d N=%d", p->M, p->N);
   const int units = sm_count() / CTAS;
-  auto kern = int8_linear_tc_kernel<BN, PAIR, TO>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::SMEM);
-  if (e == cudaSuccess) {
-    cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = CTAS;
-    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(CTAS * (tiles < units ? tiles : units)));
-    cfg.blockDim = dim3(THREADS);
-    cfg.dynamicSmemBytes = S::SMEM;
-    cfg.stream = st;
-    cfg.attrs = attr;
-    cfg.numAttrs = PAIR ? 2 : 1;
-    e = cudaLaunchKernelEx(&cfg, kern, mx, mw, *p);
-  }
-  if (e != cudaSuccess) return fail(LQ_ERR_LAUNCH, "int8_linear: %s", cudaGetErrorString(e));
-  return check_launch("int8_linear_tc_kernel");
+  return launch_clusters(int8_linear_tc_kernel<BN, PAIR, TO>, CTAS * (int)(tiles < units ? tiles : units), CTAS, S::SMEM, st, mx, mw, *p);
+}
+
+template <typename TO>
+static int launch_split(const lq_linear_problem* p, int tiles, int parts, cudaStream_t st) {
+  CUtensorMap mx, mw;
+  if (int e = encode(&mx, p->x, p->K, p->x_stride, p->M, BM)) return e;
+  if (int e = encode(&mw, p->w, p->K, p->w_stride, p->N, Split::BN)) return e;
+  return launch_clusters(int8_linear_split_kernel<TO>, tiles * parts, parts, Split::SMEM, st, mx, mw, *p, parts);
 }
 
 }  // namespace lineartc
@@ -368,8 +502,15 @@ int run_linear_tc(const lq_linear_problem* p, cudaStream_t st) {
   // Pairs of CTAs read the weights half as often from shared memory; over a few rounds their larger tiles cost more than that:
   // 8192 x 2560 -> 2560 (4.3 rounds) 54 us against 53, 4096 x 2560 -> 10576 (9) 91 against 102, 32768 x 2560 -> 10576 (73) 688 against 743
   const bool pair = mt * ((p->N + 255) / 256) >= 6 * sms;
+  // Few tiles of a long K: parts of at least 8 blocks for the CTAs of a cluster, two CTAs on an SM. 5120 -> 2560, 64 tokens: one part
+  // 14.3 us, 2, 4, 8 parts 11.0, 8.6, 8.7; 256 tokens, 2 parts: 14.5 -> 12.5; 8192 -> 1024, 33 tokens, 8 parts: 20.7 -> 7.9. To meet
+  // costs some 2 us, more than a short K has: 200 x 2560 -> 2560 9.0 -> 9.5, 100 x 1024 -> 1024 4.9 -> 6.7
+  const long long narrow = mt * ((p->N + lineartc::Split::BN - 1) / lineartc::Split::BN), blocks = (p->K + lineartc::BK - 1) / lineartc::BK;
+  int parts = blocks < 32 ? 1 : 8;
+  while (parts > 1 && (narrow * parts > 2 * sms || blocks < 8 * parts)) parts /= 2;
   return with_dtype(p->out_dtype, "int8_linear", [&](auto t) {
     using TO = decltype(t);
+    if (parts > 1) return lineartc::launch_split<TO>(p, (int)narrow, parts, st);
     if (pair) return lineartc::launch_tc<256, true, TO>(p, st);
     return best == 256 ? lineartc::launch_tc<256, false, TO>(p, st) : best == 128 ? lineartc::launch_tc<128, false, TO>(p, st) : lineartc::launch_tc<64, false, TO>(p, st);
   });

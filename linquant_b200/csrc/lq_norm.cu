@@ -19,7 +19,7 @@ enum Kind { PLAIN, ADD, ADD32, GATED };  // ADD32: the residual stream in fp32
 // A team holds one row (or group): a power of two up to 32 lanes of a warp, or all warps of the CTA.
 struct Team {
   int size;
-  float* sm;  // 32 floats; reductions take turns between two of them, so one barrier each is enough
+  float2* sm;  // 2 x 32; reductions take turns between two of them, so one barrier each is enough
   int turn = 0;
   template <typename Op>
   static __device__ __forceinline__ float over_warp(float v, Op op) {
@@ -27,25 +27,31 @@ struct Team {
     for (int m = 16; m; m >>= 1) v = op(v, __shfl_xor_sync(0xffffffffu, v, m));
     return v;
   }
-  template <typename Op>
-  __device__ __forceinline__ float reduce(float v, Op op) {  // of values that are not negative, so that 0 adds nothing
+  // The sum of s and the maximum of m (either may be left out) over the team, of values that are not negative: 0 adds nothing.
+  template <bool SUM, bool MAX>
+  __device__ __forceinline__ void reduce(float& s, float& m) {
+    auto add = [](float a, float b) { return a + b; };
+    auto max = [](float a, float b) { return max_nan(a, b); };
     if (size < 32) {
-      for (int m = size >> 1; m; m >>= 1) v = op(v, __shfl_xor_sync(0xffffffffu, v, m));
-      return v;
+      for (int k = size >> 1; k; k >>= 1) {
+        if constexpr (SUM) s = add(s, __shfl_xor_sync(0xffffffffu, s, k));
+        if constexpr (MAX) m = max(m, __shfl_xor_sync(0xffffffffu, m, k));
+      }
+      return;
     }
-    v = over_warp(v, op);
+    if constexpr (SUM) s = over_warp(s, add);
+    if constexpr (MAX) m = over_warp(m, max);
     if (size > 32) {
-      float* part = sm + 32 * turn;
+      float2* part = sm + 32 * turn;
       turn ^= 1;
       const int lane = threadIdx.x & 31;
-      if (lane == 0) part[threadIdx.x >> 5] = v;
+      if (lane == 0) part[threadIdx.x >> 5] = make_float2(s, m);
       __syncthreads();
-      v = over_warp(lane < size >> 5 ? part[lane] : 0.f, op);
+      const float2 of = lane < size >> 5 ? part[lane] : make_float2(0.f, 0.f);
+      if constexpr (SUM) s = over_warp(of.x, add);
+      if constexpr (MAX) m = over_warp(of.y, max);
     }
-    return v;
   }
-  __device__ __forceinline__ float sum(float v) { return reduce(v, [](float a, float b) { return a + b; }); }
-  __device__ __forceinline__ float max(float v) { return reduce(v, [](float a, float b) { return max_nan(a, b); }); }
 };
 
 // A thread has NV packs of VEC channels. OFF: a row may start inside a pack, the rows of all tensors at the same distance
@@ -58,22 +64,35 @@ struct Place {
   __device__ __forceinline__ bool has(int i) const { return !OFF || ((unsigned)(c + i) < (unsigned)n); }
 };
 
+// A vector of parameters, dense. Rows that start inside a pack would read theirs one by one from addresses VEC floats apart,
+// each load eight lines: these are put into shared memory once a CTA, a float of padding behind every 32, so that the lanes'
+// floats lie in different banks (post-norm, sum and norm of 1021 x 2561: 12.2 -> 11.0 us).
 template <int VEC, bool OFF>
-__device__ __forceinline__ void load_f32(const float* p, const Place<VEC, OFF>& at, float (&x)[VEC]) {  // parameters: dense
-  if constexpr (VEC % 4 == 0 && !OFF) {
-#pragma unroll
-    for (int i = 0; i < VEC; i += 4) {
-      const float4 v = __ldg(reinterpret_cast<const float4*>(p + at.c + i));
-      x[i] = v.x; x[i + 1] = v.y; x[i + 2] = v.z; x[i + 3] = v.w;
-    }
-  } else if (at.all()) {
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) x[i] = __ldg(p + at.c + i);
-  } else {
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) x[i] = at.has(i) ? __ldg(p + at.c + i) : 0.f;
+struct Params {
+  const float* p;
+  static __host__ __device__ constexpr unsigned slot(unsigned c) { return c + c / 32; }
+  static __host__ __device__ constexpr unsigned slots(int n) { return slot(n + 2 * VEC) + 1; }  // zeros before and behind
+  __device__ __forceinline__ float* stage(float* to, int n) {
+    if (p == nullptr) return to;
+    for (int c = threadIdx.x - VEC; c < n + VEC; c += blockDim.x) to[slot(c + VEC)] = (unsigned)c < (unsigned)n ? __ldg(p + c) : 0.f;
+    p = to;
+    return to + slots(n);
   }
-}
+  __device__ __forceinline__ void get(int c0, const Place<VEC, OFF>& at, float (&x)[VEC]) const {
+    if constexpr (OFF) {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) x[i] = p[slot(at.c + i + VEC)];
+    } else if constexpr (VEC % 4 == 0) {
+#pragma unroll
+      for (int i = 0; i < VEC; i += 4) {
+        const float4 v = __ldg(reinterpret_cast<const float4*>(p + c0 + at.c + i));
+        x[i] = v.x; x[i + 1] = v.y; x[i + 2] = v.z; x[i + 3] = v.w;
+      }
+    } else {
+      x[0] = __ldg(p + c0 + at.c);
+    }
+  }
+};
 template <typename TO, int VEC, bool OFF>
 __device__ __forceinline__ void store_row(TO* row, const Place<VEC, OFF>& at, const float (&y)[VEC]) {
   if (at.all()) {
@@ -101,18 +120,27 @@ __device__ __forceinline__ void store_as(void* base, size_t at_row, int dtype, c
   else store_row(reinterpret_cast<__nv_bfloat16*>(base) + at_row, at, y);
 }
 
-// CTAs walk over the rows; a row's loads are requested while the one before is summed and stored.
+// CTAs walk over the rows; a row's loads are requested while the one before is summed and stored. The register caps leave room for
+// two CTAs an SM at two loads a thread (16384 x 2560, residual and norm: 56.6 us; with 112 registers and one CTA 61.5; capped
+// at 64, which spills, 85), and for the widest CTA of each form.
 template <typename T, int VEC, int NV, Kind KIND, bool OFF>
-__global__ void __launch_bounds__(NV == 1 && !OFF || NV * VEC == 4 ? 1024 : NV == 1 ? 384 : 512) norm_kernel(const lq_norm_problem p, int team_size, long long units) {
+__global__ void __launch_bounds__(NV == 1 && !OFF || NV * VEC == 4 ? 1024 : NV == 1 ? 384 : NV == 2 ? 320 : 512, NV == 2 ? 2 : 1) norm_kernel(const lq_norm_problem p, int team_size, long long units) {
   pdl_enter();
   constexpr bool SECOND = KIND != PLAIN;
   using R = std::conditional_t<KIND == ADD32, float, T>;  // of the second input: the residual or the gate
-  __shared__ float sm[2 * 32];
+  __shared__ float2 sm[2 * 32];
   const int rank = threadIdx.x % team_size, per_row = p.D / p.group;
   const long long step = (long long)gridDim.x * (blockDim.x / team_size);
   Team team{team_size, sm};
   const float inv_n = 1.0f / (float)p.group;
   const bool has_second = KIND == GATED || p.residual != nullptr;
+  Params<VEC, OFF> weight{p.weight}, post_weight{p.post_weight}, scale_vec{p.scale_vec};
+  if constexpr (OFF) {
+    extern __shared__ float params[];
+    float* at = params;
+    for (Params<VEC, OFF>* w : {&post_weight, &scale_vec, &weight}) at = w->stage(at, p.D);
+    __syncthreads();
+  }
 
   Pack<T, VEC> raw[NV];
   constexpr int RV = VEC * sizeof(R) > 16 ? 16 / sizeof(R) : VEC;
@@ -192,39 +220,61 @@ __global__ void __launch_bounds__(NV == 1 && !OFF || NV * VEC == 4 ? 1024 : NV =
       }
     }
     request(unit + step);
-    auto rms = [&]() {
+    auto largest = [&]() {
+      float m = 0.f;
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) m = max_nan(m, fabsf(v[j][i]));
+      return m;
+    };
+    // v <- v w / rms(v), `last` what multiplies it besides. The weights come before the sum is known, which leaves one product
+    // behind the wait for it; the largest |v w| joins the sum's way, and times 1 / rms is the row's amax.
+    float amax = 0.f;
+    auto normed = [&](const Params<VEC, OFF>& w, auto with_max, auto last) {
       float s = 0.f;
 #pragma unroll
       for (int j = 0; j < NV; ++j)
 #pragma unroll
         for (int i = 0; i < VEC; ++i) s = fmaf(v[j][i], v[j][i], s);
-      return rsqrtf(fmaf(team.sum(s), inv_n, p.eps));
-    };
-    auto times = [&](float f, const float* w) {  // v f w
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
         if (!on[j]) continue;
         float ww[VEC];
-        load_f32(w + c0, at[j], ww);
+        w.get(c0, at[j], ww);
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) v[j][i] = v[j][i] * f * ww[i];
+        for (int i = 0; i < VEC; ++i) v[j][i] *= ww[i];
       }
+      last();
+      constexpr bool MAX = decltype(with_max)::value;
+      if constexpr (MAX) amax = largest();
+      team.template reduce<true, MAX>(s, amax);
+      const float f = rsqrtf(fmaf(s, inv_n, p.eps));
+      amax *= f;
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) v[j][i] *= f;
+    };
+    auto out_normed = [&](auto last) {
+      if (p.codes) normed(weight, std::true_type{}, last);
+      else normed(weight, std::false_type{}, last);
     };
 
     if constexpr (KIND == ADD || KIND == ADD32) {
-      if (p.post_weight) times(rms(), p.post_weight);
+      if (p.post_weight) normed(post_weight, std::false_type{}, [] {});
       if (has_second) {
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
           if (!on[j]) continue;
           float s[VEC];
-          if (p.scale_vec) load_f32(p.scale_vec, at[j], s);
+          if (p.scale_vec) scale_vec.get(c0, at[j], s);
 #pragma unroll
           for (int i = 0; i < VEC; ++i) v[j][i] = fmaf(p.scale_vec ? s[i] * p.residual_scale : p.residual_scale, v[j][i], g[j][i]);
           store_row(reinterpret_cast<R*>(p.residual_out) + (size_t)row * p.D, at[j], v[j]);
         }
       }
-      if (p.weight) times(rms(), p.weight);
+      if (p.weight) out_normed([] {});
     } else if constexpr (KIND == GATED) {
       auto gate = [&]() {
 #pragma unroll
@@ -233,16 +283,18 @@ __global__ void __launch_bounds__(NV == 1 && !OFF || NV * VEC == 4 ? 1024 : NV =
           for (int i = 0; i < VEC; ++i) v[j][i] *= silu(g[j][i]);
       };
       if (p.gate_first) gate();
-      times(rms(), p.weight);
-      if (!p.gate_first) gate();
+      out_normed([&] {
+        if (!p.gate_first) gate();
+      });
     }
     if (p.codes) {
-      float amax = 0.f, inv;
-#pragma unroll
-      for (int j = 0; j < NV; ++j)
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) amax = max_nan(amax, fabsf(v[j][i]));
-      const float scale = row_scale(team.max(amax), inv);
+      if constexpr (KIND == PLAIN) {
+        float none = 0.f;
+        amax = largest();
+        team.template reduce<false, true>(none, amax);
+      }
+      float inv;
+      const float scale = row_scale(amax, inv);
       if (live && rank == 0) p.scale[row] = scale;
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
@@ -280,29 +332,31 @@ static int launch_as(const lq_norm_problem* p, int packs, cudaStream_t st) {
   const long long ctas = (units + per_cta - 1) / per_cta;
   int per_sm = 0;
   auto kern = norm_kernel<T, VEC, NV, KIND, OFF>;
-  const cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, threads, 0);
+  const int params = (p->weight != nullptr) + (p->post_weight != nullptr) + (p->scale_vec != nullptr);
+  const int smem = OFF ? params * (int)Params<VEC, OFF>::slots(p->D) * (int)sizeof(float) : 0;  // three of 16384: 198 KB
+  cudaError_t e = OFF ? cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) : cudaSuccess;
+  if (e == cudaSuccess) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, threads, smem);
   if (e != cudaSuccess) return fail(LQ_ERR_LAUNCH, "norm: %s", cudaGetErrorString(e));
   const long long most = (long long)sm_count() * per_sm;
-  launch(kern, dim3((unsigned)(ctas < most ? ctas : most)), dim3(threads), 0, st, *p, team, units);
+  launch(kern, dim3((unsigned)(ctas < most ? ctas : most)), dim3(threads), smem, st, *p, team, units);
   return check_launch("norm_kernel");
 }
-// Registers hold the row, the next one on its way. Few loads a thread where rows are short of threads for the GPU (their
-// latency is what such a call costs); else two, which leaves the most rows in flight: at 32768 x 5120 (gated, bf16) NV = 1, 2,
-// 4 take 336, 242, 252 us, at 64 x 2560 2.4, 2.8, 4.1.
+// Registers hold the row, the next one on its way: two loads a thread and input where two CTAs of such threads share an SM (up to
+// 640 packs), four behind that. bf16, gated norm of 32768 x 5120: 1, 2, 4 loads 289, 182, 234 us; 20480 x 8192: 246, 233 (one
+// CTA an SM), 229, with INT8 outputs 286, 256, 231. 64 x 5120: 3.1, 2.8 us for one and two loads.
 template <typename T, Kind KIND, int VEC, bool OFF>
 static int launch_vec(const lq_norm_problem* p, cudaStream_t st) {
   const int packs = (p->group + VEC - 1) / VEC + OFF;
-  const bool few = (long long)p->rows * (p->D / p->group) <= sm_count();
   if constexpr (VEC == 1) {
     if (packs <= 1024) return launch_as<T, KIND, 1, 4, OFF>(p, packs, st);
     if (packs <= 16384) return launch_as<T, KIND, 1, 32, OFF>(p, packs, st);
   } else if constexpr (OFF) {
     if (packs <= 384) return launch_as<T, KIND, VEC, 1, OFF>(p, packs, st);
-    if (packs <= 1024) return launch_as<T, KIND, VEC, 2, OFF>(p, packs, st);
+    if (packs <= 640) return launch_as<T, KIND, VEC, 2, OFF>(p, packs, st);
     return launch_as<T, KIND, VEC, 32 / VEC, OFF>(p, packs, st);
   } else {
-    if (packs <= 32 || (few && packs <= 1024)) return launch_as<T, KIND, VEC, 1, OFF>(p, packs, st);
-    if (packs <= 1024) return launch_as<T, KIND, VEC, 2, OFF>(p, packs, st);
+    if (packs <= 32) return launch_as<T, KIND, VEC, 1, OFF>(p, packs, st);
+    if (packs <= 640) return launch_as<T, KIND, VEC, 2, OFF>(p, packs, st);
     if (packs <= 512 * 32 / VEC) return launch_as<T, KIND, VEC, 32 / VEC, OFF>(p, packs, st);
   }
   return fail(LQ_ERR_UNSUPPORTED, "norm over %d channels (at most 16384)", p->group);

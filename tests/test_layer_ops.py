@@ -497,3 +497,37 @@ def test_refusals():
         layer.rms_norm_fwd(x, w[:, 0], post_weight=w[:, 0])  # a norm of the block's output goes to a residual
     with pytest.raises(_cabi.LinQuantError):
         layer.gated_rms_norm_fwd(x, x.cpu(), randn(32))
+
+
+@pytest.mark.parametrize("out", [F16, BF16, F32])
+@pytest.mark.parametrize("M,K,N", [(8210, 100, 3500), (20011, 272, 1290)])
+def test_int8_linear_many_tiles(M, K, N, out):
+    """Pairs of CTAs on one tile, the last rows and columns ragged (M past a pair's 256 tokens by less and by more than 128)."""
+    from linquant_b200.kernels.layer import int8_linear_fwd
+
+    x, w = int_codes(M, K, -128), int_codes(N, K, -128)
+    xs, ws, b = (torch.rand(n, device="cuda") for n in (M, N, N))
+    y = int8_linear_fwd(padded(x), padded(w), ws, x_scale=xs, bias=b, out_dtype=out)
+    want = (x.double() @ w.double().t()) * xs.double()[:, None] * ws.double() + b.double()
+    # three roundings to fp32 of a product and its sum with the bias, one to the output
+    size = ((x.double() @ w.double().t()) * xs.double()[:, None] * ws.double()).abs() + b.double()
+    bound = 4 * 2.0**-24 * size + (0 if out == F32 else torch.finfo(out).eps / 2 * want.abs() + (2.0**-25 if out == F16 else 0))
+    fits = want.abs() < torch.finfo(out).max
+    assert ((y.double() - want).abs() <= bound * (1 + 2.0**-20))[fits].all()
+    most = torch.finfo(out).max
+    assert (torch.where(want > 0, y, -y).double() >= most)[~fits].all()  # behind the type's range: its largest value or infinity
+
+
+@pytest.mark.parametrize("out", [F16, BF16, F32])
+@pytest.mark.parametrize("M,K,N", [(17, 4096, 130), (40, 4111, 1001), (129, 8200, 64), (255, 16384, 2047), (30, 131071, 5)])
+def test_int8_linear_long_rows(M, K, N, out):
+    """Few tiles: parts of K that meet in a cluster. The sums are whole numbers, the same in any order."""
+    from linquant_b200.kernels.layer import int8_linear_fwd
+
+    x, w = int_codes(M, K, -128), int_codes(N, K, -128)
+    one_m, one_n = torch.ones(M, device="cuda"), torch.ones(N, device="cuda")
+    want = x.double() @ w.double().t()
+    y = int8_linear_fwd(padded(x), padded(w), one_n * 2.0**-12, x_scale=one_m * 2.0**-3, out_dtype=out)
+    # the sum rounds to fp32, scales that are powers of two round nothing, then one rounding to the output
+    assert torch.equal(y, (want.float() * 2.0**-15).to(out))
+    assert torch.equal(y, int8_linear_fwd(padded(x), padded(w), one_n * 2.0**-12, x_scale=one_m * 2.0**-3, out_dtype=out))
