@@ -2,13 +2,14 @@
 //
 //   y[m,n] = (sum_k x[m,k] w[n,k]) x_scale[m] w_scale[n] + bias[n]          INT32 sums, exact
 //
-// Kernel for few tokens, where the weights' bytes and latency count: a CTA owns 16 output channels and up to 8 MT tokens. The rows
-// of the weights come whole (2560 bytes of each at a time, two such pieces on their way) by bulk copies into shared memory; its
-// warps share K in blocks of 64 bytes and add their INT32 sums through shared memory. The reduction index may be permuted as
-// long as both operands are, so a lane takes 16 consecutive bytes of a row as the K slots of two m16n8k32 products. With values
-// for codes (VALUES) every CTA makes the codes of its tokens in shared memory while the weights are on their way.
-// 3 tokens, 5120 -> 2560 channels: fragments loaded straight from global memory, 64 bytes of a row at a time, took 8.2 us, and
-// 11.5 us with a kernel for the codes ahead of it.
+// Kernel for few tokens, where the weights' bytes and latency count: a CTA walks over tiles of 16 output channels for up to 8 MT
+// tokens. The rows of the weights come whole (2560 bytes of each at a time, two such pieces on their way) by bulk copies into
+// shared memory; its warps share K in blocks of 64 bytes and add their INT32 sums through shared memory. The reduction index may
+// be permuted as long as both operands are, so a lane takes 16 consecutive bytes of a row as the K slots of two m16n8k32 products.
+// With values for codes (VALUES) every CTA makes the codes of its tokens in shared memory while the weights are on their way.
+// 5120 -> 2560 channels: 3 tokens 6.9 us (13 MB, 2 us of memory; launch, the first bytes' latency and the sums' way through shared
+// memory are the rest), with values 9.1, with a kernel for the codes ahead 10.1; 2560 -> 10576: 8 tokens 9.2, with values 11.3.
+// A CTA for every tile, each making its codes, took 21.5 there.
 #include "lq_layer.cuh"
 #include "lq_tc.cuh"
 
@@ -39,69 +40,60 @@ struct Values {
   long long stride;
 };
 
-// The codes of rows [0, rows) of `in` at pitch `pitch` in shared memory (zeros from K on) and their scales. PV values a load.
-template <typename T, int PV, int THREADS>
+// The codes of up to 8 rows of `in` at pitch `pitch` in shared memory (zeros from K on) and their scales; PV values a load. A row
+// belongs to a power of two of warps. A thread's first HOLD loads stay in registers, what lies behind them is read again.
+template <typename T, int PV, int WARPS>
 __device__ __forceinline__ void quantize_rows_shared(const T* in, long long stride, int rows, int K, int8_t* codes, int pitch, float* scales, float* part) {
-  constexpr int R = 8;  // rows at a time: their loads are on their way together
-  const int tid = threadIdx.x, warp = tid >> 5;
-  float top[R] = {};
-#pragma unroll 2
-  for (int c = tid * PV; c < K; c += THREADS * PV) {
-    Pack<T, PV> raw[R];
+  constexpr int HOLD = 6;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, team = WARPS / (rows <= 1 ? 1 : rows <= 2 ? 2 : rows <= 4 ? 4 : 8);
+  const int row = warp / team, step = team * 32 * PV, c0 = (warp % team * 32 + lane) * PV;
+  const bool on = row < rows;
+  const T* from = in + row * stride;
+  Pack<T, PV> held[HOLD];
+  auto load = [&](int c) {
+    Pack<T, PV> raw;
+    raw.zero();
+    if (on && c < K) raw = load_pack<T, PV>(from + c);
+    return raw;
+  };
+  float top = 0.f;
+  auto largest = [&](const Pack<T, PV>& raw) {
+    float v[PV];
+    raw.get(v);
 #pragma unroll
-    for (int r = 0; r < R; ++r)
-      if (r < rows) raw[r] = load_pack<T, PV>(in + r * stride + c);
+    for (int i = 0; i < PV; ++i) top = max_nan(top, fabsf(v[i]));
+  };
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-      if (r >= rows) break;
-      float v[PV];
-      raw[r].get(v);
+  for (int h = 0; h < HOLD; ++h) held[h] = load(c0 + h * step);
 #pragma unroll
-      for (int i = 0; i < PV; ++i) top[r] = max_nan(top[r], fabsf(v[i]));
-    }
-  }
+  for (int h = 0; h < HOLD; ++h) largest(held[h]);
+  for (int c = c0 + HOLD * step; c < K; c += step) largest(load(c));
 #pragma unroll
-  for (int r = 0; r < R; ++r) {
-    if (r >= rows) break;
-#pragma unroll
-    for (int m = 16; m; m >>= 1) top[r] = max_nan(top[r], __shfl_xor_sync(0xffffffffu, top[r], m));
-    if ((tid & 31) == 0) part[r * 32 + warp] = top[r];
-  }
+  for (int m = 16; m; m >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, m));
+  if (lane == 0) part[warp] = top;
   __syncthreads();
-  float inv[R];
+  for (int w = 0; w < team; ++w) top = max_nan(top, part[row * team + w]);
+  float inv;
+  const float scale = row_scale(top, inv);
+  if (on && lane == 0 && warp % team == 0) scales[row] = scale;
+  auto store = [&](int c, const Pack<T, PV>& raw) {
+    if (!on || c >= pitch) return;
+    float v[PV];
+    raw.get(v);
+    Pack<int8_t, PV> q;
+    if constexpr (PV % 4 == 0) {
+      uint32_t* w = reinterpret_cast<uint32_t*>(&q);
 #pragma unroll
-  for (int r = 0; r < R; ++r) {
-    if (r >= rows) break;
-    float amax = 0.f;
-#pragma unroll
-    for (int w = 0; w < THREADS / 32; ++w) amax = max_nan(amax, part[r * 32 + w]);
-    const float scale = row_scale(amax, inv[r]);
-    if (tid == 0) scales[r] = scale;
-  }
-  for (int c = tid * PV; c < pitch; c += THREADS * PV) {
-    Pack<T, PV> raw[R];
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-      raw[r].zero();
-      if (r < rows && c < K) raw[r] = load_pack<T, PV>(in + r * stride + c);
+      for (int i = 0; i < PV; i += 4)
+        w[i / 4] = pack_sat_s8x2(row_code(v[i + 1], inv), row_code(v[i], inv), pack_sat_s8x2(row_code(v[i + 3], inv), row_code(v[i + 2], inv), 0u));
+    } else {
+      q.v[0] = (int8_t)row_code(v[0], inv);
     }
+    store_pack(codes + row * pitch + c, q);
+  };
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-      if (r >= rows) break;
-      float v[PV];
-      raw[r].get(v);
-      Pack<int8_t, PV> q;
-      if constexpr (PV % 4 == 0) {
-        uint32_t* w = reinterpret_cast<uint32_t*>(&q);
-#pragma unroll
-        for (int i = 0; i < PV; i += 4)
-          w[i / 4] = pack_sat_s8x2(row_code(v[i + 1], inv[r]), row_code(v[i], inv[r]), pack_sat_s8x2(row_code(v[i + 3], inv[r]), row_code(v[i + 2], inv[r]), 0u));
-      } else {
-        q.v[0] = (int8_t)row_code(v[0], inv[r]);
-      }
-      store_pack(codes + r * pitch + c, q);
-    }
-  }
+  for (int h = 0; h < HOLD; ++h) store(c0 + h * step, held[h]);
+  for (int c = c0 + HOLD * step; c < pitch; c += step) store(c, load(c));
   __syncthreads();
 }
 
@@ -113,56 +105,69 @@ static __host__ __device__ __forceinline__ int code_pitch(int K) {  // of codes 
 }
 
 template <int MT, typename TO, typename TX, int PV>
-__global__ void __launch_bounds__(std::is_same_v<TX, int8_t> ? 256 : 512) int8_linear_few_kernel(const lq_linear_problem p, const Values values) {
+__global__ void __launch_bounds__(std::is_same_v<TX, int8_t> ? 256 : 512, 2) int8_linear_few_kernel(const lq_linear_problem p, const Values values) {
   constexpr bool VALUES = !std::is_same_v<TX, int8_t>;
   constexpr int WARPS = VALUES ? 16 : 8;  // making codes takes instructions
   extern __shared__ __align__(128) int8_t dyn[];
   __shared__ int part[WARPS][8 * MT][17];
-  __shared__ float scales[8 * MT], amax[VALUES ? 8 * 32 : 1];
+  __shared__ float scales[8 * MT], amax[WARPS];
   __shared__ uint64_t bars[2];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, q = lane & 3;
-  const int n0 = blockIdx.x * 16, m0 = blockIdx.y * 8 * MT;
-  const int chunks = (p.K + KC - 1) / KC, K16 = p.K & ~15;
-  int8_t* codes = dyn + (chunks > 1 ? 2 : 1) * 16 * WP;
+  const int tiles = (p.N + 15) / 16, chunks = (p.K + KC - 1) / KC, K16 = p.K & ~15;
+  const int items = ((tiles - (int)blockIdx.x + (int)gridDim.x - 1) / (int)gridDim.x) * chunks;  // pieces of weights, one after the other
+  int8_t* codes = dyn + 2 * 16 * WP;
   const int pitch = code_pitch(p.K);
   if (tid == 0) {
     for (int i = 0; i < 2; ++i) asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;\n" ::"r"(smem_u32(&bars[i])));
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
   }
   pdl_enter();
-  auto request = [&](int c) {  // warp 0: one row a lane
-    const int bytes = min(KC, K16 - c * KC);
-    const uint32_t bar = smem_u32(&bars[c & 1]);
-    if (lane == 0) asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n" ::"r"(bar), "r"((uint32_t)(bytes > 0 ? 16 * bytes : 0)) : "memory");
+  struct At {  // of an item: its tile and piece
+    int tile, chunk;
+    __device__ __forceinline__ void next(int chunks) {
+      if (++chunk == chunks) chunk = 0, tile += gridDim.x;
+    }
+  };
+  auto request = [&](int item, const At& at) {  // warp 0: one row a lane
+    const int bytes = max(0, min(KC, K16 - at.chunk * KC));
+    const uint32_t bar = smem_u32(&bars[item & 1]);
+    if (lane == 0) asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n" ::"r"(bar), "r"((uint32_t)(16 * bytes)) : "memory");
     __syncwarp();
     if (lane < 16 && bytes > 0) {
-      const int8_t* from = p.w + (long long)min(n0 + lane, p.N - 1) * p.w_stride + (long long)c * KC;  // rows behind the last are read and not written
-      asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n" ::"r"(smem_u32(dyn + ((c & 1) * 16 + lane) * WP)),
+      const int8_t* from = p.w + (long long)min(at.tile * 16 + lane, p.N - 1) * p.w_stride + (long long)at.chunk * KC;  // rows behind the last are read and not written
+      asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n" ::"r"(smem_u32(dyn + ((item & 1) * 16 + lane) * WP)),
                    "l"(from), "r"(bytes), "r"(bar)
                    : "memory");
     }
   };
-  if (warp == 0) {
-    __syncwarp();
-    request(0);
-    if (chunks > 1) request(1);
-  }
+  At ahead{(int)blockIdx.x, 0};
+  if (warp == 0) __syncwarp();
+  for (int i = 0; i < 2 && i < items; ++i, ahead.next(chunks))
+    if (warp == 0) request(i, ahead);
+  // thread tid stores output (tid / 16, tid % 16) of a tile; its scales and bias are requested ahead
+  static_assert(8 * MT * 16 <= 32 * WARPS);
+  const int m = tid >> 4;
+  const bool mine = m < p.M;
+  const float xs = !VALUES && mine ? __ldg(p.x_scale + m) : 0.f;
   if constexpr (VALUES)
-    quantize_rows_shared<TX, PV, 32 * WARPS>(reinterpret_cast<const TX*>(values.x) + (long long)m0 * values.stride, values.stride, min(8, p.M - m0), p.K, codes, pitch, scales, amax);
+    quantize_rows_shared<TX, PV, WARPS>(reinterpret_cast<const TX*>(values.x), values.stride, p.M, p.K, codes, pitch, scales, amax);
   else
     __syncthreads();  // the barriers are there
   const int8_t* xr[MT];
 #pragma unroll
-  for (int j = 0; j < MT; ++j) xr[j] = VALUES ? codes + min(g, p.M - m0 - 1) * pitch : p.x + (long long)min(m0 + 8 * j + g, p.M - 1) * p.x_stride;
+  for (int j = 0; j < MT; ++j) xr[j] = VALUES ? codes + min(g, p.M - 1) * pitch : p.x + (long long)min(8 * j + g, p.M - 1) * p.x_stride;
   int acc[MT][4] = {};
   bool ok = true;
-  for (int c = 0; c < chunks; ++c) {
-    int8_t* w = dyn + (c & 1) * 16 * WP;
-    if (c == chunks - 1 && K16 < p.K && tid < 16) {  // what is left of a row behind its last 16 bytes
-      const int8_t* from = p.w + (long long)min(n0 + tid, p.N - 1) * p.w_stride;
-      for (int k = K16; k < p.K; ++k) w[tid * WP + k - c * KC] = from[k];
+  At at{(int)blockIdx.x, 0};
+  float ws = 0.f, bias = 0.f;
+  for (int i = 0; i < items; ++i, at.next(chunks), ahead.next(chunks)) {
+    int8_t* w = dyn + (i & 1) * 16 * WP;
+    const int n0 = at.tile * 16, on = n0 + (tid & 15), k0 = at.chunk * KC, blocks = min(KC / 64, (p.K - k0 + 63) / 64);
+    const bool last = at.chunk == chunks - 1;
+    if (at.chunk == 0 && mine && on < p.N) {
+      ws = __ldg(p.w_scale + on);
+      bias = p.bias ? __ldg(p.bias + on) : 0.f;
     }
-    const int k0 = c * KC, blocks = min(KC / 64, (p.K - k0 + 63) / 64);
     constexpr int U = (KC / 64 + WARPS - 1) / WARPS;
     uint4 b[U][MT];
 #pragma unroll
@@ -171,8 +176,14 @@ __global__ void __launch_bounds__(std::is_same_v<TX, int8_t> ? 256 : 512) int8_l
 #pragma unroll
       for (int j = 0; j < MT; ++j) b[u][j] = !VALUES ? codes16(xr[j], k, p.K) : k < pitch ? *reinterpret_cast<const uint4*>(xr[j] + k) : make_uint4(0, 0, 0, 0);
     }
-    ok = ok && mbar_wait_bounded(smem_u32(&bars[c & 1]), (uint32_t)((c >> 1) & 1));
-    if (c == chunks - 1) __syncthreads();  // the ends of the rows
+    if (last && K16 < p.K) {  // what is left of a row behind its last 16 bytes
+      if (tid < 16) {
+        const int8_t* from = p.w + (long long)min(n0 + tid, p.N - 1) * p.w_stride;
+        for (int k = K16; k < p.K; ++k) w[tid * WP + k - k0] = from[k];
+      }
+      __syncthreads();
+    }
+    ok = ok && mbar_wait_bounded(smem_u32(&bars[i & 1]), (uint32_t)((i >> 1) & 1));
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int kb = warp + u * WARPS;
@@ -184,40 +195,44 @@ __global__ void __launch_bounds__(std::is_same_v<TX, int8_t> ? 256 : 512) int8_l
         mma_s8(acc[j], lo.z, hi.z, lo.w, hi.w, b[u][j].z, b[u][j].w);
       }
     }
-    if (c + 2 < chunks) {
-      __syncthreads();
-      if (warp == 0) {
-        asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
-        request(c + 2);
-      }
+    if (last) {
+      if (chunks == 1 && i > 0) __syncthreads();  // the sums of the tile before have been read
+#pragma unroll
+      for (int j = 0; j < MT; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) part[warp][8 * j + 2 * q + (e & 1)][g + 8 * (e >> 1)] = acc[j][e], acc[j][e] = 0;
     }
-  }
-  if (!ok && p.status) atomicExch(p.status, 1);
+    ok = __syncthreads_and(ok) != 0;
+    if (!ok) {  // stores nothing more; what was requested still lands
+      for (int k = i; k < min(i + 2, items); ++k) mbar_wait_bounded(smem_u32(&bars[k & 1]), (uint32_t)((k >> 1) & 1));
+      if (tid == 0 && p.status) atomicExch(p.status, 1);
+      return;
+    }
+    if (warp == 0 && i + 2 < items) {
+      asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+      request(i + 2, ahead);
+    }
+    if (last && mine && on < p.N) {
+      int s = 0;
 #pragma unroll
-  for (int j = 0; j < MT; ++j)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) part[warp][8 * j + 2 * q + (i & 1)][g + 8 * (i >> 1)] = acc[j][i];
-  ok = __syncthreads_and(ok) != 0;
-  if (!ok) {  // stores nothing; what was requested still lands
-    for (int c = max(0, chunks - 2); c < chunks; ++c) mbar_wait_bounded(smem_u32(&bars[c & 1]), (uint32_t)((c >> 1) & 1));
-    return;
-  }
-  for (int i = tid; i < 8 * MT * 16; i += 32 * WARPS) {
-    const int m = m0 + (i >> 4), n = n0 + (i & 15);
-    if (m >= p.M || n >= p.N) continue;
-    int s = 0;
-#pragma unroll
-    for (int w = 0; w < WARPS; ++w) s += part[w][i >> 4][i & 15];
-    const float y = fmaf((float)s * (VALUES ? scales[i >> 4] : p.x_scale[m]), p.w_scale[n], p.bias ? p.bias[n] : 0.f);
-    reinterpret_cast<TO*>(p.y)[(size_t)m * p.N + n] = from_f32<TO>(y);
+      for (int v = 0; v < WARPS; ++v) s += part[v][m][tid & 15];
+      reinterpret_cast<TO*>(p.y)[(size_t)m * p.N + on] = from_f32<TO>(fmaf((float)s * (VALUES ? scales[m] : xs), ws, bias));
+    }
   }
 }
 
 template <int MT, typename TO, typename TX, int PV>
 static int launch_few(const lq_linear_problem* p, const Values& v, cudaStream_t st) {
-  const dim3 grid((p->N + 15) / 16, (p->M + 8 * MT - 1) / (8 * MT));
-  const size_t smem = (size_t)(p->K > KC ? 2 : 1) * 16 * WP + (std::is_same_v<TX, int8_t> ? 0 : (size_t)(p->M < 8 ? p->M : 8) * code_pitch(p->K));
-  const cudaError_t e = launch_opt_in(int8_linear_few_kernel<MT, TO, TX, PV>, grid, dim3(std::is_same_v<TX, int8_t> ? 256 : 512), smem, st, *p, v);
+  const size_t smem = 2 * 16 * WP + (std::is_same_v<TX, int8_t> ? 0 : (size_t)p->M * code_pitch(p->K));
+  auto kern = int8_linear_few_kernel<MT, TO, TX, PV>;
+  const int threads = std::is_same_v<TX, int8_t> ? 256 : 512;
+  int per_sm = 0;
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (e == cudaSuccess) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, threads, smem);
+  if (e == cudaSuccess) {
+    const int tiles = (p->N + 15) / 16, most = sm_count() * per_sm;
+    e = launch(kern, dim3(tiles < most ? tiles : most), dim3(threads), smem, st, *p, v);
+  }
   if (e != cudaSuccess) return fail(LQ_ERR_LAUNCH, "int8_linear: %s", cudaGetErrorString(e));
   return check_launch("int8_linear_few_kernel");
 }
@@ -245,7 +260,7 @@ extern "C" int lq_int8_linear(const lq_linear_problem* p, lq_stream stream) {
   if (int e = linear::check(p)) return e;
   if (p->M == 0) return LQ_OK;
   cudaStream_t st = (cudaStream_t)stream;
-  if (p->M > 16) return run_linear_tc(p, st);  // 5120 -> 2560 channels: 8 tokens 5.9 us here, 16 10.1, there 11.7 (8.4 from 32 on)
+  if (p->M > 16) return run_linear_tc(p, st);  // 5120 -> 2560 channels: 8 tokens 7.0 us here, 16 9.5, there 11.7 (7.9 from 32 on)
   return with_dtype(p->out_dtype, "int8_linear", [&](auto t) {
     using TO = decltype(t);
     return p->M <= 8 ? linear::launch_few<1, TO, int8_t, 1>(p, {}, st) : linear::launch_few<2, TO, int8_t, 1>(p, {}, st);
@@ -259,8 +274,9 @@ extern "C" int lq_int8_linear_values(const lq_linear_problem* p, const void* val
   if (p->M == 0) return LQ_OK;
   if (!values) return fail(LQ_ERR_NULL, "int8_linear_values: values is null");
   cudaStream_t st = (cudaStream_t)stream;
-  // up to eight tokens whose codes fit a CTA's shared memory next to the weights
-  if (p->M > 8 || (long long)p->M * linear::code_pitch(p->K) > 128 * 1024) {
+  // up to eight tokens whose codes fit a CTA's shared memory next to the weights: one launch, and 8.1 us against 9.5 (1 token), 10.8
+  // against 10.2 (5), 11.3 against 10.2 (8) at 5120 -> 2560, where the host's 2 us for another launch are not counted
+  if (p->M > 8 || (long long)p->M * linear::code_pitch(p->K) > 120 * 1024) {
     if (int e = lq_quantize_rows(values, dtype, p->M, p->K, stride, const_cast<int8_t*>(p->x), p->x_stride, const_cast<float*>(p->x_scale), stream)) return e;
     return lq_int8_linear(p, stream);
   }

@@ -351,6 +351,10 @@ __global__ void __launch_bounds__(THREADS, 2) int8_linear_split_kernel(const __g
   asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
   const uint32_t tbase = lds_u32(s_tbase);
   bool ok = true;
+  // thread tid adds the pieces rank 256 + tid + 256 parts i of four columns: the same columns each time
+  constexpr int PIECES = S::BN / 4, MOST = BM * PIECES / (2 * 32 * OUT_WARPS);
+  const int c = tid % PIECES * 4, row0 = rank * (32 * OUT_WARPS / PIECES) + tid / PIECES, rows_a_round = parts * (32 * OUT_WARPS / PIECES);
+  float ws[4], bias[4], xs[MOST];
 
   if (warp == OUT_WARPS) {
     if (lane == 0) {
@@ -381,6 +385,14 @@ __global__ void __launch_bounds__(THREADS, 2) int8_linear_split_kernel(const __g
     }
   } else {  // sums to shared memory: the stages are free once the last product is done
     const int quad = warp & 3, c0 = (warp >> 2) * 32;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const bool in = n0 + c + j < p.N;
+      ws[j] = in ? __ldg(p.w_scale + n0 + c + j) : 0.f;
+      bias[j] = in && p.bias ? __ldg(p.bias + n0 + c + j) : 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < MOST; ++i) xs[i] = row0 + i * rows_a_round < rows ? __ldg(p.x_scale + m0 + row0 + i * rows_a_round) : 0.f;
     ok = __all_sync(0xffffffffu, mbar_wait_bounded(s_acc, 0));
     asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
     if (ok && 32 * quad < rows) {
@@ -398,23 +410,20 @@ __global__ void __launch_bounds__(THREADS, 2) int8_linear_split_kernel(const __g
   cluster_sync();  // the sums of all are there
   if (warp == OUT_WARPS + 1) tmem_free<false>(tbase, S::BN);
   else if (warp < OUT_WARPS) {
-    constexpr int PIECES = S::BN / 4;
     TO* y = reinterpret_cast<TO*>(p.y);
     const bool wide = p.N % 4 == 0 && (reinterpret_cast<uintptr_t>(p.y) & (4 * sizeof(TO) - 1)) == 0;
-    for (int i = rank * 32 * OUT_WARPS + tid; i < rows * PIECES; i += parts * 32 * OUT_WARPS) {
-      const int row = i / PIECES, c = i % PIECES * 4, n = n0 + c;
-      if (n >= p.N) continue;
+#pragma unroll
+    for (int i = 0; i < MOST; ++i) {
+      const int row = row0 + i * rows_a_round, n = n0 + c;
+      if (row >= rows || n >= p.N) continue;
       int4 sum = make_int4(0, 0, 0, 0);
+#pragma unroll 4
       for (int q = 0; q < parts; ++q) {
         const int4 v = ld_cluster(in_cta(s_stage + row * S::PITCH + 4 * c, q));
         sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
       }
-      const float xs = __ldg(p.x_scale + m0 + row);
-      const int v[4] = {sum.x, sum.y, sum.z, sum.w};
-      float f[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        f[j] = n + j < p.N ? fmaf((float)v[j] * xs, __ldg(p.w_scale + n + j), p.bias ? __ldg(p.bias + n + j) : 0.f) : 0.f;
+      const float f[4] = {fmaf((float)sum.x * xs[i], ws[0], bias[0]), fmaf((float)sum.y * xs[i], ws[1], bias[1]), fmaf((float)sum.z * xs[i], ws[2], bias[2]),
+                          fmaf((float)sum.w * xs[i], ws[3], bias[3])};
       TO* to = y + (size_t)(m0 + row) * p.N + n;
       if (wide) {
         Pack<TO, 4> out;
