@@ -6,7 +6,7 @@
 // behind the last row and the last byte of K) into a ring of stages, one thread issues tcgen05.mma.kind::i8 (four steps of 32 per
 // stage) into one of two accumulators in tensor memory, and eight warps turn the other one into outputs meanwhile: INT32 to fp32,
 // both scales and the bias, through a swizzled 64-byte row per lane in shared memory, stored as pieces of 64 bytes a row.
-// Bound by the tensor pipe: 8192^3 339 us (3.24 POP/s; 366 us without pairs), 32768 x 2560 -> 10576 688 us (2.58), where what
+// Bound by the tensor pipe: 8192^3 339 us (3.24 POP/s; 366 us without pairs), 32768 x 2560 -> 10576 654 to 705 us (2.7 to 2.5, by the box's power), where what
 // torch's INT8 product reaches is 2.94 with INT32 outputs and no scales.
 // Every wait is bounded; on expiry the CTA raises the status word, lets its copies and products land, frees its tensor
 // memory and returns.

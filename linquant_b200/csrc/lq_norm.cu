@@ -7,7 +7,7 @@
 //   INT8 codes with one scale a row (amax / 127).
 //
 // Memory-bound: every input is read once into registers (VEC values a load, NV loads a thread), the sums of a row are taken
-// in fp32 by the team of threads that holds it, and y, r and the codes are written once.
+// in fp32 by the team of threads that holds it, and y, r and the codes are written once: gated norm of 32768 x 5120 bf16 182 us (5.5 TB/s; 209 with INT8 outputs), residual and norm of 16384 x 2560 56.6 us (5.9).
 #include "lq_layer.cuh"
 
 namespace lq {
