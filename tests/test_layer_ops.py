@@ -531,3 +531,19 @@ def test_int8_linear_long_rows(M, K, N, out):
     # the sum rounds to fp32, scales that are powers of two round nothing, then one rounding to the output
     assert torch.equal(y, (want.float() * 2.0**-15).to(out))
     assert torch.equal(y, int8_linear_fwd(padded(x), padded(w), one_n * 2.0**-12, x_scale=one_m * 2.0**-3, out_dtype=out))
+
+
+@pytest.mark.parametrize("heads", [False, True])
+def test_steps_of_no_sequences(heads):
+    from linquant_b200.kernels.layer import selective_scan_step, short_conv_step
+
+    state = randn(3, 4, 8, 16) if heads else randn(3, 32, 16)
+    before = state.clone()
+    u = torch.empty(0, 4, 8, device="cuda", dtype=BF16) if heads else torch.empty(0, 32, device="cuda", dtype=BF16)
+    dt = torch.empty(0, 4, device="cuda", dtype=BF16) if heads else u
+    A = -torch.rand(4, device="cuda") if heads else -torch.rand(32, 16, device="cuda")
+    none = torch.empty(0, 1, 16, device="cuda", dtype=BF16)
+    assert selective_scan_step(state, u, dt, A, none, none).shape == u.shape and torch.equal(state, before)
+    x, line = torch.empty(0, 8, device="cuda", dtype=BF16), torch.zeros(2, 3, 8, device="cuda", dtype=BF16)
+    assert short_conv_step(x, line, torch.ones(8, 4, device="cuda")).shape == x.shape
+    torch.cuda.synchronize()
