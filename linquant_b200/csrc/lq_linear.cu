@@ -221,13 +221,19 @@ __global__ void __launch_bounds__(std::is_same_v<TX, int8_t> ? 256 : 512, 2) int
   }
 }
 
+constexpr int CODES = 120 * 1024;  // bytes of codes that a CTA makes at most, next to the weights
+
+// The opt-in to shared memory is a kernel's most and not what a call needs: it belongs to the kernel on its device, and another
+// thread's smaller call between this one's opt-in and its launch would have the launch refused.
 template <int MT, typename TO, typename TX, int PV>
 static int launch_few(const lq_linear_problem* p, const Values& v, cudaStream_t st) {
-  const size_t smem = 2 * 16 * WP + (std::is_same_v<TX, int8_t> ? 0 : (size_t)p->M * code_pitch(p->K));
+  constexpr bool VALUES = !std::is_same_v<TX, int8_t>;
+  constexpr int most_smem = 2 * 16 * WP + (VALUES ? CODES : 0);
+  const size_t smem = 2 * 16 * WP + (VALUES ? (size_t)p->M * code_pitch(p->K) : 0);
   auto kern = int8_linear_few_kernel<MT, TO, TX, PV>;
-  const int threads = std::is_same_v<TX, int8_t> ? 256 : 512;
+  const int threads = VALUES ? 512 : 256;
   int per_sm = 0;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, most_smem);
   if (e == cudaSuccess) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, threads, smem);
   if (e == cudaSuccess) {
     const int tiles = (p->N + 15) / 16, most = sm_count() * per_sm;
@@ -276,7 +282,7 @@ extern "C" int lq_int8_linear_values(const lq_linear_problem* p, const void* val
   cudaStream_t st = (cudaStream_t)stream;
   // up to eight tokens whose codes fit a CTA's shared memory next to the weights: one launch, and 8.1 us against 9.5 (1 token), 10.8
   // against 10.2 (5), 11.3 against 10.2 (8) at 5120 -> 2560, where the host's 2 us for another launch are not counted
-  if (p->M > 8 || (long long)p->M * linear::code_pitch(p->K) > 120 * 1024) {
+  if (p->M > 8 || (long long)p->M * linear::code_pitch(p->K) > linear::CODES) {
     if (int e = lq_quantize_rows(values, dtype, p->M, p->K, stride, const_cast<int8_t*>(p->x), p->x_stride, const_cast<float*>(p->x_scale), stream)) return e;
     return lq_int8_linear(p, stream);
   }

@@ -14,6 +14,8 @@ namespace lq {
 
 namespace norm {
 
+constexpr int MOST = 16384;  // channels that are normed together
+
 enum Kind { PLAIN, ADD, ADD32, GATED };  // ADD32: the residual stream in fp32
 
 // A team holds one row (or group): a power of two up to 32 lanes of a warp, or all warps of the CTA.
@@ -333,8 +335,11 @@ static int launch_as(const lq_norm_problem* p, int packs, cudaStream_t st) {
   int per_sm = 0;
   auto kern = norm_kernel<T, VEC, NV, KIND, OFF>;
   const int params = (p->weight != nullptr) + (p->post_weight != nullptr) + (p->scale_vec != nullptr);
-  const int smem = OFF ? params * (int)Params<VEC, OFF>::slots(p->D) * (int)sizeof(float) : 0;  // three of 16384: 198 KB
-  cudaError_t e = OFF ? cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) : cudaSuccess;
+  // The opt-in is the most that any call needs (198 KB): it belongs to the kernel on its device, and another thread's smaller call
+  // between this one's opt-in and its launch would have the launch refused.
+  const int smem = OFF ? params * (int)Params<VEC, OFF>::slots(p->D) * (int)sizeof(float) : 0;
+  constexpr int most_smem = 3 * (int)Params<VEC, OFF>::slots(MOST) * (int)sizeof(float);
+  cudaError_t e = OFF ? cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, most_smem) : cudaSuccess;
   if (e == cudaSuccess) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, threads, smem);
   if (e != cudaSuccess) return fail(LQ_ERR_LAUNCH, "norm: %s", cudaGetErrorString(e));
   const long long most = (long long)sm_count() * per_sm;
@@ -349,7 +354,7 @@ static int launch_vec(const lq_norm_problem* p, cudaStream_t st) {
   const int packs = (p->group + VEC - 1) / VEC + OFF;
   if constexpr (VEC == 1) {
     if (packs <= 1024) return launch_as<T, KIND, 1, 4, OFF>(p, packs, st);
-    if (packs <= 16384) return launch_as<T, KIND, 1, 32, OFF>(p, packs, st);
+    if (packs <= MOST) return launch_as<T, KIND, 1, 32, OFF>(p, packs, st);
   } else if constexpr (OFF) {
     if (packs <= 384) return launch_as<T, KIND, VEC, 1, OFF>(p, packs, st);
     if (packs <= 640) return launch_as<T, KIND, VEC, 2, OFF>(p, packs, st);
@@ -359,7 +364,7 @@ static int launch_vec(const lq_norm_problem* p, cudaStream_t st) {
     if (packs <= 640) return launch_as<T, KIND, VEC, 2, OFF>(p, packs, st);
     if (packs <= 512 * 32 / VEC) return launch_as<T, KIND, VEC, 32 / VEC, OFF>(p, packs, st);
   }
-  return fail(LQ_ERR_UNSUPPORTED, "norm over %d channels (at most 16384)", p->group);
+  return fail(LQ_ERR_UNSUPPORTED, "norm over %d channels (at most %d)", p->group, MOST);
 }
 template <typename T, Kind KIND>
 static int run_kind(const lq_norm_problem* p, cudaStream_t st) {
@@ -379,7 +384,7 @@ static int run_kind(const lq_norm_problem* p, cudaStream_t st) {
     auto alike = [&](const void* t, long long pitch, int size) {
       return t == nullptr || (size == S && ((pitch - p->x_stride) * S & 15) == 0 && ((reinterpret_cast<uintptr_t>(t) ^ reinterpret_cast<uintptr_t>(p->x)) & 15) == 0);
     };
-    if (p->group == p->D && p->D <= 16384 - FULL && alike(p->gate, p->gate_stride, S) && alike(p->residual, p->residual_stride, S) &&
+    if (p->group == p->D && p->D <= MOST - FULL && alike(p->gate, p->gate_stride, S) && alike(p->residual, p->residual_stride, S) &&
         alike(p->residual_out, p->D, S) && alike(p->y, p->D, so))
       return launch_vec<T, KIND, FULL, true>(p, st);
   }
