@@ -204,9 +204,10 @@ static int launch_state_tc(const lq_ssd_problem* p, int* status, cudaStream_t st
   CUresult r = enc(&tm, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, p->q_BT, gdim, gstride, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                    CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return fail(LQ_ERR_LAUNCH, "chunk_state: cuTensorMapEncodeTiled failed with CUresult %d", (int)r);
-  const int KB = C / 128;
-  const size_t smem = (size_t)KB * 8192 + (size_t)C * 128 + sizeof(float) * C + 64 + 1024;  // N <= 128: the B tiles fit the x region
-  cudaError_t e = cudaFuncSetAttribute(ssd_chunk_state_tc_kernel<T, N>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  auto bytes = [](int chunk) { return (size_t)(chunk / 128) * 8192 + (size_t)chunk * 128 + sizeof(float) * chunk + 64 + 1024; };  // N <= 128: the B tiles fit the x region
+  const size_t smem = bytes(C);
+  // the opt-in belongs to the kernel on its device: the most that a chunk takes, so that no other thread's call lowers it before this launch
+  cudaError_t e = cudaFuncSetAttribute(ssd_chunk_state_tc_kernel<T, N>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes(256));
   if (e != cudaSuccess) return fail(LQ_ERR_LAUNCH, "chunk_state: shared memory opt-in failed: %s", cudaGetErrorString(e));
   dim3 grid(NC, p->H, p->B);
   launch(ssd_chunk_state_tc_kernel<T, N>, grid, 128, smem, st, tm, *p, status);

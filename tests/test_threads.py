@@ -10,7 +10,7 @@ from linquant_b200 import _cabi
 
 pytestmark = pytest.mark.gpu
 
-CALLS = 5000  # where each call's own size was opted in to, 5 to 18 % of the larger ones were refused
+CALLS = 5000  # where each call's own size is opted in to, 0.4 to 18 % of the larger ones are refused
 
 
 def run(calls):
@@ -61,3 +61,23 @@ def norm(D, post, rows=3):
 @pytest.mark.parametrize("calls", [lambda: (product(64), product(14000)), lambda: (norm(5201, False), norm(15001, True))], ids=["product", "norm"])
 def test_layer_operators(calls):
     assert run(calls()) == []
+
+
+def chunk_state(chunk, L=256, H=2, N=64):
+    """Chunk states of Mamba-2 by way of the transposed codes of B: a chunk's rows lie in shared memory."""
+    from linquant_b200.kernels.mamba2 import _ssd
+
+    nc = L // chunk
+    x, q = torch.randn(1, L, H, 64, device="cuda").half(), torch.ones(1, L, 1, N, device="cuda", dtype=torch.int8)
+    dt, dA, one = torch.rand(1, H, nc, chunk, device="cuda"), torch.zeros(1, H, nc, chunk, device="cuda"), torch.ones(H, 64, device="cuda")
+    call = _ssd.Call(x.device).dims(B=1, L=L, H=H, P=64, G=1, N=N, chunk=chunk)
+    call.x(x)
+    for name, t in (("q_B", q), ("q_BT", torch.empty_like(q)), ("dt", dt), ("dA", dA), ("alpha_hp", one), ("state_scale", one), ("bscale_g", one),
+                    ("states", torch.empty(1, nc, H, 64, N, device="cuda", dtype=torch.int8))):
+        call.put(name, t)
+    fn = entry("lq_ssd_chunk_state_value", C.POINTER(_ssd.SsdProblem))
+    return lambda stream: fn(C.byref(call.p), stream)
+
+
+def test_chunk_states():
+    assert run((chunk_state(128), chunk_state(256))) == []
