@@ -323,6 +323,48 @@ __global__ void __launch_bounds__(NV == 1 && !OFF || NV * VEC == 4 ? 1024 : NV =
   }
 }
 
+// Codes of rows longer than a CTA's registers hold: a CTA a row, which is read twice, the second time out of L2: 8192 x
+// 28672 bf16 123 us (5.7 TB/s of one read and the codes), 8192 x 28673, a value a load, 277 us.
+template <typename T, int VEC>
+__global__ void __launch_bounds__(512) quantize_long_kernel(const lq_norm_problem p) {
+  pdl_enter();
+  __shared__ float2 sm[2 * 32];
+  Team team{512, sm};
+  for (long long row = blockIdx.x; row < p.rows; row += gridDim.x) {
+    const T* x = reinterpret_cast<const T*>(p.x) + row * p.x_stride;
+    int8_t* out = p.codes + row * p.codes_stride;
+    float v[VEC], none = 0.f, amax = 0.f;
+#pragma unroll 4
+    for (int c = threadIdx.x * VEC; c < p.D; c += 512 * VEC) {
+      load_pack<T, VEC>(x + c).get(v);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) amax = max_nan(amax, fabsf(v[i]));
+    }
+    team.template reduce<false, true>(none, amax);
+    float inv;
+    const float scale = row_scale(amax, inv);
+    if (threadIdx.x == 0) p.scale[row] = scale;
+#pragma unroll 4
+    for (int c = threadIdx.x * VEC; c < p.D; c += 512 * VEC) {
+      load_pack<T, VEC>(x + c).get(v);
+      Pack<int8_t, VEC> q;
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) q.v[i] = (int8_t)row_code(v[i], inv);
+      store_pack(out + c, q);
+    }
+  }
+}
+template <typename T>
+static int run_long(const lq_norm_problem* p, cudaStream_t st) {
+  constexpr int FULL = 16 / sizeof(T);
+  Alignment a;
+  const bool wide = a.at(p->x).pitch(p->x_stride, sizeof(T)).pitch(p->D, sizeof(T)).bytes() == 16;
+  const int most = 4 * sm_count(), ctas = p->rows < most ? p->rows : most;
+  if (wide) launch(quantize_long_kernel<T, FULL>, dim3(ctas), dim3(512), 0, st, *p);
+  else launch(quantize_long_kernel<T, 1>, dim3(ctas), dim3(512), 0, st, *p);
+  return check_launch("quantize_long_kernel");
+}
+
 template <typename T, Kind KIND, int VEC, int NV, bool OFF>
 static int launch_as(const lq_norm_problem* p, int packs, cudaStream_t st) {
   const int need = (packs + NV - 1) / NV;
@@ -395,7 +437,7 @@ static int run(const lq_norm_problem* p, Form form, const char* what, cudaStream
   return with_dtype(p->dtype, what, [&](auto t) {
     using T = decltype(t);
     if (form == GATE) return run_kind<T, GATED>(p, st);
-    if (form == CODES) return run_kind<T, PLAIN>(p, st);
+    if (form == CODES) return p->D > MOST ? run_long<T>(p, st) : run_kind<T, PLAIN>(p, st);
     if constexpr (!std::is_same_v<T, float>) {
       if (p->residual && p->residual_f32) return run_kind<T, ADD32>(p, st);
     }

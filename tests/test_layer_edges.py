@@ -1,0 +1,59 @@
+"""Layer operators at the ends of what they take: long rows, empty batches, integers and shapes that do not fit."""
+
+import pytest
+import torch
+
+from tests import layer_reference as ref
+
+F16, BF16, F32 = torch.float16, torch.bfloat16, torch.float32
+ULP = 2.0**-24
+INF = float("inf")
+gpu = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True)
+def seed():
+    torch.manual_seed(11)
+
+
+def randn(*shape, dtype=F32):
+    return torch.randn(*shape, device="cuda").to(dtype)
+
+
+def ints(*v):
+    return torch.tensor(v, dtype=torch.int32, device="cuda")
+
+
+def int_codes(n, k):
+    return torch.randint(-128, 128, (n, k), device="cuda", dtype=torch.int8)
+
+
+# ------------------------------------------------------------------------------------- rows of more than 16384 channels
+@gpu
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("rows,K,pad", [(5, 16385, 0), (700, 16392, 0), (4, 20000, 1), (3, 28672, 8), (2, 131071, 0)])
+def test_codes_of_long_rows(rows, K, pad, dtype):
+    from linquant_b200.kernels.layer import quantize_rows_fwd
+
+    x = randn(rows, K + pad, dtype=dtype)[:, :K]
+    x[0] = 0
+    codes, scale = quantize_rows_fwd(x)
+    ref.check_codes(codes, scale, x.double().cpu())
+    x[1, 3], x[1, K - 1] = INF, float("nan")
+    _, scale = quantize_rows_fwd(x)
+    assert not torch.isfinite(scale[1]) and torch.isfinite(scale[2:]).all() and scale[0] == 0
+
+
+@gpu
+@pytest.mark.parametrize("K", [16385, 20000, 131071])
+@pytest.mark.parametrize("M", [1, 7, 8, 9, 40])
+def test_product_of_long_rows_from_values(M, K):
+    """Whatever kernel makes the codes, the product is the one of codes that were made ahead."""
+    from linquant_b200.kernels.layer import int8_linear_fwd, quantize_rows_fwd
+
+    x, (w, sw) = randn(M, K, dtype=BF16), quantize_rows_fwd(randn(24, K))
+    codes, scale = quantize_rows_fwd(x)
+    y = int8_linear_fwd(x, w, sw, out_dtype=F32)
+    assert torch.equal(y, int8_linear_fwd(codes, w, sw, x_scale=scale, out_dtype=F32))
+    want = (codes.double() @ w.double().t()) * scale.double()[:, None] * sw.double()
+    ref.check(y, want, want.abs(), 4 * ULP)
