@@ -162,7 +162,7 @@ __global__ void __launch_bounds__(128) short_conv_step_kernel(const lq_conv_prob
 
 static int check(const lq_conv_problem* p, bool step, const char* what) {
   if (!p) return fail(LQ_ERR_NULL, "%s: problem descriptor is null", what);
-  if (p->B < 0 || p->T < 0 || p->D <= 0) return fail(LQ_ERR_SHAPE, "%s: B=%d T=%d D=%d", what, p->B, p->T, p->D);
+  if (p->B < 0 || p->T < 0 || p->D <= 0 || !fits(p->T) || !fits(p->D)) return fail(LQ_ERR_SHAPE, "%s: B=%d T=%d D=%d", what, p->B, p->T, p->D);
   if (p->W < 2 || p->W > 4) return fail(LQ_ERR_UNSUPPORTED, "%s: %d taps (2, 3 or 4)", what, p->W);
   if (p->dtype < LQ_F16 || p->dtype > LQ_F32) return fail(LQ_ERR_UNSUPPORTED, "%s: dtype %d", what, p->dtype);
   if (!p->weight || ((!p->x || !p->y) && (long long)p->B * p->T > 0)) return fail(LQ_ERR_NULL, "%s: x, weight and y must be non-null", what);

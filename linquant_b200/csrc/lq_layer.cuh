@@ -115,6 +115,8 @@ static inline int with_dtype(int dtype, const char* what, F&& f) {
   return fail(LQ_ERR_UNSUPPORTED, "%s: dtype %d", what, dtype);
 }
 static inline int dtype_bytes(int dtype) { return dtype == LQ_F32 ? 4 : 2; }
+// Extents leave room in an int for the tile that holds an axis' end and the tiles requested ahead of it
+static inline bool fits(int extent) { return extent <= 0x7fffffff - (1 << 13); }
 // largest power of two (16 at most) that divides every address and byte pitch it is shown
 struct Alignment {
   uintptr_t bits = 16;

@@ -245,7 +245,7 @@ static int launch_few(const lq_linear_problem* p, const Values& v, cudaStream_t 
 
 static int check(const lq_linear_problem* p) {
   if (!p) return fail(LQ_ERR_NULL, "int8_linear: problem descriptor is null");
-  if (p->M < 0 || p->N <= 0 || p->K <= 0 || p->K > 131071) return fail(LQ_ERR_SHAPE, "int8_linear: M=%d N=%d K=%d", p->M, p->N, p->K);
+  if (p->M < 0 || p->N <= 0 || p->K <= 0 || p->K > 131071 || !fits(p->M) || !fits(p->N)) return fail(LQ_ERR_SHAPE, "int8_linear: M=%d N=%d K=%d", p->M, p->N, p->K);
   if (p->out_dtype < LQ_F16 || p->out_dtype > LQ_F32) return fail(LQ_ERR_UNSUPPORTED, "int8_linear: dtype %d", p->out_dtype);
   if (p->M == 0) return LQ_OK;
   if (!p->x || !p->w || !p->x_scale || !p->w_scale || !p->y) return fail(LQ_ERR_NULL, "int8_linear: x, w, their scales and y must be non-null");

@@ -447,7 +447,7 @@ static int run(const lq_norm_problem* p, Form form, const char* what, cudaStream
 
 static int check(const lq_norm_problem* p, const char* what) {
   if (!p) return fail(LQ_ERR_NULL, "%s: problem descriptor is null", what);
-  if (p->rows < 0 || p->D <= 0 || p->group <= 0 || p->D % p->group) return fail(LQ_ERR_SHAPE, "%s: rows=%d D=%d group=%d", what, p->rows, p->D, p->group);
+  if (p->rows < 0 || p->D <= 0 || p->group <= 0 || p->D % p->group || !fits(p->D)) return fail(LQ_ERR_SHAPE, "%s: rows=%d D=%d group=%d", what, p->rows, p->D, p->group);
   if (p->dtype < LQ_F16 || p->dtype > LQ_F32 || p->out_dtype < LQ_F16 || p->out_dtype > LQ_F32)
     return fail(LQ_ERR_UNSUPPORTED, "%s: dtype %d -> %d", what, p->dtype, p->out_dtype);
   if (p->rows > 0 && !p->x) return fail(LQ_ERR_NULL, "%s: x is null", what);

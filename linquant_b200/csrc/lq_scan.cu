@@ -761,7 +761,7 @@ static int run_step(const lq_scan_problem* p, cudaStream_t st) {
 
 static int check(const lq_scan_problem* p, bool step, const char* what) {
   if (!p) return fail(LQ_ERR_NULL, "%s: problem descriptor is null", what);
-  if (p->B < 0 || p->T < 0 || p->D <= 0 || p->G <= 0 || p->N <= 0 || p->D % p->G)
+  if (p->B < 0 || p->T < 0 || p->D <= 0 || p->G <= 0 || p->N <= 0 || p->D % p->G || !fits(p->T) || !fits(p->D))
     return fail(LQ_ERR_SHAPE, "%s: B=%d T=%d D=%d N=%d G=%d", what, p->B, p->T, p->D, p->N, p->G);
   if (p->N > 256) return fail(LQ_ERR_UNSUPPORTED, "%s: %d states a channel (at most 256)", what, p->N);
   if (p->dtype < LQ_F16 || p->dtype > LQ_F32) return fail(LQ_ERR_UNSUPPORTED, "%s: dtype %d", what, p->dtype);
@@ -769,7 +769,7 @@ static int check(const lq_scan_problem* p, bool step, const char* what) {
     return fail(LQ_ERR_NULL, "%s: u, dt, A, B, C and y must be non-null", what);
   if (!step) return p->H ? fail(LQ_ERR_UNSUPPORTED, "%s: one decay rate a head is for single tokens", what) : LQ_OK;
   if (p->T != 1) return fail(LQ_ERR_SHAPE, "%s: T=%d, one token expected", what, p->T);
-  if (p->H && (p->P <= 0 || p->H * p->P != p->D || p->H % p->G)) return fail(LQ_ERR_SHAPE, "%s: H=%d P=%d D=%d G=%d", what, p->H, p->P, p->D, p->G);
+  if (p->H && (p->P <= 0 || (long long)p->H * p->P != p->D || p->H % p->G)) return fail(LQ_ERR_SHAPE, "%s: H=%d P=%d D=%d G=%d", what, p->H, p->P, p->D, p->G);
   if (p->state_dtype < LQ_F16 || p->state_dtype > LQ_F32) return fail(LQ_ERR_UNSUPPORTED, "%s: state dtype %d", what, p->state_dtype);
   if (!p->state) return fail(LQ_ERR_NULL, "%s: state is null", what);
   if (!p->slots && p->n_slots < p->B) return fail(LQ_ERR_SHAPE, "%s: %d slots for %d sequences", what, p->n_slots, p->B);

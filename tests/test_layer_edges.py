@@ -57,3 +57,29 @@ def test_product_of_long_rows_from_values(M, K):
     assert torch.equal(y, int8_linear_fwd(codes, w, sw, x_scale=scale, out_dtype=F32))
     want = (codes.double() @ w.double().t()) * scale.double()[:, None] * sw.double()
     ref.check(y, want, want.abs(), 4 * ULP)
+
+
+# --------------------------------------------------------------------------------------------- extents near 2^31 - 1
+@pytest.mark.parametrize("entry,cls,axis", [
+    ("lq_short_conv_fwd", "ConvProblem", "T"), ("lq_short_conv_fwd", "ConvProblem", "D"), ("lq_short_conv_step", "ConvProblem", "D"),
+    ("lq_selective_scan_fwd", "ScanProblem", "T"), ("lq_selective_scan_fwd", "ScanProblem", "D"), ("lq_selective_scan_step", "ScanProblem", "D"),
+    ("lq_int8_linear", "LinearProblem", "M"), ("lq_int8_linear", "LinearProblem", "N"), ("lq_rms_norm", "NormProblem", "D")])
+def test_extents_that_tiles_would_overflow(entry, cls, axis):
+    """The number of an axis' tiles, and what is requested behind them, has to fit an int: refused ahead of any launch."""
+    import ctypes
+
+    from linquant_b200 import _cabi
+
+    p = getattr(_cabi, cls)()
+    for name, t in p._fields_:
+        if t is ctypes.c_void_p:
+            setattr(p, name, 4096)
+    values = dict(B=0, T=1, D=8, W=4, N=8, G=1, dtype=1, state_dtype=2, M=1, K=16, x_stride=16, w_stride=16, rows=0, group=8, out_dtype=1, codes_stride=16)
+    for name in values.keys() & {n for n, _ in p._fields_}:
+        setattr(p, name, values[name])
+    setattr(p, axis, 2**31 - 1)
+    if cls == "NormProblem":
+        p.group = p.D
+    fn = getattr(_cabi.lib(), entry)
+    fn.argtypes = [ctypes.POINTER(type(p)), ctypes.c_void_p]
+    assert fn(ctypes.byref(p), None) == 2
