@@ -40,13 +40,16 @@ def parameter(name, t, shape, like):
 
 
 def integers(name, t, n, like):
-    """Lengths and slots as the kernels read them: int32, dense, on the device."""
+    """Lengths and slots as the kernels read them: int32, dense, on the device. What int32 does not hold stays outside every
+    range on its side (behind the longest prompt, no slot)."""
     if t is None:
         return None
     t = torch.as_tensor(t)
     assert tuple(t.shape) == (n,), f"{name} has shape {tuple(t.shape)}, {(n,)} expected"
     if t.dtype.is_floating_point or t.dtype == torch.bool:
         raise NotImplementedError(f"{name} must be integers (got {t.dtype})")
+    if t.dtype == torch.int64:
+        t = t.clamp(-1, 2**31 - 1)
     return t.to(device=like.device, dtype=torch.int32).contiguous()
 
 

@@ -83,3 +83,23 @@ def test_extents_that_tiles_would_overflow(entry, cls, axis):
     fn = getattr(_cabi.lib(), entry)
     fn.argtypes = [ctypes.POINTER(type(p)), ctypes.c_void_p]
     assert fn(ctypes.byref(p), None) == 2
+
+
+# ------------------------------------------------------------------------------------------------- integers of 64 bits
+@gpu
+def test_lengths_and_slots_that_int32_does_not_hold():
+    """A length behind 2^31 is the whole prompt, one below 0 none of it; such slots are idle entries."""
+    from linquant_b200.kernels.layer import selective_scan_step, short_conv_fwd, short_conv_step
+
+    x, w = randn(3, 9, 32), randn(32, 4)
+    y, state = short_conv_fwd(x, w, lengths=torch.tensor([2**31 + 5, 2**32 + 4, -2**32 + 4], device="cuda"), output_final_state=True)
+    want, last = short_conv_fwd(x, w, lengths=ints(9, 9, 0), output_final_state=True)
+    assert torch.equal(y, want) and torch.equal(state, last)
+    slots = torch.tensor([2**32, -2**63, 2**31 + 1], device="cuda")
+    line = randn(4, 3, 32)
+    before = line.clone()
+    assert not short_conv_step(x[:, 0], line, w, slots=slots).any() and torch.equal(line, before)
+    h = randn(4, 32, 8)
+    before = h.clone()
+    B = randn(3, 1, 8)
+    assert not selective_scan_step(h, x[:, 0], x[:, 0], -torch.rand(32, 8, device="cuda"), B, B, slots=slots).any() and torch.equal(h, before)
