@@ -51,7 +51,7 @@ def selective_scan_step(state, u, dt, A, B, C, D=None, z=None, dt_bias=None, dt_
         assert u.dim() in (2, 3) and B.dim() == 3, "u is (b,d) or (b,H,P), B and C are (b,G,N)"
         b, (G, N), ch = u.shape[0], B.shape[1:], tuple(u.shape[1:])
         heads = u.dim() == 3
-        flat = lambda name, t: None if t is None else _layer.activation(name, t, u.shape, u).reshape(b, -1).view(u.shape)  # noqa: E731
+        flat = lambda name, t: None if t is None else _layer.activation(name, t, u.shape, u).flatten(1).view(u.shape)  # noqa: E731
         if D is not None and heads and D.dim() == 2:
             D = D.expand(ch)
         r = _cabi.host().selective_scan_step(

@@ -103,3 +103,31 @@ def test_lengths_and_slots_that_int32_does_not_hold():
     before = h.clone()
     B = randn(3, 1, 8)
     assert not selective_scan_step(h, x[:, 0], x[:, 0], -torch.rand(32, 8, device="cuda"), B, B, slots=slots).any() and torch.equal(h, before)
+
+
+# ----------------------------------------------------------------------------------------------------- empty batches
+@gpu
+@pytest.mark.parametrize("heads", [False, True])
+def test_steps_of_no_sequences_in_other_types(heads):
+    """Slots of 64 bits are converted, also where there are none."""
+    from linquant_b200.kernels.layer import selective_scan_step
+
+    state = randn(3, 4, 8, 16) if heads else randn(3, 32, 16)
+    before = state.clone()
+    u = torch.empty(0, 4, 8, device="cuda") if heads else torch.empty(0, 32, device="cuda")
+    dt = torch.empty(0, 4, device="cuda") if heads else u
+    A = -torch.rand(4, device="cuda") if heads else -torch.rand(32, 16, device="cuda")
+    none, slots = torch.empty(0, 1, 16, device="cuda"), torch.empty(0, dtype=torch.int64, device="cuda")
+    y = selective_scan_step(state, u, dt, A, none, none, z=torch.empty_like(u), slots=slots)
+    assert y.shape == u.shape and torch.equal(state, before)
+
+
+@gpu
+def test_a_gate_of_heads_in_another_order():
+    """Channels of a token that are not contiguous are copied."""
+    from linquant_b200.kernels.layer import selective_scan_step
+
+    state, u, z = randn(2, 3, 4, 16), randn(2, 3, 4), randn(2, 4, 3).transpose(1, 2)
+    dt, A, B = randn(2, 3), -torch.rand(3, device="cuda"), randn(2, 1, 16)
+    s1, s2 = state.clone(), state.clone()
+    assert torch.equal(selective_scan_step(s1, u, dt, A, B, B, z=z), selective_scan_step(s2, u, dt, A, B, B, z=z.contiguous())) and torch.equal(s1, s2)
