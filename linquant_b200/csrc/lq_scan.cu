@@ -517,6 +517,11 @@ static int run(const lq_scan_problem* p, cudaStream_t st) {
 }
 
 // ------------------------------------------------------------------------------------------------ one token
+// exp(dt A), as accurate as in the prompt's kernel: with fp32 inputs the rounding of a product with log2(e) would be the largest
+// error of a step (60 ulps at dt A = -75)
+template <typename T>
+__device__ __forceinline__ float step_decay(float dt, float A) { return sizeof(T) == 4 ? expf(dt * A) : ex2(dt * kLog2e * A); }
+
 // A row is the N states of one channel. LPR lanes hold it, VEC states each per step over N; a thread group takes R rows of
 // one head (HEADS: they share the decay, B and C) or one row with a decay rate per state.
 template <typename T, typename TS, int VEC, int R, bool HEADS>
@@ -576,13 +581,13 @@ __global__ void __launch_bounds__(128) selective_scan_step_kernel(const lq_scan_
 #pragma unroll
   for (int r = 0; r < R; ++r) acc[r] = 0.f;
   if (on) {
-    const float head_decay = HEADS ? ex2(dt * kLog2e * A[0]) : 0.f;
+    const float head_decay = HEADS ? step_decay<T>(dt, A[0]) : 0.f;
     for (int n = ln * VEC; n < p.N;) {
       float Bv[VEC], Cv[VEC], a[VEC];
       rB.get(Bv);
       rC.get(Cv);
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) a[i] = HEADS ? head_decay : ex2(dt * kLog2e * A[HEADS ? 0 : i]);
+      for (int i = 0; i < VEC; ++i) a[i] = HEADS ? head_decay : step_decay<T>(dt, A[HEADS ? 0 : i]);
 #pragma unroll
       for (int r = 0; r < R; ++r) {
         float h[VEC];
@@ -665,7 +670,7 @@ __global__ void __launch_bounds__(128) heads_step_kernel(const lq_scan_problem p
   if (on) {
     float dt = to_f32(reinterpret_cast<const T*>(p.dt)[b * p.dt_stride_b + head]) + (p.dt_bias ? p.dt_bias[head] : 0.f);
     dt = clamp_nan(p.softplus ? softplus(dt) : dt, p.dt_min, p.dt_max);
-    decay = ex2(dt * kLog2e * p.A[head]);
+    decay = step_decay<T>(dt, p.A[head]);
 #pragma unroll
     for (int i = 0; i < VEC; ++i) Bv[i] *= dt;
   }

@@ -131,3 +131,21 @@ def test_a_gate_of_heads_in_another_order():
     dt, A, B = randn(2, 3), -torch.rand(3, device="cuda"), randn(2, 1, 16)
     s1, s2 = state.clone(), state.clone()
     assert torch.equal(selective_scan_step(s1, u, dt, A, B, B, z=z), selective_scan_step(s2, u, dt, A, B, B, z=z.contiguous())) and torch.equal(s1, s2)
+
+
+# ---------------------------------------------------------------------------------------------- decay of fp32 inputs
+@gpu
+@pytest.mark.parametrize("form", ["channels", "heads of 4", "heads of 3"])
+def test_decay_of_a_step_is_that_of_expf(form):
+    """dt A is a multiple of 1/8, exact in fp32: what is left is the exponential (1 ulp, 2^-23 of it) and the product with the
+    state (half of one)."""
+    from linquant_b200.kernels.layer import selective_scan_step
+
+    n, N = 64, 16
+    A = -torch.randint(1, 600, (n, N) if form == "channels" else (n,), device="cuda") / 4.0
+    lead = () if form == "channels" else (int(form[-1]),)
+    state, u = torch.ones(1, n, *lead, N, device="cuda"), torch.zeros(1, n, *lead, device="cuda")
+    B = randn(1, 1, N)
+    selective_scan_step(state, u, torch.full((1, n), 0.5, device="cuda"), A, B, B, dt_softplus=False)
+    want = torch.exp(0.5 * A.double()).view(n, *([1] * (state.dim() - 1 - A.dim())), *A.shape[1:])
+    assert ((state[0].double() - want).abs() <= 3 * ULP * want).all()
