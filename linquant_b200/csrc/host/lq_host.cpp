@@ -727,6 +727,7 @@ PyObject* int8_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
       p.x = x.const_data_ptr<int8_t>();
       p.x_stride = aligned_rows(x, xr);
       if (a[3] == Py_None) throw NotPlain{};
+      if (x.dim() == 1 && Call::tensor(a[3]).numel() != 1) throw NotPlain{};  // f32 takes any shape for one that has no axes
       p.x_scale = c.f32(a[3], lead_of(x), true);
     } else {
       dt = out_code(ot = x.scalar_type());

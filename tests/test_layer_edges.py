@@ -149,3 +149,19 @@ def test_decay_of_a_step_is_that_of_expf(form):
     selective_scan_step(state, u, torch.full((1, n), 0.5, device="cuda"), A, B, B, dt_softplus=False)
     want = torch.exp(0.5 * A.double()).view(n, *([1] * (state.dim() - 1 - A.dim())), *A.shape[1:])
     assert ((state[0].double() - want).abs() <= 3 * ULP * want).all()
+
+
+# -------------------------------------------------------------------------------------------------------- single rows
+@gpu
+def test_scale_of_a_single_row():
+    """A row of codes without leading axes has one scale."""
+    from linquant_b200.kernels.layer import int8_linear_fwd, quantize_rows_fwd
+
+    w, sw = int_codes(4, 32), torch.rand(4, device="cuda")
+    codes, scale = quantize_rows_fwd(randn(32))
+    want = int8_linear_fwd(codes.view(1, 32), w, sw, x_scale=scale.view(1), out_dtype=F32)[0]
+    for s in (scale, scale.view(1)):
+        assert torch.equal(int8_linear_fwd(codes, w, sw, x_scale=s, out_dtype=F32), want)
+    for wrong in (torch.ones(5, device="cuda"), torch.ones(0, device="cuda")):
+        with pytest.raises(AssertionError):
+            int8_linear_fwd(codes, w, sw, x_scale=wrong)
