@@ -383,7 +383,8 @@ __global__ void __launch_bounds__(RT + 512, 1) selective_scan_kernel(const __gri
   using S = Shape<T, RT, SPT, LP, ST, TT>;
   extern __shared__ __align__(128) uint8_t smem_raw[];
   typename S::Smem& sm = *reinterpret_cast<typename S::Smem*>(smem_raw + ((128 - (smem_u32(smem_raw) & 127)) & 127));
-  const int b = blockIdx.z, grp = blockIdx.y, Dg = p.D / p.G, ch0 = blockIdx.x * S::CH;  // ch0: within the group
+  const int Dg = p.D / p.G, blocks = (Dg + S::CH - 1) / S::CH, row = blockIdx.x / blocks, b = row / p.G, grp = row - b * p.G;
+  const int ch0 = ((int)blockIdx.x - row * blocks) * S::CH;  // within the group
   if (threadIdx.x == 0) {
     for (int i = 0; i < ST; ++i) asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;\n" ::"r"(smem_u32(&sm.full[i])));
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
@@ -457,8 +458,8 @@ static int launch_scan(const lq_scan_problem* p, cudaStream_t st) {
   using S = Shape<T, RT, SPT, LP, ST, TT>;
   const int Dg = p->D / p->G;
   constexpr int E = sizeof(T);
-  const dim3 grid((Dg + S::CH - 1) / S::CH, p->G, p->B);
-  if (grid.y > 65535 || grid.z > 65535) return fail(LQ_ERR_SHAPE, "selective_scan: B=%d G=%d", p->B, p->G);
+  const long long ctas = (long long)((Dg + S::CH - 1) / S::CH) * p->G * p->B;
+  if (ctas >= (1ll << 31) - 1) return fail(LQ_ERR_SHAPE, "selective_scan: B=%d D=%d G=%d", p->B, p->D, p->G);
   // TMA: addresses, pitches and rows of 16 bytes; a pitch of 0 (an expanded input) is not one
   Maps maps = {};
   Alignment a;
@@ -490,7 +491,7 @@ static int launch_scan(const lq_scan_problem* p, cudaStream_t st) {
     const cuuint32_t cbox[3] = {S::CH, TT, 1}, nbox[4] = {S::NP, 1, TT, 1};
     if (int e = i < 3 ? encode(in[i].map, p->dtype, 3, in[i].x, chans, &pitches[i][1], cbox) : encode(in[i].map, p->dtype, 4, in[i].x, states, pitches[i], nbox)) return e;
   }
-  auto go = [&](auto kern) { return launch_opt_in(kern, grid, dim3(S::THREADS), sizeof(typename S::Smem) + 128, st, maps, *p, by8); };
+  auto go = [&](auto kern) { return launch_opt_in(kern, dim3((unsigned)ctas), dim3(S::THREADS), sizeof(typename S::Smem) + 128, st, maps, *p, by8); };
   const cudaError_t e = wide ? go(selective_scan_kernel<T, true, RT, SPT, LP, ST, TT>) : go(selective_scan_kernel<T, false, RT, SPT, LP, ST, TT>);
   if (e != cudaSuccess) return fail(LQ_ERR_LAUNCH, "selective_scan: %s", cudaGetErrorString(e));
   return check_launch("selective_scan_kernel");

@@ -165,3 +165,18 @@ def test_scale_of_a_single_row():
     for wrong in (torch.ones(5, device="cuda"), torch.ones(0, device="cuda")):
         with pytest.raises(AssertionError):
             int8_linear_fwd(codes, w, sw, x_scale=wrong)
+
+
+# -------------------------------------------------------------------------------------------- many sequences or groups
+@gpu
+@pytest.mark.parametrize("b,T,d,G,N", [(70001, 2, 3, 1, 5), (1, 3, 70000, 70000, 4), (300, 2, 600, 300, 16)])
+def test_scan_of_more_rows_than_a_grid_axis(b, T, d, G, N):
+    """Sequences times groups beyond 65535, the extent of a grid's second and third axis."""
+    from linquant_b200.kernels.layer import selective_scan_fwd
+
+    u, dt, B, C = randn(b, T, d), torch.rand(b, T, d, device="cuda") + 0.1, randn(b, T, G, N), randn(b, T, G, N)
+    A, h0 = -(torch.rand(d, N, device="cuda") + 0.5), randn(b, d, N)
+    y, h = selective_scan_fwd(u, dt, A, B, C, dt_softplus=False, initial_state=h0, output_final_state=True)
+    want, mag, end, hm = ref.scan(u, dt, A, B, C, None, None, None, False, (0, INF), h0, None)
+    ref.check(y, want, mag, 32 * T * ULP)  # 32 roundings a token at most, as in the tests of the operators
+    ref.check(h, end, hm, 32 * T * ULP)
