@@ -2,8 +2,9 @@
 
 A layer call is one residual block: residual add and norm whose kernel writes INT8 codes, the INT8 in-projection, the short
 convolution, the recurrence, the gated norm (Mamba-2; again to codes) and the INT8 out-projection. ``prefill`` takes prompts of
-different lengths (right-padded) and leaves each sequence's convolution and recurrence state in the layer's cache; ``step``
-advances any of the cached sequences by one token.
+different lengths (right-padded), each from its first token, and leaves each sequence's convolution and recurrence state in the
+layer's cache; ``step`` advances any of the cached sequences by one token. In both, a slot outside the cache marks an idle entry
+of the batch, which leaves no state.
 
 The Mamba-2 prompt runs through the INT8 SSD ops (static scales from ``calibrate``); its state, an integer carry on the
 state scale, becomes the fp32 state of the token step, in the rotated basis of B and C."""
@@ -42,6 +43,18 @@ def _randn(gen, *shape, scale=1.0):
     return torch.randn(*shape, generator=gen, device="cuda") * scale
 
 
+class _Cache:
+    """Rows of a state, one a slot, and one behind them that takes what idle entries leave: no wait for the slots' values."""
+
+    def __init__(self, slots, *shape, dtype=torch.float32):
+        self.all = torch.zeros(slots + 1, *shape, device="cuda", dtype=dtype)
+        self.rows = self.all[:slots]
+
+    def put(self, slots, values):
+        at = slots.long()
+        self.all[torch.where((at >= 0) & (at < self.rows.shape[0]), at, self.rows.shape[0])] = values
+
+
 class Mamba2Layer:
     """headdim 64; d_state 64 or 128; chunk 128 or 256. Random weights (seeded); ``slots`` sequences in the cache."""
 
@@ -60,8 +73,8 @@ class Mamba2Layer:
         want = torch.exp(torch.rand(nheads, generator=gen, device="cuda") * 4.6 - 6.9)  # steps of 0.001 to 0.1
         self.dt_bias = want + torch.log(-torch.expm1(-want))
         self.signs = torch.randint(0, 2, (ngroups, d_state), generator=gen, device="cuda").float() * 2 - 1
-        self.conv_state = torch.zeros(slots, taps - 1, self.width, device="cuda", dtype=dtype)
-        self.state = torch.zeros(slots, nheads, 64, d_state, device="cuda")
+        self._conv_cache, self._cache = _Cache(slots, taps - 1, self.width, dtype=dtype), _Cache(slots, nheads, 64, d_state)
+        self.conv_state, self.state = self._conv_cache.rows, self._cache.rows
         self.scales = None
 
     def _in(self, x, residual):
@@ -109,15 +122,16 @@ class Mamba2Layer:
     def prefill(self, x, residual, slots, lengths=None):
         """x, residual (B,T,d_model); slots (B,) int32 rows of the cache; lengths (B,) int32 or None. Returns (out, residual)."""
         assert self.scales is not None, "calibrate() first: the SSD ops take static scales"
-        S, (B, T), at = self.scales, x.shape[:2], slots.long()
+        S, (B, T) = self.scales, x.shape[:2]
         z, xBC, dt, residual = self._in(x, residual)
-        xBC, self.conv_state[at] = short_conv_fwd(xBC, self.conv, self.conv_bias, lengths=lengths, output_final_state=True)
+        xBC, last = short_conv_fwd(xBC, self.conv, self.conv_bias, lengths=lengths, output_final_state=True)
+        self._conv_cache.put(slots, last)
         xBC, dt = self._pad(xBC, dt, lengths)
         xs, qB, qC = fused_split_rotate_quant_xBC(xBC, self.signs, self.H, self.G, self.N, self.P, 1 / S["B_scale"], 1 / S["C_scale"])
         dA, step = _quant_chunk_cumsum_fwd(dt, 1.0, self.A_log, 1.0, self.chunk, dt_bias=self.dt_bias, dt_softplus=True)
         states = _quant_chunk_state_fwd_xfp_static_int8(xs, qB, step, dA, S["alpha_hp"], S["B_scale"], S["state_scale"])
         passed, _, carry = _fixedpoint_state_passing_fwd(states.flatten(3), dA[..., -1], return_carry=True)
-        self.state[at] = carry.view(B, self.H, self.P, self.N) * S["state_scale"].view(1, self.H, self.P, 1)
+        self._cache.put(slots, carry.view(B, self.H, self.P, self.N) * S["state_scale"].view(1, self.H, self.P, 1))
         cb = _quant_bmm_chunk_fwd(qC, S["C_scale"], qB, S["B_scale"], self.chunk, S["cb_scale"])
         y = _quant_chunk_scan_fwd(cb, xs, step, dA, qC, S["C_scale"], passed.view_as(states), self.D, 1.0, S["state_scale"], S["cb_scale"])
         return self._out(y[:, :T].flatten(2), z), residual
@@ -153,8 +167,8 @@ class MambaLayer:
         self.D = torch.ones(d_inner, device="cuda")
         want = torch.exp(torch.rand(d_inner, generator=gen, device="cuda") * 4.6 - 6.9)
         self.dt_bias = want + torch.log(-torch.expm1(-want))
-        self.conv_state = torch.zeros(slots, taps - 1, d_inner, device="cuda", dtype=dtype)
-        self.state = torch.zeros(slots, d_inner, d_state, device="cuda")
+        self._conv_cache, self._cache = _Cache(slots, taps - 1, d_inner, dtype=dtype), _Cache(slots, d_inner, d_state)
+        self.conv_state, self.state = self._conv_cache.rows, self._cache.rows
 
     def _in(self, x, residual):
         (codes, scale), residual = rms_norm_fwd(x, self.norm, residual=residual, quantize=True)
@@ -167,11 +181,12 @@ class MambaLayer:
 
     @torch.no_grad()
     def prefill(self, x, residual, slots, lengths=None):
-        at = slots.long()
         u, z, residual = self._in(x, residual)
-        u, self.conv_state[at] = short_conv_fwd(u, self.conv, self.conv_bias, lengths=lengths, output_final_state=True)
+        u, last = short_conv_fwd(u, self.conv, self.conv_bias, lengths=lengths, output_final_state=True)
+        self._conv_cache.put(slots, last)
         dt, B, C = self._operands(u)
-        y, self.state[at] = selective_scan_fwd(u, dt, self.A, B, C, D=self.D, z=z, dt_bias=self.dt_bias, lengths=lengths, output_final_state=True)
+        y, last = selective_scan_fwd(u, dt, self.A, B, C, D=self.D, z=z, dt_bias=self.dt_bias, lengths=lengths, output_final_state=True)
+        self._cache.put(slots, last)
         return self.out_proj(y), residual
 
     @torch.no_grad()

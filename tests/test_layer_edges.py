@@ -180,3 +180,25 @@ def test_scan_of_more_rows_than_a_grid_axis(b, T, d, G, N):
     want, mag, end, hm = ref.scan(u, dt, A, B, C, None, None, None, False, (0, INF), h0, None)
     ref.check(y, want, mag, 32 * T * ULP)  # 32 roundings a token at most, as in the tests of the operators
     ref.check(h, end, hm, 32 * T * ULP)
+
+
+# ------------------------------------------------------------------------------------------ idle entries of a prompt
+@gpu
+@pytest.mark.parametrize("kind", ["mamba2", "mamba"])
+def test_idle_entries_of_a_prompt_batch(kind):
+    """A slot outside the cache, which a token step passes over, leaves nothing in a prompt either."""
+    from linquant_b200.models import Mamba2Layer, MambaLayer
+
+    layer = Mamba2Layer(256, 8, slots=4) if kind == "mamba2" else MambaLayer(256, 512, slots=4)
+    x = randn(4, 70, 256, dtype=layer.dtype)
+    r = torch.zeros_like(x)
+    if kind == "mamba2":
+        layer.calibrate(x, r)
+    layer.prefill(x[2:3], r[2:3], ints(1))
+    want, line = layer.state[1].clone(), layer.conv_state[1].clone()
+    for t in (layer.state, layer.conv_state):
+        t.fill_(7)
+    layer.prefill(x, r, ints(-1, 4, 1, -9))
+    assert torch.equal(layer.state[1], want) and torch.equal(layer.conv_state[1], line)
+    for t in (layer.state, layer.conv_state):
+        assert (t[[0, 2, 3]] == 7).all()
