@@ -97,7 +97,10 @@ __device__ __forceinline__ void quantize_rows_shared(const T* in, long long stri
   __syncthreads();
 }
 
-constexpr int KC = 2560, WP = KC + 64;  // bytes of K at a time; pitch of a row of weights in shared memory (two rows of an access on banks of their own)
+// Bytes of K at a time: two pieces of 16 rows, 82 KB, leave room for two CTAs an SM (one next to the longest codes, 120 KB),
+// and 40 blocks of 64 are whole rounds for 8 warps. Rows of another length end in a shorter piece. WP: pitch of a row of weights in
+// shared memory (two rows of an access on banks of their own).
+constexpr int KC = 2560, WP = KC + 64;
 
 static __host__ __device__ __forceinline__ int code_pitch(int K) {  // of codes in shared memory: blocks of 64, an odd number of them
   const int p = (K + 63) / 64 * 64;
@@ -141,7 +144,6 @@ __global__ void __launch_bounds__(std::is_same_v<TX, int8_t> ? 256 : 512, 2) int
     }
   };
   At ahead{(int)blockIdx.x, 0};
-  if (warp == 0) __syncwarp();
   for (int i = 0; i < 2 && i < items; ++i, ahead.next(chunks))
     if (warp == 0) request(i, ahead);
   // thread tid stores output (tid / 16, tid % 16) of a tile; its scales and bias are requested ahead

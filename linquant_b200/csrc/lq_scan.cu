@@ -523,36 +523,33 @@ static int run(const lq_scan_problem* p, cudaStream_t st) {
 template <typename T>
 __device__ __forceinline__ float step_decay(float dt, float A) { return sizeof(T) == 4 ? expf(dt * A) : ex2(dt * kLog2e * A); }
 
-// A row is the N states of one channel. LPR lanes hold it, VEC states each per step over N; a thread group takes R rows of
-// one head (HEADS: they share the decay, B and C) or one row with a decay rate per state.
-template <typename T, typename TS, int VEC, int R, bool HEADS>
+// A row is the N states of one channel: lpr lanes hold it, VEC states each per step over N. HEADS: the channels of a head share a
+// decay (heads whose channels are no multiple of four, states off 16 bytes or too many for one access of a warp).
+template <typename T, typename TS, int VEC, bool HEADS>
 __global__ void __launch_bounds__(128) selective_scan_step_kernel(const lq_scan_problem p, int lpr, bool wide_bc) {
   pdl_enter();
   const long long idx = (long long)blockIdx.x * 128 + threadIdx.x;
-  const int ln = (int)(idx % lpr), per_b = p.D / R;
+  const int ln = (int)(idx % lpr);
   const long long unit = idx / lpr;
-  const bool live = unit < (long long)p.B * per_b;  // idle lanes still take part in the shuffles
-  const int b = live ? (int)(unit / per_b) : 0, d0 = live ? (int)(unit - (long long)b * per_b) * R : 0;
+  const bool live = unit < (long long)p.B * p.D;  // idle lanes still take part in the shuffles
+  const int b = live ? (int)(unit / p.D) : 0, d = live ? (int)(unit - (long long)b * p.D) : 0;
   const int slot = p.slots ? p.slots[b] : b;
   const bool on = live && slot >= 0 && slot < p.n_slots;
-  const int head = HEADS ? d0 / p.P : d0;
-  const int grp = HEADS ? head / (p.H / p.G) : d0 / (p.D / p.G);
+  const int head = HEADS ? d / p.P : d;
+  const int grp = HEADS ? head / (p.H / p.G) : d / (p.D / p.G);
   const T* Bm = reinterpret_cast<const T*>(p.Bm) + b * p.B_stride_b + grp * p.B_stride_g;
   const T* Cm = reinterpret_cast<const T*>(p.Cm) + b * p.C_stride_b + grp * p.C_stride_g;
-  TS* state = reinterpret_cast<TS*>(p.state) + ((size_t)(on ? slot : 0) * p.D + d0) * p.N;
-  Pack<TS, VEC> raw[R];
+  TS* state = reinterpret_cast<TS*>(p.state) + ((size_t)(on ? slot : 0) * p.D + d) * p.N;
+  Pack<TS, VEC> raw;
   Pack<T, VEC> rB, rC;
   float A[HEADS ? 1 : VEC];
   auto request = [&](int n) {
     const bool in = on && n < p.N;
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-      raw[r].zero();
-      if (in) raw[r] = load_pack<TS, VEC>(state + (size_t)r * p.N + n);
-    }
+    raw.zero();
     rB.zero();
     rC.zero();
     if (in) {
+      raw = load_pack<TS, VEC>(state + n);
       if (wide_bc) {
         rB = load_pack<T, VEC>(Bm + n);
         rC = load_pack<T, VEC>(Cm + n);
@@ -565,59 +562,40 @@ __global__ void __launch_bounds__(128) selective_scan_step_kernel(const lq_scan_
       }
       if constexpr (!HEADS) {
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) A[i] = p.A[(size_t)d0 * p.N + n + i];
+        for (int i = 0; i < VEC; ++i) A[i] = p.A[(size_t)d * p.N + n + i];
       }
     }
   };
   request(ln * VEC);  // the state first: everything else is small and comes out of the caches
-  float dt = 0.f, u[R], acc[R];
+  float dt = 0.f, u = 0.f, acc = 0.f;
   if (on) {
     dt = to_f32(reinterpret_cast<const T*>(p.dt)[b * p.dt_stride_b + head]) + (p.dt_bias ? p.dt_bias[head] : 0.f);
     if constexpr (HEADS) A[0] = p.A[head];
-#pragma unroll
-    for (int r = 0; r < R; ++r) u[r] = to_f32(reinterpret_cast<const T*>(p.u)[b * p.u_stride_b + d0 + r]);
+    u = to_f32(reinterpret_cast<const T*>(p.u)[b * p.u_stride_b + d]);
     dt = p.softplus ? softplus(dt) : dt;
     dt = clamp_nan(dt, p.dt_min, p.dt_max);
-  }
-#pragma unroll
-  for (int r = 0; r < R; ++r) acc[r] = 0.f;
-  if (on) {
-    const float head_decay = HEADS ? step_decay<T>(dt, A[0]) : 0.f;
+    const float head_decay = HEADS ? step_decay<T>(dt, A[0]) : 0.f, du = dt * u;
     for (int n = ln * VEC; n < p.N;) {
-      float Bv[VEC], Cv[VEC], a[VEC];
+      float Bv[VEC], Cv[VEC], h[VEC];
       rB.get(Bv);
       rC.get(Cv);
+      raw.get(h);
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) a[i] = HEADS ? head_decay : step_decay<T>(dt, A[HEADS ? 0 : i]);
-#pragma unroll
-      for (int r = 0; r < R; ++r) {
-        float h[VEC];
-        raw[r].get(h);
-        const float du = dt * u[r];
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-          h[i] = fmaf(a[i], h[i], du * Bv[i]);
-          acc[r] = fmaf(h[i], Cv[i], acc[r]);
-        }
-        raw[r].set(h);
-        store_pack(state + (size_t)r * p.N + n, raw[r]);
+      for (int i = 0; i < VEC; ++i) {
+        h[i] = fmaf(HEADS ? head_decay : step_decay<T>(dt, A[HEADS ? 0 : i]), h[i], du * Bv[i]);
+        acc = fmaf(h[i], Cv[i], acc);
       }
+      raw.set(h);
+      store_pack(state + n, raw);
       n += lpr * VEC;
       if (n < p.N) request(n);
     }
   }
-#pragma unroll
-  for (int r = 0; r < R; ++r)
-    for (int m = lpr >> 1; m; m >>= 1) acc[r] += __shfl_xor_sync(0xffffffffu, acc[r], m);
-#pragma unroll
-  for (int r = 0; r < R; ++r) {
-    if (!live || ln != r % lpr) continue;
-    const int d = d0 + r;
-    float v = acc[r];
-    if (p.skip) v = fmaf(p.skip[HEADS && !p.skip_has_hdim ? head : d], u[r], v);
-    if (p.z && on) v *= silu(to_f32(reinterpret_cast<const T*>(p.z)[b * p.z_stride_b + d]));
-    reinterpret_cast<T*>(p.y)[(size_t)b * p.D + d] = from_f32<T>(on ? v : 0.f);
-  }
+  for (int m = lpr >> 1; m; m >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, m);
+  if (!live || ln != 0) return;
+  if (p.skip) acc = fmaf(p.skip[HEADS && !p.skip_has_hdim ? head : d], u, acc);
+  if (p.z && on) acc *= silu(to_f32(reinterpret_cast<const T*>(p.z)[b * p.z_stride_b + d]));
+  reinterpret_cast<T*>(p.y)[(size_t)b * p.D + d] = from_f32<T>(on ? acc : 0.f);
 }
 
 // One decay a head and N states in one access of LPR lanes: a team walks over the channels of a head, R = 4 rows at a time, the
@@ -742,17 +720,17 @@ static int launch_heads(const lq_scan_problem* p, cudaStream_t st) {
   return check_launch("heads_step_kernel");
 }
 
-template <typename T, typename TS, int VEC, int R, bool HEADS>
+template <typename T, typename TS, int VEC, bool HEADS>
 static int launch_step(const lq_scan_problem* p, cudaStream_t st) {
   int lpr = 1;
   while (lpr < 32 && lpr * VEC < p->N) lpr *= 2;
-  const long long threads = (long long)p->B * (p->D / R) * lpr;
+  const long long threads = (long long)p->B * p->D * lpr;
   if (threads == 0) return LQ_OK;
   if (threads / 128 >= (1ll << 31) - 1) return fail(LQ_ERR_SHAPE, "selective_scan_step: B=%d D=%d N=%d", p->B, p->D, p->N);
   constexpr int E = sizeof(T), BYTES = VEC * E < 16 ? VEC * E : 16;
   Alignment a;
   a.at(p->Bm).at(p->Cm).pitch(p->B_stride_b, E).pitch(p->B_stride_g, E).pitch(p->C_stride_b, E).pitch(p->C_stride_g, E);
-  launch(selective_scan_step_kernel<T, TS, VEC, R, HEADS>, dim3((unsigned)((threads + 127) / 128)), dim3(128), 0, st, *p, lpr, a.bytes() >= BYTES);
+  launch(selective_scan_step_kernel<T, TS, VEC, HEADS>, dim3((unsigned)((threads + 127) / 128)), dim3(128), 0, st, *p, lpr, a.bytes() >= BYTES);
   return check_launch("selective_scan_step_kernel");
 }
 template <typename T, typename TS>
@@ -760,9 +738,9 @@ static int run_step(const lq_scan_problem* p, cudaStream_t st) {
   constexpr int FULL = 16 / sizeof(TS);
   Alignment a;
   const bool wide = a.at(p->state).pitch(p->N, sizeof(TS)).bytes() == 16;
-  if (p->H == 0) return wide ? launch_step<T, TS, FULL, 1, false>(p, st) : launch_step<T, TS, 1, 1, false>(p, st);
+  if (p->H == 0) return wide ? launch_step<T, TS, FULL, false>(p, st) : launch_step<T, TS, 1, false>(p, st);
   if (p->P % 4 == 0 && wide && p->N <= 32 * FULL) return launch_heads<T, TS, FULL>(p, st);
-  return wide ? launch_step<T, TS, FULL, 1, true>(p, st) : launch_step<T, TS, 1, 1, true>(p, st);
+  return wide ? launch_step<T, TS, FULL, true>(p, st) : launch_step<T, TS, 1, true>(p, st);
 }
 
 static int check(const lq_scan_problem* p, bool step, const char* what) {
