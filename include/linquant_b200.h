@@ -282,7 +282,8 @@ int lq_kronecker_hadamard(const void* x, void* y, int dtype, int B, int T, int H
 /* ------------------------------------------------------------------------------------------------------------
  * Operators around the recurrence of a layer: short causal convolution, selective scan, INT8 product, norms. Prompts
  * ("fwd") and single tokens ("step", the cached state updated in place). Activations are f16, bf16 or f32 with contiguous
- * channels and any token pitch (slices of a wider projection output); parameters are dense fp32. Strides are in elements.
+ * channels and any token pitch (slices of a wider projection output); parameters are dense fp32. Strides are in elements,
+ * extents at most 2^31 - 2^13.
  * No counterpart in the reference's kernels.
  * ------------------------------------------------------------------------------------------------------------ */
 typedef struct {
@@ -332,7 +333,7 @@ typedef struct {
 int lq_selective_scan_fwd(const lq_scan_problem* p, lq_stream stream);
 int lq_selective_scan_step(const lq_scan_problem* p, lq_stream stream);
 
-/* Symmetric INT8 codes of rows: scale = amax / 127, codes by the code rule; rows of codes at a pitch that is a multiple of 16
+/* Symmetric INT8 codes of rows of any length: scale = amax / 127, codes by the code rule; rows of codes at a pitch that is a multiple of 16
  * bytes. A row of zeros has scale 0 and codes 0, one with an infinity or NaN a scale that is not finite. */
 int lq_quantize_rows(const void* x, int dtype, int rows, int D, long long x_stride, int8_t* codes, long long codes_stride, float* scale,
                      lq_stream stream);
@@ -348,12 +349,12 @@ typedef struct {
 } lq_linear_problem;
 /* y[m,n] = (sum_k x[m,k] w[n,k]) x_scale[m] w_scale[n] + bias[n] */
 int lq_int8_linear(const lq_linear_problem* p, lq_stream stream);
-/* The same from values: their codes and scales as lq_quantize_rows makes them. p->x and p->x_scale name scratch for them ([M]
- * rows at x_stride bytes, [M]), which may be written. */
+/* The same from values: their codes and scales as lq_quantize_rows makes them. p->x and p->x_scale name scratch for them, always
+ * of full size (M rows at x_stride bytes, M floats): M and K decide whether it is written. */
 int lq_int8_linear_values(const lq_linear_problem* p, const void* values, int dtype, long long stride, lq_stream stream);
 
 typedef struct {
-  int rows, D, group;          /* group: channels that are normed together (divides D; the gated form only, else D) */
+  int rows, D, group;          /* group: channels that are normed together, at most 16384 (divides D; the gated form only, else D) */
   int dtype, out_dtype;
   int residual_f32;            /* the residual stream is fp32, not `dtype` */
   int gate_first;              /* norm(x silu(gate)) weight, else norm(x) weight silu(gate) */

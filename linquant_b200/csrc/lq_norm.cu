@@ -7,7 +7,11 @@
 //   INT8 codes with one scale a row (amax / 127).
 //
 // Memory-bound: every input is read once into registers (VEC values a load, NV loads a thread), the sums of a row are taken
-// in fp32 by the team of threads that holds it, and y, r and the codes are written once: gated norm of 32768 x 5120 bf16 182 us (5.5 TB/s; 209 with INT8 outputs), residual and norm of 16384 x 2560 56.6 us (5.9).
+// in fp32 by the team of threads that holds it, and y, r and the codes are written once: gated norm of 32768 x 5120 bf16 186 us
+// (5.4 TB/s; 213 with INT8 outputs, 3.9), residual and norm of 16384 x 2560 56.6 us (5.9).
+// Rows off a pack's boundary are walked in packs too where all tensors lie at the same distance behind theirs. Where they do not (an odd
+// row length next to a slice, to an fp32 residual or to another output type; groups that are no multiple of a pack) a value goes by
+// itself and rows of more than 1024 spill: gated norm of 32768 x 2561 153 us against 756 with the gate a slice.
 #include "lq_layer.cuh"
 
 namespace lq {

@@ -13,7 +13,7 @@
 // two, one barrier a tile. Inputs come as TMA tiles into a ring of ST tiles, requested ST - 2 tiles ahead of their use. Where
 // rows do not lie on 16-byte boundaries the storing warps copy them in pieces of eight or four bytes, the pieces that hold a
 // row's ends included.
-// At 1 x 16384 x 2048 with 16 states (bf16, gate): 375 us; 115 us of exponentials, 41 us of bytes. All jobs in every warp took
+// At 1 x 16384 x 2048 with 16 states (bf16, gate): 369 us; 115 us of exponentials, 41 us of bytes. All jobs in every warp took
 // 1 139 us, two jobs and plain loads 937 us, three jobs with the state index contiguous 462 us. The recurrence alone takes 259
 // us, the other two jobs alone 211 us; together shared memory is busy in 75 % of the clocks.
 #include "lq_layer.cuh"

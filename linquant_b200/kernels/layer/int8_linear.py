@@ -11,7 +11,7 @@ from ... import _cabi
 
 
 def quantize_rows_fwd(x):
-    """Symmetric INT8 codes of the rows of x (.., K) f16/bf16/f32: scale = amax / 127 in fp32, codes = x / scale rounded half
+    """Symmetric INT8 codes of the rows of x (.., K) f16/bf16/f32, of any length: scale = amax / 127 in fp32, codes = x / scale rounded half
     away from zero. Returns (codes (.., K) int8, scale (..) fp32); the rows of the codes lie at a pitch of K rounded up to 16
     bytes, as ``int8_linear_fwd`` reads them in place. Also lays out a weight (N, K) once, its scales per output channel. A
     row of zeros has scale 0; one with an infinity or NaN a scale that is not finite, and so has its product."""

@@ -39,7 +39,7 @@ def rms_norm_fwd(x, weight, residual=None, residual_scale=1.0, post_weight=None,
 
 def gated_rms_norm_fwd(x, gate, weight, group_size=None, gate_first=True, eps=1e-5, quantize=False, out_dtype=None):
     """y = norm(x silu(gate)) weight, or norm(x) weight silu(gate) with ``gate_first=False``; the norm over each
-    ``group_size`` channels (all of them without it). x, gate (.., D) of one type, the gate a slice of a wider projection
+    ``group_size`` channels, at most 16384 (all of them without it). x, gate (.., D) of one type, the gate a slice of a wider projection
     if need be; weight (D,). With ``quantize`` y comes as (codes, scale) of its rows."""
     r = _cabi.host().gated_rms_norm(x, gate, weight, group_size, gate_first, eps, quantize, out_dtype)
     if r is None:
