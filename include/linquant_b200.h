@@ -41,7 +41,7 @@ typedef void* lq_stream; /* a cudaStream_t */
 
 int lq_version(void);
 /* sizeof the descriptor structs as the library was compiled: a binding checks its own layout against these (0 = zoo, 1 = ssd,
- * 2 = workspace, 3 = conv, 4 = scan, 5 = linear, 6 = norm) */
+ * 2 = workspace, 3 = conv, 4 = scan, 5 = linear, 6 = norm, 7 = attention) */
 unsigned long long lq_struct_bytes(int which);
 const char* lq_last_error_string(void);
 
@@ -371,6 +371,29 @@ typedef struct {
 /* r = residual + residual_scale P(x), P(x) = x or norm(x) post_weight;  y = norm(r) weight  (norm(x) weight without a residual) */
 int lq_rms_norm(const lq_norm_problem* p, lq_stream stream);
 int lq_gated_rms_norm(const lq_norm_problem* p, lq_stream stream);
+
+typedef struct {
+  int B, T, H, Hk, K, V;       /* H heads of v, Hk of q and k (H / Hk share one); K <= 256 */
+  int dtype;                   /* of q, k, v, o */
+  int state_dtype;             /* step: of `state` */
+  float scale;
+  long long q_stride_b, q_stride_t, q_stride_h, k_stride_b, k_stride_t, k_stride_h; /* elements; channels contiguous */
+  long long v_stride_b, v_stride_t, v_stride_h, g_stride_b, g_stride_t, g_stride_h;
+  const void *q, *k, *v;       /* [B,T,Hk,K], [B,T,Hk,K], [B,T,H,V]; step: T = 1, strides of t are not used */
+  const float* g;              /* [B,T,H] log-decays (any strides, 0 for constants) or null */
+  const float* initial_state;  /* fwd: [B,H,K,V] or null */
+  const int* lengths;          /* fwd: as above */
+  void* o;                     /* [B,T,H,V] dense */
+  float* final_state;          /* fwd: [B,H,K,V] or null */
+  void* state;                 /* step: [n_slots,H,K,V] */
+  const int* slots;            /* step: as above */
+  int n_slots;
+} lq_attention_problem;
+/* S_t = exp(g_t) S_{t-1} + k_t v_t^T;  o_t = scale q_t S_t;  states in fp32. The workspace (0 bytes for many heads) holds the states
+ * between the segments of a call's tokens; 16-byte aligned. */
+size_t lq_linear_attention_workspace_bytes(const lq_attention_problem* p);
+int lq_linear_attention_fwd(const lq_attention_problem* p, void* workspace, size_t workspace_bytes, lq_stream stream);
+int lq_linear_attention_step(const lq_attention_problem* p, lq_stream stream);
 
 #ifdef __cplusplus
 }

@@ -648,6 +648,106 @@ PyObject* selective_scan_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// linear_attention(q, k, v, g, scale, initial_state, lengths, want_state) -> (o, state or None) | status | None
+// linear_attention_step(state, q, k, v, g, scale, slots) -> o | status | None
+struct Attention {
+  lq_attention_problem p = {};
+  at::ScalarType t;
+  // q, k [B,(T,)Hk,K], v [B,(T,)H,V], g [B,(T,)H], [H] or None; a scale of None is 1 / sqrt(K)
+  Attention(Call& c, PyObject* q_, PyObject* k_, PyObject* v_, PyObject* g_, PyObject* scale, int64_t dim) {
+    const at::Tensor& q0 = Call::tensor(q_);
+    if (!q0.is_cuda() || q0.dim() != dim) throw NotPlain{};
+    c.dev = q0.device();
+    t = q0.scalar_type();
+    const at::Tensor &q = act(c, q_, dim, t), &k = act(c, k_, dim, t), &v = act(c, v_, dim, t);
+    const int64_t h = dim - 2, B = q.size(0), T = dim == 4 ? q.size(1) : 1, H = v.size(h), K = q.size(h + 1);
+    expect(k, q.sizes());
+    if (v.size(0) != B || (dim == 4 && v.size(1) != T)) throw NotPlain{};
+    p.B = extent(B); p.T = extent(T); p.H = extent(H); p.Hk = extent(q.size(h)); p.K = extent(K); p.V = extent(v.size(h + 1));
+    p.dtype = out_code(t);
+    p.scale = scale == Py_None ? (float)(1.0 / std::sqrt((double)K)) : (float)number(scale);
+    p.q = q.const_data_ptr(); p.k = k.const_data_ptr(); p.v = v.const_data_ptr();
+    p.q_stride_b = q.stride(0); p.q_stride_h = q.stride(h);
+    p.k_stride_b = k.stride(0); p.k_stride_h = k.stride(h);
+    p.v_stride_b = v.stride(0); p.v_stride_h = v.stride(h);
+    if (dim == 4) p.q_stride_t = q.stride(1), p.k_stride_t = k.stride(1), p.v_stride_t = v.stride(1);
+    if (g_ == Py_None) return;
+    const at::Tensor& g = Call::tensor(g_);
+    if (g.device() != c.dev || g.scalar_type() != at::kFloat) throw NotPlain{};
+    p.g = g.const_data_ptr<float>();
+    if (g.dim() == 1) {
+      expect(g, {H});
+      p.g_stride_h = g.stride(0);
+    } else {
+      if (dim == 4) expect(g, {B, T, H});
+      else expect(g, {B, H});
+      p.g_stride_b = g.stride(0); p.g_stride_h = g.stride(h);
+      if (dim == 4) p.g_stride_t = g.stride(1);
+    }
+  }
+};
+PyObject* linear_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  try {
+    if (n != 8) throw NotPlain{};
+    Call c;
+    c.keep.reserve(4);
+    Attention at_(c, a[0], a[1], a[2], a[3], a[4], 4);
+    lq_attention_problem& p = at_.p;
+    c10::cuda::CUDAGuard guard(c.dev);
+    p.initial_state = c.f32(a[5], {p.B, p.H, p.K, p.V}, true);
+    p.lengths = int32(c, a[6], p.B);
+    const at::Tensor o = empty({p.B, p.T, p.H, p.V}, at_.t, c.dev);
+    p.o = o.data_ptr();
+    at::Tensor state;
+    if (flag(a[7])) {
+      state = empty({p.B, p.H, p.K, p.V}, at::kFloat, c.dev);
+      p.final_state = state.data_ptr<float>();
+    }
+    const size_t bytes = lq_linear_attention_workspace_bytes(&p);
+    uint8_t* ws = bytes ? aligned(c.hold(scratch(bytes, c.dev))) : nullptr;
+    cudaStream_t st = stream_of(c);
+    int e;
+    {
+      NoGil ng;
+      e = lq_linear_attention_fwd(&p, ws, bytes, st);
+    }
+    if (e != LQ_OK) return PyLong_FromLong(e);
+    return pair(THPVariable_Wrap(o), state.defined() ? THPVariable_Wrap(state) : none());
+  } catch (const NotPlain&) {
+    Py_RETURN_NONE;
+  }
+  END_HANDLE_TH_ERRORS
+}
+PyObject* linear_attention_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  try {
+    if (n != 7) throw NotPlain{};
+    Call c;
+    Attention at_(c, a[1], a[2], a[3], a[4], a[5], 3);
+    lq_attention_problem& p = at_.p;
+    c10::cuda::CUDAGuard guard(c.dev);
+    const at::Tensor& s = Call::tensor(a[0]);
+    if (s.device() != c.dev || !s.is_contiguous() || s.dim() != 4 || s.size(1) != p.H || s.size(2) != p.K || s.size(3) != p.V) throw NotPlain{};
+    p.state_dtype = out_code(s.scalar_type());
+    p.state = s.data_ptr();
+    p.n_slots = extent(s.size(0));
+    p.slots = int32(c, a[6], p.B);
+    const at::Tensor o = empty({p.B, p.H, p.V}, at_.t, c.dev);
+    p.o = o.data_ptr();
+    cudaStream_t st = stream_of(c);
+    int e;
+    {
+      NoGil ng;
+      e = lq_linear_attention_step(&p, st);
+    }
+    return e != LQ_OK ? PyLong_FromLong(e) : THPVariable_Wrap(o);
+  } catch (const NotPlain&) {
+    Py_RETURN_NONE;
+  }
+  END_HANDLE_TH_ERRORS
+}
+
 int64_t codes_pitch(int64_t n) { return (n + 15) / 16 * 16; }
 // [.., n] view of rows at a pitch
 at::Tensor rows_view(const at::Tensor& buf, at::IntArrayRef lead, int64_t n, int64_t pitch) {
@@ -887,6 +987,8 @@ PyMethodDef methods[] = {
     {"short_conv_step", (PyCFunction)(void*)short_conv_step, METH_FASTCALL, "short causal convolution, one token"},
     {"selective_scan", (PyCFunction)(void*)selective_scan, METH_FASTCALL, "selective scan of prompts"},
     {"selective_scan_step", (PyCFunction)(void*)selective_scan_step, METH_FASTCALL, "selective scan, one token"},
+    {"linear_attention", (PyCFunction)(void*)linear_attention, METH_FASTCALL, "linear attention of prompts"},
+    {"linear_attention_step", (PyCFunction)(void*)linear_attention_step, METH_FASTCALL, "linear attention, one token"},
     {"quantize_rows", (PyCFunction)(void*)quantize_rows, METH_FASTCALL, "symmetric INT8 codes of rows"},
     {"int8_linear", (PyCFunction)(void*)int8_linear, METH_FASTCALL, "INT8 product with token and channel scales"},
     {"rms_norm", (PyCFunction)(void*)rms_norm, METH_FASTCALL, "residual add and norms"},
