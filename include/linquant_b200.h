@@ -41,7 +41,7 @@ typedef void* lq_stream; /* a cudaStream_t */
 
 int lq_version(void);
 /* sizeof the descriptor structs as the library was compiled: a binding checks its own layout against these (0 = zoo, 1 = ssd,
- * 2 = workspace, 3 = conv, 4 = scan, 5 = linear, 6 = norm, 7 = attention) */
+ * 2 = workspace, 3 = conv, 4 = scan, 5 = linear, 6 = norm, 7 = attention, 8 = group norm) */
 unsigned long long lq_struct_bytes(int which);
 const char* lq_last_error_string(void);
 
@@ -394,6 +394,22 @@ typedef struct {
 size_t lq_linear_attention_workspace_bytes(const lq_attention_problem* p);
 int lq_linear_attention_fwd(const lq_attention_problem* p, void* workspace, size_t workspace_bytes, lq_stream stream);
 int lq_linear_attention_step(const lq_attention_problem* p, lq_stream stream);
+
+typedef struct {
+  int B, T, D, groups;         /* groups of D / groups channels */
+  int dtype;                   /* of x, gate, y */
+  int over_tokens;             /* statistics over a sequence's T tokens, else each token by itself (T = 1, B tokens) */
+  int silu;
+  float eps;
+  long long x_stride_b, x_stride_t, gate_stride_b, gate_stride_t;
+  const void *x, *gate;        /* [B,T,D]; gate or null: y *= silu(gate) */
+  const float *weight, *bias;  /* [D] or null */
+  const int* lengths;          /* over_tokens: as above */
+  void* y;                     /* [B,T,D] dense */
+} lq_group_norm_problem;
+/* y = act((x - mean) / sqrt(var + eps) weight + bias). The workspace (over_tokens) holds the sums of tiles of tokens; 8-byte aligned. */
+size_t lq_group_norm_workspace_bytes(const lq_group_norm_problem* p);
+int lq_group_norm(const lq_group_norm_problem* p, void* workspace, size_t workspace_bytes, lq_stream stream);
 
 #ifdef __cplusplus
 }

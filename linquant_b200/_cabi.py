@@ -71,6 +71,11 @@ class AttentionProblem(C.Structure):
                        void_p="q k v g initial_state lengths o final_state state slots", int_2="n_slots")
 
 
+class GroupNormProblem(C.Structure):
+    _fields_ = _fields(int="B T D groups dtype over_tokens silu", float="eps", longlong="x_stride_b x_stride_t gate_stride_b gate_stride_t",
+                       void_p="x gate weight bias lengths y")
+
+
 class LinQuantError(RuntimeError):
     pass
 

@@ -978,6 +978,64 @@ PyObject* gated_rms_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// group_norm(x, groups, weight, bias, silu, gate, eps, over_tokens, lengths) -> y | status | None.   x [..,D], or [B,T,D] over tokens
+PyObject* group_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  try {
+    if (n != 9) throw NotPlain{};
+    Call c;
+    const at::Tensor& x = Call::tensor(a[0]);
+    if (!x.is_cuda() || x.dim() < 1) throw NotPlain{};
+    c.dev = x.device();
+    c.keep.reserve(4);
+    c10::cuda::CUDAGuard guard(c.dev);
+    const int64_t D = x.size(-1);
+    lq_group_norm_problem p = {};
+    p.dtype = out_code(x.scalar_type());
+    p.D = extent(D);
+    p.groups = integer(a[1]);
+    p.silu = flag(a[4]);
+    p.eps = (float)number(a[6]);
+    p.over_tokens = flag(a[7]);
+    auto rows = [&](const at::Tensor& t, long long& sb, long long& st) {
+      if (!p.over_tokens) {
+        const Rows r(t);
+        sb = r.pitch;
+        return r.rows;
+      }
+      if (t.dim() != 3 || (D > 1 && t.stride(2) != 1)) throw NotPlain{};
+      sb = t.stride(0), st = t.stride(1);
+      return t.size(0);
+    };
+    p.B = extent(rows(x, p.x_stride_b, p.x_stride_t));
+    p.T = p.over_tokens ? extent(x.size(1)) : 1;
+    p.x = x.const_data_ptr();
+    if (a[5] != Py_None) {
+      const at::Tensor& g = Call::tensor(a[5]);
+      if (g.device() != c.dev || g.sizes() != x.sizes() || g.scalar_type() != x.scalar_type()) throw NotPlain{};
+      rows(g, p.gate_stride_b, p.gate_stride_t);
+      p.gate = g.const_data_ptr();
+    }
+    p.weight = c.f32(a[2], {D}, true);
+    p.bias = c.f32(a[3], {D}, true);
+    p.lengths = int32(c, a[8], p.B);
+    const at::Tensor y = empty(x.sizes(), x.scalar_type(), c.dev);
+    p.y = y.data_ptr();
+    const size_t bytes = lq_group_norm_workspace_bytes(&p);
+    uint8_t* ws = bytes ? aligned(c.hold(scratch(bytes, c.dev))) : nullptr;
+    cudaStream_t st = stream_of(c);
+    int e;
+    {
+      NoGil ng;
+      e = lq_group_norm(&p, ws, bytes, st);
+    }
+    return e != LQ_OK ? PyLong_FromLong(e) : THPVariable_Wrap(y);
+  } catch (const NotPlain&) {
+    Py_RETURN_NONE;
+  }
+  END_HANDLE_TH_ERRORS
+}
+
 PyMethodDef methods[] = {
     {"zoo_fwd", (PyCFunction)(void*)zoo_fwd, METH_FASTCALL, "one chunk call of a zoo cell"},
     {"split_rotate", (PyCFunction)(void*)split_rotate, METH_FASTCALL, "Mamba-2 prologue on xBC"},
@@ -993,6 +1051,7 @@ PyMethodDef methods[] = {
     {"int8_linear", (PyCFunction)(void*)int8_linear, METH_FASTCALL, "INT8 product with token and channel scales"},
     {"rms_norm", (PyCFunction)(void*)rms_norm, METH_FASTCALL, "residual add and norms"},
     {"gated_rms_norm", (PyCFunction)(void*)gated_rms_norm, METH_FASTCALL, "norm with a gate"},
+    {"group_norm", (PyCFunction)(void*)group_norm, METH_FASTCALL, "group norm with an activation"},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
