@@ -41,7 +41,7 @@ typedef void* lq_stream; /* a cudaStream_t */
 
 int lq_version(void);
 /* sizeof the descriptor structs as the library was compiled: a binding checks its own layout against these (0 = zoo, 1 = ssd,
- * 2 = workspace, 3 = conv, 4 = scan, 5 = linear, 6 = norm, 7 = attention, 8 = group norm) */
+ * 2 = workspace, 3 = conv, 4 = scan, 5 = linear, 6 = norm, 7 = attention, 8 = group norm, 9 = lora) */
 unsigned long long lq_struct_bytes(int which);
 const char* lq_last_error_string(void);
 
@@ -352,6 +352,20 @@ int lq_int8_linear(const lq_linear_problem* p, lq_stream stream);
 /* The same from values: their codes and scales as lq_quantize_rows makes them. p->x and p->x_scale name scratch for them, always
  * of full size (M rows at x_stride bytes, M floats): M and K decide whether it is written. */
 int lq_int8_linear_values(const lq_linear_problem* p, const void* values, int dtype, long long stride, lq_stream stream);
+
+typedef struct {
+  int L, R;                    /* adapters (0: none) and their rank: a multiple of 8, 128 at most */
+  int dtype;                   /* of a and b */
+  float scale;                 /* times scaling */
+  const void *a, *b;           /* [L,R,K] and [L,N,R] dense; b 16-byte aligned */
+  const int* adapters;         /* [M]: the adapter of each token; one outside 0..L-1 is none */
+  const float* scaling;        /* [L] or null */
+  float* t;                    /* scratch of lq_lora_workspace_bytes(M, R), 16-byte aligned */
+} lq_lora_problem;
+/* lq_int8_linear, or with `values` lq_int8_linear_values, and in the same rounding
+ * y[m,n] += sum_r t[m,r] b[l,n,r],  t[m,r] = scale scaling[l] sum_k x[m,k] a[l,r,k],  l = adapters[m];  x: the values, or codes times their scale */
+size_t lq_lora_workspace_bytes(int M, int R);
+int lq_lora_linear(const lq_linear_problem* p, const lq_lora_problem* q, const void* values, int dtype, long long stride, lq_stream stream);
 
 typedef struct {
   int rows, D, group;          /* group: channels that are normed together, at most 16384 (divides D; the gated form only, else D) */

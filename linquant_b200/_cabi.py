@@ -76,6 +76,10 @@ class GroupNormProblem(C.Structure):
                        void_p="x gate weight bias lengths y")
 
 
+class LoraProblem(C.Structure):
+    _fields_ = _fields(int="L R dtype", float="scale", void_p="a b adapters scaling t")
+
+
 class LinQuantError(RuntimeError):
     pass
 

@@ -791,70 +791,110 @@ PyObject* quantize_rows(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// The INT8 product of x (codes with x_scale, or values), with low-rank adapters where `lora` names them: a, b, adapters, scaling
+PyObject* linear(PyObject* x_, PyObject* w_, PyObject* w_scale, PyObject* x_scale, PyObject* bias, PyObject* out_dtype, PyObject* const* lora) {
+  Call c;
+  const at::Tensor &x = Call::tensor(x_), &w = Call::tensor(w_);
+  if (!x.is_cuda() || w.device() != x.device() || w.dim() != 2 || w.scalar_type() != at::kChar) throw NotPlain{};
+  c.dev = x.device();
+  c.keep.reserve(8);
+  c10::cuda::CUDAGuard guard(c.dev);
+  const Rows xr(x), wr(w);
+  const int64_t K = x.size(-1), N = w.size(0);
+  if (w.size(1) != K) throw NotPlain{};
+  lq_linear_problem p = {};
+  p.M = extent(xr.rows); p.N = extent(N); p.K = extent(K);
+  auto aligned_rows = [](const at::Tensor& t, const Rows& r) {
+    if ((reinterpret_cast<uintptr_t>(t.const_data_ptr()) & 15u) || (r.pitch & 15)) {
+      if (r.rows > 1 || (reinterpret_cast<uintptr_t>(t.const_data_ptr()) & 15u)) throw NotPlain{};
+      return codes_pitch(r.pitch);  // one row: its pitch is not used
+    }
+    return r.pitch;
+  };
+  p.w = w.const_data_ptr<int8_t>();
+  p.w_stride = aligned_rows(w, wr);
+  p.w_scale = c.f32(w_scale, {N}, true);
+  p.bias = c.f32(bias, {N}, true);
+  cudaStream_t st = stream_of(c);
+  int dt = -1;
+  int8_t* codes = nullptr;
+  float* scale = nullptr;
+  at::ScalarType ot = at::kBFloat16;
+  if (x.scalar_type() == at::kChar) {
+    p.x = x.const_data_ptr<int8_t>();
+    p.x_stride = aligned_rows(x, xr);
+    if (x_scale == Py_None) throw NotPlain{};
+    if (x.dim() == 1 && Call::tensor(x_scale).numel() != 1) throw NotPlain{};  // f32 takes any shape for one that has no axes
+    p.x_scale = c.f32(x_scale, lead_of(x), true);
+  } else {
+    dt = out_code(ot = x.scalar_type());
+    if (x_scale != Py_None) throw NotPlain{};
+    p.x_stride = codes_pitch(K);
+    const at::Tensor& buf = c.hold(scratch(xr.rows * (p.x_stride + 4), c.dev));
+    codes = (int8_t*)aligned(buf);
+    scale = (float*)(codes + xr.rows * p.x_stride);
+    p.x = codes;
+    p.x_scale = scale;
+  }
+  if (out_dtype != Py_None) {
+    if (!THPDtype_Check(out_dtype)) throw NotPlain{};
+    ot = ((THPDtype*)out_dtype)->scalar_type;
+  }
+  p.out_dtype = out_code(ot);
+  lq_lora_problem q = {};
+  if (lora) {
+    const at::Tensor &a = Call::tensor(lora[0]), &b = Call::tensor(lora[1]), &which = Call::tensor(lora[2]);
+    if (a.dim() != 3) throw NotPlain{};
+    const int64_t L = a.size(0), R = a.size(1);
+    expect(a, {L, R, K});
+    expect(b, {L, N, R});
+    if (a.device() != c.dev || b.device() != c.dev || a.scalar_type() != b.scalar_type() || !a.is_contiguous() || !b.is_contiguous()) throw NotPlain{};
+    if (which.device() != c.dev || which.scalar_type() != at::kInt || !which.is_contiguous() || which.sizes() != lead_of(x)) throw NotPlain{};
+    if (L > 0 && (R % 8 || (reinterpret_cast<uintptr_t>(b.const_data_ptr()) & 15u))) throw NotPlain{};
+    q.L = extent(L); q.R = extent(R);
+    q.dtype = out_code(a.scalar_type());
+    q.a = a.const_data_ptr(); q.b = b.const_data_ptr();
+    q.adapters = which.const_data_ptr<int>();
+    q.scale = 1.0f;
+    if (lora[3] != Py_None) {
+      if (THPVariable_Check(lora[3])) q.scaling = c.f32(lora[3], {L}, true);
+      else q.scale = (float)number(lora[3]);
+    }
+    q.t = (float*)aligned(c.hold(scratch(lq_lora_workspace_bytes(p.M, q.R), c.dev)));
+  }
+  std::vector<int64_t> shape(x.sizes().begin(), x.sizes().end());
+  shape.back() = N;
+  const at::Tensor y = empty(shape, ot, c.dev);
+  p.y = y.data_ptr();
+  p.status = status_word(c.dev);
+  int e;
+  {
+    NoGil ng;
+    e = lora ? lq_lora_linear(&p, &q, codes ? x.const_data_ptr() : nullptr, dt, xr.pitch, st)
+        : codes ? lq_int8_linear_values(&p, x.const_data_ptr(), dt, xr.pitch, st)
+                : lq_int8_linear(&p, st);
+  }
+  return e != LQ_OK ? PyLong_FromLong(e) : THPVariable_Wrap(y);
+}
+
 // int8_linear(x, w, w_scale, x_scale, bias, out_dtype) -> y | status | None.   x: codes with x_scale, or values
 PyObject* int8_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   try {
     if (n != 6) throw NotPlain{};
-    Call c;
-    const at::Tensor &x = Call::tensor(a[0]), &w = Call::tensor(a[1]);
-    if (!x.is_cuda() || w.device() != x.device() || w.dim() != 2 || w.scalar_type() != at::kChar) throw NotPlain{};
-    c.dev = x.device();
-    c.keep.reserve(6);
-    c10::cuda::CUDAGuard guard(c.dev);
-    const Rows xr(x), wr(w);
-    const int64_t K = x.size(-1), N = w.size(0);
-    if (w.size(1) != K) throw NotPlain{};
-    lq_linear_problem p = {};
-    p.M = extent(xr.rows); p.N = extent(N); p.K = extent(K);
-    auto aligned_rows = [](const at::Tensor& t, const Rows& r) {
-      if ((reinterpret_cast<uintptr_t>(t.const_data_ptr()) & 15u) || (r.pitch & 15)) {
-        if (r.rows > 1 || (reinterpret_cast<uintptr_t>(t.const_data_ptr()) & 15u)) throw NotPlain{};
-        return codes_pitch(r.pitch);  // one row: its pitch is not used
-      }
-      return r.pitch;
-    };
-    p.w = w.const_data_ptr<int8_t>();
-    p.w_stride = aligned_rows(w, wr);
-    p.w_scale = c.f32(a[2], {N}, true);
-    p.bias = c.f32(a[4], {N}, true);
-    cudaStream_t st = stream_of(c);
-    int dt = -1;
-    int8_t* codes = nullptr;
-    float* scale = nullptr;
-    at::ScalarType ot = at::kBFloat16;
-    if (x.scalar_type() == at::kChar) {
-      p.x = x.const_data_ptr<int8_t>();
-      p.x_stride = aligned_rows(x, xr);
-      if (a[3] == Py_None) throw NotPlain{};
-      if (x.dim() == 1 && Call::tensor(a[3]).numel() != 1) throw NotPlain{};  // f32 takes any shape for one that has no axes
-      p.x_scale = c.f32(a[3], lead_of(x), true);
-    } else {
-      dt = out_code(ot = x.scalar_type());
-      if (a[3] != Py_None) throw NotPlain{};
-      p.x_stride = codes_pitch(K);
-      const at::Tensor& buf = c.hold(scratch(xr.rows * (p.x_stride + 4), c.dev));
-      codes = (int8_t*)aligned(buf);
-      scale = (float*)(codes + xr.rows * p.x_stride);
-      p.x = codes;
-      p.x_scale = scale;
-    }
-    if (a[5] != Py_None) {
-      if (!THPDtype_Check(a[5])) throw NotPlain{};
-      ot = ((THPDtype*)a[5])->scalar_type;
-    }
-    p.out_dtype = out_code(ot);
-    std::vector<int64_t> shape(x.sizes().begin(), x.sizes().end());
-    shape.back() = N;
-    const at::Tensor y = empty(shape, ot, c.dev);
-    p.y = y.data_ptr();
-    p.status = status_word(c.dev);
-    int e;
-    {
-      NoGil ng;
-      e = codes ? lq_int8_linear_values(&p, x.const_data_ptr(), dt, xr.pitch, st) : lq_int8_linear(&p, st);
-    }
-    return e != LQ_OK ? PyLong_FromLong(e) : THPVariable_Wrap(y);
+    return linear(a[0], a[1], a[2], a[3], a[4], a[5], nullptr);
+  } catch (const NotPlain&) {
+    Py_RETURN_NONE;
+  }
+  END_HANDLE_TH_ERRORS
+}
+
+// lora_linear(x, w, w_scale, a, b, adapters, scaling, x_scale, bias, out_dtype) -> y | status | None
+PyObject* lora_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  try {
+    if (n != 10) throw NotPlain{};
+    return linear(a[0], a[1], a[2], a[7], a[8], a[9], a + 3);
   } catch (const NotPlain&) {
     Py_RETURN_NONE;
   }
@@ -1049,6 +1089,7 @@ PyMethodDef methods[] = {
     {"linear_attention_step", (PyCFunction)(void*)linear_attention_step, METH_FASTCALL, "linear attention, one token"},
     {"quantize_rows", (PyCFunction)(void*)quantize_rows, METH_FASTCALL, "symmetric INT8 codes of rows"},
     {"int8_linear", (PyCFunction)(void*)int8_linear, METH_FASTCALL, "INT8 product with token and channel scales"},
+    {"lora_linear", (PyCFunction)(void*)lora_linear, METH_FASTCALL, "INT8 product with low-rank adapters"},
     {"rms_norm", (PyCFunction)(void*)rms_norm, METH_FASTCALL, "residual add and norms"},
     {"gated_rms_norm", (PyCFunction)(void*)gated_rms_norm, METH_FASTCALL, "norm with a gate"},
     {"group_norm", (PyCFunction)(void*)group_norm, METH_FASTCALL, "group norm with an activation"},

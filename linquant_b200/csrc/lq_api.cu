@@ -104,7 +104,7 @@ extern "C" unsigned long long lq_struct_bytes(int which) {
   return which == 0 ? sizeof(lq_zoo_problem) : which == 1 ? sizeof(lq_ssd_problem) : which == 2 ? sizeof(lq_zoo_workspace)
          : which == 3 ? sizeof(lq_conv_problem) : which == 4 ? sizeof(lq_scan_problem) : which == 5 ? sizeof(lq_linear_problem)
          : which == 6 ? sizeof(lq_norm_problem) : which == 7 ? sizeof(lq_attention_problem)
-         : which == 8 ? sizeof(lq_group_norm_problem) : 0;
+         : which == 8 ? sizeof(lq_group_norm_problem) : which == 9 ? sizeof(lq_lora_problem) : 0;
 }
 extern "C" const char* lq_last_error_string(void) { return lq::g_err; }
 

@@ -10,7 +10,7 @@
 // 5120 -> 2560 channels: 3 tokens 6.9 us (13 MB, 2 us of memory; launch, the first bytes' latency and the sums' way through shared
 // memory are the rest), with values 9.1, with a kernel for the codes ahead 10.1; 2560 -> 10576: 8 tokens 9.2, with values 11.3.
 // A CTA for every tile, each making its codes, took 21.5 there.
-#include "lq_layer.cuh"
+#include "lq_lora.cuh"
 #include "lq_tc.cuh"
 
 namespace lq {
@@ -107,8 +107,8 @@ static __host__ __device__ __forceinline__ int code_pitch(int K) {  // of codes 
   return p % 128 ? p : p + 64;
 }
 
-template <int MT, typename TO, typename TX, int PV>
-__global__ void __launch_bounds__(std::is_same_v<TX, int8_t> ? 256 : 512, 2) int8_linear_few_kernel(const lq_linear_problem p, const Values values) {
+template <int MT, typename TO, typename TX, int PV, bool LORA>
+__global__ void __launch_bounds__(std::is_same_v<TX, int8_t> ? 256 : 512, 2) int8_linear_few_kernel(const lq_linear_problem p, const Values values, const Lora lora) {
   constexpr bool VALUES = !std::is_same_v<TX, int8_t>;
   constexpr int WARPS = VALUES ? 16 : 8;  // making codes takes instructions
   extern __shared__ __align__(128) int8_t dyn[];
@@ -151,6 +151,8 @@ __global__ void __launch_bounds__(std::is_same_v<TX, int8_t> ? 256 : 512, 2) int
   const int m = tid >> 4;
   const bool mine = m < p.M;
   const float xs = !VALUES && mine ? __ldg(p.x_scale + m) : 0.f;
+  int adapter = -1;
+  if constexpr (LORA) adapter = mine ? lora.of(m) : -1;
   if constexpr (VALUES)
     quantize_rows_shared<TX, PV, WARPS>(reinterpret_cast<const TX*>(values.x), values.stride, p.M, p.K, codes, pitch, scales, amax);
   else
@@ -169,6 +171,8 @@ __global__ void __launch_bounds__(std::is_same_v<TX, int8_t> ? 256 : 512, 2) int
     if (at.chunk == 0 && mine && on < p.N) {
       ws = __ldg(p.w_scale + on);
       bias = p.bias ? __ldg(p.bias + on) : 0.f;
+      if constexpr (LORA)
+        if (adapter >= 0) lora_prefetch(lora, (long long)adapter * p.N + on);
     }
     constexpr int U = (KC / 64 + WARPS - 1) / WARPS;
     uint4 b[U][MT];
@@ -218,7 +222,10 @@ __global__ void __launch_bounds__(std::is_same_v<TX, int8_t> ? 256 : 512, 2) int
       int s = 0;
 #pragma unroll
       for (int v = 0; v < WARPS; ++v) s += part[v][m][tid & 15];
-      reinterpret_cast<TO*>(p.y)[(size_t)m * p.N + on] = from_f32<TO>(fmaf((float)s * (VALUES ? scales[m] : xs), ws, bias));
+      float y = fmaf((float)s * (VALUES ? scales[m] : xs), ws, bias);
+      if constexpr (LORA)
+        if (adapter >= 0) y += lora_dot(lora, adapter, p.N, m, on);
+      reinterpret_cast<TO*>(p.y)[(size_t)m * p.N + on] = from_f32<TO>(y);
     }
   }
 }
@@ -227,22 +234,27 @@ constexpr int CODES = 120 * 1024;  // bytes of codes that a CTA makes at most, n
 
 // The opt-in to shared memory is a kernel's most and not what a call needs: it belongs to the kernel on its device, and another
 // thread's smaller call between this one's opt-in and its launch would have the launch refused.
-template <int MT, typename TO, typename TX, int PV>
-static int launch_few(const lq_linear_problem* p, const Values& v, cudaStream_t st) {
+template <int MT, typename TO, typename TX, int PV, bool LORA>
+static int launch_few_with(const lq_linear_problem* p, const Values& v, const Lora& lora, cudaStream_t st) {
   constexpr bool VALUES = !std::is_same_v<TX, int8_t>;
   constexpr int most_smem = 2 * 16 * WP + (VALUES ? CODES : 0);
   const size_t smem = 2 * 16 * WP + (VALUES ? (size_t)p->M * code_pitch(p->K) : 0);
-  auto kern = int8_linear_few_kernel<MT, TO, TX, PV>;
+  auto kern = int8_linear_few_kernel<MT, TO, TX, PV, LORA>;
   const int threads = VALUES ? 512 : 256;
   int per_sm = 0;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, most_smem);
   if (e == cudaSuccess) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, threads, smem);
   if (e == cudaSuccess) {
     const int tiles = (p->N + 15) / 16, most = sm_count() * per_sm;
-    e = launch(kern, dim3(tiles < most ? tiles : most), dim3(threads), smem, st, *p, v);
+    e = launch(kern, dim3(tiles < most ? tiles : most), dim3(threads), smem, st, *p, v, lora);
   }
   if (e != cudaSuccess) return fail(LQ_ERR_LAUNCH, "int8_linear: %s", cudaGetErrorString(e));
   return check_launch("int8_linear_few_kernel");
+}
+
+template <int MT, typename TO, typename TX, int PV>
+static int launch_few(const lq_linear_problem* p, const Values& v, const Lora* lora, cudaStream_t st) {
+  return lora ? launch_few_with<MT, TO, TX, PV, true>(p, v, *lora, st) : launch_few_with<MT, TO, TX, PV, false>(p, v, {}, st);
 }
 
 static int check(const lq_linear_problem* p) {
@@ -259,34 +271,25 @@ static int check(const lq_linear_problem* p) {
 
 }  // namespace linear
 
-int run_linear_tc(const lq_linear_problem* p, cudaStream_t st);  // lq_linear_tc.cu
+int run_linear_tc(const lq_linear_problem* p, const Lora* lora, cudaStream_t st);  // lq_linear_tc.cu
 
-}  // namespace lq
+int check_linear(const lq_linear_problem* p) { return linear::check(p); }
 
-extern "C" int lq_int8_linear(const lq_linear_problem* p, lq_stream stream) {
-  using namespace lq;
-  if (int e = linear::check(p)) return e;
-  if (p->M == 0) return LQ_OK;
-  cudaStream_t st = (cudaStream_t)stream;
-  if (p->M > 16) return run_linear_tc(p, st);  // 5120 -> 2560 channels: 8 tokens 7.0 us here, 16 9.5, there 11.7 (7.9 from 32 on)
+// `lora`: what low-rank adapters add, or null
+int run_linear(const lq_linear_problem* p, const Lora* lora, cudaStream_t st) {
+  if (p->M > 16) return run_linear_tc(p, lora, st);  // 5120 -> 2560 channels: 8 tokens 7.0 us here, 16 9.5, there 11.7 (7.9 from 32 on)
   return with_dtype(p->out_dtype, "int8_linear", [&](auto t) {
     using TO = decltype(t);
-    return p->M <= 8 ? linear::launch_few<1, TO, int8_t, 1>(p, {}, st) : linear::launch_few<2, TO, int8_t, 1>(p, {}, st);
+    return p->M <= 8 ? linear::launch_few<1, TO, int8_t, 1>(p, {}, lora, st) : linear::launch_few<2, TO, int8_t, 1>(p, {}, lora, st);
   });
 }
 
-extern "C" int lq_int8_linear_values(const lq_linear_problem* p, const void* values, int dtype, long long stride, lq_stream stream) {
-  using namespace lq;
-  if (int e = linear::check(p)) return e;
-  if (dtype < LQ_F16 || dtype > LQ_F32) return fail(LQ_ERR_UNSUPPORTED, "int8_linear_values: dtype %d", dtype);
-  if (p->M == 0) return LQ_OK;
-  if (!values) return fail(LQ_ERR_NULL, "int8_linear_values: values is null");
-  cudaStream_t st = (cudaStream_t)stream;
+int run_linear_values(const lq_linear_problem* p, const Lora* lora, const void* values, int dtype, long long stride, cudaStream_t st) {
   // up to eight tokens whose codes fit a CTA's shared memory next to the weights: one launch, and 8.1 us against 9.5 (1 token), 10.8
   // against 10.2 (5), 11.3 against 10.2 (8) at 5120 -> 2560, where the host's 2 us for another launch are not counted
   if (p->M > 8 || (long long)p->M * linear::code_pitch(p->K) > linear::CODES) {
-    if (int e = lq_quantize_rows(values, dtype, p->M, p->K, stride, const_cast<int8_t*>(p->x), p->x_stride, const_cast<float*>(p->x_scale), stream)) return e;
-    return lq_int8_linear(p, stream);
+    if (int e = lq_quantize_rows(values, dtype, p->M, p->K, stride, const_cast<int8_t*>(p->x), p->x_stride, const_cast<float*>(p->x_scale), (lq_stream)st)) return e;
+    return run_linear(p, lora, st);
   }
   return with_dtype(dtype, "int8_linear_values", [&](auto x) {
     using TX = decltype(x);
@@ -296,7 +299,23 @@ extern "C" int lq_int8_linear_values(const lq_linear_problem* p, const void* val
     return with_dtype(p->out_dtype, "int8_linear_values", [&](auto t) {
       using TO = decltype(t);
       const linear::Values v{values, stride};
-      return wide ? linear::launch_few<1, TO, TX, FULL>(p, v, st) : linear::launch_few<1, TO, TX, 1>(p, v, st);
+      return wide ? linear::launch_few<1, TO, TX, FULL>(p, v, lora, st) : linear::launch_few<1, TO, TX, 1>(p, v, lora, st);
     });
   });
+}
+
+}  // namespace lq
+
+extern "C" int lq_int8_linear(const lq_linear_problem* p, lq_stream stream) {
+  if (int e = lq::linear::check(p)) return e;
+  return p->M == 0 ? LQ_OK : lq::run_linear(p, nullptr, (cudaStream_t)stream);
+}
+
+extern "C" int lq_int8_linear_values(const lq_linear_problem* p, const void* values, int dtype, long long stride, lq_stream stream) {
+  using namespace lq;
+  if (int e = linear::check(p)) return e;
+  if (dtype < LQ_F16 || dtype > LQ_F32) return fail(LQ_ERR_UNSUPPORTED, "int8_linear_values: dtype %d", dtype);
+  if (p->M == 0) return LQ_OK;
+  if (!values) return fail(LQ_ERR_NULL, "int8_linear_values: values is null");
+  return run_linear_values(p, nullptr, values, dtype, stride, (cudaStream_t)stream);
 }

@@ -10,7 +10,7 @@
 // torch's INT8 product reaches is 2.94 with INT32 outputs and no scales.
 // Every wait is bounded; on expiry the CTA raises the status word, lets its copies and products land, frees its tensor
 // memory and returns.
-#include "lq_layer.cuh"
+#include "lq_lora.cuh"
 #include "lq_tc.cuh"
 
 namespace lq {
@@ -39,6 +39,11 @@ __device__ __forceinline__ void mbar_expect(uint32_t bar, uint32_t bytes) {
 __device__ __forceinline__ float4 lds_f4(uint32_t addr) {
   float4 v;
   asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];\n" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr));
+  return v;
+}
+__device__ __forceinline__ float2 lds_f2(uint32_t addr) {
+  float2 v;
+  asm volatile("ld.shared.v2.f32 {%0,%1}, [%2];\n" : "=f"(v.x), "=f"(v.y) : "r"(addr));
   return v;
 }
 __device__ __forceinline__ uint4 lds_u4(uint32_t addr) {
@@ -130,9 +135,9 @@ __device__ __forceinline__ void tile_at(int t, int mt, int nt, int& m, int& n) {
   m = g * GROUP + in - n * rows;
 }
 
-template <int BN, bool PAIR, typename TO>
+template <int BN, bool PAIR, typename TO, bool LORA>
 __global__ void __launch_bounds__(THREADS, 1) int8_linear_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
-                                                                    const lq_linear_problem p) {
+                                                                    const lq_linear_problem p, const Lora lora) {
   using S = Shape<BN, PAIR>;
   constexpr int CTAS = PAIR ? 2 : 1;
   extern __shared__ uint8_t smem_dyn[];
@@ -237,33 +242,75 @@ __global__ void __launch_bounds__(THREADS, 1) int8_linear_tc_kernel(const __grid
 #pragma unroll 1
       for (int c0 = 0; c0 < S::HALF; c0 += CHUNK) {
         if (n0 + c0 >= p.N) break;
-        uint32_t r[CHUNK];
-        const uint32_t from = tbase + ((uint32_t)(32 * quad) << 16) + acc * BN + half + c0;
-        if constexpr (CHUNK == 32) tmem_ld_32x32b_x32(from, r);
-        else tmem_ld_32x32b_x16(from, r);
-        asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
-        float v[CHUNK];
-#pragma unroll
-        for (int j = 0; j < CHUNK; j += 4) {
-          const float4 ws = lds_f4(cols + 4 * (c0 + j)), b = lds_f4(cols + 4 * (S::HALF + c0 + j));
-          v[j] = fmaf((float)(int)r[j] * xs, ws.x, b.x);
-          v[j + 1] = fmaf((float)(int)r[j + 1] * xs, ws.y, b.y);
-          v[j + 2] = fmaf((float)(int)r[j + 2] * xs, ws.z, b.z);
-          v[j + 3] = fmaf((float)(int)r[j + 3] * xs, ws.w, b.w);
-        }
-        __syncwarp();  // the chunk before has been read
         // rows of 64 bytes, pairs of them on the same banks: a piece at its place exclusive-or half the row's number
         auto place = [](int row, int piece) { return row * 64 + ((piece ^ ((row >> 1) & 3)) << 4); };
+        if constexpr (LORA) {  // fragments of m16n8 products: the adapters' sums are added to them
+          constexpr int NT = CHUNK / 8;
+          uint32_t r[2][CHUNK / 2];
 #pragma unroll
-        for (int j = 0; j < CHUNK; j += PER) {
-          uint4 w;
-          if constexpr (sizeof(TO) == 4) {
-            w = make_uint4(__float_as_uint(v[j]), __float_as_uint(v[j + 1]), __float_as_uint(v[j + 2]), __float_as_uint(v[j + 3]));
-          } else {
-            w = make_uint4(Act<TO>::pack2(v[j], v[j + 1]), Act<TO>::pack2(v[j + 2], v[j + 3]), Act<TO>::pack2(v[j + 4], v[j + 5]),
-                           Act<TO>::pack2(v[j + 6], v[j + 7]));
+          for (int i = 0; i < 2; ++i) {
+            const uint32_t from = tbase + ((uint32_t)(32 * quad + 16 * i) << 16) + acc * BN + half + c0;
+            if constexpr (CHUNK == 32) tmem_ld_16x256b_x4(from, r[i]);
+            else tmem_ld_16x256b_x2(from, r[i]);
           }
-          sts_u4(out + place(lane, j / PER), w);
+          asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
+          const int g = lane >> 2, t4 = lane & 3;
+          float v[2][NT][4];
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const float xs0 = __shfl_sync(0xffffffffu, xs, 16 * i + g), xs1 = __shfl_sync(0xffffffffu, xs, 16 * i + g + 8);
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+              const float2 ws = lds_f2(cols + 4 * (c0 + 8 * j + 2 * t4)), b = lds_f2(cols + 4 * (S::HALF + c0 + 8 * j + 2 * t4));
+              v[i][j][0] = fmaf((float)(int)r[i][4 * j] * xs0, ws.x, b.x);
+              v[i][j][1] = fmaf((float)(int)r[i][4 * j + 1] * xs0, ws.y, b.y);
+              v[i][j][2] = fmaf((float)(int)r[i][4 * j + 2] * xs1, ws.x, b.x);
+              v[i][j][3] = fmaf((float)(int)r[i][4 * j + 3] * xs1, ws.y, b.y);
+            }
+          }
+          lora_add<NT, sizeof(TO) == 4 ? 3 : 2>(v, lora, p.M, p.N, row0, n0 + c0);
+          __syncwarp();  // the chunk before has been read
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int j = 0; j < NT; ++j)
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                const int row = 16 * i + g + 8 * h;
+                if constexpr (sizeof(TO) == 4) {
+                  sts_u32(out + place(row, 2 * j + (t4 >> 1)) + 8 * (t4 & 1), __float_as_uint(v[i][j][2 * h]));
+                  sts_u32(out + place(row, 2 * j + (t4 >> 1)) + 8 * (t4 & 1) + 4, __float_as_uint(v[i][j][2 * h + 1]));
+                } else {
+                  sts_u32(out + place(row, j) + 4 * t4, Act<TO>::pack2(v[i][j][2 * h], v[i][j][2 * h + 1]));
+                }
+              }
+        } else {
+          uint32_t r[CHUNK];
+          const uint32_t from = tbase + ((uint32_t)(32 * quad) << 16) + acc * BN + half + c0;
+          if constexpr (CHUNK == 32) tmem_ld_32x32b_x32(from, r);
+          else tmem_ld_32x32b_x16(from, r);
+          asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
+          float v[CHUNK];
+#pragma unroll
+          for (int j = 0; j < CHUNK; j += 4) {
+            const float4 ws = lds_f4(cols + 4 * (c0 + j)), b = lds_f4(cols + 4 * (S::HALF + c0 + j));
+            v[j] = fmaf((float)(int)r[j] * xs, ws.x, b.x);
+            v[j + 1] = fmaf((float)(int)r[j + 1] * xs, ws.y, b.y);
+            v[j + 2] = fmaf((float)(int)r[j + 2] * xs, ws.z, b.z);
+            v[j + 3] = fmaf((float)(int)r[j + 3] * xs, ws.w, b.w);
+          }
+          __syncwarp();  // the chunk before has been read
+#pragma unroll
+          for (int j = 0; j < CHUNK; j += PER) {
+            uint4 w;
+            if constexpr (sizeof(TO) == 4) {
+              w = make_uint4(__float_as_uint(v[j]), __float_as_uint(v[j + 1]), __float_as_uint(v[j + 2]), __float_as_uint(v[j + 3]));
+            } else {
+              w = make_uint4(Act<TO>::pack2(v[j], v[j + 1]), Act<TO>::pack2(v[j + 2], v[j + 3]), Act<TO>::pack2(v[j + 4], v[j + 5]),
+                             Act<TO>::pack2(v[j + 6], v[j + 7]));
+            }
+            sts_u4(out + place(lane, j / PER), w);
+          }
         }
         __syncwarp();
         TO* y = reinterpret_cast<TO*>(p.y);
@@ -329,9 +376,9 @@ __device__ __forceinline__ int4 ld_cluster(uint32_t addr) {
   return v;
 }
 
-template <typename TO>
+template <typename TO, bool LORA>
 __global__ void __launch_bounds__(THREADS, 2) int8_linear_split_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
-                                                                       const lq_linear_problem p, int parts) {
+                                                                       const lq_linear_problem p, int parts, const Lora lora) {
   using S = Split;
   extern __shared__ uint8_t smem_dyn[];
   const uint32_t s_stage = (smem_u32(smem_dyn) + 1023u) & ~1023u, s_full = s_stage + S::STAGES * S::STAGE, s_empty = s_full + 8 * S::STAGES;
@@ -422,8 +469,15 @@ __global__ void __launch_bounds__(THREADS, 2) int8_linear_split_kernel(const __g
         const int4 v = ld_cluster(in_cta(s_stage + row * S::PITCH + 4 * c, q));
         sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
       }
-      const float f[4] = {fmaf((float)sum.x * xs[i], ws[0], bias[0]), fmaf((float)sum.y * xs[i], ws[1], bias[1]), fmaf((float)sum.z * xs[i], ws[2], bias[2]),
-                          fmaf((float)sum.w * xs[i], ws[3], bias[3])};
+      float f[4] = {fmaf((float)sum.x * xs[i], ws[0], bias[0]), fmaf((float)sum.y * xs[i], ws[1], bias[1]), fmaf((float)sum.z * xs[i], ws[2], bias[2]),
+                    fmaf((float)sum.w * xs[i], ws[3], bias[3])};
+      if constexpr (LORA) {
+        const int l = lora.of(m0 + row);
+        if (l >= 0)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (n + j < p.N) f[j] += lora_dot(lora, l, p.N, m0 + row, n + j);
+      }
       TO* to = y + (size_t)(m0 + row) * p.N + n;
       if (wide) {
         Pack<TO, 4> out;
@@ -476,7 +530,7 @@ static int launch_clusters(void (*kern)(KArgs...), int ctas, int cluster, size_t
 }
 
 template <int BN, bool PAIR, typename TO>
-static int launch_tc(const lq_linear_problem* p, cudaStream_t st) {
+static int launch_tc(const lq_linear_problem* p, const Lora* lora, cudaStream_t st) {
   using S = Shape<BN, PAIR>;
   constexpr int CTAS = PAIR ? 2 : 1;
   CUtensorMap mx, mw;
@@ -485,22 +539,25 @@ static int launch_tc(const lq_linear_problem* p, cudaStream_t st) {
   const long long tiles = (long long)((p->M + CTAS * BM - 1) / (CTAS * BM)) * ((p->N + BN - 1) / BN);
   if (tiles >= 1ll << 29) return fail(LQ_ERR_SHAPE, "int8_linear: M=%d N=%d", p->M, p->N);
   const int units = sm_count() / CTAS;
-  return launch_clusters(int8_linear_tc_kernel<BN, PAIR, TO>, CTAS * (int)(tiles < units ? tiles : units), CTAS, S::SMEM, st, mx, mw, *p);
+  const int ctas = CTAS * (int)(tiles < units ? tiles : units);
+  if (lora) return launch_clusters(int8_linear_tc_kernel<BN, PAIR, TO, true>, ctas, CTAS, S::SMEM, st, mx, mw, *p, *lora);
+  return launch_clusters(int8_linear_tc_kernel<BN, PAIR, TO, false>, ctas, CTAS, S::SMEM, st, mx, mw, *p, Lora{});
 }
 
 template <typename TO>
-static int launch_split(const lq_linear_problem* p, int tiles, int parts, cudaStream_t st) {
+static int launch_split(const lq_linear_problem* p, const Lora* lora, int tiles, int parts, cudaStream_t st) {
   CUtensorMap mx, mw;
   if (int e = encode(&mx, p->x, p->K, p->x_stride, p->M, BM)) return e;
   if (int e = encode(&mw, p->w, p->K, p->w_stride, p->N, Split::BN)) return e;
-  return launch_clusters(int8_linear_split_kernel<TO>, tiles * parts, parts, Split::SMEM, st, mx, mw, *p, parts);
+  if (lora) return launch_clusters(int8_linear_split_kernel<TO, true>, tiles * parts, parts, Split::SMEM, st, mx, mw, *p, parts, *lora);
+  return launch_clusters(int8_linear_split_kernel<TO, false>, tiles * parts, parts, Split::SMEM, st, mx, mw, *p, parts, Lora{});
 }
 
 }  // namespace lineartc
 
 // The widest tiles that do not leave SMs idle: rounds of tiles x the time of one, which grows with its width and a fixed part
 // (the 128 rows of x that every tile loads)
-int run_linear_tc(const lq_linear_problem* p, cudaStream_t st) {
+int run_linear_tc(const lq_linear_problem* p, const Lora* lora, cudaStream_t st) {
   const long long mt = (p->M + 127) / 128, sms = sm_count();
   int best = 256;
   long long least = 0;
@@ -519,9 +576,9 @@ int run_linear_tc(const lq_linear_problem* p, cudaStream_t st) {
   while (parts > 1 && (narrow * parts > 2 * sms || blocks < 8 * parts)) parts /= 2;
   return with_dtype(p->out_dtype, "int8_linear", [&](auto t) {
     using TO = decltype(t);
-    if (parts > 1) return lineartc::launch_split<TO>(p, (int)narrow, parts, st);
-    if (pair) return lineartc::launch_tc<256, true, TO>(p, st);
-    return best == 256 ? lineartc::launch_tc<256, false, TO>(p, st) : best == 128 ? lineartc::launch_tc<128, false, TO>(p, st) : lineartc::launch_tc<64, false, TO>(p, st);
+    if (parts > 1) return lineartc::launch_split<TO>(p, lora, (int)narrow, parts, st);
+    if (pair) return lineartc::launch_tc<256, true, TO>(p, lora, st);
+    return best == 256 ? lineartc::launch_tc<256, false, TO>(p, lora, st) : best == 128 ? lineartc::launch_tc<128, false, TO>(p, lora, st) : lineartc::launch_tc<64, false, TO>(p, lora, st);
   });
 }
 

@@ -1,0 +1,277 @@
+// INT8 product with low-rank adapters of many requests at once.
+//
+//   y[m,n] = (sum_k c[m,k] w[n,k]) x_scale[m] w_scale[n] + bias[n] + sum_r t[m,r] b[l,n,r],   t[m,r] = scaling[l] sum_k x[m,k] a[l,r,k]
+//
+// l = adapters[m]; c are x's codes. Two kernels: this file's makes t, the INT8 product's own kernels add the second sum to a tile while it
+// is still fp32 (lq_lora.cuh), so y is rounded and written once.
+// t: a CTA has a tile of 1, 16 or 64 tokens (32 of three pieces) and, of a cluster, a part of K; its four warps share that part and their sums meet in
+// shared memory, first the warps', then the CTAs', in a fixed order. Operands come from global memory straight into the fragments
+// of m16n8k16 (the reduction index permuted alike in both: a lane takes eight consecutive k). A tile whose tokens have several
+// adapters goes over its K once for each of them. Products are exact: both operands as bf16 pieces (codes and bf16 one, fp16 two, fp32
+// three; codes or fp16 with fp16 as they are), six products for fp32.
+#include "lq_lora.cuh"
+#include "lq_tc.cuh"
+
+namespace lq {
+
+namespace lora {
+
+constexpr int WARPS = 4, THREADS = 32 * WARPS, NT = 8;  // NT: tiles of 8 ranks at a time
+
+template <typename TX, typename TA>
+struct Types {
+  static constexpr bool F16 = std::is_same_v<TA, __half> && (std::is_same_v<TX, __half> || std::is_same_v<TX, int8_t>);
+  template <typename T>
+  static constexpr int pieces() { return F16 ? 1 : sizeof(T) == 4 ? 3 : std::is_same_v<T, __half> ? 2 : 1; }
+  static constexpr int NX = pieces<TX>(), NA = pieces<TA>(), KEEP = NX > NA ? NX : NA;
+};
+
+// eight consecutive values from p as words of pairs, in pieces; VEC: p on a boundary of eight values (16 bytes at most)
+template <typename T, int N, bool F16, bool VEC>
+__device__ __forceinline__ void load8(const T* p, int left, uint32_t (&w)[N][4]) {
+  float x[8];
+  if constexpr (VEC && sizeof(T) == 2 && N == 1) {  // as they are
+    const uint4 v = left > 0 ? __ldg(reinterpret_cast<const uint4*>(p)) : make_uint4(0, 0, 0, 0);
+    w[0][0] = v.x, w[0][1] = v.y, w[0][2] = v.z, w[0][3] = v.w;
+    return;
+  } else if constexpr (VEC && std::is_same_v<T, int8_t>) {
+    const uint2 v = left > 0 ? __ldg(reinterpret_cast<const uint2*>(p)) : make_uint2(0, 0);
+    const uint32_t a = v.x ^ 0x80808080u, b = v.y ^ 0x80808080u;
+    x[0] = s8_to_float<0>(a), x[1] = s8_to_float<1>(a), x[2] = s8_to_float<2>(a), x[3] = s8_to_float<3>(a);
+    x[4] = s8_to_float<0>(b), x[5] = s8_to_float<1>(b), x[6] = s8_to_float<2>(b), x[7] = s8_to_float<3>(b);
+  } else if constexpr (VEC && sizeof(T) == 2) {
+    const uint4 v = left > 0 ? __ldg(reinterpret_cast<const uint4*>(p)) : make_uint4(0, 0, 0, 0);
+    Act<T>::unpack8(v, x);
+  } else if constexpr (VEC) {
+    const float4 z = make_float4(0.f, 0.f, 0.f, 0.f), a = left > 0 ? __ldg(reinterpret_cast<const float4*>(p)) : z, b = left > 0 ? __ldg(reinterpret_cast<const float4*>(p) + 1) : z;
+    x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if constexpr (std::is_same_v<T, int8_t>) x[i] = i < left ? (float)__ldg(p + i) : 0.f;
+      else x[i] = i < left ? to_f32(p[i]) : 0.f;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (F16) {
+      w[0][i] = Act<__half>::pack2(x[2 * i], x[2 * i + 1]);
+    } else {
+      uint32_t q[N];
+      bf16_pieces<N>(x[2 * i], x[2 * i + 1], q);
+#pragma unroll
+      for (int k = 0; k < N; ++k) w[k][i] = q[k];
+    }
+  }
+}
+
+struct Shrink {
+  int M, K, L, R, RP, parts;
+  long long x_stride;          // elements
+  const void *x, *a;
+  const float* x_scale;        // of codes, or null
+  const int* adapters;
+  const float* scaling;        // [L] or null
+  float scale;
+  float* t;
+};
+
+// TILE: tokens of a CTA
+template <typename TX, typename TA, int TILE, bool VEC>
+__global__ void __launch_bounds__(THREADS) lora_shrink_kernel(const Shrink p) {
+  using Y = Types<TX, TA>;
+  constexpr int MT = (TILE + 15) / 16, ROWS = 16 * MT;
+  extern __shared__ __align__(16) float sums[];  // [WARPS][TILE][RP], then the CTA's own in the first
+  __shared__ int which[ROWS];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
+  const int rank = blockIdx.x % p.parts, m0 = blockIdx.x / p.parts * TILE;
+  pdl_enter();
+  for (int i = tid; i < ROWS; i += THREADS) {
+    const int l = i < TILE && m0 + i < p.M ? __ldg(p.adapters + m0 + i) : -1;
+    which[i] = (unsigned)l < (unsigned)p.L ? l : -1;
+  }
+  for (int i = tid; i < WARPS * TILE * p.RP; i += THREADS) sums[i] = 0.f;
+  __syncthreads();
+  const int steps = (p.K + 31) / 32, step0 = (int)((long long)steps * rank / p.parts), step1 = (int)((long long)steps * (rank + 1) / p.parts);
+  int l = -1;
+  while (true) {
+    // the next adapter of the tile, in rising order
+    int next = 0x7fffffff;
+    for (int i = lane; i < ROWS; i += 32)
+      if (which[i] > l) next = min(next, which[i]);
+    l = __reduce_min_sync(0xffffffffu, next);
+    if (l == 0x7fffffff) break;
+    for (int r0 = 0; r0 < p.R; r0 += 8 * NT) {
+      const int tiles = min(NT, (p.R - r0) / 8);
+      float acc[MT][NT][4];
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[i][j][e] = 0.f;
+      const TA* a = reinterpret_cast<const TA*>(p.a) + ((long long)l * p.R + r0 + g) * p.K;
+      const TX* x = reinterpret_cast<const TX*>(p.x);
+#pragma unroll 2
+      for (int s = step0 + warp; s < step1; s += WARPS) {
+        const int k = 32 * s + 8 * t4, left = p.K - k;
+        uint32_t xa[MT][2][Y::NX][4];
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int row = 16 * i + 8 * h + g;
+            // a token with another adapter is not read for this one
+            load8<TX, Y::NX, Y::F16, VEC>(x + (long long)(m0 + row) * p.x_stride + k, which[row] == l ? left : 0, xa[i][h]);
+          }
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+          if (j >= tiles) break;
+          uint32_t b[Y::NA][4];
+          load8<TA, Y::NA, Y::F16, VEC>(a + 8ll * j * p.K + k, left, b);
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int n = Y::NA - 1; n >= 0; --n)
+#pragma unroll
+              for (int o = Y::NX - 1; o >= 0; --o) {
+                if (n + o >= (Y::KEEP > 1 ? 3 : 1)) continue;
+#pragma unroll
+                for (int i = 0; i < MT; ++i) {
+                  if constexpr (Y::F16) mma_f16(acc[i][j], xa[i][0][o][2 * h], xa[i][1][o][2 * h], xa[i][0][o][2 * h + 1], xa[i][1][o][2 * h + 1], b[n][2 * h], b[n][2 * h + 1]);
+                  else mma_bf16(acc[i][j], xa[i][0][o][2 * h], xa[i][1][o][2 * h], xa[i][0][o][2 * h + 1], xa[i][1][o][2 * h + 1], b[n][2 * h], b[n][2 * h + 1]);
+                }
+              }
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int row = 16 * i + g + 8 * (e >> 1), r = r0 + 8 * j + 2 * t4 + (e & 1);
+            if (row < TILE && j < tiles && which[row] == l) sums[(warp * TILE + row) * p.RP + r] = acc[i][j][e];
+          }
+    }
+  }
+  __syncthreads();
+  const int values = TILE * p.RP;
+  for (int i = tid; i < values; i += THREADS) {
+    float s = sums[i];
+#pragma unroll
+    for (int w = 1; w < WARPS; ++w) s += sums[w * values + i];
+    sums[i] = s;
+  }
+  if (p.parts > 1) asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+  else __syncthreads();
+  const uint32_t base = smem_u32(sums);
+  for (int i = rank * THREADS + tid; i < values; i += p.parts * THREADS) {
+    const int row = i / p.RP, m = m0 + row;
+    if (m >= p.M) continue;
+    float s = 0.f;
+    for (int c = 0; c < p.parts; ++c) {
+      float v;
+      uint32_t at;
+      if (p.parts > 1) {
+        asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(at) : "r"(base + 4 * i), "r"(c));
+        asm volatile("ld.shared::cluster.f32 %0, [%1];\n" : "=f"(v) : "r"(at) : "memory");
+      } else {
+        v = sums[i];
+      }
+      s += v;
+    }
+    const int own = which[row];
+    if (own >= 0) {
+      s *= p.scaling ? p.scale * __ldg(p.scaling + own) : p.scale;
+      if (p.x_scale) s *= __ldg(p.x_scale + m);
+    }
+    p.t[(long long)m * p.RP + i - row * p.RP] = s;
+  }
+  if (p.parts > 1) asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");  // no CTA's sums are read any more
+}
+
+template <typename TX, typename TA, int TILE, bool VEC>
+static int shrink(const Shrink& p, int tiles, cudaStream_t st) {
+  auto kern = lora_shrink_kernel<TX, TA, TILE, VEC>;
+  constexpr int most = WARPS * TILE * 128 * 4;
+  cudaError_t e = cudaSuccess;
+  if (most > 48 * 1024) e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+  if (e == cudaSuccess) {
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = p.parts;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)tiles * p.parts);
+    cfg.blockDim = dim3(THREADS);
+    cfg.dynamicSmemBytes = (size_t)WARPS * TILE * p.RP * 4;
+    cfg.stream = st;
+    cfg.attrs = attr;
+    cfg.numAttrs = p.parts > 1 ? 2 : 1;
+    e = cudaLaunchKernelEx(&cfg, kern, p);
+  }
+  if (e != cudaSuccess) return fail(LQ_ERR_LAUNCH, "lora_linear: %s", cudaGetErrorString(e));
+  return check_launch("lora_shrink_kernel");
+}
+
+// Tokens of a CTA: one each for a decode step, whose tokens have adapters of their own; 64 or 32 where that still leaves two CTAs an SM.
+// Parts of K: two CTAs an SM, and no fewer than 128 of K for a warp.
+template <typename TX, typename TA>
+static int run_shrink(Shrink p, bool vec, cudaStream_t st) {
+  constexpr int BIG = Types<TX, TA>::KEEP == 3 ? 32 : 64;  // three pieces of 64 tokens would not fit a thread's registers
+  const int sms = sm_count(), tile = p.M <= 64 ? 1 : p.M >= 2 * BIG * sms ? BIG : 16, tiles = (p.M + tile - 1) / tile;
+  p.parts = 8;
+  while (p.parts > 1 && ((long long)tiles * p.parts > 4ll * sms || p.K < 512 * p.parts)) p.parts /= 2;
+  auto go = [&](auto v) {
+    constexpr bool VEC = decltype(v)::value;
+    if (tile == 1) return shrink<TX, TA, 1, VEC>(p, tiles, st);
+    if (tile == 16) return shrink<TX, TA, 16, VEC>(p, tiles, st);
+    return shrink<TX, TA, BIG, VEC>(p, tiles, st);
+  };
+  return vec ? go(std::true_type()) : go(std::false_type());
+}
+
+}  // namespace lora
+
+int run_linear(const lq_linear_problem* p, const Lora* lora, cudaStream_t st);                                              // lq_linear.cu
+int run_linear_values(const lq_linear_problem* p, const Lora* lora, const void* values, int dtype, long long stride, cudaStream_t st);
+int check_linear(const lq_linear_problem* p);
+
+}  // namespace lq
+
+extern "C" size_t lq_lora_workspace_bytes(int M, int R) { return M <= 0 || R <= 0 ? 0 : (size_t)M * ((R + 15) / 16 * 16) * 4; }
+
+extern "C" int lq_lora_linear(const lq_linear_problem* p, const lq_lora_problem* q, const void* values, int dtype, long long stride, lq_stream stream) {
+  using namespace lq;
+  if (int e = check_linear(p)) return e;
+  if (!q) return fail(LQ_ERR_NULL, "lora_linear: adapter descriptor is null");
+  if (q->L < 0 || q->R <= 0 || !fits(q->L)) return fail(LQ_ERR_SHAPE, "lora_linear: L=%d R=%d", q->L, q->R);
+  if (q->R % 8 || q->R > 128) return fail(LQ_ERR_UNSUPPORTED, "lora_linear: R=%d, multiples of 8 up to 128", q->R);
+  if (q->dtype < LQ_F16 || q->dtype > LQ_F32) return fail(LQ_ERR_UNSUPPORTED, "lora_linear: dtype %d", q->dtype);
+  if (values && (dtype < LQ_F16 || dtype > LQ_F32)) return fail(LQ_ERR_UNSUPPORTED, "lora_linear: dtype %d", dtype);
+  if (p->M == 0) return LQ_OK;
+  cudaStream_t st = (cudaStream_t)stream;
+  if (q->L == 0) return values ? run_linear_values(p, nullptr, values, dtype, stride, st) : run_linear(p, nullptr, st);
+  if (!q->a || !q->b || !q->adapters || !q->t) return fail(LQ_ERR_NULL, "lora_linear: a, b, adapters and t must be non-null");
+  if ((reinterpret_cast<uintptr_t>(q->b) | reinterpret_cast<uintptr_t>(q->t)) & 15u) return fail(LQ_ERR_ALIGN, "lora_linear: b and t start on 16-byte boundaries");
+  const int RP = (q->R + 15) / 16 * 16, size = dtype_bytes(q->dtype);
+  const lora::Shrink s{p->M, p->K, q->L, q->R, RP, 1, values ? stride : p->x_stride, values ? values : p->x, q->a, values ? nullptr : p->x_scale,
+                       q->adapters, q->scaling, q->scale, q->t};
+  Alignment a;
+  a.at(q->a).pitch(p->K, size);
+  Alignment x;
+  if (values) x.at(values).pitch(stride, dtype_bytes(dtype)).pitch(p->K, dtype_bytes(dtype));
+  // eight values are one or two accesses of 16 bytes and never leave their row (codes: one of 8, their rows start on 16)
+  const bool vec = a.bytes() == 16 && (size == 2 || p->K % 8 == 0) && (values ? x.bytes() == 16 && p->K % 8 == 0 : true);
+  const int e = with_dtype(q->dtype, "lora_linear", [&](auto ta) {
+    using TA = decltype(ta);
+    if (!values) return lora::run_shrink<int8_t, TA>(s, vec, st);
+    return with_dtype(dtype, "lora_linear", [&](auto tx) { return lora::run_shrink<decltype(tx), TA>(s, vec, st); });
+  });
+  if (e != LQ_OK) return e;
+  const Lora add{q->L, q->R, RP, q->dtype, q->b, q->adapters, q->t};
+  return values ? run_linear_values(p, &add, values, dtype, stride, st) : run_linear(p, &add, st);
+}

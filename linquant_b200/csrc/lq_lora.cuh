@@ -1,0 +1,134 @@
+// Low-rank adapters beside the INT8 product: what its kernels add to a tile of outputs.
+//
+//   y[m,n] += sum_r t[m,r] b[l,n,r],   l = adapters[m],   t[m,r] = scaling[l] x_scale[m] sum_k x[m,k] a[l,r,k]      (lq_lora.cu)
+#pragma once
+#include "lq_layer.cuh"
+
+namespace lq {
+
+struct Lora {
+  int L, R, RP;        // adapters; their rank, a multiple of 8; the pitch of t, a multiple of 16, zero behind R
+  int dtype;           // of b
+  const void* b;       // [L,N,R]
+  const int* adapters; // [M]: which adapter a token has; one outside 0..L-1 is none
+  const float* t;      // [M,RP]
+  __device__ __forceinline__ int of(int m) const {
+    const int l = __ldg(adapters + m);
+    return (unsigned)l < (unsigned)L ? l : -1;
+  }
+};
+
+// b[r .. r + 3] of a row as fp32; r a multiple of 4
+__device__ __forceinline__ void lora_row4(const Lora& q, long long row, int r, float (&x)[4]) {
+  const long long at = row * q.R + r;
+  if (q.dtype == LQ_F32) {
+    const float4 v = __ldg(reinterpret_cast<const float4*>(reinterpret_cast<const float*>(q.b) + at));
+    x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
+  } else {
+    const uint2 v = __ldg(reinterpret_cast<const uint2*>(reinterpret_cast<const uint16_t*>(q.b) + at));
+    if (q.dtype == LQ_F16) {
+      x[0] = Act<__half>::get(v.x, 0), x[1] = Act<__half>::get(v.x, 1), x[2] = Act<__half>::get(v.y, 0), x[3] = Act<__half>::get(v.y, 1);
+    } else {
+      x[0] = Act<__nv_bfloat16>::get(v.x, 0), x[1] = Act<__nv_bfloat16>::get(v.x, 1), x[2] = Act<__nv_bfloat16>::get(v.y, 0), x[3] = Act<__nv_bfloat16>::get(v.y, 1);
+    }
+  }
+}
+
+// A row of b on its way to L2
+__device__ __forceinline__ void lora_prefetch(const Lora& q, long long row) {
+  const int bytes = q.R * (q.dtype == LQ_F32 ? 4 : 2);
+  const char* from = reinterpret_cast<const char*>(q.b) + row * bytes;
+  for (int i = 0; i < bytes; i += 128) asm volatile("prefetch.global.L2 [%0];\n" ::"l"(from + i));
+}
+
+// The sum of one output, in fp32
+__device__ __forceinline__ float lora_dot(const Lora& q, int l, int N, int m, int n) {
+  float s = 0.f;
+  const float* t = q.t + (long long)m * q.RP;
+  const long long row = (long long)l * N + n;
+#pragma unroll 4
+  for (int r = 0; r < q.R; r += 4) {
+    float b[4];
+    lora_row4(q, row, r, b);
+    const float4 v = *reinterpret_cast<const float4*>(t + r);
+    s = fmaf(v.x, b[0], s), s = fmaf(v.y, b[1], s), s = fmaf(v.z, b[2], s), s = fmaf(v.w, b[3], s);
+  }
+  return s;
+}
+
+// fp32 pairs as N pairs of bf16 pieces, the largest first
+template <int N>
+__device__ __forceinline__ void bf16_pieces(float a, float b, uint32_t (&p)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    p[i] = Act<__nv_bfloat16>::pack2(a, b);
+    if (i + 1 < N) a -= __uint_as_float(p[i] << 16), b -= __uint_as_float(p[i] & 0xffff0000u);
+  }
+}
+
+// The sums of 32 tokens (m0 + lane) and 8 NT channels from n0, added to accumulator fragments: v[i][j] has the tokens 16 i + g (+ 8), the
+// channels 8 j + 2 q (+ 1). One pass over R for each adapter that the tokens have. The reduction index is permuted alike in both
+// operands: a lane takes four consecutive r. Both go in as PIECES bf16 pieces, products of pieces that add up to 8 PIECES bits or
+// more behind the first are left out: 16 bits for 16-bit outputs, 24 for fp32.
+template <int NT, int PIECES>
+__device__ __forceinline__ void lora_add(float (&v)[2][NT][4], const Lora& q, int M, int N, int m0, int n0) {
+  const int lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
+  const int mine = m0 + lane < M ? q.of(m0 + lane) : -1;
+  uint32_t left = __ballot_sync(0xffffffffu, mine >= 0);
+  while (left) {
+    const int l = __shfl_sync(0xffffffffu, mine, __ffs(left) - 1);
+    const uint32_t rows = __ballot_sync(0xffffffffu, mine == l);
+    left &= ~rows;
+    float s[2][NT][4];  // apart from the outputs: an infinity or NaN in b is no other adapter's
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[i][j][e] = 0.f;
+    for (int r0 = 0; r0 < q.R; r0 += 16) {
+      const int r = r0 + 4 * t4;
+      float b[NT][4];
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        const int n = n0 + 8 * j + g;
+        if (n < N && r < q.R) lora_row4(q, (long long)l * N + n, r, b[j]);
+        else b[j][0] = b[j][1] = b[j][2] = b[j][3] = 0.f;
+      }
+      uint32_t a[2][PIECES][4];
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int row = 16 * i + 8 * h + g;
+          float4 t = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (rows >> row & 1) t = *reinterpret_cast<const float4*>(q.t + (long long)(m0 + row) * q.RP + r);
+          uint32_t lo[PIECES], hi[PIECES];
+          bf16_pieces<PIECES>(t.x, t.y, lo);
+          bf16_pieces<PIECES>(t.z, t.w, hi);
+#pragma unroll
+          for (int k = 0; k < PIECES; ++k) a[i][k][h] = lo[k], a[i][k][2 + h] = hi[k];
+        }
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        uint32_t lo[PIECES], hi[PIECES];
+        bf16_pieces<PIECES>(b[j][0], b[j][1], lo);
+        bf16_pieces<PIECES>(b[j][2], b[j][3], hi);
+#pragma unroll
+        for (int k = PIECES - 1; k >= 0; --k)
+#pragma unroll
+          for (int o = PIECES - 1 - k; o >= 0; --o)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) mma_bf16(s[i][j], a[i][o][0], a[i][o][1], a[i][o][2], a[i][o][3], lo[k], hi[k]);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[i][j][e] += rows >> (16 * i + g + 8 * (e >> 1)) & 1 ? s[i][j][e] : 0.f;
+  }
+}
+
+}  // namespace lq
