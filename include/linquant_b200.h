@@ -402,6 +402,7 @@ typedef struct {
   void* state;                 /* step: [n_slots,H,K,V] */
   const int* slots;            /* step: as above */
   int n_slots;
+  int* status;                 /* fwd: as in lq_ssd_problem */
 } lq_attention_problem;
 /* S_t = exp(g_t) S_{t-1} + k_t v_t^T;  o_t = scale q_t S_t;  states in fp32. The workspace (0 bytes for many heads) holds the states
  * between the segments of a call's tokens; 16-byte aligned. */

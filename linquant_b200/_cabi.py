@@ -68,7 +68,7 @@ class AttentionProblem(C.Structure):
     _fields_ = _fields(int="B T H Hk K V dtype state_dtype", float="scale",
                        longlong="q_stride_b q_stride_t q_stride_h k_stride_b k_stride_t k_stride_h v_stride_b v_stride_t v_stride_h "
                                 "g_stride_b g_stride_t g_stride_h",
-                       void_p="q k v g initial_state lengths o final_state state slots", int_2="n_slots")
+                       void_p="q k v g initial_state lengths o final_state state slots", int_2="n_slots", void_p_2="status")
 
 
 class GroupNormProblem(C.Structure):

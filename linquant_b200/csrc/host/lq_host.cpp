@@ -704,6 +704,7 @@ PyObject* linear_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
       state = empty({p.B, p.H, p.K, p.V}, at::kFloat, c.dev);
       p.final_state = state.data_ptr<float>();
     }
+    p.status = status_word(c.dev);
     const size_t bytes = lq_linear_attention_workspace_bytes(&p);
     uint8_t* ws = bytes ? aligned(c.hold(scratch(bytes, c.dev))) : nullptr;
     cudaStream_t st = stream_of(c);

@@ -16,8 +16,7 @@
 // step of the type on each term, is of the size of the output's own. fp32 operands are three bf16 pieces each, six products.
 #include <math_constants.h>
 
-#include "lq_layer.cuh"
-#include "lq_tc.cuh"
+#include "lq_linear_attention.cuh"
 
 namespace lq {
 
@@ -38,61 +37,17 @@ __device__ __forceinline__ void cp_async16_zfill(uint32_t dst, const void* src, 
 __device__ __forceinline__ void cp_async4_zfill(uint32_t dst, const void* src, int bytes) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;\n" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
-__device__ __forceinline__ void sts_v4(uint32_t addr, const uint32_t (&v)[4]) {
-  asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};\n" ::"r"(addr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
-}
-__device__ __forceinline__ void lds_v4(uint32_t addr, uint32_t (&v)[4]) {
-  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];\n" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(addr) : "memory");
-}
-__device__ __forceinline__ float lds_f32(uint32_t addr) { return __uint_as_float(lds_u32(addr)); }
-__device__ __forceinline__ float2 lds_f2(uint32_t addr) {
-  float2 v;
-  asm volatile("ld.shared.v2.f32 {%0,%1}, [%2];\n" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
-  return v;
-}
-
 // A tile of 16-bit rows of ROWB bytes: 16-byte pieces exclusive-or the row's number, so that eight rows of a piece lie on banks of their own
 template <int ROWB>
 __device__ __forceinline__ uint32_t at(int row, int piece) {
   return row * ROWB + ((piece ^ (ROWB >= 128 ? row & 7 : (row >> 1) & 3)) << 4);
 }
 
-template <typename T>
-struct Half {  // the 16-bit type of the products
-  using type = T;
-};
-template <>
-struct Half<float> {
-  using type = __nv_bfloat16;
-};
 template <typename M>
 __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   if constexpr (std::is_same_v<M, __half>) mma_f16(c, a[0], a[1], a[2], a[3], b0, b1);
   else mma_bf16(c, a[0], a[1], a[2], a[3], b0, b1);
 }
-// fp32 pairs as N pairs of pieces, the largest first
-template <typename M, int N>
-__device__ __forceinline__ void split(float a, float b, uint32_t (&p)[N]) {
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    p[i] = Act<M>::pack2(a, b);
-    if (i + 1 < N) a -= Act<M>::get(p[i], 0), b -= Act<M>::get(p[i], 1);
-  }
-}
-// 2^n, n cut to what a normal float holds
-__device__ __forceinline__ float pow2(int n) { return __int_as_float((min(max(n, -126), 127) + 127) << 23); }
-// n with 2^n <= m < 2^(n+1); 0 for zero, infinities and NaN
-__device__ __forceinline__ int exponent(float m) {
-  const int e = (__float_as_int(m) >> 23) & 255;
-  return e == 0 || e == 255 ? 0 : e - 127;
-}
-
-struct Segments {
-  int count, tokens;  // of a segment: a multiple of 64
-  float* states;      // [count - 1][B * H][V tiles][floats of a tile]: what leaves a segment
-  float* decays;      // [count - 1][B * H]
-};
-
 // KP: channels of q and k, padded; VT: value channels of the CTA; C: tokens of a chunk
 template <typename T, int KP, int VT, int C>
 struct Shape {
@@ -103,7 +58,7 @@ struct Shape {
   static constexpr int BUFS = NP == 1 ? 2 : 1;
   static constexpr int QK = C * KP * 2, VB = C * VT * 2, SB = KP * VT * 2;
   static constexpr int TILES = NP * (2 * QK + VB);         // a buffer: q, k, v
-  static constexpr int GB = (3 * C + 4) * 4;               // running sums, what they lost to rounding, decays to the chunk's end; its whole decay, the largest of them
+  static constexpr int GB = Decay<C>::BYTES;
   static constexpr int ST = BUFS * TILES, GO = ST + NS * SB, RED = GO + GB;
   static constexpr size_t SMEM = RED + 16;
   static constexpr int REGS = KP / 64 * (VT / 8) * 4;      // of the state, a thread
@@ -161,65 +116,6 @@ __device__ __forceinline__ void load_tile(uint32_t dst, const T* src, long long 
     }
   }
 }
-
-// One warp: the chunk's running sums of g in units of log2, and the decays that follow from them. A step below -128 is one of -128: its
-// exponential is zero in fp32 either way, and the sums stay finite behind a step of minus infinity.
-template <int C>
-__device__ __forceinline__ void load_decay(float (&x)[C / 32], const lq_attention_problem& p, int b, int h, int t0, int n) {
-  const int lane = threadIdx.x & 31;
-  const float* g = p.g + b * p.g_stride_b + h * p.g_stride_h;
-#pragma unroll
-  for (int i = 0; i < C / 32; ++i) {
-    const int t = t0 + lane * (C / 32) + i;
-    x[i] = p.g != nullptr && t < n ? __ldg(g + t * p.g_stride_t) : 0.f;
-  }
-}
-template <int C>
-struct Decay {
-  static constexpr int PER = C / 32;
-  float hi[PER], lo[PER], out[PER], all, most;  // of this lane's tokens; of the whole chunk, and the largest of the decays to its end
-  __device__ __forceinline__ double of(const float (&x)[PER]) {
-    const int lane = threadIdx.x & 31;
-    double sum[PER], run = 0;
-#pragma unroll
-    for (int i = 0; i < PER; ++i) sum[i] = run += (double)(x[i] < -128.f ? -128.f : x[i]) * 1.4426950408889634;
-    double before = run;
-#pragma unroll
-    for (int m = 1; m < 32; m <<= 1) {
-      const double o = __shfl_up_sync(0xffffffffu, before, m);
-      if (lane >= m) before += o;
-    }
-    const double total = __shfl_sync(0xffffffffu, before, 31);
-    before -= run;
-    most = 0.f;
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const double s = before + sum[i];
-      hi[i] = (float)s;
-      lo[i] = (float)(s - (double)hi[i]);
-      out[i] = ex2((float)(total - s));
-      most = fmaxf(most, out[i]);
-    }
-#pragma unroll
-    for (int m = 16; m; m >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, m));
-    all = ex2((float)total);
-    return total;
-  }
-  __device__ __forceinline__ void store(uint32_t s_g) const {
-    const int lane = threadIdx.x & 31;
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const uint32_t to = s_g + 4 * (lane * PER + i);
-      sts_u32(to, __float_as_uint(hi[i]));
-      sts_u32(to + 4 * C, __float_as_uint(lo[i]));
-      sts_u32(to + 8 * C, __float_as_uint(out[i]));
-    }
-    if (lane == 0) {
-      sts_u32(s_g + 12 * C, __float_as_uint(all));
-      sts_u32(s_g + 12 * C + 4, __float_as_uint(most));
-    }
-  }
-};
 
 struct Vec {
   int q, k, v, o;  // bytes of an access
@@ -384,34 +280,9 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 2 && KP <= 128 ? 2 : 1) 
           }
         }
       }
-      const float hi0 = lds_f32(s_g + 4 * (r0 + g)), hi1 = lds_f32(s_g + 4 * (r0 + g + 8));
-      const float lo0 = lds_f32(s_g + 4 * (C + r0 + g)), lo1 = lds_f32(s_g + 4 * (C + r0 + g + 8));
-      float top0 = 0.f, top1 = 0.f;
-#pragma unroll
-      for (int j = 0; j < 2 * CS; ++j) {
-        if (j / 2 > mt) break;
-        const int col = 8 * j + 2 * t4;
-        const float2 hi = lds_f2(s_g + 4 * col), lo = lds_f2(s_g + 4 * (C + col));
-        a[j][0] = col <= r0 + g ? a[j][0] * ex2((hi0 - hi.x) + (lo0 - lo.x)) : 0.f;
-        a[j][1] = col + 1 <= r0 + g ? a[j][1] * ex2((hi0 - hi.y) + (lo0 - lo.y)) : 0.f;
-        a[j][2] = col <= r0 + g + 8 ? a[j][2] * ex2((hi1 - hi.x) + (lo1 - lo.x)) : 0.f;
-        a[j][3] = col + 1 <= r0 + g + 8 ? a[j][3] * ex2((hi1 - hi.y) + (lo1 - lo.y)) : 0.f;
-        if constexpr (F16) {
-          top0 = fmaxf(top0, fmaxf(fabsf(a[j][0]), fabsf(a[j][1])));
-          top1 = fmaxf(top1, fmaxf(fabsf(a[j][2]), fabsf(a[j][3])));
-        }
-      }
-      // fp16: rows under a power of two, so that none leaves the type's range
+      decay_products<C>(a, s_g, r0, 2 * mt + 2);
       float up0 = 1.f, up1 = 1.f;
-      if constexpr (F16) {
-#pragma unroll
-        for (int m = 1; m < 4; m <<= 1) {
-          top0 = fmaxf(top0, __shfl_xor_sync(0xffffffffu, top0, m));
-          top1 = fmaxf(top1, __shfl_xor_sync(0xffffffffu, top1, m));
-        }
-        up0 = pow2(min(14 - exponent(top0), 40));
-        up1 = pow2(min(14 - exponent(top1), 40));
-      }
+      if constexpr (F16) row_scales(a, 2 * mt + 2, up0, up1);
       uint32_t pa[S::NA][CS][4];
 #pragma unroll
       for (int j = 0; j < CS; ++j)
@@ -449,7 +320,8 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 2 && KP <= 128 ? 2 : 1) 
             }
           }
       }
-      const float f0 = ex2(hi0) * (F16 ? pow2(exp_c) : 1.f) * up0, f1 = ex2(hi1) * (F16 ? pow2(exp_c) : 1.f) * up1;
+      const float f0 = ex2(lds_f32(s_g + 4 * (r0 + g))) * (F16 ? pow2(exp_c) : 1.f) * up0;
+      const float f1 = ex2(lds_f32(s_g + 4 * (r0 + g + 8))) * (F16 ? pow2(exp_c) : 1.f) * up1;
 #pragma unroll
       for (int j = 0; j < NV; ++j) o[j][0] *= f0, o[j][1] *= f0, o[j][2] *= f1, o[j][3] *= f1;
       // and the chunk's own tokens
@@ -721,6 +593,10 @@ __global__ void __launch_bounds__(256) linear_attention_step_kernel(const lq_att
   }
 }
 
+cudaError_t launch_segment_states(const Segments& seg, int heads, long long values, cudaStream_t st) {
+  return launch(segment_states_kernel, dim3((unsigned)((values / 4 + 255) / 256)), dim3(256), 0, st, seg, heads, values, (int)(values / heads));
+}
+
 static int check(const lq_attention_problem* p, const char* what) {
   if (!p) return fail(LQ_ERR_NULL, "%s: problem descriptor is null", what);
   if (p->B < 0 || p->T < 0 || p->H <= 0 || p->Hk <= 0 || p->H % p->Hk || p->K <= 0 || p->V <= 0 || !fits(p->B) || !fits(p->T) || !fits(p->V))
@@ -731,24 +607,18 @@ static int check(const lq_attention_problem* p, const char* what) {
   return LQ_OK;
 }
 
-struct Plan {
-  int vt, regs, count, tokens;
-  long long tiles() const { return tiles_; }
-  long long tiles_;
-};
-// Segments: enough CTAs for two on an SM, none shorter than eight chunks
+// Segments: enough CTAs for every place on the GPU (two an SM; one for the tcgen05 kernel), none shorter than eight chunks
 static Plan plan(const lq_attention_problem* p) {
   Plan r;
-  const int kp = p->K <= 64 ? 64 : p->K <= 128 ? 128 : 256;
-  r.vt = kp == 256 ? 32 : 64;
-  r.regs = kp / 64 * (r.vt / 8) * 4;
-  r.tiles_ = (long long)p->B * p->H * ((p->V + r.vt - 1) / r.vt);
-  const long long room = 2ll * sm_count();
-  long long count = r.tiles_ > 0 ? room / r.tiles_ : 1;
-  const long long most = ((long long)p->T + 511) / 512;
-  count = count < 1 ? 1 : count > most ? (most < 1 ? 1 : most) : count;
-  const long long chunks = ((long long)p->T + 63) / 64;
-  const long long each = count > 0 ? (chunks + count - 1) / count : 1;
+  r.tc = tc_applies(p);
+  const int kp = p->K <= 64 && !r.tc ? 64 : p->K <= 128 ? 128 : 256, vt = kp == 256 ? 32 : 64;
+  r.regs = kp / 64 * (vt / 8) * 4;
+  r.tiles = (long long)p->B * p->H * ((p->V + vt - 1) / vt);
+  const long long chunks = ((long long)p->T + 63) / 64, room = (r.tc ? 1ll : 2ll) * sm_count();
+  long long count = r.tiles > 0 ? room / r.tiles : 1;
+  count = count > chunks / 8 ? chunks / 8 : count;
+  count = count < 1 ? 1 : count;
+  const long long each = (chunks + count - 1) / count;
   r.tokens = (int)((each < 1 ? 1 : each) * 64);
   r.count = (int)((p->T + (long long)r.tokens - 1) / r.tokens);
   if (r.count < 1) r.count = 1;
@@ -756,7 +626,7 @@ static Plan plan(const lq_attention_problem* p) {
 }
 static size_t workspace(const lq_attention_problem* p, const Plan& r) {
   if (r.count < 2) return 0;
-  return (size_t)(r.count - 1) * ((size_t)r.tiles_ * THREADS * r.regs + (((size_t)p->B * p->H + 63) / 64) * 64) * 4;
+  return (size_t)(r.count - 1) * ((size_t)r.tiles * THREADS * r.regs + (((size_t)p->B * p->H + 63) / 64) * 64) * 4;
 }
 
 static int access_bytes(const void* ptr, long long sb, long long st, long long sh, int size) {
@@ -773,14 +643,10 @@ static int run(const lq_attention_problem* p, const Plan& r, const Segments& seg
   const dim3 block(THREADS);
   cudaError_t e = cudaSuccess;
   if (seg.count > 1) {
-    e = launch_opt_in(linear_attention_kernel<T, KP, VT, C, true>, dim3((unsigned)r.tiles_, seg.count - 1), block, S::SMEM, st, *p, seg, vec);
-    if (e == cudaSuccess && seg.count > 2) {
-      const long long values = r.tiles_ * THREADS * S::REGS;
-      e = launch(segment_states_kernel, dim3((unsigned)((values / 4 + 255) / 256)), dim3(256), 0, st, seg, p->B * p->H, values,
-                 (int)(values / ((long long)p->B * p->H)));
-    }
+    e = launch_opt_in(linear_attention_kernel<T, KP, VT, C, true>, dim3((unsigned)r.tiles, seg.count - 1), block, S::SMEM, st, *p, seg, vec);
+    if (e == cudaSuccess && seg.count > 2) e = launch_segment_states(seg, p->B * p->H, r.tiles * THREADS * S::REGS, st);
   }
-  if (e == cudaSuccess) e = launch_opt_in(linear_attention_kernel<T, KP, VT, C, false>, dim3((unsigned)r.tiles_, seg.count), block, S::SMEM, st, *p, seg, vec);
+  if (e == cudaSuccess) e = launch_opt_in(linear_attention_kernel<T, KP, VT, C, false>, dim3((unsigned)r.tiles, seg.count), block, S::SMEM, st, *p, seg, vec);
   if (e != cudaSuccess) return fail(LQ_ERR_LAUNCH, "linear_attention: %s", cudaGetErrorString(e));
   return check_launch("linear_attention_kernel");
 }
@@ -806,8 +672,9 @@ extern "C" int lq_linear_attention_fwd(const lq_attention_problem* p, void* ws, 
   if (need > 0 && (ws == nullptr || bytes < need)) return fail(LQ_ERR_WORKSPACE, "linear_attention: workspace of %zu bytes, %zu needed", bytes, need);
   if (need > 0 && (reinterpret_cast<uintptr_t>(ws) & 15u)) return fail(LQ_ERR_ALIGN, "linear_attention: workspace must start on a 16-byte boundary");
   float* states = reinterpret_cast<float*>(ws);
-  const Segments seg{r.count, r.tokens, states, states + (size_t)(r.count - 1) * r.tiles_ * THREADS * r.regs};
+  const Segments seg{r.count, r.tokens, states, states + (size_t)(r.count - 1) * r.tiles * THREADS * r.regs};
   cudaStream_t st = (cudaStream_t)stream;
+  if (r.tc) return run_tc(p, r, seg, st);
   return with_dtype(p->dtype, "linear_attention", [&](auto t) {
     using T = decltype(t);
     if (p->K <= 64) return run<T, 64, 64, 64>(p, r, seg, st);
