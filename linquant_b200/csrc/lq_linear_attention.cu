@@ -9,7 +9,7 @@
 // Where a batch has too few heads for the GPU, the tokens are cut into segments: a first pass leaves every segment's own
 // state, a small kernel carries them on, and the second pass starts each segment from what enters it.
 //
-// Rounding. G is summed in 64 bits and kept as two floats, so that differences of large sums are exact; decays are 2^x of fp32
+// Rounding. G is summed and kept as two floats, so that differences of large sums are exact; decays are 2^x of fp32
 // differences. Products of 16-bit values are exact and their sums fp32. The decayed keys of the state's product are fp32 and go in
 // as three bf16 pieces (all 24 bits; fp16: two pieces under a power of two of the chunk's largest key, 22 bits), the state that q
 // reads as two pieces (16 or 22 bits), the decayed products q.k as one piece of the operands' type: their rounding, half a
@@ -220,7 +220,7 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 2 && KP <= 128 ? 2 : 1) 
   };
 
   const uint32_t s_g = s0 + S::GO;
-  double total = 0;  // warp 0: the segment's log-decay
+  Pair total;  // warp 0: the segment's log-decay
   Decay<C> next;
   float x_next[C / 32];
   if (chunks > 0) {
@@ -228,6 +228,7 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 2 && KP <= 128 ? 2 : 1) 
     if (warp == 0) {
       load_decay<C>(x_next, p, b, h, first, stop);
       total = next.of(x_next);
+      if (F16) next.largest();
       next.store(s_g);
       load_decay<C>(x_next, p, b, h, first + C, stop);
     }
@@ -246,7 +247,8 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 2 && KP <= 128 ? 2 : 1) 
     __syncthreads();  // tiles, decays and the state's pieces are there
     if (S::BUFS == 2 && c + 1 < chunks) load(c + 1, buf ^ 1);
     if (warp == 0 && c + 1 < chunks) {
-      total += next.of(x_next);
+      total = total + next.of(x_next);
+      if (F16) next.largest();
       load_decay<C>(x_next, p, b, h, t0 + 2 * C, stop);
     }
     if constexpr (!STATES) {
@@ -481,7 +483,7 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 2 && KP <= 128 ? 2 : 1) 
 #pragma unroll
       for (int j = 0; j < NT; ++j)
         to[(m * NT + j) * THREADS + tid] = make_float4(st[m][j][0] * back, st[m][j][1] * back, st[m][j][2] * back, st[m][j][3] * back);
-    if (vt == 0 && tid == 0) seg.decays[(size_t)blockIdx.y * (gridDim.x / vts) + bh] = ex2((float)total);
+    if (vt == 0 && tid == 0) seg.decays[(size_t)blockIdx.y * (gridDim.x / vts) + bh] = ex2(total.hi);
   } else {
     if (p.final_state != nullptr && (int)blockIdx.y == (n > 0 ? (n - 1) / seg.tokens : 0)) {
       float* to = p.final_state + (size_t)bh * p.K * p.V + v0;

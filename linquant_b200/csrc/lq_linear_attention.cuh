@@ -62,38 +62,57 @@ __device__ __forceinline__ void load_decay(float (&x)[C / 32], const lq_attentio
     x[i] = p.g != nullptr && t < n ? __ldg(g + t * p.g_stride_t) : 0.f;
   }
 }
+// a value as the sum of two floats, the second at most half a step of the first
+struct Pair {
+  float hi = 0.f, lo = 0.f;
+  __device__ __forceinline__ Pair() {}
+  __device__ __forceinline__ Pair(float h, float l) : hi(h), lo(l) {}
+  __device__ __forceinline__ Pair operator+(const Pair& o) const {
+    const float s = __fadd_rn(hi, o.hi), b = __fsub_rn(s, hi);
+    const float e = __fadd_rn(__fadd_rn(__fsub_rn(hi, __fsub_rn(s, b)), __fsub_rn(o.hi, b)), __fadd_rn(lo, o.lo)), h = __fadd_rn(s, e);
+    return Pair(h, __fsub_rn(e, __fsub_rn(h, s)));
+  }
+};
+
 // One warp: the chunk's running sums of g in units of log2, and the decays that follow from them. A step below -128 is one of -128: its
 // exponential is zero in fp32 either way, and the sums stay finite behind a step of minus infinity.
 template <int C>
 struct Decay {
   static constexpr int PER = C / 32, BYTES = (3 * C + 4) * 4;
-  float hi[PER], lo[PER], out[PER], all, most;  // of this lane's tokens; of the whole chunk, and the largest of the decays to its end
-  __device__ __forceinline__ double of(const float (&x)[PER]) {
+  float hi[PER], lo[PER], out[PER], all, most;  // of this lane's tokens; of the whole chunk, and the largest of `out`: of the lane, behind largest() of all
+  // Sums of two floats each: a step of the scan is a dozen dependent fp32 additions, where one in 64 bits takes several times as long
+  __device__ __forceinline__ Pair of(const float (&x)[PER]) {
     const int lane = threadIdx.x & 31;
-    double sum[PER], run = 0;
+    Pair sum[PER], run;
 #pragma unroll
-    for (int i = 0; i < PER; ++i) sum[i] = run += (double)(x[i] < -128.f ? -128.f : x[i]) * 1.4426950408889634;
-    double before = run;
+    for (int i = 0; i < PER; ++i) {
+      const float g = x[i] < -128.f ? -128.f : x[i], p = g * kLog2e;
+      const Pair step(p, fmaf(g, kLog2e, -p) + g * 1.92596299e-8f);  // log2(e) = a float and what it leaves
+      sum[i] = run = i ? run + step : step;
+    }
+    Pair before = run;
 #pragma unroll
     for (int m = 1; m < 32; m <<= 1) {
-      const double o = __shfl_up_sync(0xffffffffu, before, m);
-      if (lane >= m) before += o;
+      const Pair o(__shfl_up_sync(0xffffffffu, before.hi, m), __shfl_up_sync(0xffffffffu, before.lo, m)), both = before + o;
+      if (lane >= m) before = both;
     }
-    const double total = __shfl_sync(0xffffffffu, before, 31);
-    before -= run;
+    const Pair total(__shfl_sync(0xffffffffu, before.hi, 31), __shfl_sync(0xffffffffu, before.lo, 31));
+    const Pair first(__shfl_up_sync(0xffffffffu, before.hi, 1), __shfl_up_sync(0xffffffffu, before.lo, 1));  // what the lanes before have
     most = 0.f;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      const double s = before + sum[i];
-      hi[i] = (float)s;
-      lo[i] = (float)(s - (double)hi[i]);
-      out[i] = ex2((float)(total - s));
+      const Pair s = lane ? first + sum[i] : sum[i];
+      hi[i] = s.hi;
+      lo[i] = s.lo;
+      out[i] = ex2((total.hi - s.hi) + (total.lo - s.lo));
       most = fmaxf(most, out[i]);
     }
+    all = ex2(total.hi);
+    return total;
+  }
+  __device__ __forceinline__ void largest() {
 #pragma unroll
     for (int m = 16; m; m >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, m));
-    all = ex2((float)total);
-    return total;
   }
   // running sums, what they lost to rounding, decays to the chunk's end; its whole decay, the largest of them
   __device__ __forceinline__ void store(uint32_t s_g) const {

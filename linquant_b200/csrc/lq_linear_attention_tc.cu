@@ -5,10 +5,12 @@
 // One CTA an SM has 64 value channels of one head and walks over chunks of 64 tokens; its roles run apart by as much as the
 // buffers allow, so the only chain from chunk to chunk is the state's own (a few hundred clocks), not the chunk's four products:
 //
-//   loader warp   q, k, v tiles by TMA into a ring of stages (zeros behind K, V and T), the chunk's decays
+//   loader warp   q, k, v tiles by TMA into a ring of stages (zeros behind K, V and T)
+//   decay warps   two that take chunks in turn: the next chunk's decays, made while its tiles are on their way
 //   MMA warp      q k^T; k^T v' (both operands as they lie, token index outermost: "MN-major"); q S; P v
-//   warps 0..3    P = decayed q k^T from tensor memory to shared memory, rounded; a chunk later its outputs
-//   warps 4..7    v' = exp(G_C - G_j) v in pieces; the state, a row of K a thread in registers, S = a S + k^T v'; S rounded for q
+//   warps 0..7    two sets of four that take chunks in turn: P = decayed q k^T from tensor memory to shared memory, rounded; the outputs
+//   warps 8..15   the state, half a row of K a thread in registers: S = a S + k^T v'; S rounded for q
+//   warps 16..19  v' = exp(G_C - G_j) v in pieces
 //
 // All accumulators lie twice in tensor memory (four of 64 columns). Rounding as in lq_linear_attention.cu with the decay on v instead
 // of k (half as many values); here q reads the state as one piece of the type, the same half step as the decayed q k^T has.
@@ -26,15 +28,18 @@ namespace attentiontc {
 
 using namespace attention;
 
-constexpr int C = 64, VT = 64, WARPS = 10, LOADER = 8, ISSUER = 9;
-constexpr int TILE = C * 128, QK = 2 * TILE, STAGE = 2 * QK + TILE, STAGES = 3, SB = 128 * 128, GS = 8;  // bytes; GS: chunks whose decays are kept
+constexpr int C = 64, VT = 64, WARPS = 24, LOADER = 20, ISSUER = 21, DECAYS = 22;
+constexpr int TILE = C * 128, QK = 2 * TILE, STAGE = 2 * QK + TILE, STAGES = 3, SB = 128 * 128, GS = 8, AHEAD = 2;  // bytes; GS: chunks whose decays are kept
+// Decays of a chunk: Decay<C>'s, then for the row blocks of 16 tokens q = 1..3 those from each token before the block to its start.
+// Below the block an element's decay is that times the row's own from the start on: no exponential of its own.
+constexpr int BELOW = Decay<C>::BYTES, GB = BELOW + 96 * 4;
 
 template <typename T>
 struct Shape {
   static constexpr bool F16 = std::is_same_v<T, __half>;
   static constexpr int NV = F16 ? 2 : 3;  // pieces of v'
   static constexpr int VO = STAGES * STAGE, PO = VO + 2 * NV * TILE, SO = PO + 2 * TILE, GO = SO + 2 * SB;
-  static constexpr int RED = GO + GS * Decay<C>::BYTES, EXP = RED + 64, BARS = EXP + 16;
+  static constexpr int RED = GO + GS * GB, EXP = RED + 64, BACK = EXP + 16, SUM = BACK + 16, BARS = SUM + 16;
   static constexpr int FULL = 0, EMPTY = FULL + STAGES, S1 = EMPTY + STAGES, PF = S1 + 2, VF = PF + 2, DS = VF + 2, SF = DS + 2, OF = SF + 2, OE = OF + 2, LAST = OE + 2, COUNT = LAST + 1;
   static constexpr int TBASE = BARS + 8 * COUNT;
   static constexpr size_t SMEM = 1024 + TBASE + 8;
@@ -44,17 +49,56 @@ struct Shape {
 constexpr int T_S1 = 0, T_QS = 128, T_PV = 256, T_DS = 384;
 
 __device__ __forceinline__ void mbar_arrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];\n" ::"r"(bar) : "memory"); }
-__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity)) != 0; }
+// By every lane (each needs its own acquire of the phase), warp-uniform. One probe that does not suspend, then the hardware's own short
+// suspension: with 50 us allowed a warp comes back hundreds of clocks after its phase (94 -> 138 us for the whole kernel), with none
+// the waiting warps take the working ones' issue slots (154 us).
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile("{\n.reg .pred p;\nmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}\n" : "=r"(done) : "r"(bar), "r"(parity) : "memory");
+  if (__all_sync(0xffffffffu, done != 0u)) return true;
+  return __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity)) != 0;
+}
+__device__ __forceinline__ void tma_prefetch_4d(const CUtensorMap* map, int c0, int c1, int c2, int c3) {  // to L2
+  asm volatile("cp.async.bulk.prefetch.tensor.4d.L2.global [%0, {%1, %2, %3, %4}];\n" ::"l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(c3) : "memory");
+}
 __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, int c3, uint32_t bar) {
   asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];\n" ::"r"(dst),
                "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(bar)
                : "memory");
 }
-// warps 4..7 decide together
+// One lane of a warp, in the form the compiler knows as one: behind `lane == 0` every tensor-core instruction is issued in a loop over the
+// lanes that might be there, 45 clocks instead of the 32 that the smallest of them takes.
+__device__ __forceinline__ bool elected() {
+  uint32_t r;
+  asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}\n" : "=r"(r));
+  return r != 0;
+}
+// a ring's place and how often it has been passed, without a division a chunk
+struct Ring {
+  int s = 0;
+  uint32_t lap = 0;
+  __device__ __forceinline__ void next() {
+    if (++s == STAGES) s = 0, lap ^= 1u;
+  }
+};
+// The warps of a group decide together (the state's: barrier 2 of 256 threads, those of v': 1 of 128): none leaves while another waits there
+template <int ID, int THREADS>
 __device__ __forceinline__ bool group_and(bool ok) {
   uint32_t r;
-  asm volatile("{\n.reg .pred p, q;\nsetp.ne.b32 q, %1, 0;\nbar.red.and.pred p, 1, 128, q;\nselp.u32 %0, 1, 0, p;\n}\n" : "=r"(r) : "r"((uint32_t)ok) : "memory");
+  asm volatile("{\n.reg .pred p, q;\nsetp.ne.b32 q, %1, 0;\nbar.red.and.pred p, %2, %3, q;\nselp.u32 %0, 1, 0, p;\n}\n" : "=r"(r) : "r"((uint32_t)ok), "n"(ID), "n"(THREADS) : "memory");
   return r != 0;
+}
+// and the largest of their values; slots: a float a warp
+template <int ID, int THREADS>
+__device__ __forceinline__ float group_max(float top, uint32_t slots, bool& ok) {
+  constexpr int N = THREADS / 32;
+#pragma unroll
+  for (int m = 16; m; m >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, m));
+  if ((threadIdx.x & 31) == 0) sts_u32(slots + 4 * (threadIdx.x / 32 % N), __float_as_uint(top));
+  ok = group_and<ID, THREADS>(ok);
+#pragma unroll
+  for (int w = 0; w < N; ++w) top = fmaxf(top, lds_f32(slots + 4 * w));
+  return top;
 }
 __device__ __forceinline__ uint32_t place(int row, int piece) { return row * 128 + ((piece ^ (row & 7)) << 4); }
 __device__ __forceinline__ void before_sync() { asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory"); }
@@ -88,9 +132,9 @@ __global__ void __launch_bounds__(32 * WARPS, 1) linear_attention_tc_kernel(cons
   const int first = blockIdx.y * seg.tokens, last_token = (int)min((long long)first + seg.tokens, (long long)p.T), stop = min(n, last_token);
   const int chunks = stop > first ? (stop - first + C - 1) / C : 0;
   if (tid == 0) {
-    for (int i = 0; i < S::COUNT; ++i) {  // PF, VF, SF and OE take an arrival of each of four warps
-      const bool four = (i >= S::PF && i < S::DS) || (i >= S::SF && i < S::OF) || (i >= S::OE && i < S::LAST);
-      asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;\n" ::"r"(s_bars + 8u * i), "r"(four ? 4u : 1u));
+    for (int i = 0; i < S::COUNT; ++i) {  // arrivals of loads and decays, of a set's or the v' warps, of the state's eight, or one
+      const bool two = i < S::EMPTY, four = (i >= S::PF && i < S::DS) || (i >= S::OE && i < S::LAST), eight = i >= S::SF && i < S::OF;
+      asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;\n" ::"r"(s_bars + 8u * i), "r"(two ? 2u : four ? 4u : eight ? 8u : 1u));
     }
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
   }
@@ -105,23 +149,30 @@ __global__ void __launch_bounds__(32 * WARPS, 1) linear_attention_tc_kernel(cons
   bool ok = true;
   auto stage = [&](int c) { return s0 + (uint32_t)(c % STAGES) * STAGE; };
   auto stage_wait = [&](int c) { return warp_wait(bar(S::FULL, c % STAGES), (uint32_t)((c / STAGES) & 1)); };
-  auto decays = [&](int c) { return s0 + S::GO + (uint32_t)(c % GS) * Decay<C>::BYTES; };
+  auto decays = [&](int c) { return s0 + S::GO + (uint32_t)(c % GS) * GB; };
 
   if (warp == LOADER) {
-    double total = 0;
-    float x[C / 32];
-    load_decay<C>(x, p, b, h, first, stop);
-    Decay<C> d;
+    // The stages alone reach one chunk's time ahead, less than what memory takes: tiles go to L2 further ahead than that
+    auto fetch = [&](int c) {
+      if (c >= chunks || !elected()) return;
+      const int t0 = first + c * C;
+      tma_prefetch_4d(&map_k, 0, t0, hk, b);
+      tma_prefetch_4d(&map_k, 64, t0, hk, b);
+      if constexpr (!STATES) {
+        tma_prefetch_4d(&map_q, 0, t0, hk, b);
+        tma_prefetch_4d(&map_q, 64, t0, hk, b);
+      }
+      tma_prefetch_4d(&map_v, v0, t0, h, b);
+    };
+    Ring r;
     int c = 0;
-    for (; c < chunks; ++c) {
-      const int s = c % STAGES;
-      if (c >= STAGES && !(ok = warp_wait(bar(S::EMPTY, s), (uint32_t)((c / STAGES - 1) & 1)))) break;
-      total += d.of(x);
-      d.store(decays(c));  // its chunk eight before this one has been left by all: the stages between are empty again
-      load_decay<C>(x, p, b, h, first + (c + 1) * C, stop);
+    for (int k = STAGES; k < STAGES + AHEAD; ++k) fetch(k);
+    for (; c < chunks; ++c, r.next()) {
+      fetch(c + STAGES + AHEAD);
       __syncwarp();
-      if (lane == 0) {
-        const uint32_t to = stage(c), full = bar(S::FULL, s);
+      if (c >= STAGES && !(ok = warp_wait(bar(S::EMPTY, r.s), r.lap ^ 1u))) break;
+      if (elected()) {
+        const uint32_t to = s0 + (uint32_t)r.s * STAGE, full = bar(S::FULL, r.s);
         const int t0 = first + c * C;
         asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n" ::"r"(full), "r"((uint32_t)(STATES ? QK + TILE : STAGE)) : "memory");
         tma_load_4d(to + QK, &map_k, 0, t0, hk, b, full);
@@ -135,69 +186,110 @@ __global__ void __launch_bounds__(32 * WARPS, 1) linear_attention_tc_kernel(cons
       __syncwarp();
     }
     for (int k = max(0, c - STAGES); k < c; ++k) ok &= stage_wait(k);  // nothing may land after the CTA has gone
-    if (STATES && vt == 0 && lane == 0) seg.decays[(size_t)blockIdx.y * (gridDim.x / vts) + bh] = ex2((float)total);
+  } else if (warp >= DECAYS) {
+    const int turn = warp - DECAYS;
+    Pair total;
+    float x[2][C / 32];  // the next two chunks' on their way
+    for (int k = 0; k < 2; ++k) load_decay<C>(x[k], p, b, h, (int)min((long long)first + (turn + 2 * k) * C, (long long)stop), stop);
+    for (int c = turn; c < chunks; c += 2) {
+      Decay<C> d;
+      total = total + d.of(x[0]);
+#pragma unroll
+      for (int k = 0; k < C / 32; ++k) x[0][k] = x[1][k];
+      load_decay<C>(x[1], p, b, h, (int)min((long long)first + (c + 4ll) * C, (long long)stop), stop);
+      float below[3][2];
+#pragma unroll
+      for (int q = 1; q < 4; ++q) {
+        const float hi = __shfl_sync(0xffffffffu, d.hi[1], 8 * q - 1), lo = __shfl_sync(0xffffffffu, d.lo[1], 8 * q - 1);
+#pragma unroll
+        for (int k = 0; k < 2; ++k) below[q - 1][k] = ex2((hi - d.hi[k]) + (lo - d.lo[k]));
+      }
+      // The stage is empty: the chunk three before this one is done, and the one whose place this takes, eight before, left by all
+      if (c >= STAGES && !(ok = warp_wait(bar(S::EMPTY, c % STAGES), (uint32_t)((c / STAGES - 1) & 1)))) break;
+      d.store(decays(c));
+#pragma unroll
+      for (int q = 1; q < 4; ++q)
+        if (lane < 8 * q) {
+          const uint32_t to = decays(c) + BELOW + 4 * (8 * q * (q - 1) + 2 * lane);
+          sts_u32(to, __float_as_uint(below[q - 1][0]));
+          sts_u32(to + 4, __float_as_uint(below[q - 1][1]));
+        }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(S::FULL, c % STAGES));
+    }
+    if (STATES && lane == 0) {
+      sts_u32(s0 + S::SUM + 8 * turn, __float_as_uint(total.hi));
+      sts_u32(s0 + S::SUM + 8 * turn + 4, __float_as_uint(total.lo));
+    }
   } else if (warp == ISSUER) {
     const uint32_t id_s1 = idesc<T>(C, C, false, false), id_mn = idesc<T>(C, VT, false, true), id_ds = idesc<T>(128, VT, true, true);
-    auto scores = [&](int c) {
-      if (lane == 0) {
+    const uint64_t d_stage = desc_kmajor_sw128(s0), d_k = desc_mn_sw128(s0 + QK, TILE), d_v = desc_kmajor_sw128(s0 + S::VO), d_p = desc_kmajor_sw128(s0 + S::PO),
+                   d_s = desc_kmajor_sw128(s0 + S::SO);
+    constexpr uint32_t U = 16;  // descriptors count in units of 16 bytes
+    Ring now, ahead;
+    auto scores = [&](const Ring& r, int i) {  // q k^T
+      if (elected()) {
+        const uint64_t q = d_stage + (uint64_t)(r.s * (STAGE / U));
 #pragma unroll
         for (int ks = 0; ks < 8; ++ks) {
-          const uint32_t at = stage(c) + (ks / 4) * TILE;
-          umma_f16(tbase + T_S1 + 64 * (c & 1), desc_kmajor_sw128(at) + 2 * (ks % 4), desc_kmajor_sw128(at + QK) + 2 * (ks % 4), id_s1, ks > 0);
+          const uint64_t at = q + (ks / 4) * (TILE / U) + 2 * (ks % 4);
+          umma_f16(tbase + T_S1 + 64 * i, at, at + QK / U, id_s1, ks > 0);
         }
-        umma_commit(bar(S::S1, c & 1));
+        umma_commit(bar(S::S1, i));
       }
       __syncwarp();
     };
+    auto landed = [&](const Ring& r) { return warp_wait(bar(S::FULL, r.s), r.lap); };
     if constexpr (!STATES) {
-      if (chunks > 0 && (ok = stage_wait(0))) {
+      if (chunks > 0 && (ok = landed(ahead))) {
         after_sync();
-        scores(0);
+        scores(ahead, 0);
       }
+      ahead.next();
     }
-    for (int c = 0; c < chunks && ok; ++c) {
+    for (int c = 0; c < chunks && ok; ++c, now.next(), ahead.next()) {
       const int i = c & 1;
       const uint32_t turn = (uint32_t)((c >> 1) & 1);
+      const uint64_t stage_at = (uint64_t)(now.s * (STAGE / U));
       if constexpr (!STATES) {
         if (c + 1 < chunks) {  // P of two chunks before has been waited for: its accumulator has been read
-          if (!(ok = stage_wait(c + 1))) break;
+          if (!(ok = landed(ahead))) break;
           after_sync();
-          scores(c + 1);
+          scores(ahead, i ^ 1);
         }
       } else {
         if (c >= 2 && !(ok = warp_wait(bar(S::SF, i), turn ^ 1))) break;
       }
       if (!(ok = warp_wait(bar(S::VF, i), turn))) break;
       after_sync();
-      if (lane == 0) {  // the pieces of v', the smallest first
+      if (elected()) {  // the pieces of v', the smallest first
+        const uint64_t k = d_k + stage_at, v = d_v + (uint64_t)(i * (S::NV * TILE / U));
 #pragma unroll
         for (int w = S::NV - 1; w >= 0; --w)
 #pragma unroll
-          for (int ks = 0; ks < 4; ++ks)
-            umma_f16(tbase + T_DS + 64 * i, desc_mn_sw128(stage(c) + QK + 2048 * ks, TILE), desc_kmajor_sw128(s0 + S::VO + (i * S::NV + w) * TILE + 2048 * ks), id_ds,
-                     w < S::NV - 1 || ks > 0);
+          for (int ks = 0; ks < 4; ++ks) umma_f16(tbase + T_DS + 64 * i, k + ks * (2048 / U), v + w * (TILE / U) + ks * (2048 / U), id_ds, w < S::NV - 1 || ks > 0);
         umma_commit(bar(S::DS, i));
-        if constexpr (STATES) umma_commit(bar(S::EMPTY, c % STAGES));
+        if constexpr (STATES) umma_commit(bar(S::EMPTY, now.s));
       }
       __syncwarp();
       if constexpr (!STATES) {
         if (!(ok = warp_wait(bar(S::SF, i), turn))) break;
         if (c >= 2 && !(ok = warp_wait(bar(S::OE, i), turn ^ 1))) break;
         after_sync();
-        if (lane == 0) {
+        if (elected()) {
+          const uint64_t q = d_stage + stage_at, st = d_s + (uint64_t)(i * (SB / U));
 #pragma unroll
-          for (int ks = 0; ks < 8; ++ks)
-            umma_f16(tbase + T_QS + 64 * i, desc_kmajor_sw128(stage(c) + (ks / 4) * TILE) + 2 * (ks % 4), desc_kmajor_sw128(s0 + S::SO + i * SB + 2048 * ks), id_mn, ks > 0);
+          for (int ks = 0; ks < 8; ++ks) umma_f16(tbase + T_QS + 64 * i, q + (ks / 4) * (TILE / U) + 2 * (ks % 4), st + ks * (2048 / U), id_mn, ks > 0);
         }
         __syncwarp();
         if (!(ok = warp_wait(bar(S::PF, i), turn))) break;
         after_sync();
-        if (lane == 0) {
+        if (elected()) {
+          const uint64_t a = d_p + (uint64_t)(i * (TILE / U)), v = d_stage + stage_at + 2 * QK / U;
 #pragma unroll
-          for (int ks = 0; ks < 4; ++ks)
-            umma_f16(tbase + T_PV + 64 * i, desc_kmajor_sw128(s0 + S::PO + i * TILE) + 2 * ks, desc_kmajor_sw128(stage(c) + 2 * QK + 2048 * ks), id_mn, ks > 0);
+          for (int ks = 0; ks < 4; ++ks) umma_f16(tbase + T_PV + 64 * i, a + 2 * ks, v + ks * (2048 / U), id_mn, ks > 0);
           umma_commit(bar(S::OF, i));
-          umma_commit(bar(S::EMPTY, c % STAGES));
+          umma_commit(bar(S::EMPTY, now.s));
         }
         __syncwarp();
       }
@@ -205,50 +297,105 @@ __global__ void __launch_bounds__(32 * WARPS, 1) linear_attention_tc_kernel(cons
     if (lane == 0) umma_commit(bar(S::LAST, 0));  // every product that was issued
     __syncwarp();
     ok &= warp_wait(bar(S::LAST, 0), 0);
-  } else if (warp < 4) {
+  } else if (warp < 8) {
     if constexpr (!STATES) {
-      const int r0 = 16 * warp, g = lane >> 2, t4 = lane & 3, tiles = 2 * warp + 2;
-      const uint32_t lanes = (uint32_t)(32 * warp) << 16;  // M = 64: sixteen rows in each quarter of the lanes
+      const int set = warp >> 2, quad = warp & 3, r0 = 16 * quad, g = lane >> 2, t4 = lane & 3, tiles = 2 * quad + 2;
+      const uint32_t lanes = (uint32_t)(32 * quad) << 16;  // M = 64: sixteen rows in each quarter of the lanes
+      const uint32_t s_p = s0 + S::PO + set * TILE;
       const int cols = min(VT, p.V - v0);
       T* out = reinterpret_cast<T*>(p.o) + ((size_t)b * p.T * p.H + h) * p.V + v0;
       const size_t pitch = (size_t)p.H * p.V;
-      float up0 = 1.f, up1 = 1.f;
-      auto outputs = [&](int c, float up0, float up1) {
-        const int i = c & 1, t0 = first + c * C;
-        if (!(ok = warp_wait(bar(S::OF, i), (uint32_t)((c >> 1) & 1)))) return;
+      for (int c = set; c < chunks; c += 2) {
+        const uint32_t turn = (uint32_t)((c >> 1) & 1), s_g = decays(c);
+        const int t0 = first + c * C;
+        if (!(ok = stage_wait(c) && warp_wait(bar(S::S1, set), turn))) break;
         after_sync();
-        uint32_t qs[2][16], pv[2][16];
+        float a[8][4];
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-          tmem_ld_16x256b_x4(tbase + lanes + T_QS + 64 * i + 32 * k, qs[k]);
-          tmem_ld_16x256b_x4(tbase + lanes + T_PV + 64 * i + 32 * k, pv[k]);
-        }
-        tmem_wait();
-        before_sync();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bar(S::OE, i));
-        const uint32_t s_g = decays(c), s_p = s0 + S::PO + i * TILE;
-        float f0 = ex2(lds_f32(s_g + 4 * (r0 + g))) * p.scale, f1 = ex2(lds_f32(s_g + 4 * (r0 + g + 8))) * p.scale, c0 = p.scale, c1 = p.scale;
-        if constexpr (F16) {
-          const float e = lds_f32(s0 + S::EXP + 4 * (c & 3));
-          f0 *= e, f1 *= e, c0 /= up0, c1 /= up1;
-        }
-        const bool in0 = t0 + r0 + g < stop, in1 = t0 + r0 + g + 8 < stop;  // rows behind the sequence are zero
-        float o[8][4];
+          uint32_t r[16];
+          if (k == 0 || quad >= 2) tmem_ld_16x256b_x4(tbase + lanes + T_S1 + 64 * set + 32 * k, r);
+          tmem_wait();
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
+          for (int j = 0; j < 4; ++j)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float x = fmaf(__uint_as_float(qs[j / 4][4 * (j % 4) + e]), e < 2 ? f0 : f1, __uint_as_float(pv[j / 4][4 * (j % 4) + e]) * (e < 2 ? c0 : c1));
-            o[j][e] = (e < 2 ? in0 : in1) ? x : 0.f;
-          }
-        // through the warp's own rows of P, whose product is done
+            for (int e = 0; e < 4; ++e) a[4 * k + j][e] = 4 * k + j < tiles ? __uint_as_float(r[4 * j + e]) : 0.f;
+        }
+        const float hi0 = lds_f32(s_g + 4 * (r0 + g)), hi1 = lds_f32(s_g + 4 * (r0 + g + 8)), lo0 = lds_f32(s_g + 4 * (C + r0 + g)), lo1 = lds_f32(s_g + 4 * (C + r0 + g + 8));
+        // bf16: the scale goes in here; fp16: with the outputs, the rows get a scale of their own
+        const float own = F16 ? 1.f : p.scale;
+        float from0, from1;  // the rows' decays from the start of their block
+        {
+          const uint32_t at = s_g + 4 * max(r0 - 1, 0);
+          const float hi = quad ? lds_f32(at) : 0.f, lo = quad ? lds_f32(at + 4 * C) : 0.f;
+          from0 = ex2((hi0 - hi) + (lo0 - lo)) * own, from1 = ex2((hi1 - hi) + (lo1 - lo)) * own;
+        }
+        const uint32_t below = s_g + BELOW + 4 * (8 * quad * (quad - 1) + 2 * t4);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          sts_u32(s_p + place(r0 + g, j) + 4 * t4, Act<T>::pack2(o[j][0], o[j][1]));
-          sts_u32(s_p + place(r0 + g + 8, j) + 4 * t4, Act<T>::pack2(o[j][2], o[j][3]));
+          if (j < 2 * quad) {
+            const float2 w = lds_f2(below + 32 * j);
+            const F2 w2(w.x, w.y);
+            mul2(mul2(F2(a[j][0], a[j][1]), w2), F2(from0, from0)).get(a[j][0], a[j][1]);
+            mul2(mul2(F2(a[j][2], a[j][3]), w2), F2(from1, from1)).get(a[j][2], a[j][3]);
+          } else if (j < tiles) {
+            const int col = 8 * j + 2 * t4, row = r0 + g;
+            const float2 hi = lds_f2(s_g + 4 * col), lo = lds_f2(s_g + 4 * (C + col));
+            a[j][0] = col <= row ? a[j][0] * (ex2((hi0 - hi.x) + (lo0 - lo.x)) * own) : 0.f;
+            a[j][1] = col + 1 <= row ? a[j][1] * (ex2((hi0 - hi.y) + (lo0 - lo.y)) * own) : 0.f;
+            a[j][2] = col <= row + 8 ? a[j][2] * (ex2((hi1 - hi.x) + (lo1 - lo.x)) * own) : 0.f;
+            a[j][3] = col + 1 <= row + 8 ? a[j][3] * (ex2((hi1 - hi.y) + (lo1 - lo.y)) * own) : 0.f;
+          }
         }
+        float up0 = 1.f, up1 = 1.f;
+        if constexpr (F16) row_scales(a, tiles, up0, up1);
+        const uint32_t p0 = s_p + (r0 + g) * 128 + 4 * t4, sw = (uint32_t)(g << 4);  // rows g and g + 8 are swizzled alike
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const uint32_t to = p0 + ((uint32_t)(j << 4) ^ sw);
+          sts_u32(to, F16 ? Act<T>::pack2(a[j][0] * up0, a[j][1] * up0) : Act<T>::pack2(a[j][0], a[j][1]));
+          sts_u32(to + 1024, F16 ? Act<T>::pack2(a[j][2] * up1, a[j][3] * up1) : Act<T>::pack2(a[j][2], a[j][3]));
+        }
+        proxy_fence();
+        before_sync();
         __syncwarp();
+        if (lane == 0) mbar_arrive(bar(S::PF, set));
+        // the chunk's outputs, through the warp's own rows of P
+        float f0 = ex2(hi0) * p.scale, f1 = ex2(hi1) * p.scale, c0 = 1.f, c1 = 1.f;
+        if (!(ok = warp_wait(bar(S::OF, set), turn))) break;
+        after_sync();
+        if constexpr (F16) {
+          const float e = lds_f32(s0 + S::EXP + 4 * (c & 3));
+          f0 *= e, f1 *= e, c0 = p.scale / up0, c1 = p.scale / up1;
+        }
+        const bool whole = t0 + C <= stop, in0 = t0 + r0 + g < stop, in1 = t0 + r0 + g + 8 < stop;  // rows behind the sequence are zero
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          uint32_t qs[16], pv[16];
+          tmem_ld_16x256b_x4(tbase + lanes + T_QS + 64 * set + 32 * k, qs);
+          tmem_ld_16x256b_x4(tbase + lanes + T_PV + 64 * set + 32 * k, pv);
+          tmem_wait();
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            F2 x0(__uint_as_float(pv[4 * j]), __uint_as_float(pv[4 * j + 1])), x1(__uint_as_float(pv[4 * j + 2]), __uint_as_float(pv[4 * j + 3]));
+            if constexpr (F16) x0 = mul2(x0, F2(c0, c0)), x1 = mul2(x1, F2(c1, c1));
+            x0 = fma2(F2(__uint_as_float(qs[4 * j]), __uint_as_float(qs[4 * j + 1])), F2(f0, f0), x0);
+            x1 = fma2(F2(__uint_as_float(qs[4 * j + 2]), __uint_as_float(qs[4 * j + 3])), F2(f1, f1), x1);
+            float o[4];
+            x0.get(o[0], o[1]);
+            x1.get(o[2], o[3]);
+            if (!whole) {
+              o[0] = in0 ? o[0] : 0.f, o[1] = in0 ? o[1] : 0.f;
+              o[2] = in1 ? o[2] : 0.f, o[3] = in1 ? o[3] : 0.f;
+            }
+            const uint32_t to = p0 + ((uint32_t)((4 * k + j) << 4) ^ sw);
+            sts_u32(to, Act<T>::pack2(o[0], o[1]));
+            sts_u32(to + 1024, Act<T>::pack2(o[2], o[3]));
+          }
+        }
+        before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(S::OE, set));
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           const int row = r0 + 4 * k + (lane >> 3), piece = lane & 7, t = t0 + row;
@@ -265,170 +412,77 @@ __global__ void __launch_bounds__(32 * WARPS, 1) linear_attention_tc_kernel(cons
           }
         }
         __syncwarp();  // the rows have been read
-      };
-      for (int c = 0; c < chunks && ok; ++c) {
-        const int i = c & 1;
-        if (!(ok = stage_wait(c) && warp_wait(bar(S::S1, i), (uint32_t)((c >> 1) & 1)))) break;
-        after_sync();
-        uint32_t r[2][16];
-#pragma unroll
-        for (int k = 0; k < 2; ++k) tmem_ld_16x256b_x4(tbase + lanes + T_S1 + 64 * i + 32 * k, r[k]);
-        tmem_wait();
-        float a[8][4];
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) a[j][e] = j < tiles ? __uint_as_float(r[j / 4][4 * (j % 4) + e]) : 0.f;
-        decay_products<C>(a, decays(c), r0, tiles);
-        float w0 = 1.f, w1 = 1.f;
-        if constexpr (F16) row_scales(a, tiles, w0, w1);
-        const uint32_t s_p = s0 + S::PO + i * TILE;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          sts_u32(s_p + place(r0 + g, j) + 4 * t4, F16 ? Act<T>::pack2(a[j][0] * w0, a[j][1] * w0) : Act<T>::pack2(a[j][0], a[j][1]));
-          sts_u32(s_p + place(r0 + g + 8, j) + 4 * t4, F16 ? Act<T>::pack2(a[j][2] * w1, a[j][3] * w1) : Act<T>::pack2(a[j][2], a[j][3]));
-        }
-        proxy_fence();
-        before_sync();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bar(S::PF, i));
-        if (c > 0) outputs(c - 1, up0, up1);
-        up0 = w0, up1 = w1;
       }
-      if (ok && chunks > 0) outputs(chunks - 1, up0, up1);
       // tokens behind the sequence, from the first whole chunk that has none of it
       const int from = first + chunks * C;
-      for (long long k = tid; k < (long long)max(last_token - from, 0) * VT; k += 128) {
+      for (long long k = tid; k < (long long)max(last_token - from, 0) * VT; k += 256) {
         const int col = (int)(k % VT);
         if (col < cols) out[(size_t)(from + k / VT) * pitch + col] = from_f32<T>(0.f);
       }
     }
-  } else {
-    const int d = tid - 128, quad = warp & 3;  // a row of the state, of v' half a token
+  } else if (warp < 16) {
+    constexpr int OWN = VT / 2;  // columns of a thread
+    const int id = tid - 256, quad = warp & 3, half = (warp >> 2) & 1, d = 32 * quad + lane;  // half a row of the state
     const uint32_t lanes = (uint32_t)(32 * quad) << 16;
-    const int cols = min(VT, p.V - v0);
-    float st[VT];
+    const int cols = min(VT, p.V - v0) - OWN * half;
+    float st[OWN];
     const size_t tile = (size_t)blockIdx.x * 128 * VT;
 #pragma unroll
-    for (int j = 0; j < VT; ++j) st[j] = 0.f;
+    for (int j = 0; j < OWN; ++j) st[j] = 0.f;
     if (!STATES && blockIdx.y > 0) {
       const float4* from = reinterpret_cast<const float4*>(seg.states + (size_t)(blockIdx.y - 1) * gridDim.x * 128 * VT + tile);
 #pragma unroll
-      for (int j = 0; j < VT; j += 4) {
-        const float4 x = from[(j / 4) * 128 + d];
+      for (int j = 0; j < OWN; j += 4) {
+        const float4 x = from[(OWN / 4 * half + j / 4) * 128 + d];
         st[j] = x.x, st[j + 1] = x.y, st[j + 2] = x.z, st[j + 3] = x.w;
       }
     } else if (blockIdx.y == 0 && p.initial_state != nullptr && d < p.K) {
-      const float* from = p.initial_state + ((size_t)bh * p.K + d) * p.V + v0;
+      const float* from = p.initial_state + ((size_t)bh * p.K + d) * p.V + v0 + OWN * half;
 #pragma unroll
-      for (int j = 0; j < VT; ++j)
+      for (int j = 0; j < OWN; ++j)
         if (j < cols) st[j] = __ldg(from + j);
     }
-    auto group_max = [&](float top, int slot) {  // of warps 4..7, which leave together where a wait ran out
-#pragma unroll
-      for (int m = 16; m; m >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, m));
-      if (lane == 0) sts_u32(s0 + S::RED + 16 * slot + 4 * quad, __float_as_uint(top));
-      ok = group_and(ok);
-      const uint32_t at = s0 + S::RED + 16 * slot;
-      return fmaxf(fmaxf(lds_f32(at), lds_f32(at + 4)), fmaxf(lds_f32(at + 8), lds_f32(at + 12)));
-    };
     auto publish = [&](int c) {
       float f = 1.f;
       if constexpr (F16) {
         float top = 0.f;
 #pragma unroll
-        for (int j = 0; j < VT; ++j) top = fabsf(st[j]) < CUDART_INF_F ? fmaxf(top, fabsf(st[j])) : top;  // an infinity scales nothing
-        const int e = exponent(group_max(top, 2)) - 14;
+        for (int j = 0; j < OWN; ++j) top = fabsf(st[j]) < CUDART_INF_F ? fmaxf(top, fabsf(st[j])) : top;  // an infinity scales nothing
+        const int e = exponent(group_max<2, 256>(top, s0 + S::RED + 32, ok)) - 14;
         if (!ok) return;
         f = pow2(-e);
-        if (d == 0) sts_u32(s0 + S::EXP + 4 * (c & 3), __float_as_uint(pow2(e)));
+        if (id == 0) sts_u32(s0 + S::EXP + 4 * (c & 3), __float_as_uint(pow2(e)));
       }
       const uint32_t to = s0 + S::SO + (c & 1) * SB;
 #pragma unroll
-      for (int j = 0; j < VT; j += 8) {
+      for (int j = 0; j < OWN; j += 8) {
         uint32_t w[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) w[e] = Act<T>::pack2(F16 ? st[j + 2 * e] * f : st[j + 2 * e], F16 ? st[j + 2 * e + 1] * f : st[j + 2 * e + 1]);
-        sts_v4(to + place(d, j / 8), w);
+        sts_v4(to + place(d, OWN / 8 * half + j / 8), w);
       }
       proxy_fence();
       before_sync();
       __syncwarp();
       if (lane == 0) mbar_arrive(bar(S::SF, c & 1));
     };
-    float back = 1.f, back_next = 1.f;  // fp16: what the sums of v' are multiplied by
-    auto decayed = [&](int c) {
-      const int row = d >> 1, half = d & 1, rows = min(C, stop - first - c * C);
-      const uint32_t s_k = stage(c) + QK, s_v = stage(c) + 2 * QK, to = s0 + S::VO + (c & 1) * S::NV * TILE;
-      if (!(ok &= stage_wait(c)) && !F16) return;
-      const float w = lds_f32(decays(c) + 4 * (2 * C + row));
-      uint32_t r[4][4];
-      const bool in = row < rows;
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        if (in) lds_v4(s_v + place(row, 4 * half + q), r[q]);
-        else r[q][0] = r[q][1] = r[q][2] = r[q][3] = 0u;
-      }
-      float f = w;
-      if constexpr (F16) {
-        __half2 top = __half2half2(__ushort_as_half(0));
-#pragma unroll
-        for (int q = 0; q < 4; ++q)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) top = __hmax2(top, __habs2(*reinterpret_cast<__half2*>(&r[q][e])));
-        const float big = group_max(fminf(fmaxf(__low2float(top), __high2float(top)), 65504.f) * w, c & 1);
-        if (!ok) return;
-        const int e = max(min(exponent(big) - 14, 100), -100);
-        f = w * pow2(-e);
-        back_next = pow2(e);
-      }
-      if (!in) {  // behind the sequence
-        const uint32_t z[4] = {0u, 0u, 0u, 0u};
-#pragma unroll
-        for (int q = 0; q < 4; ++q) sts_v4(s_v + place(row, 4 * half + q), z);
-#pragma unroll
-        for (int q = 0; q < 8; ++q) sts_v4(s_k + half * TILE + place(row, q), z);
-      }
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        uint32_t w4[S::NV][4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          uint32_t pieces[S::NV];
-          split<T, S::NV>(Act<T>::get(r[q][e], 0) * f, Act<T>::get(r[q][e], 1) * f, pieces);
-#pragma unroll
-          for (int k = 0; k < S::NV; ++k) w4[k][e] = pieces[k];
-        }
-#pragma unroll
-        for (int k = 0; k < S::NV; ++k) sts_v4(to + k * TILE + place(row, 4 * half + q), w4[k]);
-      }
-      proxy_fence();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(bar(S::VF, c & 1));
-    };
-    if (chunks > 0) {
-      if constexpr (!STATES) publish(0);
-      if (ok) decayed(0);
-    }
+    if constexpr (!STATES)
+      if (chunks > 0) publish(0);
     for (int c = 0; c < chunks && ok; ++c) {
       const int i = c & 1;
-      back = back_next;
-      const float a = lds_f32(decays(c) + 12 * C);
-      if (c + 1 < chunks) {
-        decayed(c + 1);
-        if (!ok) break;
-      }
       ok = warp_wait(bar(S::DS, i), (uint32_t)((c >> 1) & 1));
-      if constexpr (F16) ok = group_and(ok);  // no warp leaves while another waits at the group's barrier
+      if constexpr (F16) ok = group_and<2, 256>(ok);
       if (!ok) break;
       after_sync();
+      uint32_t r[OWN];
+      tmem_ld_32x32b_x32(tbase + lanes + T_DS + 64 * i + OWN * half, r);
+      const float a = lds_f32(decays(c) + 12 * C), back = F16 ? lds_f32(s0 + S::BACK + 4 * (c & 3)) : 1.f;
+      tmem_wait();
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        uint32_t r[32];
-        tmem_ld_32x32b_x32(tbase + lanes + T_DS + 64 * i + 32 * k, r);
-        tmem_wait();
-#pragma unroll
-        for (int j = 0; j < 32; ++j) st[32 * k + j] = fmaf(a, st[32 * k + j], F16 ? __uint_as_float(r[j]) * back : __uint_as_float(r[j]));
+      for (int j = 0; j < OWN; j += 2) {
+        F2 x(__uint_as_float(r[j]), __uint_as_float(r[j + 1]));
+        if constexpr (F16) x = mul2(x, F2(back, back));
+        fma2(F2(a, a), F2(st[j], st[j + 1]), x).get(st[j], st[j + 1]);
       }
       if constexpr (STATES) {
         before_sync();
@@ -444,19 +498,77 @@ __global__ void __launch_bounds__(32 * WARPS, 1) linear_attention_tc_kernel(cons
       if constexpr (STATES) {
         float4* to = reinterpret_cast<float4*>(seg.states + (size_t)blockIdx.y * gridDim.x * 128 * VT + tile);
 #pragma unroll
-        for (int j = 0; j < VT; j += 4) to[(j / 4) * 128 + d] = make_float4(st[j], st[j + 1], st[j + 2], st[j + 3]);
+        for (int j = 0; j < OWN; j += 4) to[(OWN / 4 * half + j / 4) * 128 + d] = make_float4(st[j], st[j + 1], st[j + 2], st[j + 3]);
       } else if (p.final_state != nullptr && (int)blockIdx.y == (n > 0 ? (n - 1) / seg.tokens : 0) && d < p.K) {
-        float* to = p.final_state + ((size_t)bh * p.K + d) * p.V + v0;
+        float* to = p.final_state + ((size_t)bh * p.K + d) * p.V + v0 + OWN * half;
 #pragma unroll
-        for (int j = 0; j < VT; ++j)
+        for (int j = 0; j < OWN; ++j)
           if (j < cols) to[j] = st[j];
       }
+    }
+  } else {
+    const int id = tid - 512, row = id >> 1, half = id & 1;  // half a token a thread
+    for (int c = 0; c < chunks; ++c) {
+      const int i = c & 1, rows = min(C, stop - first - c * C);
+      const uint32_t s_k = stage(c) + QK, s_v = stage(c) + 2 * QK, to = s0 + S::VO + i * S::NV * TILE;
+      ok = stage_wait(c) && (c < 2 || warp_wait(bar(S::DS, i), (uint32_t)(((c >> 1) + 1) & 1)));  // the product that read this buffer is done
+      if (!F16 && !ok) break;
+      float f = lds_f32(decays(c) + 4 * (2 * C + row));
+      uint32_t r[4][4];
+      const bool in = row < rows;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        if (in) lds_v4(s_v + place(row, 4 * half + q), r[q]);
+        else r[q][0] = r[q][1] = r[q][2] = r[q][3] = 0u;
+      }
+      if constexpr (F16) {
+        __half2 top = __half2half2(__ushort_as_half(0));
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) top = __hmax2(top, __habs2(*reinterpret_cast<__half2*>(&r[q][e])));
+        const float big = group_max<1, 128>(fminf(fmaxf(__low2float(top), __high2float(top)), 65504.f) * f, s0 + S::RED + 16 * i, ok);
+        if (!ok) break;
+        const int e = max(min(exponent(big) - 14, 100), -100);
+        f *= pow2(-e);
+        if (id == 0) sts_u32(s0 + S::BACK + 4 * (c & 3), __float_as_uint(pow2(e)));  // what the sums of v' are multiplied by
+      }
+      if (!in) {  // behind the sequence
+        const uint32_t z[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+        for (int q = 0; q < 4; ++q) sts_v4(s_v + place(row, 4 * half + q), z);
+#pragma unroll
+        for (int q = 0; q < 8; ++q) sts_v4(s_k + half * TILE + place(row, q), z);
+      }
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        uint32_t w4[S::NV][4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if constexpr (F16) {
+            uint32_t pieces[2];
+            split<T, 2>(Act<T>::get(r[q][e], 0) * f, Act<T>::get(r[q][e], 1) * f, pieces);
+            w4[0][e] = pieces[0], w4[1][e] = pieces[1];
+          } else {
+            split3_pair(mul2(F2(Act<T>::get(r[q][e], 0), Act<T>::get(r[q][e], 1)), F2(f, f)), w4[0][e], w4[1][e], w4[S::NV - 1][e]);
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < S::NV; ++k) sts_v4(to + k * TILE + place(row, 4 * half + q), w4[k]);
+      }
+      proxy_fence();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(S::VF, i));
     }
   }
   if (!ok && lane == 0 && p.status != nullptr) atomicExch(p.status, 1);
   __syncwarp();
   before_sync();
   __syncthreads();
+  if (STATES && vt == 0 && tid == 0) {
+    const Pair even(lds_f32(s0 + S::SUM), lds_f32(s0 + S::SUM + 4)), odd(lds_f32(s0 + S::SUM + 8), lds_f32(s0 + S::SUM + 12));
+    seg.decays[(size_t)blockIdx.y * (gridDim.x / vts) + bh] = ex2((even + odd).hi);
+  }
   if (warp == ISSUER) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tbase), "r"(512u) : "memory");
 }
 
