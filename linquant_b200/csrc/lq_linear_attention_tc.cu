@@ -40,13 +40,13 @@ struct Shape {
   static constexpr int NV = F16 ? 2 : 3;  // pieces of v'
   static constexpr int VO = STAGES * STAGE, PO = VO + 2 * NV * TILE, SO = PO + 2 * TILE, GO = SO + 2 * SB;
   static constexpr int RED = GO + GS * GB, EXP = RED + 64, BACK = EXP + 16, SUM = BACK + 16, BARS = SUM + 16;
-  static constexpr int FULL = 0, EMPTY = FULL + STAGES, S1 = EMPTY + STAGES, PF = S1 + 2, VF = PF + 2, DS = VF + 2, SF = DS + 2, OF = SF + 2, OE = OF + 2, LAST = OE + 2, COUNT = LAST + 1;
+  static constexpr int FULL = 0, EMPTY = FULL + STAGES, S1 = EMPTY + STAGES, PF = S1 + 2, VF = PF + 2, DS = VF + 2, SF = DS + 2, OF = SF + 2, OE = OF + 2, DR = OE + 1, LAST = DR + 1, COUNT = LAST + 1;
   static constexpr int TBASE = BARS + 8 * COUNT;
   static constexpr size_t SMEM = 1024 + TBASE + 8;
   static_assert(SMEM <= 232448);
 };
-// tensor memory: columns of the accumulators
-constexpr int T_S1 = 0, T_QS = 128, T_PV = 256, T_DS = 384;
+// tensor memory: columns of the accumulators; q k^T twice, k^T v' a tile for each piece of v'
+constexpr int T_S1 = 0, T_QS = 128, T_PV = 192, T_DS = 256;
 
 __device__ __forceinline__ void mbar_arrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];\n" ::"r"(bar) : "memory"); }
 // By every lane (each needs its own acquire of the phase), warp-uniform. One probe that does not suspend, then the hardware's own short
@@ -57,6 +57,11 @@ __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity) {
   asm volatile("{\n.reg .pred p;\nmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}\n" : "=r"(done) : "r"(bar), "r"(parity) : "memory");
   if (__all_sync(0xffffffffu, done != 0u)) return true;
   return __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity)) != 0;
+}
+__device__ __forceinline__ void tma_store_4d(const CUtensorMap* map, uint32_t src, int c0, int c1, int c2, int c3) {
+  asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.bulk_group [%0, {%2, %3, %4, %5}], [%1];\n" ::"l"(reinterpret_cast<uint64_t>(map)), "r"(src), "r"(c0),
+               "r"(c1), "r"(c2), "r"(c3)
+               : "memory");
 }
 __device__ __forceinline__ void tma_prefetch_4d(const CUtensorMap* map, int c0, int c1, int c2, int c3) {  // to L2
   asm volatile("cp.async.bulk.prefetch.tensor.4d.L2.global [%0, {%1, %2, %3, %4}];\n" ::"l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(c3) : "memory");
@@ -117,8 +122,8 @@ __device__ __forceinline__ uint64_t desc_mn_sw128(uint32_t saddr, int apart) {
 
 template <typename T, bool STATES>
 __global__ void __launch_bounds__(32 * WARPS, 1) linear_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
-                                                                            const __grid_constant__ CUtensorMap map_v, const lq_attention_problem p,
-                                                                            const Segments seg, const int wide) {
+                                                                            const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_o,
+                                                                            const lq_attention_problem p, const Segments seg, const int wide) {
   using S = Shape<T>;
   constexpr bool F16 = S::F16;
   extern __shared__ __align__(1024) uint8_t smem_dyn[];
@@ -133,7 +138,7 @@ __global__ void __launch_bounds__(32 * WARPS, 1) linear_attention_tc_kernel(cons
   const int chunks = stop > first ? (stop - first + C - 1) / C : 0;
   if (tid == 0) {
     for (int i = 0; i < S::COUNT; ++i) {  // arrivals of loads and decays, of a set's or the v' warps, of the state's eight, or one
-      const bool two = i < S::EMPTY, four = (i >= S::PF && i < S::DS) || (i >= S::OE && i < S::LAST), eight = i >= S::SF && i < S::OF;
+      const bool two = i < S::EMPTY, four = (i >= S::PF && i < S::DS) || i == S::OE, eight = (i >= S::SF && i < S::OF) || i == S::DR;
       asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;\n" ::"r"(s_bars + 8u * i), "r"(two ? 2u : four ? 4u : eight ? 8u : 1u));
     }
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
@@ -222,8 +227,8 @@ __global__ void __launch_bounds__(32 * WARPS, 1) linear_attention_tc_kernel(cons
       sts_u32(s0 + S::SUM + 8 * turn + 4, __float_as_uint(total.lo));
     }
   } else if (warp == ISSUER) {
-    const uint32_t id_s1 = idesc<T>(C, C, false, false), id_mn = idesc<T>(C, VT, false, true), id_ds = idesc<T>(128, VT, true, true);
-    const uint64_t d_stage = desc_kmajor_sw128(s0), d_k = desc_mn_sw128(s0 + QK, TILE), d_v = desc_kmajor_sw128(s0 + S::VO), d_p = desc_kmajor_sw128(s0 + S::PO),
+    const uint32_t id_s1 = idesc<T>(C, C, false, false), id_mn = idesc<T>(C, VT, false, true), id_ds = idesc<T>(128, S::NV * VT, true, true);
+    const uint64_t d_stage = desc_kmajor_sw128(s0), d_k = desc_mn_sw128(s0 + QK, TILE), d_v = desc_mn_sw128(s0 + S::VO, TILE), d_p = desc_kmajor_sw128(s0 + S::PO),
                    d_s = desc_kmajor_sw128(s0 + S::SO);
     constexpr uint32_t U = 16;  // descriptors count in units of 16 bytes
     Ring now, ahead;
@@ -257,29 +262,26 @@ __global__ void __launch_bounds__(32 * WARPS, 1) linear_attention_tc_kernel(cons
           after_sync();
           scores(ahead, i ^ 1);
         }
-      } else {
-        if (c >= 2 && !(ok = warp_wait(bar(S::SF, i), turn ^ 1))) break;
       }
       if (!(ok = warp_wait(bar(S::VF, i), turn))) break;
+      if (c >= 1 && !(ok = warp_wait(bar(S::DR, 0), (uint32_t)((c - 1) & 1)))) break;
       after_sync();
-      if (elected()) {  // the pieces of v', the smallest first
+      if (elected()) {  // all pieces of v' side by side: k is read once
         const uint64_t k = d_k + stage_at, v = d_v + (uint64_t)(i * (S::NV * TILE / U));
 #pragma unroll
-        for (int w = S::NV - 1; w >= 0; --w)
-#pragma unroll
-          for (int ks = 0; ks < 4; ++ks) umma_f16(tbase + T_DS + 64 * i, k + ks * (2048 / U), v + w * (TILE / U) + ks * (2048 / U), id_ds, w < S::NV - 1 || ks > 0);
+        for (int ks = 0; ks < 4; ++ks) umma_f16(tbase + T_DS, k + ks * (2048 / U), v + ks * (2048 / U), id_ds, ks > 0);
         umma_commit(bar(S::DS, i));
         if constexpr (STATES) umma_commit(bar(S::EMPTY, now.s));
       }
       __syncwarp();
       if constexpr (!STATES) {
         if (!(ok = warp_wait(bar(S::SF, i), turn))) break;
-        if (c >= 2 && !(ok = warp_wait(bar(S::OE, i), turn ^ 1))) break;
+        if (c >= 1 && !(ok = warp_wait(bar(S::OE, 0), (uint32_t)((c - 1) & 1)))) break;
         after_sync();
         if (elected()) {
           const uint64_t q = d_stage + stage_at, st = d_s + (uint64_t)(i * (SB / U));
 #pragma unroll
-          for (int ks = 0; ks < 8; ++ks) umma_f16(tbase + T_QS + 64 * i, q + (ks / 4) * (TILE / U) + 2 * (ks % 4), st + ks * (2048 / U), id_mn, ks > 0);
+          for (int ks = 0; ks < 8; ++ks) umma_f16(tbase + T_QS, q + (ks / 4) * (TILE / U) + 2 * (ks % 4), st + ks * (2048 / U), id_mn, ks > 0);
         }
         __syncwarp();
         if (!(ok = warp_wait(bar(S::PF, i), turn))) break;
@@ -287,7 +289,7 @@ __global__ void __launch_bounds__(32 * WARPS, 1) linear_attention_tc_kernel(cons
         if (elected()) {
           const uint64_t a = d_p + (uint64_t)(i * (TILE / U)), v = d_stage + stage_at + 2 * QK / U;
 #pragma unroll
-          for (int ks = 0; ks < 4; ++ks) umma_f16(tbase + T_PV + 64 * i, a + 2 * ks, v + ks * (2048 / U), id_mn, ks > 0);
+          for (int ks = 0; ks < 4; ++ks) umma_f16(tbase + T_PV, a + 2 * ks, v + ks * (2048 / U), id_mn, ks > 0);
           umma_commit(bar(S::OF, i));
           umma_commit(bar(S::EMPTY, now.s));
         }
@@ -349,6 +351,8 @@ __global__ void __launch_bounds__(32 * WARPS, 1) linear_attention_tc_kernel(cons
         }
         float up0 = 1.f, up1 = 1.f;
         if constexpr (F16) row_scales(a, tiles, up0, up1);
+        if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;\n" ::: "memory");  // the outputs before have left these rows
+        __syncwarp();
         const uint32_t p0 = s_p + (r0 + g) * 128 + 4 * t4, sw = (uint32_t)(g << 4);  // rows g and g + 8 are swizzled alike
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
@@ -369,12 +373,17 @@ __global__ void __launch_bounds__(32 * WARPS, 1) linear_attention_tc_kernel(cons
           f0 *= e, f1 *= e, c0 = p.scale / up0, c1 = p.scale / up1;
         }
         const bool whole = t0 + C <= stop, in0 = t0 + r0 + g < stop, in1 = t0 + r0 + g + 8 < stop;  // rows behind the sequence are zero
-#pragma unroll
+#pragma unroll 1
         for (int k = 0; k < 2; ++k) {
           uint32_t qs[16], pv[16];
-          tmem_ld_16x256b_x4(tbase + lanes + T_QS + 64 * set + 32 * k, qs);
-          tmem_ld_16x256b_x4(tbase + lanes + T_PV + 64 * set + 32 * k, pv);
+          tmem_ld_16x256b_x4(tbase + lanes + T_QS + 32 * k, qs);
+          tmem_ld_16x256b_x4(tbase + lanes + T_PV + 32 * k, pv);
           tmem_wait();
+          if (k == 1) {
+            before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar(S::OE, 0));
+          }
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             F2 x0(__uint_as_float(pv[4 * j]), __uint_as_float(pv[4 * j + 1])), x1(__uint_as_float(pv[4 * j + 2]), __uint_as_float(pv[4 * j + 3]));
@@ -393,26 +402,27 @@ __global__ void __launch_bounds__(32 * WARPS, 1) linear_attention_tc_kernel(cons
             sts_u32(to + 1024, Act<T>::pack2(o[2], o[3]));
           }
         }
-        before_sync();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bar(S::OE, set));
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const int row = r0 + 4 * k + (lane >> 3), piece = lane & 7, t = t0 + row;
-          uint32_t w[4];
-          lds_v4(s_p + place(row, piece), w);
-          if (t >= last_token || piece * 8 >= cols) continue;
-          T* to = out + (size_t)t * pitch + piece * 8;
-          if (wide) {
-            *reinterpret_cast<uint4*>(to) = make_uint4(w[0], w[1], w[2], w[3]);
-          } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-              if (piece * 8 + e < cols) reinterpret_cast<uint16_t*>(to)[e] = (uint16_t)(w[e / 2] >> (16 * (e & 1)));
+        if (wide) {  // the warp's sixteen rows by TMA; what lies behind T or V is cut off
+          proxy_fence();
+          __syncwarp();
+          if (lane == 0) {
+            tma_store_4d(&map_o, s_p + r0 * 128, v0, t0 + r0, h, b);
+            asm volatile("cp.async.bulk.commit_group;\n" ::: "memory");
           }
+        } else {
+          __syncwarp();
+          for (int k = lane; k < 16 * VT; k += 32) {
+            const int row = r0 + k / VT, col = k % VT;
+            if (t0 + row >= last_token || col >= cols) continue;
+            uint16_t w;
+            asm volatile("ld.shared.u16 %0, [%1];\n" : "=h"(w) : "r"(s_p + place(row, col >> 3) + (col & 7) * 2) : "memory");
+            reinterpret_cast<uint16_t*>(out)[(size_t)(t0 + row) * pitch + col] = w;
+          }
+          __syncwarp();
         }
-        __syncwarp();  // the rows have been read
       }
+      if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;\n" ::: "memory");
+      __syncwarp();
       // tokens behind the sequence, from the first whole chunk that has none of it
       const int from = first + chunks * C;
       for (long long k = tid; k < (long long)max(last_token - from, 0) * VT; k += 256) {
@@ -474,21 +484,26 @@ __global__ void __launch_bounds__(32 * WARPS, 1) linear_attention_tc_kernel(cons
       if constexpr (F16) ok = group_and<2, 256>(ok);
       if (!ok) break;
       after_sync();
-      uint32_t r[OWN];
-      tmem_ld_32x32b_x32(tbase + lanes + T_DS + 64 * i + OWN * half, r);
       const float a = lds_f32(decays(c) + 12 * C), back = F16 ? lds_f32(s0 + S::BACK + 4 * (c & 3)) : 1.f;
-      tmem_wait();
 #pragma unroll
-      for (int j = 0; j < OWN; j += 2) {
-        F2 x(__uint_as_float(r[j]), __uint_as_float(r[j + 1]));
-        if constexpr (F16) x = mul2(x, F2(back, back));
-        fma2(F2(a, a), F2(st[j], st[j + 1]), x).get(st[j], st[j + 1]);
+      for (int j = 0; j < OWN; j += 2) mul2(F2(st[j], st[j + 1]), F2(a, a)).get(st[j], st[j + 1]);
+#pragma unroll 1
+      for (int w = S::NV - 1; w >= 0; --w) {  // the smallest piece first
+        uint32_t r[OWN];
+        tmem_ld_32x32b_x32(tbase + lanes + T_DS + VT * w + OWN * half, r);
+        tmem_wait();
+        if (w == 0) {
+          before_sync();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar(S::DR, 0));
+        }
+#pragma unroll
+        for (int j = 0; j < OWN; j += 2) {
+          const F2 x(__uint_as_float(r[j]), __uint_as_float(r[j + 1])), y(st[j], st[j + 1]);
+          (F16 ? fma2(x, F2(back, back), y) : add2(x, y)).get(st[j], st[j + 1]);
+        }
       }
-      if constexpr (STATES) {
-        before_sync();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bar(S::SF, i));
-      } else if (c + 1 < chunks) {
+      if (!STATES && c + 1 < chunks) {
         if (c >= 1) ok &= warp_wait(bar(S::OF, i ^ 1), (uint32_t)(((c - 1) >> 1) & 1));
         if (!F16 && !ok) break;
         publish(c + 1);
@@ -514,19 +529,17 @@ __global__ void __launch_bounds__(32 * WARPS, 1) linear_attention_tc_kernel(cons
       ok = stage_wait(c) && (c < 2 || warp_wait(bar(S::DS, i), (uint32_t)(((c >> 1) + 1) & 1)));  // the product that read this buffer is done
       if (!F16 && !ok) break;
       float f = lds_f32(decays(c) + 4 * (2 * C + row));
-      uint32_t r[4][4];
       const bool in = row < rows;
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        if (in) lds_v4(s_v + place(row, 4 * half + q), r[q]);
-        else r[q][0] = r[q][1] = r[q][2] = r[q][3] = 0u;
-      }
       if constexpr (F16) {
         __half2 top = __half2half2(__ushort_as_half(0));
 #pragma unroll
-        for (int q = 0; q < 4; ++q)
+        for (int q = 0; q < 4; ++q) {
+          uint32_t x[4];
+          if (in) lds_v4(s_v + place(row, 4 * half + q), x);
+          else x[0] = x[1] = x[2] = x[3] = 0u;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) top = __hmax2(top, __habs2(*reinterpret_cast<__half2*>(&r[q][e])));
+          for (int e = 0; e < 4; ++e) top = __hmax2(top, __habs2(*reinterpret_cast<__half2*>(&x[e])));
+        }
         const float big = group_max<1, 128>(fminf(fmaxf(__low2float(top), __high2float(top)), 65504.f) * f, s0 + S::RED + 16 * i, ok);
         if (!ok) break;
         const int e = max(min(exponent(big) - 14, 100), -100);
@@ -540,17 +553,19 @@ __global__ void __launch_bounds__(32 * WARPS, 1) linear_attention_tc_kernel(cons
 #pragma unroll
         for (int q = 0; q < 8; ++q) sts_v4(s_k + half * TILE + place(row, q), z);
       }
-#pragma unroll
+#pragma unroll 1
       for (int q = 0; q < 4; ++q) {
-        uint32_t w4[S::NV][4];
+        uint32_t w4[S::NV][4], x[4];
+        if (F16 || in) lds_v4(s_v + place(row, 4 * half + q), x);
+        else x[0] = x[1] = x[2] = x[3] = 0u;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           if constexpr (F16) {
             uint32_t pieces[2];
-            split<T, 2>(Act<T>::get(r[q][e], 0) * f, Act<T>::get(r[q][e], 1) * f, pieces);
+            split<T, 2>(Act<T>::get(x[e], 0) * f, Act<T>::get(x[e], 1) * f, pieces);
             w4[0][e] = pieces[0], w4[1][e] = pieces[1];
           } else {
-            split3_pair(mul2(F2(Act<T>::get(r[q][e], 0), Act<T>::get(r[q][e], 1)), F2(f, f)), w4[0][e], w4[1][e], w4[S::NV - 1][e]);
+            split3_pair(mul2(F2(Act<T>::get(x[e], 0), Act<T>::get(x[e], 1)), F2(f, f)), w4[0][e], w4[1][e], w4[S::NV - 1][e]);
           }
         }
 #pragma unroll
@@ -572,14 +587,14 @@ __global__ void __launch_bounds__(32 * WARPS, 1) linear_attention_tc_kernel(cons
   if (warp == ISSUER) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tbase), "r"(512u) : "memory");
 }
 
-// rows of `width` channels as boxes of 64 tokens x 64 channels, zero behind the last channel and token
-static int encode(CUtensorMap* m, bool f16, const void* base, int width, int T, int heads, int B, long long st, long long sh, long long sb) {
+// rows of `width` channels as boxes of `rows` tokens x 64 channels, zero behind the last channel and token
+static int encode(CUtensorMap* m, bool f16, const void* base, int width, int T, int heads, int B, long long st, long long sh, long long sb, int rows = C) {
   EncodeTiledFn enc = encode_tiled_fn();
   if (enc == nullptr) return fail(LQ_ERR_LAUNCH, "linear_attention: the driver does not export cuTensorMapEncodeTiled");
   const cuuint64_t gdim[4] = {(cuuint64_t)width, (cuuint64_t)T, (cuuint64_t)heads, (cuuint64_t)B};
   // an axis of one has any stride
   const cuuint64_t gstride[3] = {T > 1 ? (cuuint64_t)st * 2 : 1024, heads > 1 ? (cuuint64_t)sh * 2 : 1024, B > 1 ? (cuuint64_t)sb * 2 : 1024};
-  const cuuint32_t box[4] = {64, (cuuint32_t)C, 1, 1}, estr[4] = {1, 1, 1, 1};
+  const cuuint32_t box[4] = {64, (cuuint32_t)rows, 1, 1}, estr[4] = {1, 1, 1, 1};
   const CUresult r = enc(m, f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), gdim, gstride, box, estr,
                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? LQ_OK : fail(LQ_ERR_LAUNCH, "linear_attention: cuTensorMapEncodeTiled failed with CUresult %d", (int)r);
@@ -593,13 +608,16 @@ static int run(const lq_attention_problem* p, const Plan& r, const Segments& seg
   if (int e = encode(&k, S::F16, p->k, p->K, p->T, p->Hk, p->B, p->k_stride_t, p->k_stride_h, p->k_stride_b)) return e;
   if (int e = encode(&v, S::F16, p->v, p->V, p->T, p->H, p->B, p->v_stride_t, p->v_stride_h, p->v_stride_b)) return e;
   const int wide = p->V % 8 == 0 && (reinterpret_cast<uintptr_t>(p->o) & 15u) == 0;
+  CUtensorMap o = q;
+  if (wide)
+    if (int e = encode(&o, S::F16, p->o, p->V, p->T, p->H, p->B, (long long)p->H * p->V, p->V, (long long)p->T * p->H * p->V, 16)) return e;
   const dim3 block(32 * WARPS);
   cudaError_t e = cudaSuccess;
   if (seg.count > 1) {
-    e = launch_opt_in(linear_attention_tc_kernel<T, true>, dim3((unsigned)r.tiles, seg.count - 1), block, S::SMEM, st, q, k, v, *p, seg, wide);
+    e = launch_opt_in(linear_attention_tc_kernel<T, true>, dim3((unsigned)r.tiles, seg.count - 1), block, S::SMEM, st, q, k, v, o, *p, seg, wide);
     if (e == cudaSuccess && seg.count > 2) e = launch_segment_states(seg, p->B * p->H, r.tiles * 128 * VT, st);
   }
-  if (e == cudaSuccess) e = launch_opt_in(linear_attention_tc_kernel<T, false>, dim3((unsigned)r.tiles, seg.count), block, S::SMEM, st, q, k, v, *p, seg, wide);
+  if (e == cudaSuccess) e = launch_opt_in(linear_attention_tc_kernel<T, false>, dim3((unsigned)r.tiles, seg.count), block, S::SMEM, st, q, k, v, o, *p, seg, wide);
   if (e != cudaSuccess) return fail(LQ_ERR_LAUNCH, "linear_attention: %s", cudaGetErrorString(e));
   return check_launch("linear_attention_tc_kernel");
 }
