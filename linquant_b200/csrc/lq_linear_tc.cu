@@ -237,6 +237,12 @@ __global__ void __launch_bounds__(THREADS, 1) int8_linear_tc_kernel(const __grid
         sts_u32(cols + 4 * (S::HALF + c), __float_as_uint(in && p.bias ? __ldg(p.bias + n0 + c) : 0.f));
       }
       __syncwarp();
+      auto low = [&] {
+        if constexpr (LORA) return LoraTile<CHUNK / 8, sizeof(TO) == 4 ? 3 : 2>(lora, p.M, p.N, row0);
+        else return 0;
+      }();
+      if constexpr (LORA)
+        if (n0 < p.N) low.begin(n0);
       if (!(ok = __all_sync(0xffffffffu, wait(s_acc + 8 * acc, (uint32_t)((i / 2) & 1))))) break;
       asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
 #pragma unroll 1
@@ -268,7 +274,8 @@ __global__ void __launch_bounds__(THREADS, 1) int8_linear_tc_kernel(const __grid
               v[i][j][3] = fmaf((float)(int)r[i][4 * j + 3] * xs1, ws.y, b.y);
             }
           }
-          lora_add<NT, sizeof(TO) == 4 ? 3 : 2>(v, lora, p.M, p.N, row0, n0 + c0);
+          low.add(v);
+          if (c0 + CHUNK < S::HALF && n0 + c0 + CHUNK < p.N) low.begin(n0 + c0 + CHUNK);  // on its way while this chunk is stored
           __syncwarp();  // the chunk before has been read
 #pragma unroll
           for (int i = 0; i < 2; ++i)

@@ -4,7 +4,7 @@
 //
 // l = adapters[m]; c are x's codes. Two kernels: this file's makes t, the INT8 product's own kernels add the second sum to a tile while it
 // is still fp32 (lq_lora.cuh), so y is rounded and written once.
-// t: a CTA has a tile of 1, 16 or 64 tokens (32 of three pieces) and, of a cluster, a part of K; its four warps share that part and their sums meet in
+// t: a CTA has a tile of 1, 16 or 32 tokens and, of a cluster, a part of K; its four warps share that part and their sums meet in
 // shared memory, first the warps', then the CTAs', in a fixed order. Operands come from global memory straight into the fragments
 // of m16n8k16 (the reduction index permuted alike in both: a lane takes eight consecutive k). A tile whose tokens have several
 // adapters goes over its K once for each of them. Products are exact: both operands as bf16 pieces (codes and bf16 one, fp16 two, fp32
@@ -16,7 +16,7 @@ namespace lq {
 
 namespace lora {
 
-constexpr int WARPS = 4, THREADS = 32 * WARPS, NT = 8;  // NT: tiles of 8 ranks at a time
+constexpr int WARPS = 4, THREADS = 32 * WARPS;
 
 template <typename TX, typename TA>
 struct Types {
@@ -26,44 +26,69 @@ struct Types {
   static constexpr int NX = pieces<TX>(), NA = pieces<TA>(), KEEP = NX > NA ? NX : NA;
 };
 
-// eight consecutive values from p as words of pairs, in pieces; VEC: p on a boundary of eight values (16 bytes at most)
-template <typename T, int N, bool F16, bool VEC>
-__device__ __forceinline__ void load8(const T* p, int left, uint32_t (&w)[N][4]) {
-  float x[8];
-  if constexpr (VEC && sizeof(T) == 2 && N == 1) {  // as they are
-    const uint4 v = left > 0 ? __ldg(reinterpret_cast<const uint4*>(p)) : make_uint4(0, 0, 0, 0);
-    w[0][0] = v.x, w[0][1] = v.y, w[0][2] = v.z, w[0][3] = v.w;
-    return;
-  } else if constexpr (VEC && std::is_same_v<T, int8_t>) {
-    const uint2 v = left > 0 ? __ldg(reinterpret_cast<const uint2*>(p)) : make_uint2(0, 0);
-    const uint32_t a = v.x ^ 0x80808080u, b = v.y ^ 0x80808080u;
-    x[0] = s8_to_float<0>(a), x[1] = s8_to_float<1>(a), x[2] = s8_to_float<2>(a), x[3] = s8_to_float<3>(a);
-    x[4] = s8_to_float<0>(b), x[5] = s8_to_float<1>(b), x[6] = s8_to_float<2>(b), x[7] = s8_to_float<3>(b);
-  } else if constexpr (VEC && sizeof(T) == 2) {
-    const uint4 v = left > 0 ? __ldg(reinterpret_cast<const uint4*>(p)) : make_uint4(0, 0, 0, 0);
-    Act<T>::unpack8(v, x);
-  } else if constexpr (VEC) {
-    const float4 z = make_float4(0.f, 0.f, 0.f, 0.f), a = left > 0 ? __ldg(reinterpret_cast<const float4*>(p)) : z, b = left > 0 ? __ldg(reinterpret_cast<const float4*>(p) + 1) : z;
-    x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
-  } else {
+// Eight consecutive values, on their way and then as words of pairs in pieces. VEC: they start on a boundary of eight values (16 bytes at most)
+template <typename T, bool VEC>
+struct Eight {
+  static constexpr int WORDS = VEC ? 2 * sizeof(T) : 8;
+  uint32_t w[WORDS];
+  __device__ __forceinline__ void load(const T* p, int left) {  // what lies `left` values or more behind p is zero and not read
+    if constexpr (VEC) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      if constexpr (std::is_same_v<T, int8_t>) x[i] = i < left ? (float)__ldg(p + i) : 0.f;
-      else x[i] = i < left ? to_f32(p[i]) : 0.f;
-    }
-  }
+      for (int i = 0; i < WORDS; ++i) w[i] = 0u;
+      if (left <= 0) return;
+      if constexpr (WORDS == 2) {
+        const uint2 v = __ldg(reinterpret_cast<const uint2*>(p));
+        w[0] = v.x, w[1] = v.y;
+      } else {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if constexpr (F16) {
-      w[0][i] = Act<__half>::pack2(x[2 * i], x[2 * i + 1]);
+        for (int i = 0; i < WORDS; i += 4) {
+          const uint4 v = __ldg(reinterpret_cast<const uint4*>(p) + i / 4);
+          w[i] = v.x, w[i + 1] = v.y, w[i + 2] = v.z, w[i + 3] = v.w;
+        }
+      }
     } else {
-      uint32_t q[N];
-      bf16_pieces<N>(x[2 * i], x[2 * i + 1], q);
 #pragma unroll
-      for (int k = 0; k < N; ++k) w[k][i] = q[k];
+      for (int i = 0; i < 8; ++i) {
+        float x = 0.f;
+        if (i < left) {
+          if constexpr (std::is_same_v<T, int8_t>) x = (float)__ldg(p + i);
+          else x = to_f32(p[i]);
+        }
+        w[i] = __float_as_uint(x);
+      }
     }
   }
-}
+  template <int N, bool F16>
+  __device__ __forceinline__ void pieces(uint32_t (&q)[N][4]) const {
+    if constexpr (VEC && sizeof(T) == 2 && N == 1) {  // as they are
+#pragma unroll
+      for (int i = 0; i < 4; ++i) q[0][i] = w[i];
+    } else {
+      float x[8];
+      if constexpr (VEC && std::is_same_v<T, int8_t>) {
+        const uint32_t a = w[0] ^ 0x80808080u, b = w[1] ^ 0x80808080u;
+        x[0] = s8_to_float<0>(a), x[1] = s8_to_float<1>(a), x[2] = s8_to_float<2>(a), x[3] = s8_to_float<3>(a);
+        x[4] = s8_to_float<0>(b), x[5] = s8_to_float<1>(b), x[6] = s8_to_float<2>(b), x[7] = s8_to_float<3>(b);
+      } else if constexpr (VEC && sizeof(T) == 2) {
+        Act<T>::unpack8(make_uint4(w[0], w[1], w[2], w[3]), x);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = __uint_as_float(w[i]);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (F16) {
+          q[0][i] = Act<__half>::pack2(x[2 * i], x[2 * i + 1]);
+        } else {
+          uint32_t r[N];
+          bf16_pieces<N>(x[2 * i], x[2 * i + 1], r);
+#pragma unroll
+          for (int k = 0; k < N; ++k) q[k][i] = r[k];
+        }
+      }
+    }
+  }
+};
 
 struct Shrink {
   int M, K, L, R, RP, parts;
@@ -76,8 +101,8 @@ struct Shrink {
   float* t;
 };
 
-// TILE: tokens of a CTA
-template <typename TX, typename TA, int TILE, bool VEC>
+// TILE: tokens of a CTA; NT: tiles of 8 ranks at a time
+template <typename TX, typename TA, int TILE, bool VEC, int NT>
 __global__ void __launch_bounds__(THREADS) lora_shrink_kernel(const Shrink p) {
   using Y = Types<TX, TA>;
   constexpr int MT = (TILE + 15) / 16, ROWS = 16 * MT;
@@ -110,38 +135,52 @@ __global__ void __launch_bounds__(THREADS) lora_shrink_kernel(const Shrink p) {
         for (int j = 0; j < NT; ++j)
 #pragma unroll
           for (int e = 0; e < 4; ++e) acc[i][j][e] = 0.f;
-      const TA* a = reinterpret_cast<const TA*>(p.a) + ((long long)l * p.R + r0 + g) * p.K;
-      const TX* x = reinterpret_cast<const TX*>(p.x);
-#pragma unroll 2
-      for (int s = step0 + warp; s < step1; s += WARPS) {
-        const int k = 32 * s + 8 * t4, left = p.K - k;
-        uint32_t xa[MT][2][Y::NX][4];
+      const TA* a = reinterpret_cast<const TA*>(p.a) + ((long long)l * p.R + r0 + g) * p.K + 8 * t4;
+      const TX* x = reinterpret_cast<const TX*>(p.x) + (long long)(m0 + g) * p.x_stride + 8 * t4;
+      bool own[MT][2];  // a token with another adapter is not read for this one
 #pragma unroll
-        for (int i = 0; i < MT; ++i)
+      for (int i = 0; i < MT; ++i) own[i][0] = which[16 * i + g] == l, own[i][1] = which[16 * i + g + 8] == l;
+      // U steps of 32 on their way
+      constexpr int U = MT * Eight<TX, VEC>::WORDS * 2 + NT * Eight<TA, VEC>::WORDS <= 24 ? 4 : MT * Eight<TX, VEC>::WORDS * 2 + NT * Eight<TA, VEC>::WORDS <= 48 ? 2 : 1;
+      for (int s0 = step0 + warp; s0 < step1; s0 += U * WARPS) {
+        Eight<TX, VEC> rx[U][MT][2];
+        Eight<TA, VEC> ra[U][NT];
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const int row = 16 * i + 8 * h + g;
-            // a token with another adapter is not read for this one
-            load8<TX, Y::NX, Y::F16, VEC>(x + (long long)(m0 + row) * p.x_stride + k, which[row] == l ? left : 0, xa[i][h]);
-          }
+        for (int u = 0; u < U; ++u) {
+          const int s = s0 + u * WARPS, k = 32 * s, left = s < step1 ? p.K - k - 8 * t4 : 0;
 #pragma unroll
-        for (int j = 0; j < NT; ++j) {
-          if (j >= tiles) break;
-          uint32_t b[Y::NA][4];
-          load8<TA, Y::NA, Y::F16, VEC>(a + 8ll * j * p.K + k, left, b);
+          for (int i = 0; i < MT; ++i)
 #pragma unroll
-          for (int h = 0; h < 2; ++h)
+            for (int h = 0; h < 2; ++h) rx[u][i][h].load(x + (long long)(16 * i + 8 * h) * p.x_stride + k, own[i][h] ? left : 0);
 #pragma unroll
-            for (int n = Y::NA - 1; n >= 0; --n)
+          for (int j = 0; j < NT; ++j) ra[u][j].load(a + 8ll * j * p.K + k, j < tiles ? left : 0);
+        }
 #pragma unroll
-              for (int o = Y::NX - 1; o >= 0; --o) {
-                if (n + o >= (Y::KEEP > 1 ? 3 : 1)) continue;
+        for (int u = 0; u < U; ++u) {
+          uint32_t xa[MT][2][Y::NX][4];
 #pragma unroll
-                for (int i = 0; i < MT; ++i) {
-                  if constexpr (Y::F16) mma_f16(acc[i][j], xa[i][0][o][2 * h], xa[i][1][o][2 * h], xa[i][0][o][2 * h + 1], xa[i][1][o][2 * h + 1], b[n][2 * h], b[n][2 * h + 1]);
-                  else mma_bf16(acc[i][j], xa[i][0][o][2 * h], xa[i][1][o][2 * h], xa[i][0][o][2 * h + 1], xa[i][1][o][2 * h + 1], b[n][2 * h], b[n][2 * h + 1]);
+          for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) rx[u][i][h].template pieces<Y::NX, Y::F16>(xa[i][h]);
+#pragma unroll
+          for (int j = 0; j < NT; ++j) {
+            if (j >= tiles) break;
+            uint32_t b[Y::NA][4];
+            ra[u][j].template pieces<Y::NA, Y::F16>(b);
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+              for (int n = Y::NA - 1; n >= 0; --n)
+#pragma unroll
+                for (int o = Y::NX - 1; o >= 0; --o) {
+                  if (n + o >= (Y::KEEP > 1 ? 3 : 1)) continue;
+#pragma unroll
+                  for (int i = 0; i < MT; ++i) {
+                    if constexpr (Y::F16) mma_f16(acc[i][j], xa[i][0][o][2 * h], xa[i][1][o][2 * h], xa[i][0][o][2 * h + 1], xa[i][1][o][2 * h + 1], b[n][2 * h], b[n][2 * h + 1]);
+                    else mma_bf16(acc[i][j], xa[i][0][o][2 * h], xa[i][1][o][2 * h], xa[i][0][o][2 * h + 1], xa[i][1][o][2 * h + 1], b[n][2 * h], b[n][2 * h + 1]);
+                  }
                 }
-              }
+          }
         }
       }
 #pragma unroll
@@ -191,9 +230,9 @@ __global__ void __launch_bounds__(THREADS) lora_shrink_kernel(const Shrink p) {
   if (p.parts > 1) asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");  // no CTA's sums are read any more
 }
 
-template <typename TX, typename TA, int TILE, bool VEC>
+template <typename TX, typename TA, int TILE, bool VEC, int NT>
 static int shrink(const Shrink& p, int tiles, cudaStream_t st) {
-  auto kern = lora_shrink_kernel<TX, TA, TILE, VEC>;
+  auto kern = lora_shrink_kernel<TX, TA, TILE, VEC, NT>;
   constexpr int most = WARPS * TILE * 128 * 4;
   cudaError_t e = cudaSuccess;
   if (most > 48 * 1024) e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
@@ -217,21 +256,22 @@ static int shrink(const Shrink& p, int tiles, cudaStream_t st) {
   return check_launch("lora_shrink_kernel");
 }
 
-// Tokens of a CTA: one each for a decode step, whose tokens have adapters of their own; 64 or 32 where that still leaves two CTAs an SM.
-// Parts of K: two CTAs an SM, and no fewer than 128 of K for a warp.
+// Tokens of a CTA: one each for a decode step, whose tokens have adapters of their own; 32 where that leaves a CTA an SM, so that a's rows are
+// read for twice as many. Parts of K: up to four CTAs an SM, and no fewer than 128 of K for a warp.
 template <typename TX, typename TA>
 static int run_shrink(Shrink p, bool vec, cudaStream_t st) {
-  constexpr int BIG = Types<TX, TA>::KEEP == 3 ? 32 : 64;  // three pieces of 64 tokens would not fit a thread's registers
-  const int sms = sm_count(), tile = p.M <= 64 ? 1 : p.M >= 2 * BIG * sms ? BIG : 16, tiles = (p.M + tile - 1) / tile;
+  const int sms = sm_count(), tile = p.M <= 64 ? 1 : p.M >= 32 * sms ? 32 : 16, tiles = (p.M + tile - 1) / tile;
   p.parts = 8;
   while (p.parts > 1 && ((long long)tiles * p.parts > 4ll * sms || p.K < 512 * p.parts)) p.parts /= 2;
-  auto go = [&](auto v) {
+  auto go = [&](auto v, auto nt) {
     constexpr bool VEC = decltype(v)::value;
-    if (tile == 1) return shrink<TX, TA, 1, VEC>(p, tiles, st);
-    if (tile == 16) return shrink<TX, TA, 16, VEC>(p, tiles, st);
-    return shrink<TX, TA, BIG, VEC>(p, tiles, st);
+    constexpr int NT = decltype(nt)::value;
+    if (tile == 1) return shrink<TX, TA, 1, VEC, NT>(p, tiles, st);
+    if (tile == 16) return shrink<TX, TA, 16, VEC, NT>(p, tiles, st);
+    return shrink<TX, TA, 32, VEC, NT>(p, tiles, st);
   };
-  return vec ? go(std::true_type()) : go(std::false_type());
+  auto width = [&](auto v) { return p.R <= 16 ? go(v, std::integral_constant<int, 2>()) : go(v, std::integral_constant<int, 8>()); };
+  return vec ? width(std::true_type()) : width(std::false_type());
 }
 
 }  // namespace lora

@@ -66,69 +66,113 @@ __device__ __forceinline__ void bf16_pieces(float a, float b, uint32_t (&p)[N]) 
   }
 }
 
-// The sums of 32 tokens (m0 + lane) and 8 NT channels from n0, added to accumulator fragments: v[i][j] has the tokens 16 i + g (+ 8), the
-// channels 8 j + 2 q (+ 1). One pass over R for each adapter that the tokens have. The reduction index is permuted alike in both
-// operands: a lane takes four consecutive r. Both go in as PIECES bf16 pieces, products of pieces that add up to 8 PIECES bits or
-// more behind the first are left out: 16 bits for 16-bit outputs, 24 for fp32.
+// The sums of 32 tokens (m0 + lane) and 8 NT channels, added to accumulator fragments: v[i][j] has the tokens 16 i + g (+ 8), the
+// channels 8 j + 2 q (+ 1) from n0. One pass over R for each adapter that the tokens have, the operands of the next step requested before
+// the products of this one. The reduction index is permuted alike in both operands: a lane takes four consecutive r. Both go in as
+// PIECES bf16 pieces (b of bf16: one), products of pieces that add up to 8 PIECES bits or more behind the first are left out: 16
+// bits for 16-bit outputs, 24 for fp32.
 template <int NT, int PIECES>
-__device__ __forceinline__ void lora_add(float (&v)[2][NT][4], const Lora& q, int M, int N, int m0, int n0) {
-  const int lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
-  const int mine = m0 + lane < M ? q.of(m0 + lane) : -1;
-  uint32_t left = __ballot_sync(0xffffffffu, mine >= 0);
-  while (left) {
-    const int l = __shfl_sync(0xffffffffu, mine, __ffs(left) - 1);
-    const uint32_t rows = __ballot_sync(0xffffffffu, mine == l);
+struct LoraTile {
+  const Lora& q;
+  int N, n0, m0, mine, l = 0, r0 = 0;
+  uint32_t all, rows = 0, left = 0;
+  float b[NT][4];
+  float4 t[2][2];
+  __device__ __forceinline__ LoraTile(const Lora& q, int M, int N, int m0) : q(q), N(N), m0(m0) {
+    const int lane = threadIdx.x & 31;
+    mine = m0 + lane < M ? q.of(m0 + lane) : -1;
+    all = __ballot_sync(0xffffffffu, mine >= 0);
+  }
+  __device__ __forceinline__ void next_adapter() {
+    l = __shfl_sync(0xffffffffu, mine, __ffs(left) - 1);
+    rows = __ballot_sync(0xffffffffu, mine == l);
     left &= ~rows;
-    float s[2][NT][4];  // apart from the outputs: an infinity or NaN in b is no other adapter's
+    r0 = 0;
+  }
+  __device__ __forceinline__ void request() {
+    const int lane = threadIdx.x & 31, g = lane >> 2, r = r0 + 4 * (lane & 3);
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-      for (int j = 0; j < NT; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) s[i][j][e] = 0.f;
-    for (int r0 = 0; r0 < q.R; r0 += 16) {
-      const int r = r0 + 4 * t4;
-      float b[NT][4];
-#pragma unroll
-      for (int j = 0; j < NT; ++j) {
-        const int n = n0 + 8 * j + g;
-        if (n < N && r < q.R) lora_row4(q, (long long)l * N + n, r, b[j]);
-        else b[j][0] = b[j][1] = b[j][2] = b[j][3] = 0.f;
-      }
-      uint32_t a[2][PIECES][4];
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int row = 16 * i + 8 * h + g;
-          float4 t = make_float4(0.f, 0.f, 0.f, 0.f);
-          if (rows >> row & 1) t = *reinterpret_cast<const float4*>(q.t + (long long)(m0 + row) * q.RP + r);
-          uint32_t lo[PIECES], hi[PIECES];
-          bf16_pieces<PIECES>(t.x, t.y, lo);
-          bf16_pieces<PIECES>(t.z, t.w, hi);
-#pragma unroll
-          for (int k = 0; k < PIECES; ++k) a[i][k][h] = lo[k], a[i][k][2 + h] = hi[k];
-        }
-#pragma unroll
-      for (int j = 0; j < NT; ++j) {
-        uint32_t lo[PIECES], hi[PIECES];
-        bf16_pieces<PIECES>(b[j][0], b[j][1], lo);
-        bf16_pieces<PIECES>(b[j][2], b[j][3], hi);
-#pragma unroll
-        for (int k = PIECES - 1; k >= 0; --k)
-#pragma unroll
-          for (int o = PIECES - 1 - k; o >= 0; --o)
-#pragma unroll
-            for (int i = 0; i < 2; ++i) mma_bf16(s[i][j], a[i][o][0], a[i][o][1], a[i][o][2], a[i][o][3], lo[k], hi[k]);
-      }
+    for (int j = 0; j < NT; ++j) {
+      const int n = n0 + 8 * j + g;
+      if (n < N && r < q.R) lora_row4(q, (long long)l * N + n, r, b[j]);
+      else b[j][0] = b[j][1] = b[j][2] = b[j][3] = 0.f;
     }
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
-      for (int j = 0; j < NT; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[i][j][e] += rows >> (16 * i + g + 8 * (e >> 1)) & 1 ? s[i][j][e] : 0.f;
+      for (int h = 0; h < 2; ++h) {
+        const int row = 16 * i + 8 * h + g;
+        t[i][h] = rows >> row & 1 ? *reinterpret_cast<const float4*>(q.t + (long long)(m0 + row) * q.RP + r) : make_float4(0.f, 0.f, 0.f, 0.f);
+      }
   }
-}
+  // the first operands for the channels from n
+  __device__ __forceinline__ void begin(int n) {
+    if (!all) return;
+    n0 = n;
+    left = all;
+    next_adapter();
+    request();
+  }
+  __device__ __forceinline__ void add(float (&v)[2][NT][4]) {
+    if (!all) return;
+    const int lane = threadIdx.x & 31, g = lane >> 2;
+    bool more = true;
+    while (more) {
+      const uint32_t now = rows;
+      float s[2][NT][4];  // apart from the outputs: an infinity or NaN in b is no other adapter's
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[i][j][e] = 0.f;
+      bool same = true;
+      while (same) {
+        uint32_t a[2][PIECES][4], w[NT][PIECES][2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            uint32_t lo[PIECES], hi[PIECES];
+            bf16_pieces<PIECES>(t[i][h].x, t[i][h].y, lo);
+            bf16_pieces<PIECES>(t[i][h].z, t[i][h].w, hi);
+#pragma unroll
+            for (int k = 0; k < PIECES; ++k) a[i][k][h] = lo[k], a[i][k][2 + h] = hi[k];
+          }
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+          uint32_t lo[PIECES], hi[PIECES];
+          bf16_pieces<PIECES>(b[j][0], b[j][1], lo);
+          bf16_pieces<PIECES>(b[j][2], b[j][3], hi);
+#pragma unroll
+          for (int k = 0; k < PIECES; ++k) w[j][k][0] = lo[k], w[j][k][1] = hi[k];
+        }
+        r0 += 16;
+        same = r0 < q.R;
+        if (!same) {
+          more = left != 0;
+          if (more) next_adapter();
+        }
+        if (same || more) request();
+#pragma unroll
+        for (int k = PIECES - 1; k >= 0; --k) {
+          if (k > 0 && q.dtype == LQ_BF16) continue;
+#pragma unroll
+          for (int o = PIECES - 1 - k; o >= 0; --o)
+#pragma unroll
+            for (int j = 0; j < NT; ++j)
+#pragma unroll
+              for (int i = 0; i < 2; ++i) mma_bf16(s[i][j], a[i][o][0], a[i][o][1], a[i][o][2], a[i][o][3], w[j][k][0], w[j][k][1]);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[i][j][e] += now >> (16 * i + g + 8 * (e >> 1)) & 1 ? s[i][j][e] : 0.f;
+    }
+  }
+};
 
 }  // namespace lq
