@@ -242,7 +242,10 @@ __global__ void __launch_bounds__(THREADS, 1) int8_linear_tc_kernel(const __grid
         else return 0;
       }();
       if constexpr (LORA)
-        if (n0 < p.N) low.begin(n0);
+        if (n0 < p.N) {
+          low.prefetch(n0, S::HALF);
+          low.begin(n0);
+        }
       if (!(ok = __all_sync(0xffffffffu, wait(s_acc + 8 * acc, (uint32_t)((i / 2) & 1))))) break;
       asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
 #pragma unroll 1
@@ -552,7 +555,8 @@ static int launch_tc(const lq_linear_problem* p, const Lora* lora, cudaStream_t 
 }
 
 template <typename TO>
-static int launch_split(const lq_linear_problem* p, const Lora* lora, int tiles, int parts, cudaStream_t st) {
+static int launch_split(const lq_linear_problem* p, const Lora* lora, int parts, cudaStream_t st) {
+  const int tiles = (p->M + 127) / 128 * ((p->N + Split::BN - 1) / Split::BN);
   CUtensorMap mx, mw;
   if (int e = encode(&mx, p->x, p->K, p->x_stride, p->M, BM)) return e;
   if (int e = encode(&mw, p->w, p->K, p->w_stride, p->N, Split::BN)) return e;
@@ -561,6 +565,19 @@ static int launch_split(const lq_linear_problem* p, const Lora* lora, int tiles,
 }
 
 }  // namespace lineartc
+
+static int parts_of(const lq_linear_problem* p) {
+  // Few tiles of a long K: parts of at least 8 blocks for the CTAs of a cluster, two CTAs on an SM. 5120 -> 2560, 64 tokens: one part
+  // 14.3 us, 2, 4, 8 parts 11.0, 8.6, 8.7; 256 tokens, 2 parts: 14.5 -> 12.5; 8192 -> 1024, 33 tokens, 8 parts: 20.7 -> 7.9. To meet
+  // costs some 2 us, more than a short K has: 200 x 2560 -> 2560 9.0 -> 9.5, 100 x 1024 -> 1024 4.9 -> 6.7
+  const long long mt = (p->M + 127) / 128, sms = sm_count(), narrow = mt * ((p->N + lineartc::Split::BN - 1) / lineartc::Split::BN),
+                  blocks = (p->K + lineartc::BK - 1) / lineartc::BK;
+  int parts = blocks < 32 ? 1 : 8;
+  while (parts > 1 && (narrow * parts > 2 * sms || blocks < 8 * parts)) parts /= 2;
+  return parts;
+}
+
+bool linear_takes_halves(const lq_linear_problem* p) { return p->M > 16 && p->out_dtype != LQ_F32 && parts_of(p) == 1; }
 
 // The widest tiles that do not leave SMs idle: rounds of tiles x the time of one, which grows with its width and a fixed part
 // (the 128 rows of x that every tile loads)
@@ -575,15 +592,10 @@ int run_linear_tc(const lq_linear_problem* p, const Lora* lora, cudaStream_t st)
   // Pairs of CTAs read the weights half as often from shared memory; over a few rounds their larger tiles cost more than that:
   // 8192 x 2560 -> 2560 (4.3 rounds) 54 us against 53, 4096 x 2560 -> 10576 (9) 91 against 102, 32768 x 2560 -> 10576 (73) 688 against 743
   const bool pair = mt * ((p->N + 255) / 256) >= 6 * sms;
-  // Few tiles of a long K: parts of at least 8 blocks for the CTAs of a cluster, two CTAs on an SM. 5120 -> 2560, 64 tokens: one part
-  // 14.3 us, 2, 4, 8 parts 11.0, 8.6, 8.7; 256 tokens, 2 parts: 14.5 -> 12.5; 8192 -> 1024, 33 tokens, 8 parts: 20.7 -> 7.9. To meet
-  // costs some 2 us, more than a short K has: 200 x 2560 -> 2560 9.0 -> 9.5, 100 x 1024 -> 1024 4.9 -> 6.7
-  const long long narrow = mt * ((p->N + lineartc::Split::BN - 1) / lineartc::Split::BN), blocks = (p->K + lineartc::BK - 1) / lineartc::BK;
-  int parts = blocks < 32 ? 1 : 8;
-  while (parts > 1 && (narrow * parts > 2 * sms || blocks < 8 * parts)) parts /= 2;
+  const int parts = parts_of(p);
   return with_dtype(p->out_dtype, "int8_linear", [&](auto t) {
     using TO = decltype(t);
-    if (parts > 1) return lineartc::launch_split<TO>(p, lora, (int)narrow, parts, st);
+    if (parts > 1) return lineartc::launch_split<TO>(p, lora, parts, st);
     if (pair) return lineartc::launch_tc<256, true, TO>(p, lora, st);
     return best == 256 ? lineartc::launch_tc<256, false, TO>(p, lora, st) : best == 128 ? lineartc::launch_tc<128, false, TO>(p, lora, st) : lineartc::launch_tc<64, false, TO>(p, lora, st);
   });

@@ -31,20 +31,16 @@ template <typename T, bool VEC>
 struct Eight {
   static constexpr int WORDS = VEC ? 2 * sizeof(T) : 8;
   uint32_t w[WORDS];
-  __device__ __forceinline__ void load(const T* p, int left) {  // what lies `left` values or more behind p is zero and not read
-    if constexpr (VEC) {
+  // VEC: always read (a load behind a condition would have to land before the next one is issued); else what lies `left` values or more behind p is not
+  __device__ __forceinline__ void load(const T* p, int left) {
+    if constexpr (VEC && WORDS == 2) {
+      const uint2 v = __ldg(reinterpret_cast<const uint2*>(p));
+      w[0] = v.x, w[1] = v.y;
+    } else if constexpr (VEC) {
 #pragma unroll
-      for (int i = 0; i < WORDS; ++i) w[i] = 0u;
-      if (left <= 0) return;
-      if constexpr (WORDS == 2) {
-        const uint2 v = __ldg(reinterpret_cast<const uint2*>(p));
-        w[0] = v.x, w[1] = v.y;
-      } else {
-#pragma unroll
-        for (int i = 0; i < WORDS; i += 4) {
-          const uint4 v = __ldg(reinterpret_cast<const uint4*>(p) + i / 4);
-          w[i] = v.x, w[i + 1] = v.y, w[i + 2] = v.z, w[i + 3] = v.w;
-        }
+      for (int i = 0; i < WORDS; i += 4) {
+        const uint4 v = __ldg(reinterpret_cast<const uint4*>(p) + i / 4);
+        w[i] = v.x, w[i + 1] = v.y, w[i + 2] = v.z, w[i + 3] = v.w;
       }
     } else {
 #pragma unroll
@@ -57,6 +53,10 @@ struct Eight {
         w[i] = __float_as_uint(x);
       }
     }
+  }
+  __device__ __forceinline__ void keep(bool in) {
+#pragma unroll
+    for (int i = 0; i < WORDS; ++i) w[i] = in ? w[i] : 0u;
   }
   template <int N, bool F16>
   __device__ __forceinline__ void pieces(uint32_t (&q)[N][4]) const {
@@ -98,6 +98,7 @@ struct Shrink {
   const int* adapters;
   const float* scaling;        // [L] or null
   float scale;
+  int halves;                  // t as pieces: for four values each their bf16 roundings, then those of what is left
   float* t;
 };
 
@@ -135,25 +136,45 @@ __global__ void __launch_bounds__(THREADS) lora_shrink_kernel(const Shrink p) {
         for (int j = 0; j < NT; ++j)
 #pragma unroll
           for (int e = 0; e < 4; ++e) acc[i][j][e] = 0.f;
-      const TA* a = reinterpret_cast<const TA*>(p.a) + ((long long)l * p.R + r0 + g) * p.K + 8 * t4;
-      const TX* x = reinterpret_cast<const TX*>(p.x) + (long long)(m0 + g) * p.x_stride + 8 * t4;
-      bool own[MT][2];  // a token with another adapter is not read for this one
+      // what lies behind the last token, rank or channel is read from inside and made zero
+      const TA* a[NT];
+      const TX* x[MT][2];
+      bool own[MT][2];  // a token with another adapter is zero for this one
 #pragma unroll
-      for (int i = 0; i < MT; ++i) own[i][0] = which[16 * i + g] == l, own[i][1] = which[16 * i + g + 8] == l;
+      for (int j = 0; j < NT; ++j) a[j] = reinterpret_cast<const TA*>(p.a) + ((long long)l * p.R + min(r0 + 8 * j + g, p.R - 1)) * p.K;
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int row = 16 * i + 8 * h + g;
+          own[i][h] = which[row] == l;
+          x[i][h] = reinterpret_cast<const TX*>(p.x) + (long long)(own[i][h] ? m0 + row : m0) * p.x_stride;
+        }
       // U steps of 32 on their way
-      constexpr int U = MT * Eight<TX, VEC>::WORDS * 2 + NT * Eight<TA, VEC>::WORDS <= 24 ? 4 : MT * Eight<TX, VEC>::WORDS * 2 + NT * Eight<TA, VEC>::WORDS <= 48 ? 2 : 1;
+      constexpr int BYTES = MT * Eight<TX, VEC>::WORDS * 2 + NT * Eight<TA, VEC>::WORDS, U = BYTES <= 24 ? 4 : BYTES <= 48 ? 2 : 1;
       for (int s0 = step0 + warp; s0 < step1; s0 += U * WARPS) {
         Eight<TX, VEC> rx[U][MT][2];
         Eight<TA, VEC> ra[U][NT];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-          const int s = s0 + u * WARPS, k = 32 * s, left = s < step1 ? p.K - k - 8 * t4 : 0;
+          const int k = 32 * (s0 + u * WARPS) + 8 * t4, left = s0 + u * WARPS < step1 ? p.K - k : 0, at = VEC ? min(k, p.K - 8) : k;
 #pragma unroll
           for (int i = 0; i < MT; ++i)
 #pragma unroll
-            for (int h = 0; h < 2; ++h) rx[u][i][h].load(x + (long long)(16 * i + 8 * h) * p.x_stride + k, own[i][h] ? left : 0);
+            for (int h = 0; h < 2; ++h) rx[u][i][h].load(x[i][h] + at, left);
 #pragma unroll
-          for (int j = 0; j < NT; ++j) ra[u][j].load(a + 8ll * j * p.K + k, j < tiles ? left : 0);
+          for (int j = 0; j < NT; ++j)
+            if (VEC || j < tiles) ra[u][j].load(a[j] + at, left);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const bool in = s0 + u * WARPS < step1 && p.K - 32 * (s0 + u * WARPS) - 8 * t4 > 0;
+#pragma unroll
+          for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) rx[u][i][h].keep(in && own[i][h]);
+#pragma unroll
+          for (int j = 0; j < NT; ++j) ra[u][j].keep(in && j < tiles);
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
@@ -205,27 +226,35 @@ __global__ void __launch_bounds__(THREADS) lora_shrink_kernel(const Shrink p) {
   if (p.parts > 1) asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");
   else __syncthreads();
   const uint32_t base = smem_u32(sums);
-  for (int i = rank * THREADS + tid; i < values; i += p.parts * THREADS) {
+  for (int i = 4 * (rank * THREADS + tid); i < values; i += 4 * p.parts * THREADS) {  // four of a row
     const int row = i / p.RP, m = m0 + row;
     if (m >= p.M) continue;
-    float s = 0.f;
+    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
     for (int c = 0; c < p.parts; ++c) {
-      float v;
-      uint32_t at;
+      float4 v;
+      uint32_t at = base + 4 * i;
       if (p.parts > 1) {
         asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(at) : "r"(base + 4 * i), "r"(c));
-        asm volatile("ld.shared::cluster.f32 %0, [%1];\n" : "=f"(v) : "r"(at) : "memory");
+        asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];\n" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at) : "memory");
       } else {
-        v = sums[i];
+        v = *reinterpret_cast<const float4*>(sums + i);
       }
-      s += v;
+      s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
     }
     const int own = which[row];
     if (own >= 0) {
-      s *= p.scaling ? p.scale * __ldg(p.scaling + own) : p.scale;
-      if (p.x_scale) s *= __ldg(p.x_scale + m);
+      float f = p.scaling ? p.scale * __ldg(p.scaling + own) : p.scale;
+      if (p.x_scale) f *= __ldg(p.x_scale + m);
+      s.x *= f, s.y *= f, s.z *= f, s.w *= f;
     }
-    p.t[(long long)m * p.RP + i - row * p.RP] = s;
+    uint4 w = make_uint4(__float_as_uint(s.x), __float_as_uint(s.y), __float_as_uint(s.z), __float_as_uint(s.w));
+    if (p.halves) {
+      uint32_t lo[2], hi[2];
+      bf16_pieces<2>(s.x, s.y, lo);
+      bf16_pieces<2>(s.z, s.w, hi);
+      w = make_uint4(lo[0], hi[0], lo[1], hi[1]);
+    }
+    *reinterpret_cast<uint4*>(p.t + (long long)m * p.RP + i - row * p.RP) = w;
   }
   if (p.parts > 1) asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");  // no CTA's sums are read any more
 }
@@ -279,6 +308,7 @@ static int run_shrink(Shrink p, bool vec, cudaStream_t st) {
 int run_linear(const lq_linear_problem* p, const Lora* lora, cudaStream_t st);                                              // lq_linear.cu
 int run_linear_values(const lq_linear_problem* p, const Lora* lora, const void* values, int dtype, long long stride, cudaStream_t st);
 int check_linear(const lq_linear_problem* p);
+bool linear_takes_halves(const lq_linear_problem* p);  // whether the kernel that runs reads t as two pieces
 
 }  // namespace lq
 
@@ -299,7 +329,7 @@ extern "C" int lq_lora_linear(const lq_linear_problem* p, const lq_lora_problem*
   if ((reinterpret_cast<uintptr_t>(q->b) | reinterpret_cast<uintptr_t>(q->t)) & 15u) return fail(LQ_ERR_ALIGN, "lora_linear: b and t start on 16-byte boundaries");
   const int RP = (q->R + 15) / 16 * 16, size = dtype_bytes(q->dtype);
   const lora::Shrink s{p->M, p->K, q->L, q->R, RP, 1, values ? stride : p->x_stride, values ? values : p->x, q->a, values ? nullptr : p->x_scale,
-                       q->adapters, q->scaling, q->scale, q->t};
+                       q->adapters, q->scaling, q->scale, linear_takes_halves(p), q->t};
   Alignment a;
   a.at(q->a).pitch(p->K, size);
   Alignment x;
