@@ -277,7 +277,7 @@ int check_linear(const lq_linear_problem* p) { return linear::check(p); }
 
 // `lora`: what low-rank adapters add, or null
 int run_linear(const lq_linear_problem* p, const Lora* lora, cudaStream_t st) {
-  if (p->M > 16) return run_linear_tc(p, lora, st);  // 5120 -> 2560 channels: 8 tokens 7.0 us here, 16 9.5, there 11.7 (7.9 from 32 on)
+  if (p->M > kFewTokens) return run_linear_tc(p, lora, st);  // 5120 -> 2560 channels: 8 tokens 7.0 us here, 16 9.5, there 11.7 (7.9 from 32 on)
   return with_dtype(p->out_dtype, "int8_linear", [&](auto t) {
     using TO = decltype(t);
     return p->M <= 8 ? linear::launch_few<1, TO, int8_t, 1>(p, {}, lora, st) : linear::launch_few<2, TO, int8_t, 1>(p, {}, lora, st);

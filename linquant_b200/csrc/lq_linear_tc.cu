@@ -41,11 +41,6 @@ __device__ __forceinline__ float4 lds_f4(uint32_t addr) {
   asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];\n" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr));
   return v;
 }
-__device__ __forceinline__ float2 lds_f2(uint32_t addr) {
-  float2 v;
-  asm volatile("ld.shared.v2.f32 {%0,%1}, [%2];\n" : "=f"(v.x), "=f"(v.y) : "r"(addr));
-  return v;
-}
 __device__ __forceinline__ uint4 lds_u4(uint32_t addr) {
   uint4 v;
   asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];\n" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
@@ -237,90 +232,67 @@ __global__ void __launch_bounds__(THREADS, 1) int8_linear_tc_kernel(const __grid
         sts_u32(cols + 4 * (S::HALF + c), __float_as_uint(in && p.bias ? __ldg(p.bias + n0 + c) : 0.f));
       }
       __syncwarp();
-      auto low = [&] {
-        if constexpr (LORA) return LoraTile<CHUNK / 8, sizeof(TO) == 4 ? 3 : 2>(lora, p.M, p.N, row0);
-        else return 0;
-      }();
-      if constexpr (LORA)
-        if (n0 < p.N) {
-          low.prefetch(n0, S::HALF);
-          low.begin(n0);
+      // What the adapter of this lane's row adds to the next chunk, from where it has been left in y: on its way while the chunk before is stored
+      [[maybe_unused]] Pack<TO, PER> low[CHUNK / PER];
+      [[maybe_unused]] const bool adapted = LORA && row0 + lane < p.M && lora.of(row0 + lane) >= 0;
+      [[maybe_unused]] auto share = [&](int c0) {
+        if (!adapted || c0 >= S::HALF) return;
+        const TO* from = reinterpret_cast<const TO*>(p.y) + (size_t)(row0 + lane) * p.N + n0 + c0;
+#pragma unroll
+        for (int j = 0; j < CHUNK; j += PER) {
+          if (wide) {
+            if (n0 + c0 + j < p.N) low[j / PER] = load_pack<TO, PER>(from + j);
+          } else {
+#pragma unroll
+            for (int e = 0; e < PER; ++e) low[j / PER].v[e] = n0 + c0 + j + e < p.N ? from[j + e] : from_f32<TO>(0.f);
+          }
         }
+      };
+      if constexpr (LORA) share(0);
       if (!(ok = __all_sync(0xffffffffu, wait(s_acc + 8 * acc, (uint32_t)((i / 2) & 1))))) break;
       asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
 #pragma unroll 1
       for (int c0 = 0; c0 < S::HALF; c0 += CHUNK) {
         if (n0 + c0 >= p.N) break;
+        uint32_t r[CHUNK];
+        const uint32_t from = tbase + ((uint32_t)(32 * quad) << 16) + acc * BN + half + c0;
+        if constexpr (CHUNK == 32) tmem_ld_32x32b_x32(from, r);
+        else tmem_ld_32x32b_x16(from, r);
+        asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
+        float v[CHUNK];
+#pragma unroll
+        for (int j = 0; j < CHUNK; j += 4) {
+          const float4 ws = lds_f4(cols + 4 * (c0 + j)), b = lds_f4(cols + 4 * (S::HALF + c0 + j));
+          v[j] = fmaf((float)(int)r[j] * xs, ws.x, b.x);
+          v[j + 1] = fmaf((float)(int)r[j + 1] * xs, ws.y, b.y);
+          v[j + 2] = fmaf((float)(int)r[j + 2] * xs, ws.z, b.z);
+          v[j + 3] = fmaf((float)(int)r[j + 3] * xs, ws.w, b.w);
+        }
+        if constexpr (LORA) {
+          if (adapted) {
+#pragma unroll
+            for (int j = 0; j < CHUNK; j += PER) {
+              float x[PER];
+              low[j / PER].get(x);
+#pragma unroll
+              for (int e = 0; e < PER; ++e) v[j + e] += x[e];
+            }
+          }
+          share(c0 + CHUNK);
+        }
+        __syncwarp();  // the chunk before has been read
         // rows of 64 bytes, pairs of them on the same banks: a piece at its place exclusive-or half the row's number
         auto place = [](int row, int piece) { return row * 64 + ((piece ^ ((row >> 1) & 3)) << 4); };
-        if constexpr (LORA) {  // fragments of m16n8 products: the adapters' sums are added to them
-          constexpr int NT = CHUNK / 8;
-          uint32_t r[2][CHUNK / 2];
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const uint32_t from = tbase + ((uint32_t)(32 * quad + 16 * i) << 16) + acc * BN + half + c0;
-            if constexpr (CHUNK == 32) tmem_ld_16x256b_x4(from, r[i]);
-            else tmem_ld_16x256b_x2(from, r[i]);
+        for (int j = 0; j < CHUNK; j += PER) {
+          uint4 w;
+          if constexpr (sizeof(TO) == 4) {
+            w = make_uint4(__float_as_uint(v[j]), __float_as_uint(v[j + 1]), __float_as_uint(v[j + 2]), __float_as_uint(v[j + 3]));
+          } else {
+            w = make_uint4(Act<TO>::pack2(v[j], v[j + 1]), Act<TO>::pack2(v[j + 2], v[j + 3]), Act<TO>::pack2(v[j + 4], v[j + 5]),
+                           Act<TO>::pack2(v[j + 6], v[j + 7]));
           }
-          asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
-          const int g = lane >> 2, t4 = lane & 3;
-          float v[2][NT][4];
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const float xs0 = __shfl_sync(0xffffffffu, xs, 16 * i + g), xs1 = __shfl_sync(0xffffffffu, xs, 16 * i + g + 8);
-#pragma unroll
-            for (int j = 0; j < NT; ++j) {
-              const float2 ws = lds_f2(cols + 4 * (c0 + 8 * j + 2 * t4)), b = lds_f2(cols + 4 * (S::HALF + c0 + 8 * j + 2 * t4));
-              v[i][j][0] = fmaf((float)(int)r[i][4 * j] * xs0, ws.x, b.x);
-              v[i][j][1] = fmaf((float)(int)r[i][4 * j + 1] * xs0, ws.y, b.y);
-              v[i][j][2] = fmaf((float)(int)r[i][4 * j + 2] * xs1, ws.x, b.x);
-              v[i][j][3] = fmaf((float)(int)r[i][4 * j + 3] * xs1, ws.y, b.y);
-            }
-          }
-          low.add(v);
-          if (c0 + CHUNK < S::HALF && n0 + c0 + CHUNK < p.N) low.begin(n0 + c0 + CHUNK);  // on its way while this chunk is stored
-          __syncwarp();  // the chunk before has been read
-#pragma unroll
-          for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int j = 0; j < NT; ++j)
-#pragma unroll
-              for (int h = 0; h < 2; ++h) {
-                const int row = 16 * i + g + 8 * h;
-                if constexpr (sizeof(TO) == 4) {
-                  sts_u32(out + place(row, 2 * j + (t4 >> 1)) + 8 * (t4 & 1), __float_as_uint(v[i][j][2 * h]));
-                  sts_u32(out + place(row, 2 * j + (t4 >> 1)) + 8 * (t4 & 1) + 4, __float_as_uint(v[i][j][2 * h + 1]));
-                } else {
-                  sts_u32(out + place(row, j) + 4 * t4, Act<TO>::pack2(v[i][j][2 * h], v[i][j][2 * h + 1]));
-                }
-              }
-        } else {
-          uint32_t r[CHUNK];
-          const uint32_t from = tbase + ((uint32_t)(32 * quad) << 16) + acc * BN + half + c0;
-          if constexpr (CHUNK == 32) tmem_ld_32x32b_x32(from, r);
-          else tmem_ld_32x32b_x16(from, r);
-          asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
-          float v[CHUNK];
-#pragma unroll
-          for (int j = 0; j < CHUNK; j += 4) {
-            const float4 ws = lds_f4(cols + 4 * (c0 + j)), b = lds_f4(cols + 4 * (S::HALF + c0 + j));
-            v[j] = fmaf((float)(int)r[j] * xs, ws.x, b.x);
-            v[j + 1] = fmaf((float)(int)r[j + 1] * xs, ws.y, b.y);
-            v[j + 2] = fmaf((float)(int)r[j + 2] * xs, ws.z, b.z);
-            v[j + 3] = fmaf((float)(int)r[j + 3] * xs, ws.w, b.w);
-          }
-          __syncwarp();  // the chunk before has been read
-#pragma unroll
-          for (int j = 0; j < CHUNK; j += PER) {
-            uint4 w;
-            if constexpr (sizeof(TO) == 4) {
-              w = make_uint4(__float_as_uint(v[j]), __float_as_uint(v[j + 1]), __float_as_uint(v[j + 2]), __float_as_uint(v[j + 3]));
-            } else {
-              w = make_uint4(Act<TO>::pack2(v[j], v[j + 1]), Act<TO>::pack2(v[j + 2], v[j + 3]), Act<TO>::pack2(v[j + 4], v[j + 5]),
-                             Act<TO>::pack2(v[j + 6], v[j + 7]));
-            }
-            sts_u4(out + place(lane, j / PER), w);
-          }
+          sts_u4(out + place(lane, j / PER), w);
         }
         __syncwarp();
         TO* y = reinterpret_cast<TO*>(p.y);
@@ -481,14 +453,12 @@ __global__ void __launch_bounds__(THREADS, 2) int8_linear_split_kernel(const __g
       }
       float f[4] = {fmaf((float)sum.x * xs[i], ws[0], bias[0]), fmaf((float)sum.y * xs[i], ws[1], bias[1]), fmaf((float)sum.z * xs[i], ws[2], bias[2]),
                     fmaf((float)sum.w * xs[i], ws[3], bias[3])};
-      if constexpr (LORA) {
-        const int l = lora.of(m0 + row);
-        if (l >= 0)
+      TO* to = y + (size_t)(m0 + row) * p.N + n;
+      if constexpr (LORA)  // the adapter's share has been left there
+        if (lora.of(m0 + row) >= 0)
 #pragma unroll
           for (int j = 0; j < 4; ++j)
-            if (n + j < p.N) f[j] += lora_dot(lora, l, p.N, m0 + row, n + j);
-      }
-      TO* to = y + (size_t)(m0 + row) * p.N + n;
+            if (n + j < p.N) f[j] += to_f32(to[j]);
       if (wide) {
         Pack<TO, 4> out;
         out.set(f);
@@ -555,8 +525,7 @@ static int launch_tc(const lq_linear_problem* p, const Lora* lora, cudaStream_t 
 }
 
 template <typename TO>
-static int launch_split(const lq_linear_problem* p, const Lora* lora, int parts, cudaStream_t st) {
-  const int tiles = (p->M + 127) / 128 * ((p->N + Split::BN - 1) / Split::BN);
+static int launch_split(const lq_linear_problem* p, const Lora* lora, int tiles, int parts, cudaStream_t st) {
   CUtensorMap mx, mw;
   if (int e = encode(&mx, p->x, p->K, p->x_stride, p->M, BM)) return e;
   if (int e = encode(&mw, p->w, p->K, p->w_stride, p->N, Split::BN)) return e;
@@ -566,21 +535,9 @@ static int launch_split(const lq_linear_problem* p, const Lora* lora, int parts,
 
 }  // namespace lineartc
 
-static int parts_of(const lq_linear_problem* p) {
-  // Few tiles of a long K: parts of at least 8 blocks for the CTAs of a cluster, two CTAs on an SM. 5120 -> 2560, 64 tokens: one part
-  // 14.3 us, 2, 4, 8 parts 11.0, 8.6, 8.7; 256 tokens, 2 parts: 14.5 -> 12.5; 8192 -> 1024, 33 tokens, 8 parts: 20.7 -> 7.9. To meet
-  // costs some 2 us, more than a short K has: 200 x 2560 -> 2560 9.0 -> 9.5, 100 x 1024 -> 1024 4.9 -> 6.7
-  const long long mt = (p->M + 127) / 128, sms = sm_count(), narrow = mt * ((p->N + lineartc::Split::BN - 1) / lineartc::Split::BN),
-                  blocks = (p->K + lineartc::BK - 1) / lineartc::BK;
-  int parts = blocks < 32 ? 1 : 8;
-  while (parts > 1 && (narrow * parts > 2 * sms || blocks < 8 * parts)) parts /= 2;
-  return parts;
-}
-
-bool linear_takes_halves(const lq_linear_problem* p) { return p->M > 16 && p->out_dtype != LQ_F32 && parts_of(p) == 1; }
-
 // The widest tiles that do not leave SMs idle: rounds of tiles x the time of one, which grows with its width and a fixed part
 // (the 128 rows of x that every tile loads)
+// `lora`: the rows to whose outputs something has been left to add, or null
 int run_linear_tc(const lq_linear_problem* p, const Lora* lora, cudaStream_t st) {
   const long long mt = (p->M + 127) / 128, sms = sm_count();
   int best = 256;
@@ -592,10 +549,15 @@ int run_linear_tc(const lq_linear_problem* p, const Lora* lora, cudaStream_t st)
   // Pairs of CTAs read the weights half as often from shared memory; over a few rounds their larger tiles cost more than that:
   // 8192 x 2560 -> 2560 (4.3 rounds) 54 us against 53, 4096 x 2560 -> 10576 (9) 91 against 102, 32768 x 2560 -> 10576 (73) 688 against 743
   const bool pair = mt * ((p->N + 255) / 256) >= 6 * sms;
-  const int parts = parts_of(p);
+  // Few tiles of a long K: parts of at least 8 blocks for the CTAs of a cluster, two CTAs on an SM. 5120 -> 2560, 64 tokens: one part
+  // 14.3 us, 2, 4, 8 parts 11.0, 8.6, 8.7; 256 tokens, 2 parts: 14.5 -> 12.5; 8192 -> 1024, 33 tokens, 8 parts: 20.7 -> 7.9. To meet
+  // costs some 2 us, more than a short K has: 200 x 2560 -> 2560 9.0 -> 9.5, 100 x 1024 -> 1024 4.9 -> 6.7
+  const long long narrow = mt * ((p->N + lineartc::Split::BN - 1) / lineartc::Split::BN), blocks = (p->K + lineartc::BK - 1) / lineartc::BK;
+  int parts = blocks < 32 ? 1 : 8;
+  while (parts > 1 && (narrow * parts > 2 * sms || blocks < 8 * parts)) parts /= 2;
   return with_dtype(p->out_dtype, "int8_linear", [&](auto t) {
     using TO = decltype(t);
-    if (parts > 1) return lineartc::launch_split<TO>(p, lora, parts, st);
+    if (parts > 1) return lineartc::launch_split<TO>(p, lora, (int)narrow, parts, st);
     if (pair) return lineartc::launch_tc<256, true, TO>(p, lora, st);
     return best == 256 ? lineartc::launch_tc<256, false, TO>(p, lora, st) : best == 128 ? lineartc::launch_tc<128, false, TO>(p, lora, st) : lineartc::launch_tc<64, false, TO>(p, lora, st);
   });

@@ -2,8 +2,10 @@
 //
 //   y[m,n] = (sum_k c[m,k] w[n,k]) x_scale[m] w_scale[n] + bias[n] + sum_r t[m,r] b[l,n,r],   t[m,r] = scaling[l] sum_k x[m,k] a[l,r,k]
 //
-// l = adapters[m]; c are x's codes. Two kernels: this file's makes t, the INT8 product's own kernels add the second sum to a tile while it
-// is still fp32 (lq_lora.cuh), so y is rounded and written once.
+// l = adapters[m]; c are x's codes. This file's first kernel makes t. Up to 16 tokens the INT8 product's kernel adds the second sum to its own in
+// fp32 (lq_lora.cuh). For more this file's second kernel leaves it in y and the product's kernels add it from there: what runs beside the
+// tcgen05 product on an SM's tensor cores waits for them (warp products in its epilogue: 510 us where the product alone takes 302, at
+// 16384 x 2560 -> 10576 with rank 16; fp32 products there: 680).
 // t: a CTA has a tile of 1, 16 or 32 tokens and, of a cluster, a part of K; its four warps share that part and their sums meet in
 // shared memory, first the warps', then the CTAs', in a fixed order. Operands come from global memory straight into the fragments
 // of m16n8k16 (the reduction index permuted alike in both: a lane takes eight consecutive k). A tile whose tokens have several
@@ -98,7 +100,6 @@ struct Shrink {
   const int* adapters;
   const float* scaling;        // [L] or null
   float scale;
-  int halves;                  // t as pieces: for four values each their bf16 roundings, then those of what is left
   float* t;
 };
 
@@ -247,14 +248,7 @@ __global__ void __launch_bounds__(THREADS) lora_shrink_kernel(const Shrink p) {
       if (p.x_scale) f *= __ldg(p.x_scale + m);
       s.x *= f, s.y *= f, s.z *= f, s.w *= f;
     }
-    uint4 w = make_uint4(__float_as_uint(s.x), __float_as_uint(s.y), __float_as_uint(s.z), __float_as_uint(s.w));
-    if (p.halves) {
-      uint32_t lo[2], hi[2];
-      bf16_pieces<2>(s.x, s.y, lo);
-      bf16_pieces<2>(s.z, s.w, hi);
-      w = make_uint4(lo[0], hi[0], lo[1], hi[1]);
-    }
-    *reinterpret_cast<uint4*>(p.t + (long long)m * p.RP + i - row * p.RP) = w;
+    *reinterpret_cast<float4*>(p.t + (long long)m * p.RP + i - row * p.RP) = s;
   }
   if (p.parts > 1) asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");  // no CTA's sums are read any more
 }
@@ -303,12 +297,178 @@ static int run_shrink(Shrink p, bool vec, cudaStream_t st) {
   return vec ? width(std::true_type()) : width(std::false_type());
 }
 
+// ---- the second product: y[m,n] = sum_r t[m,r] b[l,n,r] for the tokens that have an adapter
+constexpr int SPAN = 64, CHUNK = 32, CT = CHUNK / 8;  // channels of a warp, at a time, in tiles of 8
+
+// A warp: 32 tokens, SPAN channels. Over the adapters that the tokens have and their ranks in steps of 16; a step's operands are requested before
+// the products of the one ahead. The reduction index is permuted alike in both operands: a lane takes four consecutive r. Both are
+// bf16 pieces: two (three for fp32 outputs) of t and of fp16 and fp32 b, products below 16 (24) bits behind the first left out.
+// The INT8 product's kernel reads y again, adds its own sum in fp32 and rounds once more: this rounding is of the adapters' share alone.
+// Bound by the bytes of y.
+template <typename TO, typename TB>
+__global__ void __launch_bounds__(THREADS, sizeof(TO) == 2 ? 5 : 3) lora_expand_kernel(const Lora q, int M, int N, TO* y) {
+  constexpr int PT = sizeof(TO) == 4 ? 3 : 2, PB = std::is_same_v<TB, __nv_bfloat16> ? 1 : PT;
+  __shared__ __align__(16) uint8_t stage[WARPS][32 * 128];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
+  const int m0 = blockIdx.y * 32, n0 = (blockIdx.x * WARPS + warp) * SPAN;
+  pdl_enter();
+  if (n0 >= N) return;
+  constexpr int PER = 16 / sizeof(TO), ROW = CHUNK / PER;  // values of 16 bytes; such pieces of a row's chunk
+  const int mine = m0 + lane < M ? q.of(m0 + lane) : -1;
+  const uint32_t all = __ballot_sync(0xffffffffu, mine >= 0);
+  if (!all) return;
+  const bool wide = ((size_t)N * sizeof(TO)) % 16 == 0 && (reinterpret_cast<uintptr_t>(y) & 15u) == 0;
+  const uint32_t out = smem_u32(stage[warp]);
+  auto place = [](int row, int piece) { return row * 128 + ((piece ^ (row & 7)) << 4); };
+
+  // the step that is on its way
+  int l = 0, r0 = 0, c0 = 0;
+  uint32_t rows = 0, left = 0;
+  Pack<TB, 4> b[CT];
+  float4 t[2][2];
+  auto next_adapter = [&] {
+    l = __shfl_sync(0xffffffffu, mine, __ffs(left) - 1);
+    rows = __ballot_sync(0xffffffffu, mine == l);
+    left &= ~rows;
+    r0 = 0;
+  };
+  auto request = [&] {
+    const int r = r0 + 4 * t4, rb = min(r, q.R - 4);  // behind R t is zero, and b is made so
+    const TB* from = reinterpret_cast<const TB*>(q.b) + (long long)l * N * q.R + rb;
+#pragma unroll
+    for (int j = 0; j < CT; ++j) b[j] = load_pack<TB, 4>(from + (long long)min(n0 + c0 + 8 * j + g, N - 1) * q.R);  // behind N nothing is stored
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int row = 16 * i + 8 * h + g;  // of tokens with another adapter what comes of it is not kept
+        t[i][h] = *reinterpret_cast<const float4*>(q.t + (long long)min(m0 + row, M - 1) * q.RP + r);
+      }
+  };
+  left = all;
+  next_adapter();
+  request();
+  while (true) {
+    const uint32_t now = rows;
+    const int at = c0;
+    float s[2][CT][4];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int j = 0; j < CT; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[i][j][e] = 0.f;
+    bool same = true, done = false, end = false;  // the adapter goes on; the chunk is complete; nothing is left
+    while (same) {
+      uint32_t a[2][PT][4], w[CT][PB][2];
+      const bool inside = r0 + 4 * t4 < q.R;
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          uint32_t lo[PT], hi[PT];
+          bf16_pieces<PT>(t[i][h].x, t[i][h].y, lo);
+          bf16_pieces<PT>(t[i][h].z, t[i][h].w, hi);
+#pragma unroll
+          for (int k = 0; k < PT; ++k) a[i][k][h] = lo[k], a[i][k][2 + h] = hi[k];
+        }
+#pragma unroll
+      for (int j = 0; j < CT; ++j) {
+        if constexpr (PB == 1) {
+          const uint2 x = *reinterpret_cast<const uint2*>(&b[j]);
+          w[j][0][0] = inside ? x.x : 0u, w[j][0][1] = inside ? x.y : 0u;
+        } else {
+          float x[4];
+          b[j].get(x);
+          uint32_t lo[PB], hi[PB];
+          bf16_pieces<PB>(inside ? x[0] : 0.f, inside ? x[1] : 0.f, lo);
+          bf16_pieces<PB>(inside ? x[2] : 0.f, inside ? x[3] : 0.f, hi);
+#pragma unroll
+          for (int k = 0; k < PB; ++k) w[j][k][0] = lo[k], w[j][k][1] = hi[k];
+        }
+      }
+      r0 += 16;
+      same = r0 < q.R;
+      if (!same) {
+        if (left == 0) {
+          done = true;
+          c0 += CHUNK;
+          end = c0 >= SPAN || n0 + c0 >= N;
+          left = all;
+        }
+        if (!end) next_adapter();
+      }
+      if (!end) request();
+#pragma unroll
+      for (int k = PB - 1; k >= 0; --k)
+#pragma unroll
+        for (int o = PT - 1; o >= 0; --o) {
+          if (k + o >= PT) continue;
+#pragma unroll
+          for (int j = 0; j < CT; ++j)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) mma_bf16(s[i][j], a[i][o][0], a[i][o][1], a[i][o][2], a[i][o][3], w[j][k][0], w[j][k][1]);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int row = 16 * i + 8 * h + g;
+        if (!(now >> row & 1)) continue;
+#pragma unroll
+        for (int j = 0; j < CT; ++j) {
+          const int byte = (8 * j + 2 * t4) * (int)sizeof(TO);
+          const uint32_t to = out + place(row, byte >> 4) + (byte & 15);
+          if constexpr (sizeof(TO) == 4) {
+            sts_u32(to, __float_as_uint(s[i][j][2 * h]));
+            sts_u32(to + 4, __float_as_uint(s[i][j][2 * h + 1]));
+          } else {
+            sts_u32(to, Act<TO>::pack2(s[i][j][2 * h], s[i][j][2 * h + 1]));
+          }
+        }
+      }
+    if (done) {
+      __syncwarp();
+      if (wide) {
+#pragma unroll
+        for (int k = 0; k < ROW; ++k) {
+          const int row = 32 / ROW * k + lane / ROW, piece = lane % ROW, n = n0 + at + piece * PER;
+          if (all >> row & 1 && n < N)
+            *reinterpret_cast<uint4*>(y + (size_t)(m0 + row) * N + n) = *reinterpret_cast<const uint4*>(stage[warp] + place(row, piece));
+        }
+      } else {
+        for (int row = 0; row < 32; ++row) {
+          const int byte = lane * (int)sizeof(TO);
+          if (all >> row & 1 && n0 + at + lane < N)
+            y[(size_t)(m0 + row) * N + n0 + at + lane] = *reinterpret_cast<const TO*>(stage[warp] + place(row, byte >> 4) + (byte & 15));
+        }
+      }
+      __syncwarp();  // the chunk has been read
+    }
+    if (end) return;
+  }
+}
+
+static int expand(const Lora& q, const lq_linear_problem* p, cudaStream_t st) {
+  return with_dtype(p->out_dtype, "lora_linear", [&](auto t) {
+    using TO = decltype(t);
+    const long long rows = ((long long)p->M + 31) / 32;
+    if (rows > 65535) return fail(LQ_ERR_SHAPE, "lora_linear: M=%d", p->M);
+    return with_dtype(q.dtype, "lora_linear", [&](auto tb) {
+      using TB = decltype(tb);
+      const cudaError_t e = launch(lora_expand_kernel<TO, TB>, dim3((p->N + WARPS * SPAN - 1) / (WARPS * SPAN), (unsigned)rows), dim3(THREADS), 0, st, q, p->M, p->N,
+                                   reinterpret_cast<TO*>(p->y));
+      return e != cudaSuccess ? fail(LQ_ERR_LAUNCH, "lora_linear: %s", cudaGetErrorString(e)) : check_launch("lora_expand_kernel");
+    });
+  });
+}
+
 }  // namespace lora
 
 int run_linear(const lq_linear_problem* p, const Lora* lora, cudaStream_t st);                                              // lq_linear.cu
 int run_linear_values(const lq_linear_problem* p, const Lora* lora, const void* values, int dtype, long long stride, cudaStream_t st);
 int check_linear(const lq_linear_problem* p);
-bool linear_takes_halves(const lq_linear_problem* p);  // whether the kernel that runs reads t as two pieces
 
 }  // namespace lq
 
@@ -329,7 +489,7 @@ extern "C" int lq_lora_linear(const lq_linear_problem* p, const lq_lora_problem*
   if ((reinterpret_cast<uintptr_t>(q->b) | reinterpret_cast<uintptr_t>(q->t)) & 15u) return fail(LQ_ERR_ALIGN, "lora_linear: b and t start on 16-byte boundaries");
   const int RP = (q->R + 15) / 16 * 16, size = dtype_bytes(q->dtype);
   const lora::Shrink s{p->M, p->K, q->L, q->R, RP, 1, values ? stride : p->x_stride, values ? values : p->x, q->a, values ? nullptr : p->x_scale,
-                       q->adapters, q->scaling, q->scale, linear_takes_halves(p), q->t};
+                       q->adapters, q->scaling, q->scale, q->t};
   Alignment a;
   a.at(q->a).pitch(p->K, size);
   Alignment x;
@@ -343,5 +503,7 @@ extern "C" int lq_lora_linear(const lq_linear_problem* p, const lq_lora_problem*
   });
   if (e != LQ_OK) return e;
   const Lora add{q->L, q->R, RP, q->dtype, q->b, q->adapters, q->t};
+  if (p->M > kFewTokens)
+    if (int e2 = lora::expand(add, p, st)) return e2;
   return values ? run_linear_values(p, &add, values, dtype, stride, st) : run_linear(p, &add, st);
 }

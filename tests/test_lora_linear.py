@@ -27,10 +27,13 @@ def ints(*v):
     return torch.tensor(v, dtype=torch.int32, device="cuda")
 
 
-def low_error(dtype, K, R):
+def low_error(dtype, K, R, M):
     """Of the adapters' sum, relative to its terms' magnitudes. x a: one rounding (the tensor core cuts off, 2^-23) for each 16 of K and
-    piece (six at most), 16 where the parts meet; t b the same over R. 16-bit outputs on tcgen05 take t and b as 16 bits each."""
-    return (6 * (K / 16 + R / 16 + 2) + 32) * 2 * ULP + (0 if dtype == F32 else 2.0**-15)
+    piece (six at most), 16 where the parts meet; t b the same over R. 16-bit outputs of more than 16 tokens take t and b as 16 bits
+    each, and the sum is left in the output's type before the shared one joins it: half a step of that type, of a sum that is no
+    larger than its terms' magnitudes together."""
+    exact = (6 * (K / 16 + R / 16 + 2) + 32) * 2 * ULP
+    return exact if dtype == F32 else exact + 2.0**-15 + (ref.UNIT[dtype] if M > 16 else 0)
 
 
 def want_of(x, codes, x_scale, w, w_scale, a, b, which, scaling, bias):
@@ -52,7 +55,7 @@ def want_of(x, codes, x_scale, w, w_scale, a, b, which, scaling, bias):
 
 def agree(y, want, K, R):
     base, mag, low = want
-    e = low_error(y.dtype, K, R)
+    e = low_error(y.dtype, K, R, y.shape[0])
     ref.check(y, base, mag * (4 * ULP / e) + low, e)
 
 
