@@ -100,6 +100,7 @@ struct Shrink {
   const int* adapters;
   const float* scaling;        // [L] or null
   float scale;
+  int halves;                  // t as pieces: of four values their bf16 roundings, then those of what is left
   float* t;
 };
 
@@ -248,7 +249,14 @@ __global__ void __launch_bounds__(THREADS) lora_shrink_kernel(const Shrink p) {
       if (p.x_scale) f *= __ldg(p.x_scale + m);
       s.x *= f, s.y *= f, s.z *= f, s.w *= f;
     }
-    *reinterpret_cast<float4*>(p.t + (long long)m * p.RP + i - row * p.RP) = s;
+    uint4 w = make_uint4(__float_as_uint(s.x), __float_as_uint(s.y), __float_as_uint(s.z), __float_as_uint(s.w));
+    if (p.halves) {
+      uint32_t lo[2], hi[2];
+      bf16_pieces<2>(s.x, s.y, lo);
+      bf16_pieces<2>(s.z, s.w, hi);
+      w = make_uint4(lo[0], hi[0], lo[1], hi[1]);
+    }
+    *reinterpret_cast<uint4*>(p.t + (long long)m * p.RP + i - row * p.RP) = w;
   }
   if (p.parts > 1) asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");  // no CTA's sums are read any more
 }
@@ -280,12 +288,12 @@ static int shrink(const Shrink& p, int tiles, cudaStream_t st) {
 }
 
 // Tokens of a CTA: one each for a decode step, whose tokens have adapters of their own; 32 where that leaves a CTA an SM, so that a's rows are
-// read for twice as many. Parts of K: up to four CTAs an SM, and no fewer than 128 of K for a warp.
+// read for twice as many. Parts of K: up to four CTAs an SM, and no fewer than 64 of K for a warp.
 template <typename TX, typename TA>
 static int run_shrink(Shrink p, bool vec, cudaStream_t st) {
   const int sms = sm_count(), tile = p.M <= 64 ? 1 : p.M >= 32 * sms ? 32 : 16, tiles = (p.M + tile - 1) / tile;
   p.parts = 8;
-  while (p.parts > 1 && ((long long)tiles * p.parts > 4ll * sms || p.K < 512 * p.parts)) p.parts /= 2;
+  while (p.parts > 1 && ((long long)tiles * p.parts > 4ll * sms || p.K < 256 * p.parts)) p.parts /= 2;
   auto go = [&](auto v, auto nt) {
     constexpr bool VEC = decltype(v)::value;
     constexpr int NT = decltype(nt)::value;
@@ -293,19 +301,19 @@ static int run_shrink(Shrink p, bool vec, cudaStream_t st) {
     if (tile == 16) return shrink<TX, TA, 16, VEC, NT>(p, tiles, st);
     return shrink<TX, TA, 32, VEC, NT>(p, tiles, st);
   };
-  auto width = [&](auto v) { return p.R <= 16 ? go(v, std::integral_constant<int, 2>()) : go(v, std::integral_constant<int, 8>()); };
+  auto width = [&](auto v) { return p.R <= 16 ? go(v, std::integral_constant<int, 2>()) : p.R <= 32 ? go(v, std::integral_constant<int, 4>()) : go(v, std::integral_constant<int, 8>()); };
   return vec ? width(std::true_type()) : width(std::false_type());
 }
 
 // ---- the second product: y[m,n] = sum_r t[m,r] b[l,n,r] for the tokens that have an adapter
-constexpr int SPAN = 64, CHUNK = 32, CT = CHUNK / 8;  // channels of a warp, at a time, in tiles of 8
+constexpr int CHUNK = 32, CT = CHUNK / 8;  // channels at a time, in tiles of 8
 
 // A warp: 32 tokens, SPAN channels. Over the adapters that the tokens have and their ranks in steps of 16; a step's operands are requested before
 // the products of the one ahead. The reduction index is permuted alike in both operands: a lane takes four consecutive r. Both are
 // bf16 pieces: two (three for fp32 outputs) of t and of fp16 and fp32 b, products below 16 (24) bits behind the first left out.
 // The INT8 product's kernel reads y again, adds its own sum in fp32 and rounds once more: this rounding is of the adapters' share alone.
 // Bound by the bytes of y.
-template <typename TO, typename TB>
+template <typename TO, typename TB, int SPAN>
 __global__ void __launch_bounds__(THREADS, sizeof(TO) == 2 ? 5 : 3) lora_expand_kernel(const Lora q, int M, int N, TO* y) {
   constexpr int PT = sizeof(TO) == 4 ? 3 : 2, PB = std::is_same_v<TB, __nv_bfloat16> ? 1 : PT;
   __shared__ __align__(16) uint8_t stage[WARPS][32 * 128];
@@ -325,7 +333,13 @@ __global__ void __launch_bounds__(THREADS, sizeof(TO) == 2 ? 5 : 3) lora_expand_
   int l = 0, r0 = 0, c0 = 0;
   uint32_t rows = 0, left = 0;
   Pack<TB, 4> b[CT];
-  float4 t[2][2];
+  uint4 t[2][2];
+  if (SPAN == 32) {  // few tokens: every adapter's rows of b on their way to L2, by its first one
+    const uint32_t like = __match_any_sync(0xffffffffu, mine);
+    const TB* from = reinterpret_cast<const TB*>(q.b) + ((long long)mine * N + n0) * q.R;
+    if (mine >= 0 && (like & ((1u << lane) - 1)) == 0)
+      asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;\n" ::"l"(from), "r"((uint32_t)(min(SPAN, N - n0) * q.R * (int)sizeof(TB))) : "memory");
+  }
   auto next_adapter = [&] {
     l = __shfl_sync(0xffffffffu, mine, __ffs(left) - 1);
     rows = __ballot_sync(0xffffffffu, mine == l);
@@ -334,15 +348,21 @@ __global__ void __launch_bounds__(THREADS, sizeof(TO) == 2 ? 5 : 3) lora_expand_
   };
   auto request = [&] {
     const int r = r0 + 4 * t4, rb = min(r, q.R - 4);  // behind R t is zero, and b is made so
-    const TB* from = reinterpret_cast<const TB*>(q.b) + (long long)l * N * q.R + rb;
+    const int n = n0 + c0 + g;
+    if (n0 + c0 + CHUNK <= N) {
+      const TB* from = reinterpret_cast<const TB*>(q.b) + ((long long)l * N + n) * q.R + rb;
 #pragma unroll
-    for (int j = 0; j < CT; ++j) b[j] = load_pack<TB, 4>(from + (long long)min(n0 + c0 + 8 * j + g, N - 1) * q.R);  // behind N nothing is stored
+      for (int j = 0; j < CT; ++j) b[j] = load_pack<TB, 4>(from + 8 * j * q.R);
+    } else {  // behind N nothing is stored
+#pragma unroll
+      for (int j = 0; j < CT; ++j) b[j] = load_pack<TB, 4>(reinterpret_cast<const TB*>(q.b) + ((long long)l * N + min(n + 8 * j, N - 1)) * q.R + rb);
+    }
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int row = 16 * i + 8 * h + g;  // of tokens with another adapter what comes of it is not kept
-        t[i][h] = *reinterpret_cast<const float4*>(q.t + (long long)min(m0 + row, M - 1) * q.RP + r);
+        t[i][h] = *reinterpret_cast<const uint4*>(q.t + (long long)min(m0 + row, M - 1) * q.RP + r);
       }
   };
   left = all;
@@ -366,11 +386,15 @@ __global__ void __launch_bounds__(THREADS, sizeof(TO) == 2 ? 5 : 3) lora_expand_
       for (int i = 0; i < 2; ++i)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          uint32_t lo[PT], hi[PT];
-          bf16_pieces<PT>(t[i][h].x, t[i][h].y, lo);
-          bf16_pieces<PT>(t[i][h].z, t[i][h].w, hi);
+          if constexpr (PT == 2) {  // as the first kernel has left them
+            a[i][0][h] = t[i][h].x, a[i][0][2 + h] = t[i][h].y, a[i][1][h] = t[i][h].z, a[i][1][2 + h] = t[i][h].w;
+          } else {
+            uint32_t lo[PT], hi[PT];
+            bf16_pieces<PT>(__uint_as_float(t[i][h].x), __uint_as_float(t[i][h].y), lo);
+            bf16_pieces<PT>(__uint_as_float(t[i][h].z), __uint_as_float(t[i][h].w), hi);
 #pragma unroll
-          for (int k = 0; k < PT; ++k) a[i][k][h] = lo[k], a[i][k][2 + h] = hi[k];
+            for (int k = 0; k < PT; ++k) a[i][k][h] = lo[k], a[i][k][2 + h] = hi[k];
+          }
         }
 #pragma unroll
       for (int j = 0; j < CT; ++j) {
@@ -457,9 +481,12 @@ static int expand(const Lora& q, const lq_linear_problem* p, cudaStream_t st) {
     if (rows > 65535) return fail(LQ_ERR_SHAPE, "lora_linear: M=%d", p->M);
     return with_dtype(q.dtype, "lora_linear", [&](auto tb) {
       using TB = decltype(tb);
-      const cudaError_t e = launch(lora_expand_kernel<TO, TB>, dim3((p->N + WARPS * SPAN - 1) / (WARPS * SPAN), (unsigned)rows), dim3(THREADS), 0, st, q, p->M, p->N,
-                                   reinterpret_cast<TO*>(p->y));
-      return e != cudaSuccess ? fail(LQ_ERR_LAUNCH, "lora_linear: %s", cudaGetErrorString(e)) : check_launch("lora_expand_kernel");
+      // few tokens: warps of 32 channels, as many as there can be, each of which goes over all adapters of its tokens one after the other
+      auto go = [&](auto kern, int span) {
+        const cudaError_t e = launch(kern, dim3((p->N + WARPS * span - 1) / (WARPS * span), (unsigned)rows), dim3(THREADS), 0, st, q, p->M, p->N, reinterpret_cast<TO*>(p->y));
+        return e != cudaSuccess ? fail(LQ_ERR_LAUNCH, "lora_linear: %s", cudaGetErrorString(e)) : check_launch("lora_expand_kernel");
+      };
+      return rows * ((p->N + 127) / 128) <= 10ll * sm_count() ? go(lora_expand_kernel<TO, TB, 32>, 32) : go(lora_expand_kernel<TO, TB, 128>, 128);
     });
   });
 }
@@ -489,7 +516,7 @@ extern "C" int lq_lora_linear(const lq_linear_problem* p, const lq_lora_problem*
   if ((reinterpret_cast<uintptr_t>(q->b) | reinterpret_cast<uintptr_t>(q->t)) & 15u) return fail(LQ_ERR_ALIGN, "lora_linear: b and t start on 16-byte boundaries");
   const int RP = (q->R + 15) / 16 * 16, size = dtype_bytes(q->dtype);
   const lora::Shrink s{p->M, p->K, q->L, q->R, RP, 1, values ? stride : p->x_stride, values ? values : p->x, q->a, values ? nullptr : p->x_scale,
-                       q->adapters, q->scaling, q->scale, q->t};
+                       q->adapters, q->scaling, q->scale, p->M > kFewTokens && p->out_dtype != LQ_F32, q->t};
   Alignment a;
   a.at(q->a).pitch(p->K, size);
   Alignment x;

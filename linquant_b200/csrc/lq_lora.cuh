@@ -16,7 +16,7 @@ struct Lora {
   int dtype;           // of b
   const void* b;       // [L,N,R]
   const int* adapters; // [M]: which adapter a token has; one outside 0..L-1 is none
-  const float* t;      // [M,RP]
+  const float* t;      // [M,RP]; 16-bit outputs of more than kFewTokens tokens: as two bf16 pieces of four values each
   __device__ __forceinline__ int of(int m) const {
     const int l = __ldg(adapters + m);
     return (unsigned)l < (unsigned)L ? l : -1;
