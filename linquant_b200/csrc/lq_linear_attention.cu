@@ -507,20 +507,30 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 2 && KP <= 128 ? 2 : 1) 
   }
 }
 
-// What leaves a segment: its own state and, decayed, what entered it. One thread has four values of all segments.
-__global__ void __launch_bounds__(256) segment_states_kernel(const Segments seg, int heads, long long values, int values_a_head) {
+// What leaves a segment: its own state and, decayed, what entered it. One thread has four values of all segments, eight of them on their way.
+__global__ void __launch_bounds__(128) segment_states_kernel(const Segments seg, int heads, long long values, int values_a_head) {
+  constexpr int U = 8;
   pdl_enter();
-  const long long i = (blockIdx.x * 256ll + threadIdx.x) * 4;
+  const long long i = (blockIdx.x * 128ll + threadIdx.x) * 4;
   if (i >= values) return;
-  const int bh = (int)(i / values_a_head);
-  float4 s = *reinterpret_cast<const float4*>(seg.states + i);
-  float4 next = *reinterpret_cast<const float4*>(seg.states + values + i);
-  for (int k = 1; k < seg.count - 1; ++k) {
-    const float4 own = next;
-    const float a = __ldg(seg.decays + (size_t)k * heads + bh);
-    if (k + 1 < seg.count - 1) next = *reinterpret_cast<const float4*>(seg.states + (size_t)(k + 1) * values + i);
-    s = make_float4(fmaf(a, s.x, own.x), fmaf(a, s.y, own.y), fmaf(a, s.z, own.z), fmaf(a, s.w, own.w));
-    *reinterpret_cast<float4*>(seg.states + (size_t)k * values + i) = s;
+  const int bh = (int)(i / values_a_head), last = seg.count - 2;  // the last segment's is not there
+  float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int k0 = 0; k0 <= last; k0 += U) {
+    float4 own[U];
+    float a[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int k = min(k0 + u, last);
+      own[u] = *reinterpret_cast<const float4*>(seg.states + (size_t)k * values + i);
+      a[u] = __ldg(seg.decays + (size_t)k * heads + bh);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int k = k0 + u;
+      if (k > last) break;
+      s = k == 0 ? own[u] : make_float4(fmaf(a[u], s.x, own[u].x), fmaf(a[u], s.y, own[u].y), fmaf(a[u], s.z, own[u].z), fmaf(a[u], s.w, own[u].w));
+      if (k > 0) *reinterpret_cast<float4*>(seg.states + (size_t)k * values + i) = s;
+    }
   }
 }
 
@@ -596,7 +606,7 @@ __global__ void __launch_bounds__(256) linear_attention_step_kernel(const lq_att
 }
 
 cudaError_t launch_segment_states(const Segments& seg, int heads, long long values, cudaStream_t st) {
-  return launch(segment_states_kernel, dim3((unsigned)((values / 4 + 255) / 256)), dim3(256), 0, st, seg, heads, values, (int)(values / heads));
+  return launch(segment_states_kernel, dim3((unsigned)((values / 4 + 127) / 128)), dim3(128), 0, st, seg, heads, values, (int)(values / heads));
 }
 
 static int check(const lq_attention_problem* p, const char* what) {
@@ -609,16 +619,17 @@ static int check(const lq_attention_problem* p, const char* what) {
   return LQ_OK;
 }
 
-// Segments: enough CTAs for every place on the GPU (two an SM; one for the tcgen05 kernel), none shorter than eight chunks
+// Segments: enough CTAs for every place on the GPU (two an SM, one of fp32 operands or for the tcgen05 kernel). None is shorter than eight
+// chunks, or two of fp32 operands, whose chunks take ten times as long
 static Plan plan(const lq_attention_problem* p) {
   Plan r;
   r.tc = tc_applies(p);
   const int kp = p->K <= 64 && !r.tc ? 64 : p->K <= 128 ? 128 : 256, vt = kp == 256 ? 32 : 64;
   r.regs = kp / 64 * (vt / 8) * 4;
   r.tiles = (long long)p->B * p->H * ((p->V + vt - 1) / vt);
-  const long long chunks = ((long long)p->T + 63) / 64, room = (r.tc ? 1ll : 2ll) * sm_count();
+  const long long chunks = ((long long)p->T + 63) / 64, room = (r.tc || p->dtype == LQ_F32 ? 1ll : 2ll) * sm_count(), least = p->dtype == LQ_F32 ? 2 : 8;
   long long count = r.tiles > 0 ? room / r.tiles : 1;
-  count = count > chunks / 8 ? chunks / 8 : count;
+  count = count > chunks / least ? chunks / least : count;
   count = count < 1 ? 1 : count;
   const long long each = (chunks + count - 1) / count;
   r.tokens = (int)((each < 1 ? 1 : each) * 64);
