@@ -50,9 +50,15 @@ class _Cache:
         self.all = torch.zeros(slots + 1, *shape, device="cuda", dtype=dtype)
         self.rows = self.all[:slots]
 
-    def put(self, slots, values):
+    def _at(self, slots):
         at = slots.long()
-        self.all[torch.where((at >= 0) & (at < self.rows.shape[0]), at, self.rows.shape[0])] = values
+        return torch.where((at >= 0) & (at < self.rows.shape[0]), at, self.rows.shape[0])
+
+    def put(self, slots, values):
+        self.all[self._at(slots)] = values
+
+    def take(self, slots):
+        return self.all[self._at(slots)]
 
 
 class Mamba2Layer:
