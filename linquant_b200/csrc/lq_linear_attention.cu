@@ -4,7 +4,7 @@
 //
 // Prompts, by chunks of C tokens: with G the running sum of g inside a chunk and S the state that enters it
 //   o_i = scale (exp(G_i) q_i S + sum_{j<=i} exp(G_i - G_j) (q_i . k_j) v_j),   S' = exp(G_C) S + sum_j exp(G_C - G_j) k_j v_j^T
-// so a chunk is four matrix products. A CTA of four warps has VT value channels of one head, keeps its part of the state in the
+// so a chunk is four matrix products. A CTA has VT value channels of one head, keeps its part of the state in the
 // accumulators of the last product and walks over the chunks: the data are read once, and nothing but o is written.
 // Where a batch has too few heads for the GPU, the tokens are cut into segments: a first pass leaves every segment's own
 // state, a small kernel carries them on, and the second pass starts each segment from what enters it.
@@ -21,8 +21,6 @@
 namespace lq {
 
 namespace attention {
-
-constexpr int THREADS = 128;
 
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];\n" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
@@ -61,30 +59,35 @@ struct Shape {
   static constexpr int GB = Decay<C>::BYTES;
   static constexpr int ST = BUFS * TILES, GO = ST + NS * SB, RED = GO + GB;
   static constexpr size_t SMEM = RED + 16;
-  static constexpr int REGS = KP / 64 * (VT / 8) * 4;      // of the state, a thread
-  static constexpr int WPM = 64 / C;                       // warps that share 16 rows of the output
+  // Warps: fp32 operands to 128 channels, whose tiles leave room for one CTA an SM, take eight (611 tokens of 6 heads, 72 x 100: one warp a scheduler
+  // waits for its own results five clocks of six)
+  static constexpr int WARPS = sizeof(T) == 4 && KP <= 128 ? 8 : 4, THREADS = 32 * WARPS;
+  static constexpr int WPM = 16 * WARPS / C;               // warps that share 16 rows of the output
+  static constexpr int ROWS = WARPS < KP / 16 ? WARPS : KP / 16;  // warps along the state's rows; the others along its columns
+  static constexpr int MT = KP / 16 / ROWS, NT = VT / 8 / (WARPS / ROWS);  // a warp's tiles of the state
+  static constexpr int REGS = MT * NT * 4;                 // of the state, a thread
 };
 
 // Rows of a chunk to a tile: 16-bit values as they are, fp32 as three tiles of bf16 pieces. `vec`: bytes of an access that every row start allows.
-template <typename T, int COLS, int C, int PIECE>
+template <typename T, int COLS, int C, int PIECE, int NTHREADS>
 __device__ __forceinline__ void load_tile(uint32_t dst, const T* src, long long stride, int rows, int cols, int vec) {
   constexpr int ROWB = COLS * 2, PER = COLS / 8;
   if constexpr (sizeof(T) == 2) {
     if (vec == 16) {
 #pragma unroll 4
-      for (int i = threadIdx.x; i < C * PER; i += THREADS) {
+      for (int i = threadIdx.x; i < C * PER; i += NTHREADS) {
         const int row = i / PER, p = i % PER, bytes = row < rows ? min(max(cols - p * 8, 0) * 2, 16) : 0;
         cp_async16_zfill(dst + at<ROWB>(row, p), bytes ? src + row * stride + p * 8 : src, bytes);
       }
     } else if (vec >= 4) {
 #pragma unroll 4
-      for (int i = threadIdx.x; i < C * PER * 4; i += THREADS) {
+      for (int i = threadIdx.x; i < C * PER * 4; i += NTHREADS) {
         const int row = i / (PER * 4), e = i % (PER * 4), bytes = row < rows ? min(max(cols - e * 2, 0) * 2, 4) : 0;
         cp_async4_zfill(dst + at<ROWB>(row, e >> 2) + (e & 3) * 4, bytes ? src + row * stride + e * 2 : src, bytes);
       }
     } else {
 #pragma unroll 4
-      for (int i = threadIdx.x; i < C * COLS; i += THREADS) {
+      for (int i = threadIdx.x; i < C * COLS; i += NTHREADS) {
         const int row = i / COLS, e = i % COLS;
         uint16_t v = 0;
         if (row < rows && e < cols) v = __ldg(reinterpret_cast<const unsigned short*>(src) + row * stride + e);
@@ -92,8 +95,8 @@ __device__ __forceinline__ void load_tile(uint32_t dst, const T* src, long long 
       }
     }
   } else {
-#pragma unroll 2
-    for (int i = threadIdx.x; i < C * PER; i += THREADS) {
+#pragma unroll 4
+    for (int i = threadIdx.x; i < C * PER; i += NTHREADS) {
       const int row = i / PER, p = i % PER;
       const float* from = src + row * stride + p * 8;
       float x[8];
@@ -117,16 +120,25 @@ __device__ __forceinline__ void load_tile(uint32_t dst, const T* src, long long 
   }
 }
 
+// A chunk's rows on their way to L2
+template <int NTHREADS>
+__device__ __forceinline__ void prefetch_tile(const float* src, long long stride, int rows, int cols) {
+  const int lines = (cols + 31) / 32;
+  for (int i = threadIdx.x; i < rows * lines; i += NTHREADS)
+    asm volatile("prefetch.global.L2 [%0];\n" ::"l"(src + i / lines * stride + i % lines * 32));
+}
+
 struct Vec {
   int q, k, v, o;  // bytes of an access
 };
 
 template <typename T, int KP, int VT, int C, bool STATES>
-__global__ void __launch_bounds__(THREADS, sizeof(T) == 2 && KP <= 128 ? 2 : 1) linear_attention_kernel(const lq_attention_problem p, const Segments seg, const Vec vec) {
+__global__ void __launch_bounds__(sizeof(T) == 4 && KP <= 128 ? 256 : 128, sizeof(T) == 2 && KP <= 128 ? 2 : 1) linear_attention_kernel(const lq_attention_problem p, const Segments seg, const Vec vec) {
   using S = Shape<T, KP, VT, C>;
   using M = typename S::M;
   constexpr bool F16 = S::F16;
-  constexpr int NP = S::NP, MT = KP / 64, NT = VT / 8, KS = KP / 16, CS = C / 16;
+  constexpr int NP = S::NP, MT = S::MT, NT = S::NT, KS = KP / 16, CS = C / 16;
+  constexpr int SIDE = 2;  // pairs of sums side by side: a sum's products wait for one another
   extern __shared__ __align__(128) uint8_t smem_dyn[];
   const uint32_t s0 = smem_u32(smem_dyn), s_state = s0 + S::ST, s_red = s0 + S::RED;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
@@ -141,8 +153,8 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 2 && KP <= 128 ? 2 : 1) 
   const T* v = reinterpret_cast<const T*>(p.v) + b * p.v_stride_b + h * p.v_stride_h + v0;
   const int cols = min(VT, p.V - v0);
 
-  float st[MT][NT][4];  // rows d0 + 16 m + g (+ 8), columns 8 j + 2 t4 (+ 1); fp16: times 2^-exp_w
-  const int d0 = warp * (KP / 4);
+  float st[MT][NT][4];  // rows d0 + 16 m + g (+ 8), columns 8 (js + j) + 2 t4 (+ 1); fp16: times 2^-exp_w
+  const int d0 = warp % S::ROWS * (16 * MT), js = warp / S::ROWS * NT;
   int exp_w = 0;
 #pragma unroll
   for (int m = 0; m < MT; ++m)
@@ -150,15 +162,15 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 2 && KP <= 128 ? 2 : 1) 
     for (int j = 0; j < NT; ++j)
 #pragma unroll
       for (int e = 0; e < 4; ++e) st[m][j][e] = 0.f;
-  const size_t tile = (size_t)blockIdx.x * THREADS * S::REGS;
+  const size_t tile = (size_t)blockIdx.x * S::THREADS * S::REGS;
   if (blockIdx.y > 0) {
     if constexpr (!STATES) {
-      const float4* from = reinterpret_cast<const float4*>(seg.states + (size_t)(blockIdx.y - 1) * gridDim.x * THREADS * S::REGS + tile);
+      const float4* from = reinterpret_cast<const float4*>(seg.states + (size_t)(blockIdx.y - 1) * gridDim.x * S::THREADS * S::REGS + tile);
 #pragma unroll
       for (int m = 0; m < MT; ++m)
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
-          const float4 x = from[(m * NT + j) * THREADS + tid];
+          const float4 x = from[(m * NT + j) * S::THREADS + tid];
           st[m][j][0] = x.x, st[m][j][1] = x.y, st[m][j][2] = x.z, st[m][j][3] = x.w;
         }
     }
@@ -170,7 +182,7 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 2 && KP <= 128 ? 2 : 1) 
       for (int j = 0; j < NT; ++j)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const int d = d0 + 16 * m + g + 8 * (e >> 1), c = 8 * j + 2 * t4 + (e & 1);
+          const int d = d0 + 16 * m + g + 8 * (e >> 1), c = 8 * (js + j) + 2 * t4 + (e & 1);
           if (d < p.K && c < cols) st[m][j][e] = __ldg(from + (size_t)d * p.V + c);
         }
   }
@@ -178,9 +190,9 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 2 && KP <= 128 ? 2 : 1) 
   auto load = [&](int c, int buf) {
     const int t0 = first + c * C, rows = min(C, stop - t0);
     const uint32_t to = s0 + buf * S::TILES;
-    if constexpr (!STATES) load_tile<T, KP, C, S::QK>(to, q + t0 * p.q_stride_t, p.q_stride_t, rows, p.K, vec.q);
-    load_tile<T, KP, C, S::QK>(to + NP * S::QK, k + t0 * p.k_stride_t, p.k_stride_t, rows, p.K, vec.k);
-    load_tile<T, VT, C, S::VB>(to + 2 * NP * S::QK, v + t0 * p.v_stride_t, p.v_stride_t, rows, cols, vec.v);
+    if constexpr (!STATES) load_tile<T, KP, C, S::QK, S::THREADS>(to, q + t0 * p.q_stride_t, p.q_stride_t, rows, p.K, vec.q);
+    load_tile<T, KP, C, S::QK, S::THREADS>(to + NP * S::QK, k + t0 * p.k_stride_t, p.k_stride_t, rows, p.K, vec.k);
+    load_tile<T, VT, C, S::VB, S::THREADS>(to + 2 * NP * S::QK, v + t0 * p.v_stride_t, p.v_stride_t, rows, cols, vec.v);
     cp_async_commit();
   };
   // what q reads: the state in pieces; fp16: under a power of two that all warps share
@@ -212,7 +224,7 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 2 && KP <= 128 ? 2 : 1) 
         for (int j = 0; j < NT; ++j) {
           uint32_t w[S::NS];
           split<M, S::NS>(st[m][j][2 * r] * f, st[m][j][2 * r + 1] * f, w);
-          const uint32_t to = s_state + at<VT * 2>(d, j) + 4 * t4;
+          const uint32_t to = s_state + at<VT * 2>(d, js + j) + 4 * t4;
 #pragma unroll
           for (int i = 0; i < S::NS; ++i) sts_u32(to + i * S::SB, w[i]);
         }
@@ -246,6 +258,12 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 2 && KP <= 128 ? 2 : 1) 
     cp_async_wait<0>();
     __syncthreads();  // tiles, decays and the state's pieces are there
     if (S::BUFS == 2 && c + 1 < chunks) load(c + 1, buf ^ 1);
+    if constexpr (sizeof(T) == 4) {
+      const int t1 = t0 + C, rows = min(C, stop - t1);
+      if (!STATES) prefetch_tile<S::THREADS>(q + t1 * p.q_stride_t, p.q_stride_t, rows, p.K);
+      prefetch_tile<S::THREADS>(k + t1 * p.k_stride_t, p.k_stride_t, rows, p.K);
+      prefetch_tile<S::THREADS>(v + t1 * p.v_stride_t, p.v_stride_t, rows, cols);
+    }
     if (warp == 0 && c + 1 < chunks) {
       total = total + next.of(x_next);
       if (F16) next.largest();
@@ -253,7 +271,7 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 2 && KP <= 128 ? 2 : 1) 
     }
     if constexpr (!STATES) {
       const int mt = warp / S::WPM, r0 = 16 * mt;  // rows of this warp; of the VT columns it has its share
-      constexpr int NV = NT / S::WPM;
+      constexpr int NV = VT / 8 / S::WPM, SV = NV >= 4 ? SIDE : 1;
       const int j0 = warp % S::WPM * NV;
       // decayed products of q and k
       float a[2 * CS][4];
@@ -264,21 +282,26 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 2 && KP <= 128 ? 2 : 1) 
       const int arow = r0 + (lane & 15), apiece = lane >> 4;
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
+        if (16 * ks >= p.K) break;
         uint32_t qa[NP][4];
 #pragma unroll
         for (int i = 0; i < NP; ++i) ldsm4(qa[i], s_q + i * S::QK + at<KP * 2>(arow, 2 * ks + apiece));
 #pragma unroll
-        for (int j = 0; j < CS; ++j) {
+        for (int j = 0; j < CS; j += SIDE) {
           if (j > mt) break;
 #pragma unroll
           for (int i = NP - 1; i >= 0; --i) {
-            uint32_t kb[4];
-            ldsm4(kb, s_k + i * S::QK + at<KP * 2>(16 * j + (lane & 7) + (lane >> 4) * 8, 2 * ks + ((lane >> 3) & 1)));
+            uint32_t kb[SIDE][4];
 #pragma unroll
-            for (int o = NP - 1 - i; o >= 0; --o) {
-              mma<M>(a[2 * j], qa[o], kb[0], kb[1]);
-              mma<M>(a[2 * j + 1], qa[o], kb[2], kb[3]);
-            }
+            for (int u = 0; u < SIDE; ++u) ldsm4(kb[u], s_k + i * S::QK + at<KP * 2>(16 * (j + u) + (lane & 7) + (lane >> 4) * 8, 2 * ks + ((lane >> 3) & 1)));
+#pragma unroll
+            for (int o = NP - 1 - i; o >= 0; --o)
+#pragma unroll
+              for (int u = 0; u < SIDE; ++u) {
+                if (j + u > mt) break;
+                mma<M>(a[2 * (j + u)], qa[o], kb[u][0], kb[u][1]);
+                mma<M>(a[2 * (j + u) + 1], qa[o], kb[u][2], kb[u][3]);
+              }
           }
         }
       }
@@ -305,20 +328,25 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 2 && KP <= 128 ? 2 : 1) 
         for (int e = 0; e < 4; ++e) o[j][e] = 0.f;
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
+        if (16 * ks >= p.K) break;
         uint32_t qa[NP][4];
 #pragma unroll
         for (int i = 0; i < NP; ++i) ldsm4(qa[i], s_q + i * S::QK + at<KP * 2>(arow, 2 * ks + apiece));
 #pragma unroll
-        for (int j = 0; j < NV; j += 2)
+        for (int j = 0; j < NV; j += 2 * SV)
 #pragma unroll
           for (int i = S::NS - 1; i >= 0; --i) {
-            uint32_t sb[4];
-            ldsm4t(sb, s_state + i * S::SB + at<VT * 2>(16 * ks + (lane & 15), j0 + j + (lane >> 4)));
+            uint32_t sb[SV][4];
+#pragma unroll
+            for (int u = 0; u < SV; ++u) ldsm4t(sb[u], s_state + i * S::SB + at<VT * 2>(16 * ks + (lane & 15), j0 + j + 2 * u + (lane >> 4)));
 #pragma unroll
             for (int w = NP - 1; w >= 0; --w) {
               if (w + i >= S::NS) continue;
-              mma<M>(o[j], qa[w], sb[0], sb[1]);
-              mma<M>(o[j + 1], qa[w], sb[2], sb[3]);
+#pragma unroll
+              for (int u = 0; u < SV; ++u) {
+                mma<M>(o[j + 2 * u], qa[w], sb[u][0], sb[u][1]);
+                mma<M>(o[j + 2 * u + 1], qa[w], sb[u][2], sb[u][3]);
+              }
             }
           }
       }
@@ -331,16 +359,19 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 2 && KP <= 128 ? 2 : 1) 
       for (int ks = 0; ks < CS; ++ks) {
         if (ks > mt) break;
 #pragma unroll
-        for (int j = 0; j < NV; j += 2)
+        for (int j = 0; j < NV; j += 2 * SV)
 #pragma unroll
           for (int i = NP - 1; i >= 0; --i) {
-            uint32_t vb[4];
-            ldsm4t(vb, s_v + i * S::VB + at<VT * 2>(16 * ks + (lane & 15), j0 + j + (lane >> 4)));
+            uint32_t vb[SV][4];
 #pragma unroll
-            for (int w = S::NA - 1 - i; w >= 0; --w) {
-              mma<M>(o[j], pa[w][ks], vb[0], vb[1]);
-              mma<M>(o[j + 1], pa[w][ks], vb[2], vb[3]);
-            }
+            for (int u = 0; u < SV; ++u) ldsm4t(vb[u], s_v + i * S::VB + at<VT * 2>(16 * ks + (lane & 15), j0 + j + 2 * u + (lane >> 4)));
+#pragma unroll
+            for (int w = S::NA - 1 - i; w >= 0; --w)
+#pragma unroll
+              for (int u = 0; u < SV; ++u) {
+                mma<M>(o[j + 2 * u], pa[w][ks], vb[u][0], vb[u][1]);
+                mma<M>(o[j + 2 * u + 1], pa[w][ks], vb[u][2], vb[u][3]);
+              }
           }
       }
       const float c0 = F16 ? p.scale / up0 : p.scale, c1 = F16 ? p.scale / up1 : p.scale;
@@ -452,16 +483,19 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 2 && KP <= 128 ? 2 : 1) 
             for (int i = 0; i < S::NK; ++i) kp[i][e] = pieces[i];
           }
 #pragma unroll
-          for (int j = 0; j < NT; j += 2)
+          for (int j = 0; j < NT; j += 2 * SIDE)
 #pragma unroll
             for (int i = NP - 1; i >= 0; --i) {
-              uint32_t vb[4];
-              ldsm4t(vb, s_v + i * S::VB + at<VT * 2>(16 * ks + (lane & 15), j + (lane >> 4)));
+              uint32_t vb[SIDE][4];
 #pragma unroll
-              for (int w = S::NK - 1 - i; w >= 0; --w) {
-                mma<M>(st[m][j], kp[w], vb[0], vb[1]);
-                mma<M>(st[m][j + 1], kp[w], vb[2], vb[3]);
-              }
+              for (int u = 0; u < SIDE; ++u) ldsm4t(vb[u], s_v + i * S::VB + at<VT * 2>(16 * ks + (lane & 15), js + j + 2 * u + (lane >> 4)));
+#pragma unroll
+              for (int w = S::NK - 1 - i; w >= 0; --w)
+#pragma unroll
+                for (int u = 0; u < SIDE; ++u) {
+                  mma<M>(st[m][j + 2 * u], kp[w], vb[u][0], vb[u][1]);
+                  mma<M>(st[m][j + 2 * u + 1], kp[w], vb[u][2], vb[u][3]);
+                }
             }
         }
       }
@@ -477,12 +511,12 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 2 && KP <= 128 ? 2 : 1) 
 
   const float back = F16 ? pow2(exp_w) : 1.f;
   if constexpr (STATES) {
-    float4* to = reinterpret_cast<float4*>(seg.states + (size_t)blockIdx.y * gridDim.x * THREADS * S::REGS + tile);
+    float4* to = reinterpret_cast<float4*>(seg.states + (size_t)blockIdx.y * gridDim.x * S::THREADS * S::REGS + tile);
 #pragma unroll
     for (int m = 0; m < MT; ++m)
 #pragma unroll
       for (int j = 0; j < NT; ++j)
-        to[(m * NT + j) * THREADS + tid] = make_float4(st[m][j][0] * back, st[m][j][1] * back, st[m][j][2] * back, st[m][j][3] * back);
+        to[(m * NT + j) * S::THREADS + tid] = make_float4(st[m][j][0] * back, st[m][j][1] * back, st[m][j][2] * back, st[m][j][3] * back);
     if (vt == 0 && tid == 0) seg.decays[(size_t)blockIdx.y * (gridDim.x / vts) + bh] = ex2(total.hi);
   } else {
     if (p.final_state != nullptr && (int)blockIdx.y == (n > 0 ? (n - 1) / seg.tokens : 0)) {
@@ -493,14 +527,14 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 2 && KP <= 128 ? 2 : 1) 
         for (int j = 0; j < NT; ++j)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const int d = d0 + 16 * m + g + 8 * (e >> 1), col = 8 * j + 2 * t4 + (e & 1);
+            const int d = d0 + 16 * m + g + 8 * (e >> 1), col = 8 * (js + j) + 2 * t4 + (e & 1);
             if (d < p.K && col < cols) to[(size_t)d * p.V + col] = st[m][j][e] * back;
           }
     }
     // tokens behind the sequence, from the first whole chunk that has none of it
     T* out = reinterpret_cast<T*>(p.o) + ((size_t)b * p.T * p.H + h) * p.V + v0;
     const int from = first + chunks * C;
-    for (long long i = tid; i < (long long)max(last_token - from, 0) * VT; i += THREADS) {
+    for (long long i = tid; i < (long long)max(last_token - from, 0) * VT; i += S::THREADS) {
       const int col = (int)(i % VT);
       if (col < cols) out[(size_t)(from + i / VT) * p.H * p.V + col] = from_f32<T>(0.f);
     }
@@ -625,7 +659,7 @@ static Plan plan(const lq_attention_problem* p) {
   Plan r;
   r.tc = tc_applies(p);
   const int kp = p->K <= 64 && !r.tc ? 64 : p->K <= 128 ? 128 : 256, vt = kp == 256 ? 32 : 64;
-  r.regs = kp / 64 * (vt / 8) * 4;
+  r.floats = kp * vt;
   r.tiles = (long long)p->B * p->H * ((p->V + vt - 1) / vt);
   const long long chunks = ((long long)p->T + 63) / 64, room = (r.tc || p->dtype == LQ_F32 ? 1ll : 2ll) * sm_count(), least = p->dtype == LQ_F32 ? 2 : 8;
   long long count = r.tiles > 0 ? room / r.tiles : 1;
@@ -639,7 +673,7 @@ static Plan plan(const lq_attention_problem* p) {
 }
 static size_t workspace(const lq_attention_problem* p, const Plan& r) {
   if (r.count < 2) return 0;
-  return (size_t)(r.count - 1) * ((size_t)r.tiles * THREADS * r.regs + (((size_t)p->B * p->H + 63) / 64) * 64) * 4;
+  return (size_t)(r.count - 1) * ((size_t)r.tiles * r.floats + (((size_t)p->B * p->H + 63) / 64) * 64) * 4;
 }
 
 static int access_bytes(const void* ptr, long long sb, long long st, long long sh, int size) {
@@ -653,11 +687,11 @@ static int run(const lq_attention_problem* p, const Plan& r, const Segments& seg
   const int size = sizeof(T);
   const Vec vec{access_bytes(p->q, p->q_stride_b, p->q_stride_t, p->q_stride_h, size), access_bytes(p->k, p->k_stride_b, p->k_stride_t, p->k_stride_h, size),
                 access_bytes(p->v, p->v_stride_b, p->v_stride_t, p->v_stride_h, size), access_bytes(p->o, p->V, p->V, p->V, size)};
-  const dim3 block(THREADS);
+  const dim3 block(S::THREADS);
   cudaError_t e = cudaSuccess;
   if (seg.count > 1) {
     e = launch_opt_in(linear_attention_kernel<T, KP, VT, C, true>, dim3((unsigned)r.tiles, seg.count - 1), block, S::SMEM, st, *p, seg, vec);
-    if (e == cudaSuccess && seg.count > 2) e = launch_segment_states(seg, p->B * p->H, r.tiles * THREADS * S::REGS, st);
+    if (e == cudaSuccess && seg.count > 2) e = launch_segment_states(seg, p->B * p->H, r.tiles * S::THREADS * S::REGS, st);
   }
   if (e == cudaSuccess) e = launch_opt_in(linear_attention_kernel<T, KP, VT, C, false>, dim3((unsigned)r.tiles, seg.count), block, S::SMEM, st, *p, seg, vec);
   if (e != cudaSuccess) return fail(LQ_ERR_LAUNCH, "linear_attention: %s", cudaGetErrorString(e));
@@ -685,7 +719,7 @@ extern "C" int lq_linear_attention_fwd(const lq_attention_problem* p, void* ws, 
   if (need > 0 && (ws == nullptr || bytes < need)) return fail(LQ_ERR_WORKSPACE, "linear_attention: workspace of %zu bytes, %zu needed", bytes, need);
   if (need > 0 && (reinterpret_cast<uintptr_t>(ws) & 15u)) return fail(LQ_ERR_ALIGN, "linear_attention: workspace must start on a 16-byte boundary");
   float* states = reinterpret_cast<float*>(ws);
-  const Segments seg{r.count, r.tokens, states, states + (size_t)(r.count - 1) * r.tiles * THREADS * r.regs};
+  const Segments seg{r.count, r.tokens, states, states + (size_t)(r.count - 1) * r.tiles * r.floats};
   cudaStream_t st = (cudaStream_t)stream;
   if (r.tc) return run_tc(p, r, seg, st);
   return with_dtype(p->dtype, "linear_attention", [&](auto t) {

@@ -171,7 +171,7 @@ __device__ __forceinline__ void row_scales(const float (&a)[NJ][4], int tiles, f
 // lq_linear_attention_tc.cu: the kernel for many tokens of 16-bit operands on tcgen05, where it applies
 bool tc_applies(const lq_attention_problem* p);
 struct Plan {
-  int regs, count, tokens;  // floats of a state's tile a thread (of 128); segments and their tokens
+  int floats, count, tokens;  // of a state's tile; segments and their tokens
   long long tiles;          // B * H * V tiles
   bool tc;
 };
