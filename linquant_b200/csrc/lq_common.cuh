@@ -20,11 +20,17 @@ int sm_count();  // of the current device
 // stream-serialisation attribute and open with pdl_enter(), which waits until everything before has completed and is
 // visible: the launch itself (block scheduling, instruction and parameter fetch) then overlaps the end of the kernel before,
 // 1 to 3 us per kernel, which is a third of a short prompt's time (a Mamba-2 layer on one chunk: 55 -> 38 us). All
-// memory traffic, barrier set-up and tensor-memory allocation stay behind the wait. No kernel triggers its successor
+// memory traffic, barrier set-up and tensor-memory allocation stay behind the wait. Kernels do not trigger their successors
 // early: CTAs that are placed while a kernel is still running fill whatever SMs have room, several to an SM, and the serial
 // state passes then keep that uneven placement to their end (DeltaNet, 1 x 1024 tokens: 75 us instead of 60).
 __device__ __forceinline__ void pdl_enter() {
   asm volatile("griddepcontrol.wait;\n" ::: "memory");
+}
+// The next kernel may be placed once every CTA has come here; its own pdl_enter() still waits for this one's end. Only behind this kernel's
+// pdl_enter(): what ran before it has then completed for the next one too, which may read that ahead of its wait. The kernels of
+// low-rank adapters, whose successor needs their results at its end only, are the ones that do it.
+__device__ __forceinline__ void pdl_trigger() {
+  asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
 }
 template <typename... KArgs, typename... Args>
 static inline cudaError_t launch(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, Args&&... args) {

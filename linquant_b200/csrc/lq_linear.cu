@@ -124,7 +124,7 @@ __global__ void __launch_bounds__(std::is_same_v<TX, int8_t> ? 256 : 512, 2) int
     for (int i = 0; i < 2; ++i) asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;\n" ::"r"(smem_u32(&bars[i])));
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
   }
-  pdl_enter();
+  if constexpr (!LORA) pdl_enter();  // with adapters it is t alone that the kernel ahead makes
   struct At {  // of an item: its tile and piece
     int tile, chunk;
     __device__ __forceinline__ void next(int chunks) {
@@ -212,12 +212,15 @@ __global__ void __launch_bounds__(std::is_same_v<TX, int8_t> ? 256 : 512, 2) int
     if (!ok) {  // stores nothing more; what was requested still lands
       for (int k = i; k < min(i + 2, items); ++k) mbar_wait_bounded(smem_u32(&bars[k & 1]), (uint32_t)((k >> 1) & 1));
       if (tid == 0 && p.status) atomicExch(p.status, 1);
+      if constexpr (LORA) pdl_enter();
       return;
     }
     if (warp == 0 && i + 2 < items) {
       asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
       request(i + 2, ahead);
     }
+    if constexpr (LORA)
+      if (last) pdl_enter();
     if (last && mine && on < p.N) {
       int s = 0;
 #pragma unroll
@@ -284,10 +287,12 @@ int run_linear(const lq_linear_problem* p, const Lora* lora, cudaStream_t st) {
   });
 }
 
+// up to eight tokens whose codes fit a CTA's shared memory next to the weights: one launch, and 8.1 us against 9.5 (1 token), 10.8
+// against 10.2 (5), 11.3 against 10.2 (8) at 5120 -> 2560, where the host's 2 us for another launch are not counted
+bool linear_makes_codes(const lq_linear_problem* p) { return p->M <= 8 && (long long)p->M * linear::code_pitch(p->K) <= linear::CODES; }
+
 int run_linear_values(const lq_linear_problem* p, const Lora* lora, const void* values, int dtype, long long stride, cudaStream_t st) {
-  // up to eight tokens whose codes fit a CTA's shared memory next to the weights: one launch, and 8.1 us against 9.5 (1 token), 10.8
-  // against 10.2 (5), 11.3 against 10.2 (8) at 5120 -> 2560, where the host's 2 us for another launch are not counted
-  if (p->M > 8 || (long long)p->M * linear::code_pitch(p->K) > linear::CODES) {
+  if (!linear_makes_codes(p)) {
     if (int e = lq_quantize_rows(values, dtype, p->M, p->K, stride, const_cast<int8_t*>(p->x), p->x_stride, const_cast<float*>(p->x_scale), (lq_stream)st)) return e;
     return run_linear(p, lora, st);
   }

@@ -142,7 +142,7 @@ __global__ void __launch_bounds__(THREADS, 1) int8_linear_tc_kernel(const __grid
   const int rank = PAIR ? (int)cluster_rank() : 0, first = blockIdx.x / CTAS, step = gridDim.x / CTAS;
   const int mt = (p.M + CTAS * BM - 1) / (CTAS * BM), nt = (p.N + BN - 1) / BN, tiles = mt * nt, kblocks = (p.K + BK - 1) / BK;
 
-  pdl_enter();
+  if constexpr (!LORA) pdl_enter();  // with adapters the kernel ahead makes their share alone, which the outputs wait for
   if (tid == 0) {
     for (int i = 0; i < S::STAGES; ++i) {
       mbar_init(s_full + 8 * i, 1);
@@ -218,6 +218,7 @@ __global__ void __launch_bounds__(THREADS, 1) int8_linear_tc_kernel(const __grid
     const int quad = warp & 3, half = (warp >> 2) * S::HALF;
     const uint32_t out = s_out + warp * 32 * 64, cols = s_cols + warp * 2 * S::HALF * 4;
     const bool wide = ((size_t)p.N * sizeof(TO)) % 16 == 0 && (reinterpret_cast<uintptr_t>(p.y) & 15u) == 0;
+    if constexpr (LORA) pdl_enter();
     int i = 0;
     for (int t = first; t < tiles; t += step, ++i) {
       int m, n;
@@ -369,7 +370,7 @@ __global__ void __launch_bounds__(THREADS, 2) int8_linear_split_kernel(const __g
   const int nt = (p.N + S::BN - 1) / S::BN, m0 = tile / nt * BM, n0 = tile % nt * S::BN, rows = min(BM, p.M - m0);
   const int kblocks = (p.K + BK - 1) / BK, kb0 = kblocks * rank / parts, count = kblocks * (rank + 1) / parts - kb0;
 
-  pdl_enter();
+  if constexpr (!LORA) pdl_enter();
   if (tid == 0) {
     for (int i = 0; i < 2 * S::STAGES + 1; ++i) mbar_init(s_full + 8 * i, 1);
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
@@ -439,6 +440,7 @@ __global__ void __launch_bounds__(THREADS, 2) int8_linear_split_kernel(const __g
   cluster_sync();  // the sums of all are there
   if (warp == OUT_WARPS + 1) tmem_free<false>(tbase, S::BN);
   else if (warp < OUT_WARPS) {
+    if constexpr (LORA) pdl_enter();  // the adapters' share
     TO* y = reinterpret_cast<TO*>(p.y);
     const bool wide = p.N % 4 == 0 && (reinterpret_cast<uintptr_t>(p.y) & (4 * sizeof(TO) - 1)) == 0;
 #pragma unroll

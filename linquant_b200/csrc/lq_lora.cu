@@ -114,6 +114,7 @@ __global__ void __launch_bounds__(THREADS) lora_shrink_kernel(const Shrink p) {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
   const int rank = blockIdx.x % p.parts, m0 = blockIdx.x / p.parts * TILE;
   pdl_enter();
+  pdl_trigger();
   for (int i = tid; i < ROWS; i += THREADS) {
     const int l = i < TILE && m0 + i < p.M ? __ldg(p.adapters + m0 + i) : -1;
     which[i] = (unsigned)l < (unsigned)p.L ? l : -1;
@@ -319,12 +320,10 @@ __global__ void __launch_bounds__(THREADS, sizeof(TO) == 2 ? 5 : 3) lora_expand_
   __shared__ __align__(16) uint8_t stage[WARPS][32 * 128];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
   const int m0 = blockIdx.y * 32, n0 = (blockIdx.x * WARPS + warp) * SPAN;
-  pdl_enter();
   if (n0 >= N) return;
   constexpr int PER = 16 / sizeof(TO), ROW = CHUNK / PER;  // values of 16 bytes; such pieces of a row's chunk
   const int mine = m0 + lane < M ? q.of(m0 + lane) : -1;
   const uint32_t all = __ballot_sync(0xffffffffu, mine >= 0);
-  if (!all) return;
   const bool wide = ((size_t)N * sizeof(TO)) % 16 == 0 && (reinterpret_cast<uintptr_t>(y) & 15u) == 0;
   const uint32_t out = smem_u32(stage[warp]);
   auto place = [](int row, int piece) { return row * 128 + ((piece ^ (row & 7)) << 4); };
@@ -340,6 +339,9 @@ __global__ void __launch_bounds__(THREADS, sizeof(TO) == 2 ? 5 : 3) lora_expand_
     if (mine >= 0 && (like & ((1u << lane) - 1)) == 0)
       asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;\n" ::"l"(from), "r"((uint32_t)(min(SPAN, N - n0) * q.R * (int)sizeof(TB))) : "memory");
   }
+  pdl_enter();  // t; what ran before the kernel that makes it has completed
+  pdl_trigger();
+  if (!all) return;
   auto next_adapter = [&] {
     l = __shfl_sync(0xffffffffu, mine, __ffs(left) - 1);
     rows = __ballot_sync(0xffffffffu, mine == l);
@@ -496,6 +498,7 @@ static int expand(const Lora& q, const lq_linear_problem* p, cudaStream_t st) {
 int run_linear(const lq_linear_problem* p, const Lora* lora, cudaStream_t st);                                              // lq_linear.cu
 int run_linear_values(const lq_linear_problem* p, const Lora* lora, const void* values, int dtype, long long stride, cudaStream_t st);
 int check_linear(const lq_linear_problem* p);
+bool linear_makes_codes(const lq_linear_problem* p);
 
 }  // namespace lq
 
@@ -523,6 +526,10 @@ extern "C" int lq_lora_linear(const lq_linear_problem* p, const lq_lora_problem*
   if (values) x.at(values).pitch(stride, dtype_bytes(dtype)).pitch(p->K, dtype_bytes(dtype));
   // eight values are one or two accesses of 16 bytes and never leave their row (codes: one of 8, their rows start on 16)
   const bool vec = a.bytes() == 16 && (size == 2 || p->K % 8 == 0) && (values ? x.bytes() == 16 && p->K % 8 == 0 : true);
+  // Codes first: the kernel that makes t lets its successors start, which read them ahead of its end
+  const bool rows = values && !linear_makes_codes(p);
+  if (rows)
+    if (int e = lq_quantize_rows(values, dtype, p->M, p->K, stride, const_cast<int8_t*>(p->x), p->x_stride, const_cast<float*>(p->x_scale), stream)) return e;
   const int e = with_dtype(q->dtype, "lora_linear", [&](auto ta) {
     using TA = decltype(ta);
     if (!values) return lora::run_shrink<int8_t, TA>(s, vec, st);
@@ -532,5 +539,5 @@ extern "C" int lq_lora_linear(const lq_linear_problem* p, const lq_lora_problem*
   const Lora add{q->L, q->R, RP, q->dtype, q->b, q->adapters, q->t};
   if (p->M > kFewTokens)
     if (int e2 = lora::expand(add, p, st)) return e2;
-  return values ? run_linear_values(p, &add, values, dtype, stride, st) : run_linear(p, &add, st);
+  return values && !rows ? run_linear_values(p, &add, values, dtype, stride, st) : run_linear(p, &add, st);
 }

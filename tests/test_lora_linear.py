@@ -200,3 +200,33 @@ def test_refusals(what, error):
         lora_linear_fwd(x.char() if what == "codes" else x, w, ws, a[..., :16] if what == "a" else a, b[:1] if what == "b" else b.float() if what == "mixed" else b,
                         which[:2] if what == "adapters" else which.float() if what == "float" else which, scaling=randn(3) if what == "scaling" else None,
                         out_dtype=torch.float64 if what == "out" else None)
+
+
+@gpu
+@pytest.mark.parametrize("M", [3, 11, 40, 300, 5000])
+@pytest.mark.parametrize("form", ["codes", BF16])
+def test_kernels_that_overlap(M, form):
+    """The product starts while t and the adapters' share are being made: calls one behind the other, each on rows that the kernel ahead
+    of it has just written, have the bits of calls that wait for the device in between."""
+    from linquant_b200.kernels.layer import lora_linear_fwd, quantize_rows_fwd
+
+    K, N, L, R = 640, 1000, 5, 24
+    w, ws, a, b = weights(N, K, R, L, BF16)
+    which = torch.randint(-1, L, (M,), device="cuda").int()
+    source = [randn(M, K, dtype=BF16) for _ in range(4)]
+
+    def call(i, x):
+        x.copy_(source[i % 4])
+        if form == "codes":
+            codes, xs = quantize_rows_fwd(x)
+            return lora_linear_fwd(codes, w, ws, a, b, which, scaling=0.5, x_scale=xs, out_dtype=BF16)
+        return lora_linear_fwd(x, w, ws, a, b, which, scaling=0.5)
+
+    want, x = [], torch.empty(M, K, device="cuda", dtype=BF16)
+    for i in range(4):
+        want.append(call(i, x))
+        torch.cuda.synchronize()
+    for round in range(6):
+        got = [call(i, x) for i in range(8)]
+        torch.cuda.synchronize()
+        assert all(torch.equal(y, want[i % 4]) for i, y in enumerate(got)), round
