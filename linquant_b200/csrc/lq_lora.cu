@@ -310,23 +310,21 @@ static int run_shrink(Shrink p, bool vec, cudaStream_t st) {
 constexpr int CHUNK = 32, CT = CHUNK / 8;  // channels at a time, in tiles of 8
 
 // A warp: 32 tokens, SPAN channels. Over the adapters that the tokens have and their ranks in steps of 16; a step's operands are requested before
-// the products of the one ahead. The reduction index is permuted alike in both operands: a lane takes four consecutive r. Both are
+// the products of the one ahead. The reduction index is permuted alike in both operands: a lane takes four consecutive r; and the channels of
+// a chunk, column 2 i + e of tile j being channel 8 i + 2 j + e, so that a lane holds eight consecutive ones of a row. Both operands are
 // bf16 pieces: two (three for fp32 outputs) of t and of fp16 and fp32 b, products below 16 (24) bits behind the first left out.
 // The INT8 product's kernel reads y again, adds its own sum in fp32 and rounds once more: this rounding is of the adapters' share alone.
 // Bound by the bytes of y.
 template <typename TO, typename TB, int SPAN>
-__global__ void __launch_bounds__(THREADS, sizeof(TO) == 2 ? 5 : 3) lora_expand_kernel(const Lora q, int M, int N, TO* y) {
+__global__ void __launch_bounds__(THREADS, sizeof(TO) == 2 ? 4 : 3) lora_expand_kernel(const Lora q, int M, int N, TO* y) {
   constexpr int PT = sizeof(TO) == 4 ? 3 : 2, PB = std::is_same_v<TB, __nv_bfloat16> ? 1 : PT;
-  __shared__ __align__(16) uint8_t stage[WARPS][32 * 128];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
   const int m0 = blockIdx.y * 32, n0 = (blockIdx.x * WARPS + warp) * SPAN;
   if (n0 >= N) return;
-  constexpr int PER = 16 / sizeof(TO), ROW = CHUNK / PER;  // values of 16 bytes; such pieces of a row's chunk
+  constexpr int PER = 16 / sizeof(TO);  // values of 16 bytes
   const int mine = m0 + lane < M ? q.of(m0 + lane) : -1;
   const uint32_t all = __ballot_sync(0xffffffffu, mine >= 0);
   const bool wide = ((size_t)N * sizeof(TO)) % 16 == 0 && (reinterpret_cast<uintptr_t>(y) & 15u) == 0;
-  const uint32_t out = smem_u32(stage[warp]);
-  auto place = [](int row, int piece) { return row * 128 + ((piece ^ (row & 7)) << 4); };
 
   // the step that is on its way
   int l = 0, r0 = 0, c0 = 0;
@@ -350,14 +348,14 @@ __global__ void __launch_bounds__(THREADS, sizeof(TO) == 2 ? 5 : 3) lora_expand_
   };
   auto request = [&] {
     const int r = r0 + 4 * t4, rb = min(r, q.R - 4);  // behind R t is zero, and b is made so
-    const int n = n0 + c0 + g;
+    const int n = n0 + c0 + 8 * (g >> 1) + (g & 1);
     if (n0 + c0 + CHUNK <= N) {
       const TB* from = reinterpret_cast<const TB*>(q.b) + ((long long)l * N + n) * q.R + rb;
 #pragma unroll
-      for (int j = 0; j < CT; ++j) b[j] = load_pack<TB, 4>(from + 8 * j * q.R);
+      for (int j = 0; j < CT; ++j) b[j] = load_pack<TB, 4>(from + 2 * j * q.R);
     } else {  // behind N nothing is stored
 #pragma unroll
-      for (int j = 0; j < CT; ++j) b[j] = load_pack<TB, 4>(reinterpret_cast<const TB*>(q.b) + ((long long)l * N + min(n + 8 * j, N - 1)) * q.R + rb);
+      for (int j = 0; j < CT; ++j) b[j] = load_pack<TB, 4>(reinterpret_cast<const TB*>(q.b) + ((long long)l * N + min(n + 2 * j, N - 1)) * q.R + rb);
     }
 #pragma unroll
     for (int i = 0; i < 2; ++i)
@@ -380,7 +378,7 @@ __global__ void __launch_bounds__(THREADS, sizeof(TO) == 2 ? 5 : 3) lora_expand_
       for (int j = 0; j < CT; ++j)
 #pragma unroll
         for (int e = 0; e < 4; ++e) s[i][j][e] = 0.f;
-    bool same = true, done = false, end = false;  // the adapter goes on; the chunk is complete; nothing is left
+    bool same = true, end = false;  // the adapter goes on; nothing is left
     while (same) {
       uint32_t a[2][PT][4], w[CT][PB][2];
       const bool inside = r0 + 4 * t4 < q.R;
@@ -417,7 +415,6 @@ __global__ void __launch_bounds__(THREADS, sizeof(TO) == 2 ? 5 : 3) lora_expand_
       same = r0 < q.R;
       if (!same) {
         if (left == 0) {
-          done = true;
           c0 += CHUNK;
           end = c0 >= SPAN || n0 + c0 >= N;
           left = all;
@@ -442,36 +439,24 @@ __global__ void __launch_bounds__(THREADS, sizeof(TO) == 2 ? 5 : 3) lora_expand_
       for (int h = 0; h < 2; ++h) {
         const int row = 16 * i + 8 * h + g;
         if (!(now >> row & 1)) continue;
+        const int n = n0 + at + 8 * t4;
+        TO* to = y + (size_t)(m0 + row) * N + n;
 #pragma unroll
-        for (int j = 0; j < CT; ++j) {
-          const int byte = (8 * j + 2 * t4) * (int)sizeof(TO);
-          const uint32_t to = out + place(row, byte >> 4) + (byte & 15);
-          if constexpr (sizeof(TO) == 4) {
-            sts_u32(to, __float_as_uint(s[i][j][2 * h]));
-            sts_u32(to + 4, __float_as_uint(s[i][j][2 * h + 1]));
+        for (int c = 0; c < 8; c += PER) {
+          Pack<TO, PER> out;
+          float x[PER];
+#pragma unroll
+          for (int v = 0; v < PER; ++v) x[v] = s[i][(c + v) / 2][2 * h + (v & 1)];
+          out.set(x);
+          if (wide) {
+            if (n + c < N) store_pack(to + c, out);
           } else {
-            sts_u32(to, Act<TO>::pack2(s[i][j][2 * h], s[i][j][2 * h + 1]));
+#pragma unroll
+            for (int v = 0; v < PER; ++v)
+              if (n + c + v < N) to[c + v] = out.v[v];
           }
         }
       }
-    if (done) {
-      __syncwarp();
-      if (wide) {
-#pragma unroll
-        for (int k = 0; k < ROW; ++k) {
-          const int row = 32 / ROW * k + lane / ROW, piece = lane % ROW, n = n0 + at + piece * PER;
-          if (all >> row & 1 && n < N)
-            *reinterpret_cast<uint4*>(y + (size_t)(m0 + row) * N + n) = *reinterpret_cast<const uint4*>(stage[warp] + place(row, piece));
-        }
-      } else {
-        for (int row = 0; row < 32; ++row) {
-          const int byte = lane * (int)sizeof(TO);
-          if (all >> row & 1 && n0 + at + lane < N)
-            y[(size_t)(m0 + row) * N + n0 + at + lane] = *reinterpret_cast<const TO*>(stage[warp] + place(row, byte >> 4) + (byte & 15));
-        }
-      }
-      __syncwarp();  // the chunk has been read
-    }
     if (end) return;
   }
 }
