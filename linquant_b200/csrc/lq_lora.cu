@@ -319,7 +319,7 @@ template <typename TO, typename TB, int SPAN>
 __global__ void __launch_bounds__(THREADS, sizeof(TO) == 2 ? 4 : 3) lora_expand_kernel(const Lora q, int M, int N, TO* y) {
   constexpr int PT = sizeof(TO) == 4 ? 3 : 2, PB = std::is_same_v<TB, __nv_bfloat16> ? 1 : PT;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
-  const int m0 = blockIdx.y * 32, n0 = (blockIdx.x * WARPS + warp) * SPAN;
+  const int columns = (N + WARPS * SPAN - 1) / (WARPS * SPAN), m0 = (int)(blockIdx.x / columns) * 32, n0 = ((int)(blockIdx.x % columns) * WARPS + warp) * SPAN;
   if (n0 >= N) return;
   constexpr int PER = 16 / sizeof(TO);  // values of 16 bytes
   const int mine = m0 + lane < M ? q.of(m0 + lane) : -1;
@@ -465,12 +465,13 @@ static int expand(const Lora& q, const lq_linear_problem* p, cudaStream_t st) {
   return with_dtype(p->out_dtype, "lora_linear", [&](auto t) {
     using TO = decltype(t);
     const long long rows = ((long long)p->M + 31) / 32;
-    if (rows > 65535) return fail(LQ_ERR_SHAPE, "lora_linear: M=%d", p->M);
     return with_dtype(q.dtype, "lora_linear", [&](auto tb) {
       using TB = decltype(tb);
       // few tokens: warps of 32 channels, as many as there can be, each of which goes over all adapters of its tokens one after the other
       auto go = [&](auto kern, int span) {
-        const cudaError_t e = launch(kern, dim3((p->N + WARPS * span - 1) / (WARPS * span), (unsigned)rows), dim3(THREADS), 0, st, q, p->M, p->N, reinterpret_cast<TO*>(p->y));
+        const long long ctas = rows * ((p->N + WARPS * span - 1) / (WARPS * span));
+        if (ctas >= 1ll << 31) return fail(LQ_ERR_SHAPE, "lora_linear: M=%d N=%d", p->M, p->N);
+        const cudaError_t e = launch(kern, dim3((unsigned)ctas), dim3(THREADS), 0, st, q, p->M, p->N, reinterpret_cast<TO*>(p->y));
         return e != cudaSuccess ? fail(LQ_ERR_LAUNCH, "lora_linear: %s", cudaGetErrorString(e)) : check_launch("lora_expand_kernel");
       };
       return rows * ((p->N + 127) / 128) <= 10ll * sm_count() ? go(lora_expand_kernel<TO, TB, 32>, 32) : go(lora_expand_kernel<TO, TB, 128>, 128);

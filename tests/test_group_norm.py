@@ -207,3 +207,20 @@ def test_refusals(what, error):
                        weight=randn(15) if what == "weight" else None, gate={"gate": x[:, :4], "gate_type": x.half()}.get(what),
                        over_tokens=what in ("dims", "lengths_n"),
                        lengths=torch.tensor([1, 2, 3] if what == "lengths_n" else [1, 2], device="cuda") if what.startswith("lengths") else None)
+
+
+@gpu
+def test_rows_behind_32_bits():
+    """2.2e9 values: the last rows have what they have by themselves."""
+    from linquant_b200.kernels.layer import group_norm_fwd
+
+    x = torch.empty(2_100_003, 1032, device="cuda", dtype=torch.bfloat16).normal_()
+    y = group_norm_fwd(x, 2)
+    tail = x[-77:].clone()
+    assert torch.equal(y[-77:], group_norm_fwd(tail, 2)) and torch.equal(y[:77], group_norm_fwd(x[:77].clone(), 2))
+    del y
+    z = group_norm_fwd(x.unsqueeze(0), 2, over_tokens=True, lengths=torch.tensor([130], device="cuda", dtype=torch.int32))
+    # tiles of another length add in another order: fp32 roundings of the mean and variance, then a step of bf16 that may fall to the other side
+    alone = group_norm_fwd(x[:130].clone().unsqueeze(0), 2, over_tokens=True)[0].float()
+    assert ((z[0, :130].float() - alone).abs() <= alone.abs() * 2.0**-7 + 2.0**-16).all()
+    assert not z[0, -1000:].any()

@@ -338,3 +338,75 @@ def test_refusals(what):
             linear_attention_step(randn(2, 4, 24, 16).transpose(2, 3), q[:, 0], k[:, 0], v[:, 0], g[:, 0])
         else:
             linear_attention_step(randn(1, 4, 16, 24), q[:, 0], k[:, 0], v[:, 0], g[:, 0])  # a row fewer than sequences
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("what", ["batch", "heads", "tokens", "all"])
+def test_operands_that_repeat(dtype, what):
+    """Broadcast operands, whose strides are zero."""
+    from linquant_b200.kernels.layer import linear_attention_fwd, linear_attention_step
+
+    B, T, H, K, V = 2, 90, 3, 64, 72
+    one = {"batch": (1, T, H), "heads": (B, T, 1), "tokens": (B, 1, H), "all": (1, 1, 1)}[what]
+    q, k, v = (randn(*one, n, dtype=dtype).expand(B, T, H, n) for n in (K, K, V))
+    g = (-torch.rand(*one, device="cuda")).expand(B, T, H)
+    o, state = linear_attention_fwd(q, k, v, g, output_final_state=True)
+    agree(o, state, recurrence(q, k, v, g, None, None, None), dtype, T)
+    cache = randn(B, H, K, V)
+    want = recurrence(q[:, :1], k[:, :1], v[:, :1], g[:, :1], None, cache.clone(), None)
+    o = linear_attention_step(cache, q[:, 0], k[:, 0], v[:, 0], g[:, 0])
+    agree(o.unsqueeze(1), cache, want, dtype, 1)
+
+
+@gpu
+@pytest.mark.parametrize("K,dtype", [(64, BF16), (136, F16)])
+def test_outputs_behind_32_bits(K, dtype):
+    """2.3e9 outputs and values; the last sequence counts its first tokens only."""
+    from linquant_b200.kernels.layer import linear_attention_fwd
+
+    B, T, H, V = 2, 70000, 128, 128
+    n = ints(65, 130)
+    q, k = randn(B, T, 1, K, dtype=dtype), randn(B, T, 1, K, dtype=dtype)
+    v = torch.empty(B, T, H, V, device="cuda", dtype=dtype)
+    v[:, :130] = randn(B, 130, H, V, dtype=dtype)
+    g = -torch.rand(H, device="cuda")
+    o, state = linear_attention_fwd(q, k, v, g, lengths=n, output_final_state=True)
+    agree(o[:, :130], state, recurrence(q[:, :130], k[:, :130], v[:, :130], g, None, None, n), dtype, 130)
+    assert not o[:, 130:].any()
+
+
+@gpu
+def test_from_two_threads():
+    """Calls whose kernels differ in shared memory and workspaces, each on a stream of its own: every one has its own result."""
+    import threading
+
+    from linquant_b200.kernels.layer import group_norm_fwd, linear_attention_fwd, lora_linear_fwd, quantize_rows_fwd
+
+    def calls(dtype, K, T, M, R):
+        q, k, v, g = inputs(1, T, 2, 2, K, 64, dtype)
+        x = randn(M, 320, dtype=dtype)
+        w, ws = quantize_rows_fwd(randn(96, 320))
+        a, b, which = randn(3, R, 320, dtype=dtype), randn(3, 96, R, dtype=dtype), torch.randint(-1, 3, (M,), device="cuda").int()
+        return lambda: (linear_attention_fwd(q, k, v, g)[0], lora_linear_fwd(x, w, ws, a, b, which), group_norm_fwd(x.unsqueeze(0), 5, over_tokens=True))
+
+    jobs = [calls(F32, 100, 300, 90, 128), calls(BF16, 64, 1500, 3, 8), calls(F16, 200, 90, 700, 40)]
+    want = [job() for job in jobs]
+    torch.cuda.synchronize()
+    bad, start = [], threading.Barrier(len(jobs))
+
+    def work(job, expected):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            start.wait()
+            for _ in range(200):
+                got = job()
+                torch.cuda.current_stream().synchronize()
+                if not all(torch.equal(a, b) for a, b in zip(got, expected)):
+                    bad.append(expected[0].dtype)
+
+    threads = [threading.Thread(target=work, args=z) for z in zip(jobs, want)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert bad == []

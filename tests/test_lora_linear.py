@@ -230,3 +230,20 @@ def test_kernels_that_overlap(M, form):
         got = [call(i, x) for i in range(8)]
         torch.cuda.synchronize()
         assert all(torch.equal(y, want[i % 4]) for i, y in enumerate(got)), round
+
+
+@gpu
+def test_outputs_behind_32_bits():
+    """2.1 million tokens, 2.2e9 outputs: rows at both ends and around the 65536th tile of 32."""
+    from linquant_b200.kernels.layer import lora_linear_fwd, quantize_rows_fwd
+
+    M, K, N, R, L = 2_100_003, 16, 1032, 8, 3
+    w, ws, a, b = weights(N, K, R, L, BF16)
+    x = randn(M, K, dtype=BF16)
+    which = (torch.arange(M, device="cuda") // 1000 % 4).int()  # the fourth: none
+    y = lora_linear_fwd(x, w, ws, a, b, which, scaling=0.5)
+    rows = torch.cat([torch.arange(n, n + 40, device="cuda") for n in (0, 65535 * 32 - 20, M - 40)])
+    codes, xs = quantize_rows_fwd(x[rows])
+    base, mag, low = want_of(x[rows], codes, xs, w, ws, a, b, which[rows], 0.5, None)
+    e = low_error(BF16, K, R, M)
+    ref.check(y[rows], base, mag * (4 * ULP / e) + low, e)
