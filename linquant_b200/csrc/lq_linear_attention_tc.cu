@@ -10,7 +10,7 @@
 //   MMA warp      q k^T; k^T v' (both operands as they lie, token index outermost: "MN-major"); q S; P v
 //   warps 0..7    two sets of four that take chunks in turn: P = decayed q k^T from tensor memory to shared memory, rounded; the outputs
 //   warps 8..15   the state, half a row of K a thread in registers: S = a S + k^T v'; S rounded for q
-//   warps 16..19  v' = exp(G_C - G_j) v in pieces
+//   warps 16..19  v' = exp(G_C - G_j) v in pieces (where only segments' states are made, warps 0..3 take every other chunk)
 //
 // All accumulators lie twice in tensor memory (four of 64 columns). Rounding as in lq_linear_attention.cu with the decay on v instead
 // of k (half as many values); here q reads the state as one piece of the type, the same half step as the decayed q k^T has.
@@ -78,7 +78,7 @@ struct Ring {
     if (++s == STAGES) s = 0, lap ^= 1u;
   }
 };
-// The warps of a group decide together (the state's: barrier 2 of 256 threads, those of v': 1 of 128): none leaves while another waits there
+// The warps of a group decide together (the state's: barrier 2 of 256 threads, those of v': 1 and 3 of 128): none leaves while another waits there
 template <int ID, int THREADS>
 __device__ __forceinline__ bool group_and(bool ok) {
   uint32_t r;
@@ -277,7 +277,7 @@ __global__ void __launch_bounds__(32 * WARPS, 1) linear_attention_tc_kernel(cons
     if (elected()) umma_commit(bar(S::LAST, 0));  // every product that was issued
     __syncwarp();
     ok &= warp_wait(bar(S::LAST, 0), 0);
-  } else if (warp < 8) {
+  } else if (!STATES && warp < 8) {
     if constexpr (!STATES) {
       const int set = warp >> 2, quad = warp & 3, r0 = 16 * quad, g = lane >> 2, t4 = lane & 3;
       const uint32_t lanes = (uint32_t)(32 * quad) << 16;  // M = 64: sixteen rows in each quarter of the lanes
@@ -434,7 +434,7 @@ __global__ void __launch_bounds__(32 * WARPS, 1) linear_attention_tc_kernel(cons
         if (col < cols) out[(size_t)(from + k / VT) * pitch + col] = from_f32<T>(0.f);
       }
     }
-  } else if (warp < 16) {
+  } else if (warp >= 8 && warp < 16) {
     if (lane == 0) mbar_arrive(bar(S::VR, 0)), mbar_arrive(bar(S::VR, 1));  // nothing to be read before the first two chunks
     constexpr int OWN = VT / 2;  // columns of a thread
     const int id = tid - 256, quad = warp & 3, half = (warp >> 2) & 1, d = 32 * quad + lane;  // half a row of the state
@@ -520,9 +520,10 @@ __global__ void __launch_bounds__(32 * WARPS, 1) linear_attention_tc_kernel(cons
           if (j < cols) to[j] = st[j];
       }
     }
-  } else {
-    const int id = tid - 512, row = id >> 1, half = id & 1;  // half a token a thread
-    for (int c = 0; c < chunks; ++c) {
+  } else if (warp >= 16 || warp < 4) {
+    const bool second = warp < 4;  // of segments' states alone: two sets, which take chunks in turn
+    const int id = tid & 127, row = id >> 1, half = id & 1;  // half a token a thread
+    for (int c = second; c < chunks; c += STATES ? 2 : 1) {
       const int i = c & 1, rows = min(C, stop - first - c * C);
       const uint32_t s_k = stage(c) + QK, s_v = stage(c) + 2 * QK, to = s0 + S::VO + i * S::NV * TILE;
       ok = stage_wait(c) && (c < 2 || warp_wait(bar(S::DS, i), (uint32_t)(((c >> 1) + 1) & 1)));  // the product that read this buffer is done
@@ -539,7 +540,8 @@ __global__ void __launch_bounds__(32 * WARPS, 1) linear_attention_tc_kernel(cons
 #pragma unroll
           for (int e = 0; e < 4; ++e) top = __hmax2(top, __habs2(*reinterpret_cast<__half2*>(&x[e])));
         }
-        const float big = group_max<1, 128>(fminf(fmaxf(__low2float(top), __high2float(top)), 65504.f) * f, s0 + S::RED + 16 * i, ok);
+        const float mine = fminf(fmaxf(__low2float(top), __high2float(top)), 65504.f) * f;
+        const float big = STATES && second ? group_max<3, 128>(mine, s0 + S::RED + 16 * i, ok) : group_max<1, 128>(mine, s0 + S::RED + 16 * i, ok);
         if (!ok) break;
         const int e = max(min(exponent(big) - 14, 100), -100);
         f *= pow2(-e);
