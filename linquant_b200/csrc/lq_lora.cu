@@ -292,13 +292,14 @@ static int shrink(const Shrink& p, int tiles, cudaStream_t st) {
 // read for twice as many. Parts of K: up to four CTAs an SM, and no fewer than 64 of K for a warp.
 template <typename TX, typename TA>
 static int run_shrink(Shrink p, bool vec, cudaStream_t st) {
-  const int sms = sm_count(), tile = p.M <= 64 ? 1 : p.M >= 32 * sms ? 32 : 16, tiles = (p.M + tile - 1) / tile;
+  const int sms = sm_count(), tile = p.M <= 64 ? 1 : p.M >= 32 * sms ? 32 : p.M <= 4 * sms ? 8 : 16, tiles = (p.M + tile - 1) / tile;
   p.parts = 8;
   while (p.parts > 1 && ((long long)tiles * p.parts > 4ll * sms || p.K < 256 * p.parts)) p.parts /= 2;
   auto go = [&](auto v, auto nt) {
     constexpr bool VEC = decltype(v)::value;
     constexpr int NT = decltype(nt)::value;
     if (tile == 1) return shrink<TX, TA, 1, VEC, NT>(p, tiles, st);
+    if (tile == 8) return shrink<TX, TA, 8, VEC, NT>(p, tiles, st);
     if (tile == 16) return shrink<TX, TA, 16, VEC, NT>(p, tiles, st);
     return shrink<TX, TA, 32, VEC, NT>(p, tiles, st);
   };
@@ -315,14 +316,14 @@ constexpr int CHUNK = 32, CT = CHUNK / 8;  // channels at a time, in tiles of 8
 // bf16 pieces: two (three for fp32 outputs) of t and of fp16 and fp32 b, products below 16 (24) bits behind the first left out.
 // The INT8 product's kernel reads y again, adds its own sum in fp32 and rounds once more: this rounding is of the adapters' share alone.
 // Bound by the bytes of y.
-template <typename TO, typename TB, int SPAN>
-__global__ void __launch_bounds__(THREADS, sizeof(TO) == 2 ? 4 : 3) lora_expand_kernel(const Lora q, int M, int N, TO* y) {
+template <typename TO, typename TB, int SPAN, int MI>
+__global__ void __launch_bounds__(THREADS, sizeof(TO) == 2 ? (MI == 1 ? 6 : 4) : 3) lora_expand_kernel(const Lora q, int M, int N, TO* y) {
   constexpr int PT = sizeof(TO) == 4 ? 3 : 2, PB = std::is_same_v<TB, __nv_bfloat16> ? 1 : PT;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
-  const int columns = (N + WARPS * SPAN - 1) / (WARPS * SPAN), m0 = (int)(blockIdx.x / columns) * 32, n0 = ((int)(blockIdx.x % columns) * WARPS + warp) * SPAN;
+  const int columns = (N + WARPS * SPAN - 1) / (WARPS * SPAN), m0 = (int)(blockIdx.x / columns) * (16 * MI), n0 = ((int)(blockIdx.x % columns) * WARPS + warp) * SPAN;
   if (n0 >= N) return;
   constexpr int PER = 16 / sizeof(TO);  // values of 16 bytes
-  const int mine = m0 + lane < M ? q.of(m0 + lane) : -1;
+  const int mine = lane < 16 * MI && m0 + lane < M ? q.of(m0 + lane) : -1;
   const uint32_t all = __ballot_sync(0xffffffffu, mine >= 0);
   const bool wide = ((size_t)N * sizeof(TO)) % 16 == 0 && (reinterpret_cast<uintptr_t>(y) & 15u) == 0;
 
@@ -330,7 +331,7 @@ __global__ void __launch_bounds__(THREADS, sizeof(TO) == 2 ? 4 : 3) lora_expand_
   int l = 0, r0 = 0, c0 = 0;
   uint32_t rows = 0, left = 0;
   Pack<TB, 4> b[CT];
-  uint4 t[2][2];
+  uint4 t[MI][2];
   if (SPAN == 32) {  // few tokens: every adapter's rows of b on their way to L2, by its first one
     const uint32_t like = __match_any_sync(0xffffffffu, mine);
     const TB* from = reinterpret_cast<const TB*>(q.b) + ((long long)mine * N + n0) * q.R;
@@ -358,7 +359,7 @@ __global__ void __launch_bounds__(THREADS, sizeof(TO) == 2 ? 4 : 3) lora_expand_
       for (int j = 0; j < CT; ++j) b[j] = load_pack<TB, 4>(reinterpret_cast<const TB*>(q.b) + ((long long)l * N + min(n + 2 * j, N - 1)) * q.R + rb);
     }
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < MI; ++i)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int row = 16 * i + 8 * h + g;  // of tokens with another adapter what comes of it is not kept
@@ -371,19 +372,19 @@ __global__ void __launch_bounds__(THREADS, sizeof(TO) == 2 ? 4 : 3) lora_expand_
   while (true) {
     const uint32_t now = rows;
     const int at = c0;
-    float s[2][CT][4];
+    float s[MI][CT][4];
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < MI; ++i)
 #pragma unroll
       for (int j = 0; j < CT; ++j)
 #pragma unroll
         for (int e = 0; e < 4; ++e) s[i][j][e] = 0.f;
     bool same = true, end = false;  // the adapter goes on; nothing is left
     while (same) {
-      uint32_t a[2][PT][4], w[CT][PB][2];
+      uint32_t a[MI][PT][4], w[CT][PB][2];
       const bool inside = r0 + 4 * t4 < q.R;
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+      for (int i = 0; i < MI; ++i)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           if constexpr (PT == 2) {  // as the first kernel has left them
@@ -430,11 +431,11 @@ __global__ void __launch_bounds__(THREADS, sizeof(TO) == 2 ? 4 : 3) lora_expand_
 #pragma unroll
           for (int j = 0; j < CT; ++j)
 #pragma unroll
-            for (int i = 0; i < 2; ++i) mma_bf16(s[i][j], a[i][o][0], a[i][o][1], a[i][o][2], a[i][o][3], w[j][k][0], w[j][k][1]);
+            for (int i = 0; i < MI; ++i) mma_bf16(s[i][j], a[i][o][0], a[i][o][1], a[i][o][2], a[i][o][3], w[j][k][0], w[j][k][1]);
         }
     }
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < MI; ++i)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int row = 16 * i + 8 * h + g;
@@ -464,17 +465,17 @@ __global__ void __launch_bounds__(THREADS, sizeof(TO) == 2 ? 4 : 3) lora_expand_
 static int expand(const Lora& q, const lq_linear_problem* p, cudaStream_t st) {
   return with_dtype(p->out_dtype, "lora_linear", [&](auto t) {
     using TO = decltype(t);
-    const long long rows = ((long long)p->M + 31) / 32;
     return with_dtype(q.dtype, "lora_linear", [&](auto tb) {
       using TB = decltype(tb);
       // few tokens: warps of 32 channels, as many as there can be, each of which goes over all adapters of its tokens one after the other
-      auto go = [&](auto kern, int span) {
+      auto go = [&](auto kern, int span, int tokens) {
+        const long long rows = ((long long)p->M + tokens - 1) / tokens;
         const long long ctas = rows * ((p->N + WARPS * span - 1) / (WARPS * span));
         if (ctas >= 1ll << 31) return fail(LQ_ERR_SHAPE, "lora_linear: M=%d N=%d", p->M, p->N);
         const cudaError_t e = launch(kern, dim3((unsigned)ctas), dim3(THREADS), 0, st, q, p->M, p->N, reinterpret_cast<TO*>(p->y));
         return e != cudaSuccess ? fail(LQ_ERR_LAUNCH, "lora_linear: %s", cudaGetErrorString(e)) : check_launch("lora_expand_kernel");
       };
-      return rows * ((p->N + 127) / 128) <= 10ll * sm_count() ? go(lora_expand_kernel<TO, TB, 32>, 32) : go(lora_expand_kernel<TO, TB, 128>, 128);
+      return ((long long)p->M + 31) / 32 * ((p->N + 127) / 128) <= 10ll * sm_count() ? go(lora_expand_kernel<TO, TB, 32, 1>, 32, 16) : go(lora_expand_kernel<TO, TB, 128, 2>, 128, 32);
     });
   });
 }
