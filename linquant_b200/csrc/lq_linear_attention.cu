@@ -139,6 +139,26 @@ __global__ void __launch_bounds__(sizeof(T) == 4 && KP <= 128 ? 256 : 128, sizeo
   constexpr bool F16 = S::F16;
   constexpr int NP = S::NP, MT = S::MT, NT = S::NT, KS = KP / 16, CS = C / 16;
   constexpr int SIDE = 2;  // pairs of sums side by side: a sum's products wait for one another
+  // fp32 operands: the six products of a step sum by themselves and join the others by an addition that rounds. The tensor core cuts
+  // its sums off, always towards zero: over the 72 products of an output or those of all tokens of a state that adds up to 1e-6.
+  constexpr bool APART = NP == 3;
+  float own[APART ? SIDE : 1][2][4];
+  auto sum = [&](float (&all)[4], int u, int half) -> float(&)[4] {
+    if constexpr (APART) return own[u][half];
+    else return all;
+  };
+  auto start = [&]() {
+    if constexpr (APART)
+#pragma unroll
+      for (int u = 0; u < SIDE; ++u)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) own[u][e >> 2][e & 3] = 0.f;
+  };
+  auto join = [&](float (&all)[4], int u, int half) {
+    if constexpr (APART)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) all[e] += own[u][half][e];
+  };
   extern __shared__ __align__(128) uint8_t smem_dyn[];
   const uint32_t s0 = smem_u32(smem_dyn), s_state = s0 + S::ST, s_red = s0 + S::RED;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
@@ -289,6 +309,7 @@ __global__ void __launch_bounds__(sizeof(T) == 4 && KP <= 128 ? 256 : 128, sizeo
 #pragma unroll
         for (int j = 0; j < CS; j += SIDE) {
           if (j > mt) break;
+          start();
 #pragma unroll
           for (int i = NP - 1; i >= 0; --i) {
             uint32_t kb[SIDE][4];
@@ -299,10 +320,12 @@ __global__ void __launch_bounds__(sizeof(T) == 4 && KP <= 128 ? 256 : 128, sizeo
 #pragma unroll
               for (int u = 0; u < SIDE; ++u) {
                 if (j + u > mt) break;
-                mma<M>(a[2 * (j + u)], qa[o], kb[u][0], kb[u][1]);
-                mma<M>(a[2 * (j + u) + 1], qa[o], kb[u][2], kb[u][3]);
+                mma<M>(sum(a[2 * (j + u)], u, 0), qa[o], kb[u][0], kb[u][1]);
+                mma<M>(sum(a[2 * (j + u) + 1], u, 1), qa[o], kb[u][2], kb[u][3]);
               }
           }
+#pragma unroll
+          for (int u = 0; u < SIDE; ++u) join(a[2 * (j + u)], u, 0), join(a[2 * (j + u) + 1], u, 1);
         }
       }
       decay_products<C>(a, s_g, r0, 2 * mt + 2);
@@ -333,7 +356,8 @@ __global__ void __launch_bounds__(sizeof(T) == 4 && KP <= 128 ? 256 : 128, sizeo
 #pragma unroll
         for (int i = 0; i < NP; ++i) ldsm4(qa[i], s_q + i * S::QK + at<KP * 2>(arow, 2 * ks + apiece));
 #pragma unroll
-        for (int j = 0; j < NV; j += 2 * SV)
+        for (int j = 0; j < NV; j += 2 * SV) {
+          start();
 #pragma unroll
           for (int i = S::NS - 1; i >= 0; --i) {
             uint32_t sb[SV][4];
@@ -344,11 +368,14 @@ __global__ void __launch_bounds__(sizeof(T) == 4 && KP <= 128 ? 256 : 128, sizeo
               if (w + i >= S::NS) continue;
 #pragma unroll
               for (int u = 0; u < SV; ++u) {
-                mma<M>(o[j + 2 * u], qa[w], sb[u][0], sb[u][1]);
-                mma<M>(o[j + 2 * u + 1], qa[w], sb[u][2], sb[u][3]);
+                mma<M>(sum(o[j + 2 * u], u, 0), qa[w], sb[u][0], sb[u][1]);
+                mma<M>(sum(o[j + 2 * u + 1], u, 1), qa[w], sb[u][2], sb[u][3]);
               }
             }
           }
+#pragma unroll
+          for (int u = 0; u < SV; ++u) join(o[j + 2 * u], u, 0), join(o[j + 2 * u + 1], u, 1);
+        }
       }
       const float f0 = ex2(lds_f32(s_g + 4 * (r0 + g))) * (F16 ? pow2(exp_c) : 1.f) * up0;
       const float f1 = ex2(lds_f32(s_g + 4 * (r0 + g + 8))) * (F16 ? pow2(exp_c) : 1.f) * up1;
@@ -359,7 +386,8 @@ __global__ void __launch_bounds__(sizeof(T) == 4 && KP <= 128 ? 256 : 128, sizeo
       for (int ks = 0; ks < CS; ++ks) {
         if (ks > mt) break;
 #pragma unroll
-        for (int j = 0; j < NV; j += 2 * SV)
+        for (int j = 0; j < NV; j += 2 * SV) {
+          start();
 #pragma unroll
           for (int i = NP - 1; i >= 0; --i) {
             uint32_t vb[SV][4];
@@ -369,10 +397,13 @@ __global__ void __launch_bounds__(sizeof(T) == 4 && KP <= 128 ? 256 : 128, sizeo
             for (int w = S::NA - 1 - i; w >= 0; --w)
 #pragma unroll
               for (int u = 0; u < SV; ++u) {
-                mma<M>(o[j + 2 * u], pa[w][ks], vb[u][0], vb[u][1]);
-                mma<M>(o[j + 2 * u + 1], pa[w][ks], vb[u][2], vb[u][3]);
+                mma<M>(sum(o[j + 2 * u], u, 0), pa[w][ks], vb[u][0], vb[u][1]);
+                mma<M>(sum(o[j + 2 * u + 1], u, 1), pa[w][ks], vb[u][2], vb[u][3]);
               }
           }
+#pragma unroll
+          for (int u = 0; u < SV; ++u) join(o[j + 2 * u], u, 0), join(o[j + 2 * u + 1], u, 1);
+        }
       }
       const float c0 = F16 ? p.scale / up0 : p.scale, c1 = F16 ? p.scale / up1 : p.scale;
       const bool in0 = t0 + r0 + g < stop, in1 = t0 + r0 + g + 8 < stop;
@@ -483,7 +514,8 @@ __global__ void __launch_bounds__(sizeof(T) == 4 && KP <= 128 ? 256 : 128, sizeo
             for (int i = 0; i < S::NK; ++i) kp[i][e] = pieces[i];
           }
 #pragma unroll
-          for (int j = 0; j < NT; j += 2 * SIDE)
+          for (int j = 0; j < NT; j += 2 * SIDE) {
+            start();
 #pragma unroll
             for (int i = NP - 1; i >= 0; --i) {
               uint32_t vb[SIDE][4];
@@ -493,10 +525,13 @@ __global__ void __launch_bounds__(sizeof(T) == 4 && KP <= 128 ? 256 : 128, sizeo
               for (int w = S::NK - 1 - i; w >= 0; --w)
 #pragma unroll
                 for (int u = 0; u < SIDE; ++u) {
-                  mma<M>(st[m][j + 2 * u], kp[w], vb[u][0], vb[u][1]);
-                  mma<M>(st[m][j + 2 * u + 1], kp[w], vb[u][2], vb[u][3]);
+                  mma<M>(sum(st[m][j + 2 * u], u, 0), kp[w], vb[u][0], vb[u][1]);
+                  mma<M>(sum(st[m][j + 2 * u + 1], u, 1), kp[w], vb[u][2], vb[u][3]);
                 }
             }
+#pragma unroll
+            for (int u = 0; u < SIDE; ++u) join(st[m][j + 2 * u], u, 0), join(st[m][j + 2 * u + 1], u, 1);
+          }
         }
       }
     }
