@@ -688,15 +688,17 @@ static int check(const lq_attention_problem* p, const char* what) {
   return LQ_OK;
 }
 
-// Segments: enough CTAs for every place on the GPU (two an SM, one of fp32 operands or for the tcgen05 kernel). None is shorter than eight
-// chunks, or two of fp32 operands, whose chunks take ten times as long
+// Segments: enough CTAs for every place on the GPU (two an SM, one of fp32 operands or for the tcgen05 kernel). None is shorter than four
+// chunks, two of fp32 operands, whose chunks take ten times as long, and calls of fewer than twelve stay whole. 16 heads of 128 x 128, bf16: 512
+// tokens whole 12.4 us, in two 14.7; 1024 whole 21.3, in four 17.3; 4 heads, 2048: in four 22.4, in eight 16.3. fp32, 6 heads of
+// 72 x 100, 611 tokens: whole 155, in two 113
 static Plan plan(const lq_attention_problem* p) {
   Plan r;
   r.tc = tc_applies(p);
   const int kp = p->K <= 64 && !r.tc ? 64 : p->K <= 128 ? 128 : 256, vt = kp == 256 ? 32 : 64;
   r.floats = kp * vt;
   r.tiles = (long long)p->B * p->H * ((p->V + vt - 1) / vt);
-  const long long chunks = ((long long)p->T + 63) / 64, room = (r.tc || p->dtype == LQ_F32 ? 1ll : 2ll) * sm_count(), least = p->dtype == LQ_F32 ? 2 : 8;
+  const long long chunks = ((long long)p->T + 63) / 64, room = (r.tc || p->dtype == LQ_F32 ? 1ll : 2ll) * sm_count(), least = p->dtype == LQ_F32 ? 2 : chunks < 12 ? 12 : 4;
   long long count = r.tiles > 0 ? room / r.tiles : 1;
   count = count > chunks / least ? chunks / least : count;
   count = count < 1 ? 1 : count;
@@ -789,8 +791,9 @@ extern "C" int lq_linear_attention_step(const lq_attention_problem* p, lq_stream
         return e != cudaSuccess ? fail(LQ_ERR_LAUNCH, "linear_attention_step: %s", cudaGetErrorString(e)) : check_launch("linear_attention_step_kernel");
       };
       if (bytes == 16) {
-        // few heads: narrow columns, so that more SMs share the states
-        if ((long long)p->B * p->H * ((p->V + 32 * FULL - 1) / (32 * FULL)) < 2ll * sm_count()) return go(linear_attention_step_kernel<T, TS, FULL, 8>, 8 * FULL);
+        // Few heads: narrow columns, so that more SMs share the states, as long as a round of CTAs takes them (16 heads of 128 x 128, fp32:
+        // one sequence 2.1 us, 3.4 with wide ones; 6 sequences 3.1 and 3.6; 8 sequences 4.5 and 3.7)
+        if (4ll * p->B * p->H * ((p->V + 32 * FULL - 1) / (32 * FULL)) <= 3ll * sm_count()) return go(linear_attention_step_kernel<T, TS, FULL, 8>, 8 * FULL);
         return go(linear_attention_step_kernel<T, TS, FULL, 32>, 32 * FULL);
       }
       return go(linear_attention_step_kernel<T, TS, 1, 32>, 32);

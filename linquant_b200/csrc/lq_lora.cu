@@ -6,7 +6,7 @@
 // fp32 (lq_lora.cuh). For more this file's second kernel leaves it in y and the product's kernels add it from there: what runs beside the
 // tcgen05 product on an SM's tensor cores waits for them (warp products in its epilogue: 510 us where the product alone takes 302, at
 // 16384 x 2560 -> 10576 with rank 16; fp32 products there: 680).
-// t: a CTA has a tile of 1, 16 or 32 tokens and, of a cluster, a part of K; its four warps share that part and their sums meet in
+// t: a CTA has a tile of 1, 8 or 16 tokens and, of a cluster, a part of K; its four warps share that part and their sums meet in
 // shared memory, first the warps', then the CTAs', in a fixed order. Operands come from global memory straight into the fragments
 // of m16n8k16 (the reduction index permuted alike in both: a lane takes eight consecutive k). A tile whose tokens have several
 // adapters goes over its K once for each of them. Products are exact: both operands as bf16 pieces (codes and bf16 one, fp16 two, fp32
@@ -288,11 +288,13 @@ static int shrink(const Shrink& p, int tiles, cudaStream_t st) {
   return check_launch("lora_shrink_kernel");
 }
 
-// Tokens of a CTA: one each for a decode step, whose tokens have adapters of their own; 32 where that leaves a CTA an SM, so that a's rows are
-// read for twice as many. Parts of K: up to four CTAs an SM, and no fewer than 64 of K for a warp.
+// Tokens of a CTA: one for few tokens, each of which may have an adapter of its own, as long as a's rows, read once for each, are few (100 x 2560
+// of as many adapters, rank 16: 22 us where eight take 30; 256 x 5120 in runs of 7, rank 32: 36 and 27); eight up to four tokens an SM, whose
+// tiles have fewer adapters to go through (333 tokens in runs of 7, rank 32: 34 us, 37 with sixteen); then sixteen (4000 tokens in runs of
+// 500: 46 us, 49 with eight; 32 were no better). Parts of K: up to four CTAs an SM, and no fewer than 64 of K for a warp.
 template <typename TX, typename TA>
 static int run_shrink(Shrink p, bool vec, cudaStream_t st) {
-  const int sms = sm_count(), tile = p.M <= 64 ? 1 : p.M >= 32 * sms ? 32 : p.M <= 4 * sms ? 8 : 16, tiles = (p.M + tile - 1) / tile;
+  const int sms = sm_count(), tile = (long long)p.M * p.R <= 4096 ? 1 : p.M <= 4 * sms ? 8 : 16, tiles = (p.M + tile - 1) / tile;
   p.parts = 8;
   while (p.parts > 1 && ((long long)tiles * p.parts > 4ll * sms || p.K < 256 * p.parts)) p.parts /= 2;
   auto go = [&](auto v, auto nt) {
@@ -300,8 +302,7 @@ static int run_shrink(Shrink p, bool vec, cudaStream_t st) {
     constexpr int NT = decltype(nt)::value;
     if (tile == 1) return shrink<TX, TA, 1, VEC, NT>(p, tiles, st);
     if (tile == 8) return shrink<TX, TA, 8, VEC, NT>(p, tiles, st);
-    if (tile == 16) return shrink<TX, TA, 16, VEC, NT>(p, tiles, st);
-    return shrink<TX, TA, 32, VEC, NT>(p, tiles, st);
+    return shrink<TX, TA, 16, VEC, NT>(p, tiles, st);
   };
   auto width = [&](auto v) { return p.R <= 16 ? go(v, std::integral_constant<int, 2>()) : p.R <= 32 ? go(v, std::integral_constant<int, 4>()) : go(v, std::integral_constant<int, 8>()); };
   return vec ? width(std::true_type()) : width(std::false_type());
@@ -310,12 +311,12 @@ static int run_shrink(Shrink p, bool vec, cudaStream_t st) {
 // ---- the second product: y[m,n] = sum_r t[m,r] b[l,n,r] for the tokens that have an adapter
 constexpr int CHUNK = 32, CT = CHUNK / 8;  // channels at a time, in tiles of 8
 
-// A warp: 32 tokens, SPAN channels. Over the adapters that the tokens have and their ranks in steps of 16; a step's operands are requested before
+// A warp: 16 MI tokens, SPAN channels. Over the adapters that the tokens have and their ranks in steps of 16; a step's operands are requested before
 // the products of the one ahead. The reduction index is permuted alike in both operands: a lane takes four consecutive r; and the channels of
 // a chunk, column 2 i + e of tile j being channel 8 i + 2 j + e, so that a lane holds eight consecutive ones of a row. Both operands are
 // bf16 pieces: two (three for fp32 outputs) of t and of fp16 and fp32 b, products below 16 (24) bits behind the first left out.
 // The INT8 product's kernel reads y again, adds its own sum in fp32 and rounds once more: this rounding is of the adapters' share alone.
-// Bound by the bytes of y.
+// Many tokens: bound by y's bytes (16384 x 10576, rank 16: 90 us, 3.9 TB/s, with a third of the issue slots). Few: by L2's latency.
 template <typename TO, typename TB, int SPAN, int MI>
 __global__ void __launch_bounds__(THREADS, sizeof(TO) == 2 ? (MI == 1 ? 6 : 4) : 3) lora_expand_kernel(const Lora q, int M, int N, TO* y) {
   constexpr int PT = sizeof(TO) == 4 ? 3 : 2, PB = std::is_same_v<TB, __nv_bfloat16> ? 1 : PT;
@@ -467,7 +468,9 @@ static int expand(const Lora& q, const lq_linear_problem* p, cudaStream_t st) {
     using TO = decltype(t);
     return with_dtype(q.dtype, "lora_linear", [&](auto tb) {
       using TB = decltype(tb);
-      // few tokens: warps of 32 channels, as many as there can be, each of which goes over all adapters of its tokens one after the other
+      // Few tokens: warps of 16 of them and 32 channels, as many as there can be, each of which goes over all adapters of its tokens one after
+      // the other (333 x 10576, rank 32, runs of 7: 34 us where the others' warps of 32 and 128 take 53; 1000 x 2560 25 and 27). Many: these
+      // read b half as often (1000 x 10576, rank 16: 45 us and 49, 16384 tokens 475 and 559)
       auto go = [&](auto kern, int span, int tokens) {
         const long long rows = ((long long)p->M + tokens - 1) / tokens;
         const long long ctas = rows * ((p->N + WARPS * span - 1) / (WARPS * span));
