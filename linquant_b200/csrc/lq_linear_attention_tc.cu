@@ -16,6 +16,9 @@
 // of k (half as many values); here q reads the state as one piece of the type, the same half step as the decayed q k^T has.
 // fp16: rows of P, v' of a chunk and the state q reads each under a power of two of their largest value.
 // Behind a sequence's last token k and v are made zero in shared memory: a NaN there times a weight of zero would be one.
+// 4 x 4096 x 16 heads of 128 x 128, bf16, slices of a projection: 91 us. Bound by the steps a chunk
+// takes from q k^T by way of P to the outputs, two sets in turn: tensor pipe 47 % busy, issue slots 55 %, HBM 34 %. One prompt of 32768, 8 heads,
+// fp16: 150 us, of which 52 the first pass over its segments.
 // Every wait is bounded; on expiry the CTA raises the status word, lets its copies and products land, frees its tensor memory
 // and returns.
 #include <math_constants.h>

@@ -11,6 +11,10 @@
 // of m16n8k16 (the reduction index permuted alike in both: a lane takes eight consecutive k). A tile whose tokens have several
 // adapters goes over its K once for each of them. Products are exact: both operands as bf16 pieces (codes and bf16 one, fp16 two, fp32
 // three; codes or fp16 with fp16 as they are), six products for fp32.
+// Both kernels let their successors start at once (pdl_trigger()): the product's loads and sums run beside them, and wait for t or the share where
+// it is added. 3 tokens, 5120 -> 2560, rank 16: 11.4 us in a row, 15.6 without, 9.3 the product alone.
+// t of 333 x 2560 codes, rank 32, 24 adapters in runs of 7: 11 us, bound by latency, a tile's adapters one after the other; of 16384 x 2560, rank 16:
+// 22 us (42 MB of codes from HBM or L2, half of the issue slots).
 #include "lq_lora.cuh"
 #include "lq_tc.cuh"
 
