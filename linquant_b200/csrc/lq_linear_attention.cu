@@ -12,8 +12,7 @@
 // Rounding. G is summed and kept as two floats, so that differences of large sums are exact; decays are 2^x of fp32
 // differences. Products of 16-bit values are exact and their sums fp32. The decayed keys of the state's product are fp32 and go in
 // as three bf16 pieces (all 24 bits; fp16: two pieces under a power of two of the chunk's largest key, 22 bits), the state that q
-// reads as two pieces (16 or 22 bits), the decayed products q.k as one piece of the operands' type: their rounding, half a
-// step of the type on each term, is of the size of the output's own. fp32 operands are three bf16 pieces each, six products.
+// reads and the decayed products q.k as two pieces (16 or 22 bits). fp32 operands are three bf16 pieces each, six products.
 //
 // 16-bit prompts whose rows TMA takes run in lq_linear_attention_tc.cu (4 x 4096 x 16 heads of 128 x 128, bf16: 91 us, 334 here). What is left
 // is bound by warp MMA's own latencies: 5 x 611 x 6 heads of 72 x 100, fp32, 87 us with the call, tensor pipe 29 % busy, HBM 1 %.
@@ -55,7 +54,7 @@ struct Shape {
   using M = typename Half<T>::type;
   static constexpr bool F16 = std::is_same_v<T, __half>;
   static constexpr int NP = sizeof(T) == 4 ? 3 : 1;        // pieces of q, k, v
-  static constexpr int NK = F16 ? 2 : 3, NS = sizeof(T) == 4 ? 3 : 2, NA = NP;  // pieces of decayed keys, of the state, of decayed q.k
+  static constexpr int NK = F16 ? 2 : 3, NS = sizeof(T) == 4 ? 3 : 2, NA = NS;  // pieces of decayed keys, of the state, of decayed q.k
   static constexpr int BUFS = NP == 1 ? 2 : 1;
   static constexpr int QK = C * KP * 2, VB = C * VT * 2, SB = KP * VT * 2;
   static constexpr int TILES = NP * (2 * QK + VB);         // a buffer: q, k, v

@@ -13,7 +13,8 @@
 //   warps 16..19  v' = exp(G_C - G_j) v in pieces (where only segments' states are made, warps 0..3 take every other chunk)
 //
 // All accumulators lie twice in tensor memory (four of 64 columns). Rounding as in lq_linear_attention.cu with the decay on v instead
-// of k (half as many values); here q reads the state as one piece of the type, the same half step as the decayed q k^T has.
+// of k (half as many values); here q reads the state, and v the decayed q k^T, as one piece of the type: half a step of the type on each
+// term, of the size of the output's own rounding.
 // fp16: rows of P, v' of a chunk and the state q reads each under a power of two of their largest value.
 // Behind a sequence's last token k and v are made zero in shared memory: a NaN there times a weight of zero would be one.
 // 4 x 4096 x 16 heads of 128 x 128, bf16, slices of a projection: 91 us. Bound by the steps a chunk
@@ -630,9 +631,10 @@ static int run(const lq_attention_problem* p, const Plan& r, const Segments& seg
 
 namespace attention {
 
-// 16-bit operands whose rows TMA can fetch: every start on a 16-byte boundary, strides that move forwards
+// 16-bit operands whose rows TMA can fetch: every start on a 16-byte boundary, strides that move forwards. More than one chunk of tokens: a
+// single one has nothing to overlap, and its outputs, sums of a few terms each rounded once more, would show it
 bool tc_applies(const lq_attention_problem* p) {
-  if (p->dtype == LQ_F32 || p->K > 128 || p->T < 1) return false;
+  if (p->dtype == LQ_F32 || p->K > 128 || p->T <= attentiontc::C) return false;
   auto rows = [&](const void* base, int heads, long long st, long long sh, long long sb) {
     auto fits = [](int extent, long long stride) { return extent <= 1 || (stride > 0 && stride % 8 == 0 && stride < (1ll << 38)); };
     return (reinterpret_cast<uintptr_t>(base) & 15u) == 0 && fits(p->T, st) && fits(heads, sh) && fits(p->B, sb);
