@@ -230,7 +230,7 @@ __global__ void __launch_bounds__(THREADS) lora_shrink_kernel(const Shrink p) {
     for (int w = 1; w < WARPS; ++w) s += sums[w * values + i];
     sums[i] = s;
   }
-  if (p.parts > 1) asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+  if (p.parts > 1) cluster_sync();
   else __syncthreads();
   const uint32_t base = smem_u32(sums);
   for (int i = 4 * (rank * THREADS + tid); i < values; i += 4 * p.parts * THREADS) {  // four of a row
@@ -263,7 +263,7 @@ __global__ void __launch_bounds__(THREADS) lora_shrink_kernel(const Shrink p) {
     }
     *reinterpret_cast<uint4*>(p.t + (long long)m * p.RP + i - row * p.RP) = w;
   }
-  if (p.parts > 1) asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");  // no CTA's sums are read any more
+  if (p.parts > 1) cluster_sync();  // no CTA's sums are read any more
 }
 
 template <typename TX, typename TA, int TILE, bool VEC, int NT>

@@ -18,6 +18,12 @@ __device__ __forceinline__ bool mbar_wait_bounded(uint32_t bar, uint32_t parity)
   }
   return false;
 }
+// All threads of a cluster; what they wrote before is visible to all behind it. Both instructions want whole warps at once, and lanes that
+// come from loops of different lengths are not together by themselves.
+__device__ __forceinline__ void cluster_sync() {
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+}
 // shared-memory accesses by 32-bit shared address (no generic-address arithmetic)
 __device__ __forceinline__ uint32_t lds_u32(uint32_t addr) {
   uint32_t v;
