@@ -86,6 +86,7 @@ struct Ring {
 template <int ID, int THREADS>
 __device__ __forceinline__ bool group_and(bool ok) {
   uint32_t r;
+  __syncwarp();  // bar.red is for whole warps at once
   asm volatile("{\n.reg .pred p, q;\nsetp.ne.b32 q, %1, 0;\nbar.red.and.pred p, %2, %3, q;\nselp.u32 %0, 1, 0, p;\n}\n" : "=r"(r) : "r"((uint32_t)ok), "n"(ID), "n"(THREADS) : "memory");
   return r != 0;
 }

@@ -19,3 +19,10 @@ def test_cluster_barriers(name):
     for m in re.finditer(r"barrier\.cluster\.arrive", text):
         before = text[:m.start()].rstrip().removesuffix('asm volatile("').rstrip()
         assert before.endswith("__syncwarp();"), f"{name}: line {text[:m.start()].count(chr(10)) + 1}"
+
+
+def test_decisions_of_a_group_of_warps():
+    """Linear attention: one lane of each warp has just stored its warp's largest value."""
+    text = open(os.path.join(build.CSRC, "lq_linear_attention_tc.cu")).read()
+    assert text.count("bar.red.") == 1
+    assert "__syncwarp();" in text[text.index("bool group_and(bool ok)"):text.index("bar.red.")]
