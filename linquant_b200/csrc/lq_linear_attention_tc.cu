@@ -36,7 +36,7 @@ constexpr int C = 64, VT = 64, WARPS = 24, DECAYS = 20, ISSUER = 22, LOADER = 23
 constexpr int TILE = C * 128, QK = 2 * TILE, STAGE = 2 * QK + TILE, STAGES = 3, SB = 128 * 128, GS = 8;  // bytes; GS: chunks whose decays are kept
 // Decays of a chunk: Decay<C>'s, then for the row blocks of 16 tokens q = 1..3 those from each token before the block to its start.
 // Below the block an element's decay is that times the row's own from the start on: no exponential of its own.
-constexpr int GROWTH = 12 * C + 4, BELOW = Decay<C>::BYTES, GB = BELOW + 96 * 4;  // GROWTH: the sum of what is above zero
+constexpr int BELOW = Decay<C>::BYTES, GB = BELOW + 96 * 4;
 
 template <typename T>
 struct Shape {
@@ -182,13 +182,6 @@ __global__ void __launch_bounds__(32 * WARPS, 1) linear_attention_tc_kernel(cons
     for (int c = turn; c < chunks; c += 2) {
       Decay<C> d;
       total = total + d.of(x[0]);
-      float growth = 0.f;
-      if constexpr (F16) {
-#pragma unroll
-        for (int k = 0; k < C / 32; ++k) growth += fmaxf(x[0][k], 0.f) * kLog2e;
-#pragma unroll
-        for (int m = 16; m; m >>= 1) growth += __shfl_xor_sync(0xffffffffu, growth, m);
-      }
 #pragma unroll
       for (int k = 0; k < C / 32; ++k) x[0][k] = x[1][k];
       load_decay<C>(x[1], p, b, h, (int)min((long long)first + (c + 4ll) * C, (long long)stop), stop);
@@ -201,7 +194,6 @@ __global__ void __launch_bounds__(32 * WARPS, 1) linear_attention_tc_kernel(cons
       }
       // The stage is empty: the chunk three before this one is done, and the one whose place this takes, eight before, left by all
       if (c >= STAGES && !(ok = done_wait(c - STAGES))) break;
-      if constexpr (F16) d.most = growth;
       d.store(decays(c));
 #pragma unroll
       for (int q = 1; q < 4; ++q)
@@ -300,35 +292,28 @@ __global__ void __launch_bounds__(32 * WARPS, 1) linear_attention_tc_kernel(cons
         // Loops over blocks of 16 columns are not unrolled: five roles' code passes through the instruction cache every chunk
         const uint32_t t_s1 = tbase + lanes + T_S1 + 64 * set, p0 = s_p + (r0 + g) * 128 + 4 * t4, sw = (uint32_t)(g << 4);  // rows g and g + 8 are swizzled alike
         const float hi0 = lds_f32(s_g + 4 * (r0 + g)), hi1 = lds_f32(s_g + 4 * (r0 + g + 8)), lo0 = lds_f32(s_g + 4 * (C + r0 + g)), lo1 = lds_f32(s_g + 4 * (C + r0 + g + 8));
-        // bf16: the scale goes in here; fp16: with the outputs, the rows get a scale of their own, under the largest |q k| and, should decays grow, their growth
-        float own0 = F16 ? 1.f : p.scale, own1 = own0;
+        const uint32_t at = s_g + 4 * max(r0 - 1, 0), below = s_g + BELOW + 4 * (8 * quad * (quad - 1) + 2 * t4);
+        const float hi = lds_f32(at), lo = lds_f32(at + 4 * C);
+        float from0 = ex2((hi0 - hi) + (lo0 - lo)), from1 = ex2((hi1 - hi) + (lo1 - lo));  // from the start of their block
+        // the block on the diagonal: nothing above it, not even zero times what is there
+        auto diagonal = [&](float (&x)[8], float own0, float own1) {
+          uint32_t r[8];
+          tmem_ld_16x256b_x2(t_s1 + r0, r);
+          tmem_wait();
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int col = 8 * e + 2 * t4;
+            const float2 h = lds_f2(s_g + 4 * (r0 + col)), l = lds_f2(s_g + 4 * (C + r0 + col));
+            x[4 * e] = col <= g ? __uint_as_float(r[4 * e]) * (ex2((hi0 - h.x) + (lo0 - l.x)) * own0) : 0.f;
+            x[4 * e + 1] = col + 1 <= g ? __uint_as_float(r[4 * e + 1]) * (ex2((hi0 - h.y) + (lo0 - l.y)) * own0) : 0.f;
+            x[4 * e + 2] = col <= g + 8 ? __uint_as_float(r[4 * e + 2]) * (ex2((hi1 - h.x) + (lo1 - l.x)) * own1) : 0.f;
+            x[4 * e + 3] = col + 1 <= g + 8 ? __uint_as_float(r[4 * e + 3]) * (ex2((hi1 - h.y) + (lo1 - l.y)) * own1) : 0.f;
+          }
+        };
+        // bf16: the scale goes in here; fp16: with the outputs, a row goes under a power of two of its largest decayed product
+        float up0 = 1.f, up1 = 1.f, d[8];
         if constexpr (F16) {
           float top0 = 0.f, top1 = 0.f;
-#pragma unroll 1
-          for (int jj = 0; jj <= quad; ++jj) {
-            uint32_t r[8];
-            tmem_ld_16x256b_x2(t_s1 + 16 * jj, r);
-            tmem_wait();
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              const int over = jj < quad ? -16 : 8 * (e >> 2) + 2 * t4 + (e & 1) - g;  // columns behind row g
-              if (e & 2) top1 = over <= 8 ? fmaxf(top1, fabsf(__uint_as_float(r[e]))) : top1;
-              else top0 = over <= 0 ? fmaxf(top0, fabsf(__uint_as_float(r[e]))) : top0;
-            }
-          }
-#pragma unroll
-          for (int m = 1; m < 4; m <<= 1) {
-            top0 = fmaxf(top0, __shfl_xor_sync(0xffffffffu, top0, m));
-            top1 = fmaxf(top1, __shfl_xor_sync(0xffffffffu, top1, m));
-          }
-          const int grow = 14 - (int)fminf(ceilf(lds_f32(s_g + GROWTH)), 250.f);
-          own0 = pow2(min(grow - exponent(top0), 40)), own1 = pow2(min(grow - exponent(top1), 40));
-        }
-        const float up0 = own0, up1 = own1;
-        {
-          const uint32_t at = s_g + 4 * max(r0 - 1, 0), below = s_g + BELOW + 4 * (8 * quad * (quad - 1) + 2 * t4);
-          const float hi = lds_f32(at), lo = lds_f32(at + 4 * C);
-          const float from0 = ex2((hi0 - hi) + (lo0 - lo)) * own0, from1 = ex2((hi1 - hi) + (lo1 - lo)) * own1;  // from the start of their block
 #pragma unroll 1
           for (int jj = 0; jj < quad; ++jj) {
             uint32_t r[8];
@@ -337,37 +322,57 @@ __global__ void __launch_bounds__(32 * WARPS, 1) linear_attention_tc_kernel(cons
             tmem_wait();
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-              float x[4];
-              mul2(mul2(F2(__uint_as_float(r[4 * e]), __uint_as_float(r[4 * e + 1])), F2(w[e].x, w[e].y)), F2(from0, from0)).get(x[0], x[1]);
-              mul2(mul2(F2(__uint_as_float(r[4 * e + 2]), __uint_as_float(r[4 * e + 3])), F2(w[e].x, w[e].y)), F2(from1, from1)).get(x[2], x[3]);
-              const uint32_t to = p0 + ((uint32_t)((2 * jj + e) << 4) ^ sw);
-              sts_u32(to, Act<T>::pack2(x[0], x[1]));
-              sts_u32(to + 1024, Act<T>::pack2(x[2], x[3]));
+              top0 = fmaxf(top0, fmaxf(fabsf(__uint_as_float(r[4 * e])) * w[e].x, fabsf(__uint_as_float(r[4 * e + 1])) * w[e].y));
+              top1 = fmaxf(top1, fmaxf(fabsf(__uint_as_float(r[4 * e + 2])) * w[e].x, fabsf(__uint_as_float(r[4 * e + 3])) * w[e].y));
             }
           }
+          top0 *= from0, top1 *= from1;
+          diagonal(d, 1.f, 1.f);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            if (e & 2) top1 = fmaxf(top1, fabsf(d[e]));
+            else top0 = fmaxf(top0, fabsf(d[e]));
+          }
+#pragma unroll
+          for (int m = 1; m < 4; m <<= 1) {
+            top0 = fmaxf(top0, __shfl_xor_sync(0xffffffffu, top0, m));
+            top1 = fmaxf(top1, __shfl_xor_sync(0xffffffffu, top1, m));
+          }
+          up0 = pow2(min(14 - exponent(top0), 40)), up1 = pow2(min(14 - exponent(top1), 40));
+        } else {
+          from0 *= p.scale, from1 *= p.scale;
         }
-        {
+#pragma unroll 1
+        for (int jj = 0; jj < quad; ++jj) {
           uint32_t r[8];
-          tmem_ld_16x256b_x2(t_s1 + r0, r);
+          tmem_ld_16x256b_x2(t_s1 + 16 * jj, r);
+          const float2 w[2] = {lds_f2(below + 64 * jj), lds_f2(below + 64 * jj + 32)};
           tmem_wait();
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {  // the block on the diagonal: nothing above it, not even zero times what is there
-            const int col = 8 * e + 2 * t4;
-            const float2 h = lds_f2(s_g + 4 * (r0 + col)), l = lds_f2(s_g + 4 * (C + r0 + col));
-            const float x0 = col <= g ? __uint_as_float(r[4 * e]) * (ex2((hi0 - h.x) + (lo0 - l.x)) * own0) : 0.f;
-            const float x1 = col + 1 <= g ? __uint_as_float(r[4 * e + 1]) * (ex2((hi0 - h.y) + (lo0 - l.y)) * own0) : 0.f;
-            const float x2 = col <= g + 8 ? __uint_as_float(r[4 * e + 2]) * (ex2((hi1 - h.x) + (lo1 - l.x)) * own1) : 0.f;
-            const float x3 = col + 1 <= g + 8 ? __uint_as_float(r[4 * e + 3]) * (ex2((hi1 - h.y) + (lo1 - l.y)) * own1) : 0.f;
-            const uint32_t to = p0 + ((uint32_t)((2 * quad + e) << 4) ^ sw);
-            sts_u32(to, Act<T>::pack2(x0, x1));
-            sts_u32(to + 1024, Act<T>::pack2(x2, x3));
+          for (int e = 0; e < 2; ++e) {
+            float x[4];
+            F2 y0 = mul2(mul2(F2(__uint_as_float(r[4 * e]), __uint_as_float(r[4 * e + 1])), F2(w[e].x, w[e].y)), F2(from0, from0));
+            F2 y1 = mul2(mul2(F2(__uint_as_float(r[4 * e + 2]), __uint_as_float(r[4 * e + 3])), F2(w[e].x, w[e].y)), F2(from1, from1));
+            if constexpr (F16) y0 = mul2(y0, F2(up0, up0)), y1 = mul2(y1, F2(up1, up1));  // last: with a large decay ahead it might leave fp32
+            y0.get(x[0], x[1]);
+            y1.get(x[2], x[3]);
+            const uint32_t to = p0 + ((uint32_t)((2 * jj + e) << 4) ^ sw);
+            sts_u32(to, Act<T>::pack2(x[0], x[1]));
+            sts_u32(to + 1024, Act<T>::pack2(x[2], x[3]));
           }
+        }
+        if constexpr (!F16) diagonal(d, p.scale, p.scale);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const uint32_t to = p0 + ((uint32_t)((2 * quad + e) << 4) ^ sw);
+          sts_u32(to, Act<T>::pack2(d[4 * e] * up0, d[4 * e + 1] * up0));
+          sts_u32(to + 1024, Act<T>::pack2(d[4 * e + 2] * up1, d[4 * e + 3] * up1));
+        }
 #pragma unroll 1
-          for (int j = 2 * quad + 2; j < 8; ++j) {
-            const uint32_t to = p0 + ((uint32_t)(j << 4) ^ sw);
-            sts_u32(to, 0u);
-            sts_u32(to + 1024, 0u);
-          }
+        for (int j = 2 * quad + 2; j < 8; ++j) {
+          const uint32_t to = p0 + ((uint32_t)(j << 4) ^ sw);
+          sts_u32(to, 0u);
+          sts_u32(to + 1024, 0u);
         }
         proxy_fence();
         before_sync();
