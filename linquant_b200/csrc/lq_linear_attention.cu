@@ -11,7 +11,7 @@
 //
 // Rounding. G is summed and kept as two floats, so that differences of large sums are exact; decays are 2^x of fp32
 // differences. Products of 16-bit values are exact and their sums fp32. The decayed keys of the state's product are fp32 and go in
-// as three bf16 pieces (all 24 bits; fp16: two pieces under a power of two of the chunk's largest key, 22 bits), the state that q
+// as three bf16 pieces (all 24 bits; fp16: two pieces under a power of two of the largest of them, 22 bits), the state that q
 // reads and the decayed products q.k as two pieces (16 or 22 bits). fp32 operands are three bf16 pieces each, six products.
 //
 // 16-bit prompts whose rows TMA takes run in lq_linear_attention_tc.cu (4 x 4096 x 16 heads of 128 x 128, bf16: 91 us, 334 here). What is left
@@ -262,7 +262,6 @@ __global__ void __launch_bounds__(sizeof(T) == 4 && KP <= 128 ? 256 : 128, sizeo
     if (warp == 0) {
       load_decay<C>(x_next, p, b, h, first, stop);
       total = next.of(x_next);
-      if (F16) next.largest();
       next.store(s_g);
       load_decay<C>(x_next, p, b, h, first + C, stop);
     }
@@ -288,7 +287,6 @@ __global__ void __launch_bounds__(sizeof(T) == 4 && KP <= 128 ? 256 : 128, sizeo
     }
     if (warp == 0 && c + 1 < chunks) {
       total = total + next.of(x_next);
-      if (F16) next.largest();
       load_decay<C>(x_next, p, b, h, t0 + 2 * C, stop);
     }
     if constexpr (!STATES) {
@@ -465,21 +463,24 @@ __global__ void __launch_bounds__(sizeof(T) == 4 && KP <= 128 ? 256 : 128, sizeo
           for (int i = 0; i < NP; ++i) ldsm4t(ka[i][ks], s_k + i * S::QK + at<KP * 2>(16 * ks + (lane & 7) + (lane >> 4) * 8, piece));
         float down = 1.f;
         if constexpr (F16) {
-          if (m == 0) {  // a power of two above the warp's largest decayed key
-            __half2 top = __half2half2(__ushort_as_half(0));
+          if (m == 0) {  // a power of two above the warp's largest decayed key, each under its own token's decay
+            float big = 0.f;
 #pragma unroll
-            for (int mm = 0; mm < MT; ++mm)
+            for (int ks = 0; ks < CS; ++ks) {
+              const float2 w0 = lds_f2(s_g + 4 * (2 * C + 16 * ks + 2 * t4)), w1 = lds_f2(s_g + 4 * (2 * C + 16 * ks + 8 + 2 * t4));
+              __half2 top[2] = {__half2half2(__ushort_as_half(0)), __half2half2(__ushort_as_half(0))};  // of tokens 2 t4 (+ 1), and of those 8 behind them
 #pragma unroll
-              for (int ks = 0; ks < CS; ++ks) {
+              for (int mm = 0; mm < MT; ++mm) {
                 uint32_t r[4];
                 ldsm4t(r, s_k + at<KP * 2>(16 * ks + (lane & 7) + (lane >> 4) * 8, (d0 + 16 * mm) / 8 + ((lane >> 3) & 1)));
 #pragma unroll
-                for (int e = 0; e < 4; ++e) top = __hmax2(top, __habs2(*reinterpret_cast<__half2*>(&r[e])));
+                for (int e = 0; e < 4; ++e) top[e >> 1] = __hmax2(top[e >> 1], __habs2(*reinterpret_cast<__half2*>(&r[e])));
               }
-            float big = fmaxf(__low2float(top), __high2float(top));
+              big = fmaxf(big, fmaxf(fminf(__low2float(top[0]), 65504.f) * w0.x, fminf(__high2float(top[0]), 65504.f) * w0.y));
+              big = fmaxf(big, fmaxf(fminf(__low2float(top[1]), 65504.f) * w1.x, fminf(__high2float(top[1]), 65504.f) * w1.y));
+            }
 #pragma unroll
             for (int x = 16; x; x >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, x));
-            big = fminf(big, 65504.f) * lds_f32(s_g + 12 * C + 4);
             const int to = big > 0.f ? max(min(exponent(big) - 14, 100), -100) : exp_w;
             const float move = pow2(exp_w - to);
 #pragma unroll

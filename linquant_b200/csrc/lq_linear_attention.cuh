@@ -78,8 +78,8 @@ struct Pair {
 // exponential is zero in fp32 either way, and the sums stay finite behind a step of minus infinity.
 template <int C>
 struct Decay {
-  static constexpr int PER = C / 32, BYTES = (3 * C + 4) * 4;
-  float hi[PER], lo[PER], out[PER], all, most;  // of this lane's tokens; of the whole chunk, and the largest of `out`: of the lane, behind largest() of all
+  static constexpr int PER = C / 32, BYTES = (3 * C + 4) * 4;  // on a 16-byte boundary again
+  float hi[PER], lo[PER], out[PER], all;  // of this lane's tokens; of the whole chunk
   // Sums of two floats each: a step of the scan is a dozen dependent fp32 additions, where one in 64 bits takes several times as long
   __device__ __forceinline__ Pair of(const float (&x)[PER]) {
     const int lane = threadIdx.x & 31;
@@ -98,23 +98,17 @@ struct Decay {
     }
     const Pair total(__shfl_sync(0xffffffffu, before.hi, 31), __shfl_sync(0xffffffffu, before.lo, 31));
     const Pair first(__shfl_up_sync(0xffffffffu, before.hi, 1), __shfl_up_sync(0xffffffffu, before.lo, 1));  // what the lanes before have
-    most = 0.f;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       const Pair s = lane ? first + sum[i] : sum[i];
       hi[i] = s.hi;
       lo[i] = s.lo;
       out[i] = ex2((total.hi - s.hi) + (total.lo - s.lo));
-      most = fmaxf(most, out[i]);
     }
     all = ex2(total.hi);
     return total;
   }
-  __device__ __forceinline__ void largest() {
-#pragma unroll
-    for (int m = 16; m; m >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, m));
-  }
-  // running sums, what they lost to rounding, decays to the chunk's end; its whole decay, the largest of them
+  // running sums, what they lost to rounding, decays to the chunk's end; its whole decay
   __device__ __forceinline__ void store(uint32_t s_g) const {
     const int lane = threadIdx.x & 31;
 #pragma unroll
@@ -124,10 +118,7 @@ struct Decay {
       sts_u32(to + 4 * C, __float_as_uint(lo[i]));
       sts_u32(to + 8 * C, __float_as_uint(out[i]));
     }
-    if (lane == 0) {
-      sts_u32(s_g + 12 * C, __float_as_uint(all));
-      sts_u32(s_g + 12 * C + 4, __float_as_uint(most));
-    }
+    if (lane == 0) sts_u32(s_g + 12 * C, __float_as_uint(all));
   }
 };
 

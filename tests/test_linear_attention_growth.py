@@ -95,7 +95,7 @@ def test_decays_that_grow(what, dtype, K, V, pad):
 
 @gpu
 @pytest.mark.parametrize("large", ["k", "v"])
-@pytest.mark.parametrize("K,V,pad", [(128, 128, 0), (64, 64, 0)])
+@pytest.mark.parametrize("K,V,pad", [(128, 128, 0), (64, 64, 0), (72, 64, 1)])
 def test_a_reset_behind_large_values(K, V, pad, large):
     """fp16: before a step of minus infinity keys (values) are 2^35 times those behind it. What a row, or the state, keeps has its own precision."""
     from linquant_b200.kernels.layer import linear_attention_fwd
