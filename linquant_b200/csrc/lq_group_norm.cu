@@ -345,7 +345,7 @@ __global__ void __launch_bounds__(WIDE, VEC >= 4 ? 1 : 2) group_norm_apply_kerne
   const float inv_n = n > 0 ? 1.f / (float)n : 0.f;
   for (int g = warp; g < groups; g += blockDim.x / 32) {
     const float2* sums = t.sums + (size_t)b * t.count * p.groups + g0 + g;
-    auto tokens_of = [&](int i) { return (float)min(max(n - i * t.tokens, 0), t.tokens); };
+    auto tokens_of = [&](int i) { return i < t.count ? (float)min(max(n - i * t.tokens, 0), t.tokens) : 0.f; };  // behind the last tile i tokens may pass 32 bits
     float mean = 0.f, m2 = 0.f;
     if (t.count <= 128) {
       float2 v[4];
