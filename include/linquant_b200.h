@@ -361,10 +361,12 @@ typedef struct {
   const int* adapters;         /* [M]: the adapter of each token; one outside 0..L-1 is none */
   const float* scaling;        /* [L] or null */
   float* t;                    /* scratch of lq_lora_workspace_bytes(M, R), 16-byte aligned */
+  float* share;                /* scratch of lq_lora_share_bytes(M, N, out_dtype), 16-byte aligned; null where that is 0 */
 } lq_lora_problem;
 /* lq_int8_linear, or with `values` lq_int8_linear_values, and in the same rounding
  * y[m,n] += sum_r t[m,r] b[l,n,r],  t[m,r] = scale scaling[l] sum_k x[m,k] a[l,r,k],  l = adapters[m];  x: the values, or codes times their scale */
 size_t lq_lora_workspace_bytes(int M, int R);
+size_t lq_lora_share_bytes(int M, int N, int out_dtype); /* the fp32 sums over r of more than 16 tokens with 16-bit outputs: 1 GiB, or 1024 tokens of wide rows, at most */
 int lq_lora_linear(const lq_linear_problem* p, const lq_lora_problem* q, const void* values, int dtype, long long stride, lq_stream stream);
 
 typedef struct {

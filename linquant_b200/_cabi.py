@@ -77,7 +77,7 @@ class GroupNormProblem(C.Structure):
 
 
 class LoraProblem(C.Structure):
-    _fields_ = _fields(int="L R dtype", float="scale", void_p="a b adapters scaling t")
+    _fields_ = _fields(int="L R dtype", float="scale", void_p="a b adapters scaling t share")
 
 
 class LinQuantError(RuntimeError):

@@ -862,6 +862,8 @@ PyObject* linear(PyObject* x_, PyObject* w_, PyObject* w_scale, PyObject* x_scal
       else q.scale = (float)number(lora[3]);
     }
     q.t = (float*)aligned(c.hold(scratch(lq_lora_workspace_bytes(p.M, q.R), c.dev)));
+    const size_t bytes = q.L > 0 ? lq_lora_share_bytes(p.M, p.N, p.out_dtype) : 0;
+    if (bytes) q.share = (float*)aligned(c.hold(scratch(bytes, c.dev)));
   }
   std::vector<int64_t> shape(x.sizes().begin(), x.sizes().end());
   shape.back() = N;

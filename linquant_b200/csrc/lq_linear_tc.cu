@@ -230,19 +230,25 @@ __global__ void __launch_bounds__(THREADS, 1) int8_linear_tc_kernel(const __grid
         sts_u32(cols + 4 * (S::HALF + c), __float_as_uint(in && p.bias ? __ldg(p.bias + n0 + c) : 0.f));
       }
       __syncwarp();
-      // What the adapter of this lane's row adds to the next chunk, from where it has been left in y: on its way while the chunk before is stored
-      [[maybe_unused]] Pack<TO, PER> low[CHUNK / PER];
+      // What the adapter of this lane's row adds to the next chunk: on its way while the chunk before is stored
+      [[maybe_unused]] float4 low[CHUNK / 4];
       [[maybe_unused]] const bool adapted = LORA && row0 + lane < p.M && lora.of(row0 + lane) >= 0;
       [[maybe_unused]] auto share = [&](int c0) {
         if (!adapted || c0 >= S::HALF) return;
-        const TO* from = reinterpret_cast<const TO*>(p.y) + (size_t)(row0 + lane) * p.N + n0 + c0;
+        if constexpr (sizeof(TO) == 2) {
 #pragma unroll
-        for (int j = 0; j < CHUNK; j += PER) {
-          if (wide) {
-            if (n0 + c0 + j < p.N) low[j / PER] = load_pack<TO, PER>(from + j);
-          } else {
+          for (int j = 0; j < CHUNK; j += 4)
+            if (n0 + c0 + j < p.N) low[j / 4] = *reinterpret_cast<const float4*>(lora.share_at(row0 + lane, n0 + c0 + j));
+        } else {
+          const float* from = lora.share + (size_t)(row0 + lane) * p.N + n0 + c0;
 #pragma unroll
-            for (int e = 0; e < PER; ++e) low[j / PER].v[e] = n0 + c0 + j + e < p.N ? from[j + e] : from_f32<TO>(0.f);
+          for (int j = 0; j < CHUNK; j += 4) {
+            if (wide) {
+              if (n0 + c0 + j < p.N) low[j / 4] = *reinterpret_cast<const float4*>(from + j);
+            } else {
+              auto at = [&](int e) { return n0 + c0 + j + e < p.N ? from[j + e] : 0.f; };
+              low[j / 4] = make_float4(at(0), at(1), at(2), at(3));
+            }
           }
         }
       };
@@ -269,12 +275,7 @@ __global__ void __launch_bounds__(THREADS, 1) int8_linear_tc_kernel(const __grid
         if constexpr (LORA) {
           if (adapted) {
 #pragma unroll
-            for (int j = 0; j < CHUNK; j += PER) {
-              float x[PER];
-              low[j / PER].get(x);
-#pragma unroll
-              for (int e = 0; e < PER; ++e) v[j + e] += x[e];
-            }
+            for (int j = 0; j < CHUNK; j += 4) v[j] += low[j / 4].x, v[j + 1] += low[j / 4].y, v[j + 2] += low[j / 4].z, v[j + 3] += low[j / 4].w;
           }
           share(c0 + CHUNK);
         }
@@ -453,11 +454,13 @@ __global__ void __launch_bounds__(THREADS, 2) int8_linear_split_kernel(const __g
       float f[4] = {fmaf((float)sum.x * xs[i], ws[0], bias[0]), fmaf((float)sum.y * xs[i], ws[1], bias[1]), fmaf((float)sum.z * xs[i], ws[2], bias[2]),
                     fmaf((float)sum.w * xs[i], ws[3], bias[3])};
       TO* to = y + (size_t)(m0 + row) * p.N + n;
-      if constexpr (LORA)  // the adapter's share has been left there
-        if (lora.of(m0 + row) >= 0)
+      if constexpr (LORA)
+        if (lora.of(m0 + row) >= 0) {
+          const float* low = sizeof(TO) == 2 ? lora.share_at(m0 + row, n) : lora.share + (size_t)(m0 + row) * p.N + n;
 #pragma unroll
           for (int j = 0; j < 4; ++j)
-            if (n + j < p.N) f[j] += to_f32(to[j]);
+            if (n + j < p.N) f[j] += low[j];
+        }
       if (wide) {
         Pack<TO, 4> out;
         out.set(f);
@@ -536,7 +539,7 @@ static int launch_split(const lq_linear_problem* p, const Lora* lora, int tiles,
 
 // The widest tiles that do not leave SMs idle: rounds of tiles x the time of one, which grows with its width and a fixed part
 // (the 128 rows of x that every tile loads)
-// `lora`: the rows to whose outputs something has been left to add, or null
+// `lora`: the rows to whose outputs something is to be added, and where it lies, or null
 int run_linear_tc(const lq_linear_problem* p, const Lora* lora, cudaStream_t st) {
   const long long mt = (p->M + 127) / 128, sms = sm_count();
   int best = 256;

@@ -3,8 +3,8 @@
 //   y[m,n] = (sum_k c[m,k] w[n,k]) x_scale[m] w_scale[n] + bias[n] + sum_r t[m,r] b[l,n,r],   t[m,r] = scaling[l] sum_k x[m,k] a[l,r,k]
 //
 // l = adapters[m]; c are x's codes. This file's first kernel makes t. Up to 16 tokens the INT8 product's kernel adds the second sum to its own in
-// fp32 (lq_lora.cuh). For more this file's second kernel leaves it in y and the product's kernels add it from there: what runs beside the
-// tcgen05 product on an SM's tensor cores waits for them (warp products in its epilogue: 510 us where the product alone takes 302, at
+// fp32 (lq_lora.cuh). For more this file's second kernel leaves it in fp32 scratch (for fp32 outputs in y itself) and the product's kernels add it
+// from there, to the sum that is then rounded once. What runs beside the tcgen05 product on an SM's tensor cores waits for them (warp products in its epilogue: 510 us where the product alone takes 302, at
 // 16384 x 2560 -> 10576 with rank 16; fp32 products there: 680).
 // t: a CTA has a tile of 1, 8 or 16 tokens and, of a cluster, a part of K; its four warps share that part and their sums meet in
 // shared memory, first the warps', then the CTAs', in a fixed order. Operands come from global memory straight into the fragments
@@ -315,22 +315,20 @@ static int run_shrink(Shrink p, bool vec, cudaStream_t st) {
 // ---- the second product: y[m,n] = sum_r t[m,r] b[l,n,r] for the tokens that have an adapter
 constexpr int CHUNK = 32, CT = CHUNK / 8;  // channels at a time, in tiles of 8
 
-// A warp: 16 MI tokens, SPAN channels. Over the adapters that the tokens have and their ranks in steps of 16; a step's operands are requested before
+// A warp: 16 MI tokens, SPAN channels; PT: pieces of t, two for 16-bit outputs and three for fp32. Over the adapters that the tokens have and their ranks in steps of 16; a step's operands are requested before
 // the products of the one ahead. The reduction index is permuted alike in both operands: a lane takes four consecutive r; and the channels of
 // a chunk, column 2 i + e of tile j being channel 8 i + 2 j + e, so that a lane holds eight consecutive ones of a row. Both operands are
-// bf16 pieces: two (three for fp32 outputs) of t and of fp16 and fp32 b, products below 16 (24) bits behind the first left out.
-// The INT8 product's kernel reads y again, adds its own sum in fp32 and rounds once more: this rounding is of the adapters' share alone.
-// Many tokens: bound by y's bytes (16384 x 10576, rank 16: 90 us, 3.9 TB/s, with a third of the issue slots). Few: by L2's latency.
-template <typename TO, typename TB, int SPAN, int MI>
-__global__ void __launch_bounds__(THREADS, sizeof(TO) == 2 ? (MI == 1 ? 6 : 4) : 3) lora_expand_kernel(const Lora q, int M, int N, TO* y) {
-  constexpr int PT = sizeof(TO) == 4 ? 3 : 2, PB = std::is_same_v<TB, __nv_bfloat16> ? 1 : PT;
+// bf16 pieces: PT of t and of fp16 and fp32 b, products below 16 (24) bits behind the first left out.
+// Many tokens: bound by the share's bytes (16384 x 10576, rank 16: 147 us, 4.7 TB/s). Few: by L2's latency.
+template <int PT, typename TB, int SPAN, int MI>
+__global__ void __launch_bounds__(THREADS, PT == 2 ? (MI == 1 ? 6 : 4) : 3) lora_expand_kernel(const Lora q, int M, int N) {
+  constexpr int PB = std::is_same_v<TB, __nv_bfloat16> ? 1 : PT;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
   const int columns = (N + WARPS * SPAN - 1) / (WARPS * SPAN), m0 = (int)(blockIdx.x / columns) * (16 * MI), n0 = ((int)(blockIdx.x % columns) * WARPS + warp) * SPAN;
   if (n0 >= N) return;
-  constexpr int PER = 16 / sizeof(TO);  // values of 16 bytes
   const int mine = lane < 16 * MI && m0 + lane < M ? q.of(m0 + lane) : -1;
   const uint32_t all = __ballot_sync(0xffffffffu, mine >= 0);
-  const bool wide = ((size_t)N * sizeof(TO)) % 16 == 0 && (reinterpret_cast<uintptr_t>(y) & 15u) == 0;
+  const bool wide = PT == 2 || (N % 4 == 0 && (reinterpret_cast<uintptr_t>(q.share) & 15u) == 0);
 
   // the step that is on its way
   int l = 0, r0 = 0, c0 = 0;
@@ -446,20 +444,17 @@ __global__ void __launch_bounds__(THREADS, sizeof(TO) == 2 ? (MI == 1 ? 6 : 4) :
         const int row = 16 * i + 8 * h + g;
         if (!(now >> row & 1)) continue;
         const int n = n0 + at + 8 * t4;
-        TO* to = y + (size_t)(m0 + row) * N + n;
 #pragma unroll
-        for (int c = 0; c < 8; c += PER) {
-          Pack<TO, PER> out;
-          float x[PER];
-#pragma unroll
-          for (int v = 0; v < PER; ++v) x[v] = s[i][(c + v) / 2][2 * h + (v & 1)];
-          out.set(x);
+        for (int c = 0; c < 8; c += 4) {
+          const float4 x = make_float4(s[i][c / 2][2 * h], s[i][c / 2][2 * h + 1], s[i][c / 2 + 1][2 * h], s[i][c / 2 + 1][2 * h + 1]);
+          float* to = PT == 2 ? q.share_at(m0 + row, n + c) : q.share + (size_t)(m0 + row) * N + n + c;
           if (wide) {
-            if (n + c < N) store_pack(to + c, out);
+            if (n + c < N) *reinterpret_cast<float4*>(to) = x;
           } else {
-#pragma unroll
-            for (int v = 0; v < PER; ++v)
-              if (n + c + v < N) to[c + v] = out.v[v];
+            if (n + c < N) to[0] = x.x;
+            if (n + c + 1 < N) to[1] = x.y;
+            if (n + c + 2 < N) to[2] = x.z;
+            if (n + c + 3 < N) to[3] = x.w;
           }
         }
       }
@@ -468,24 +463,37 @@ __global__ void __launch_bounds__(THREADS, sizeof(TO) == 2 ? (MI == 1 ? 6 : 4) :
 }
 
 static int expand(const Lora& q, const lq_linear_problem* p, cudaStream_t st) {
-  return with_dtype(p->out_dtype, "lora_linear", [&](auto t) {
-    using TO = decltype(t);
-    return with_dtype(q.dtype, "lora_linear", [&](auto tb) {
-      using TB = decltype(tb);
+  return with_dtype(q.dtype, "lora_linear", [&](auto tb) {
+    using TB = decltype(tb);
+    auto pieces = [&](auto pt) {
+      constexpr int PT = decltype(pt)::value;
       // Few tokens: warps of 16 of them and 32 channels, as many as there can be, each of which goes over all adapters of its tokens one after
-      // the other (333 x 10576, rank 32, runs of 7: 34 us where the others' warps of 32 and 128 take 53; 1000 x 2560 25 and 27). Many: these
-      // read b half as often (1000 x 10576, rank 16: 45 us and 49, 16384 tokens 475 and 559)
+      // the other (333 x 10576, rank 32, runs of 7: 40 us where the others' warps of 32 and 128 take 63; 1000 x 2560 25 and 27). Many: these
+      // read b half as often (1000 x 10576, rank 16: 49 us and 54, 16384 tokens 519 and 595)
       auto go = [&](auto kern, int span, int tokens) {
         const long long rows = ((long long)p->M + tokens - 1) / tokens;
         const long long ctas = rows * ((p->N + WARPS * span - 1) / (WARPS * span));
         if (ctas >= 1ll << 31) return fail(LQ_ERR_SHAPE, "lora_linear: M=%d N=%d", p->M, p->N);
-        const cudaError_t e = launch(kern, dim3((unsigned)ctas), dim3(THREADS), 0, st, q, p->M, p->N, reinterpret_cast<TO*>(p->y));
+        const cudaError_t e = launch(kern, dim3((unsigned)ctas), dim3(THREADS), 0, st, q, p->M, p->N);
         return e != cudaSuccess ? fail(LQ_ERR_LAUNCH, "lora_linear: %s", cudaGetErrorString(e)) : check_launch("lora_expand_kernel");
       };
-      return ((long long)p->M + 31) / 32 * ((p->N + 127) / 128) <= 10ll * sm_count() ? go(lora_expand_kernel<TO, TB, 32, 1>, 32, 16) : go(lora_expand_kernel<TO, TB, 128, 2>, 128, 32);
-    });
+      return ((long long)p->M + 31) / 32 * ((p->N + 127) / 128) <= 10ll * sm_count() ? go(lora_expand_kernel<PT, TB, 32, 1>, 32, 16) : go(lora_expand_kernel<PT, TB, 128, 2>, 128, 32);
+    };
+    return p->out_dtype == LQ_F32 ? pieces(std::integral_constant<int, 3>()) : pieces(std::integral_constant<int, 2>());
   });
 }
+
+// 16-bit outputs of more than kFewTokens tokens: in slabs whose fp32 shares take about 1 GiB (and 1024 tokens at least), each made and added
+// before the next one's. None has few tokens: they are of one size, but for the rounding to whole blocks of 32
+struct Slabs {
+  long long M, count, blocks;
+  Slabs(int m, int N) : M(m), blocks(((long long)N + 3) / 4) {
+    const long long most = (1ll << 26) / blocks < 1024 ? 1024 : (1ll << 26) / blocks;
+    count = (M + most - 1) / most;
+  }
+  int start(long long i) const { return i >= count ? (int)M : (int)(M * i / count & ~31ll); }
+  size_t bytes() const { return (size_t)((M + count - 1) / count / 32 + 2) * 32 * blocks * 16; }
+};
 
 }  // namespace lora
 
@@ -497,6 +505,10 @@ bool linear_makes_codes(const lq_linear_problem* p);
 }  // namespace lq
 
 extern "C" size_t lq_lora_workspace_bytes(int M, int R) { return M <= 0 || R <= 0 ? 0 : (size_t)M * ((R + 15) / 16 * 16) * 4; }
+extern "C" size_t lq_lora_share_bytes(int M, int N, int out_dtype) {
+  if (M <= lq::kFewTokens || N <= 0 || out_dtype == LQ_F32) return 0;
+  return lq::lora::Slabs(M, N).bytes();
+}
 
 extern "C" int lq_lora_linear(const lq_linear_problem* p, const lq_lora_problem* q, const void* values, int dtype, long long stride, lq_stream stream) {
   using namespace lq;
@@ -512,6 +524,9 @@ extern "C" int lq_lora_linear(const lq_linear_problem* p, const lq_lora_problem*
   if (!q->a || !q->b || !q->adapters || !q->t) return fail(LQ_ERR_NULL, "lora_linear: a, b, adapters and t must be non-null");
   if ((reinterpret_cast<uintptr_t>(q->b) | reinterpret_cast<uintptr_t>(q->t)) & 15u) return fail(LQ_ERR_ALIGN, "lora_linear: b and t start on 16-byte boundaries");
   const int RP = (q->R + 15) / 16 * 16, size = dtype_bytes(q->dtype);
+  const bool scratch = lq_lora_share_bytes(p->M, p->N, p->out_dtype) > 0;
+  if (scratch && !q->share) return fail(LQ_ERR_NULL, "lora_linear: share must be non-null for 16-bit outputs of %d tokens", p->M);
+  if (scratch && (reinterpret_cast<uintptr_t>(q->share) & 15u)) return fail(LQ_ERR_ALIGN, "lora_linear: share starts on a 16-byte boundary");
   const lora::Shrink s{p->M, p->K, q->L, q->R, RP, 1, values ? stride : p->x_stride, values ? values : p->x, q->a, values ? nullptr : p->x_scale,
                        q->adapters, q->scaling, q->scale, p->M > kFewTokens && p->out_dtype != LQ_F32, q->t};
   Alignment a;
@@ -530,8 +545,27 @@ extern "C" int lq_lora_linear(const lq_linear_problem* p, const lq_lora_problem*
     return with_dtype(dtype, "lora_linear", [&](auto tx) { return lora::run_shrink<decltype(tx), TA>(s, vec, st); });
   });
   if (e != LQ_OK) return e;
-  const Lora add{q->L, q->R, RP, q->dtype, q->b, q->adapters, q->t};
-  if (p->M > kFewTokens)
+  Lora add{q->L, q->R, RP, q->dtype, q->b, q->adapters, q->t, nullptr, 0};
+  if (p->M <= kFewTokens) return values && !rows ? run_linear_values(p, &add, values, dtype, stride, st) : run_linear(p, &add, st);
+  if (!scratch) {
+    add.share = reinterpret_cast<float*>(p->y);
     if (int e2 = lora::expand(add, p, st)) return e2;
-  return values && !rows ? run_linear_values(p, &add, values, dtype, stride, st) : run_linear(p, &add, st);
+    return run_linear(p, &add, st);
+  }
+  const lora::Slabs slabs(p->M, p->N);
+  add.share = q->share;
+  add.blocks = (int)slabs.blocks;
+  for (long long i = 0; i < slabs.count; ++i) {
+    const int from = slabs.start(i);
+    lq_linear_problem part = *p;
+    part.M = slabs.start(i + 1) - from;
+    part.x = p->x + from * p->x_stride;
+    part.x_scale = p->x_scale + from;
+    part.y = reinterpret_cast<uint16_t*>(p->y) + (size_t)from * p->N;
+    add.adapters = q->adapters + from;
+    add.t = q->t + (size_t)from * RP;
+    if (int e2 = lora::expand(add, &part, st)) return e2;
+    if (int e2 = run_linear(&part, &add, st)) return e2;
+  }
+  return LQ_OK;
 }

@@ -2,8 +2,8 @@
 //
 //   y[m,n] += sum_r t[m,r] b[l,n,r],   l = adapters[m],   t[m,r] = scaling[l] x_scale[m] sum_k x[m,k] a[l,r,k]      (lq_lora.cu)
 //
-// Few tokens (at most 16): the product's kernel makes the sum itself. More: a kernel of its own has left it in y, in y's type, for the rows
-// that have an adapter.
+// Few tokens (at most 16): the product's kernel makes the sum itself. More: a kernel of its own has left it in fp32 for the rows that have an
+// adapter (`share`), so that it joins the shared sum before either is rounded to y's type.
 #pragma once
 #include "lq_layer.cuh"
 
@@ -17,6 +17,13 @@ struct Lora {
   const void* b;       // [L,N,R]
   const int* adapters; // [M]: which adapter a token has; one outside 0..L-1 is none
   const float* t;      // [M,RP]; 16-bit outputs of more than kFewTokens tokens: as two bf16 pieces of four values each
+  // More than kFewTokens tokens. fp32 outputs: y itself, rows of N values. Else blocks of 32 tokens x 4 channels, channels before tokens: where the
+  // product's lanes have a token each they read whole lines (in rows a line is fetched twice: 16384 x 2560 -> 10576, rank 16, 674 us, 514)
+  float* share;
+  int blocks;          // of 4 channels; 0 for rows
+  __device__ __forceinline__ float* share_at(int m, int n) const {  // n: a multiple of 4
+    return share + ((((long long)(m >> 5) * blocks + (n >> 2)) << 5) + (m & 31)) * 4;
+  }
   __device__ __forceinline__ int of(int m) const {
     const int l = __ldg(adapters + m);
     return (unsigned)l < (unsigned)L ? l : -1;

@@ -32,7 +32,10 @@ def lora_linear_fwd(x, w, w_scale, lora_a, lora_b, adapters, scaling=None, x_sca
     lora_a (L,R,K), lora_b (L,N,R) of one type, f16/bf16/f32; R up to 128, a multiple of 8 is read in place, others are copied:
     lay adapters out once with ``stack_adapters``. ``adapters`` (..): which of the L each row has; one outside 0..L-1 has none.
     ``scaling`` a number or (L,). Rows that lie next to one another with one adapter share its reads. Returns y (.., N) in
-    ``out_dtype`` (x's type; bf16 for codes)."""
+    ``out_dtype`` (x's type; bf16 for codes).
+
+    The share is an fp32 sum whatever y's type, and joins the shared product's before either is rounded: it may be larger than y's type holds. With
+    16-bit outputs of more than 16 rows x a and b go into it as two bf16 numbers each (16 bits), and it takes up to 1 GiB of scratch."""
     r = _cabi.host().lora_linear(x, w, w_scale, lora_a, lora_b, adapters, scaling, x_scale, bias, out_dtype)
     if r is None:
         _layer.require_cuda(x, "lora_linear_fwd")
