@@ -31,7 +31,7 @@ def lora_linear_fwd(x, w, w_scale, lora_a, lora_b, adapters, scaling=None, x_sca
 
     lora_a (L,R,K), lora_b (L,N,R) of one type, f16/bf16/f32; R up to 128, a multiple of 8 is read in place, others are copied:
     lay adapters out once with ``stack_adapters``. ``adapters`` (..): which of the L each row has; one outside 0..L-1 has none.
-    ``scaling`` a number or (L,). Rows that lie next to one another with one adapter share its reads. Returns y (.., N) in
+    ``scaling`` a number, one on the device or (L,). Rows that lie next to one another with one adapter share its reads. Returns y (.., N) in
     ``out_dtype`` (x's type; bf16 for codes).
 
     The share is an fp32 sum whatever y's type, and joins the shared product's before either is rounded: it may be larger than y's type holds. With
@@ -54,12 +54,14 @@ def lora_linear_fwd(x, w, w_scale, lora_a, lora_b, adapters, scaling=None, x_sca
         lead, pad = x.shape[:-1], -lora_a.shape[1] % 8
         adapters = torch.as_tensor(adapters)
         assert adapters.shape == lead, f"adapters has shape {tuple(adapters.shape)}, {tuple(lead)} expected"
+        if torch.is_tensor(scaling) and scaling.dim() == 0:  # on the device it is read there
+            scaling = scaling.expand(lora_a.shape[0]) if scaling.is_cuda else float(scaling)
         if pad:
             lora_a, lora_b = F.pad(lora_a, (0, 0, 0, pad)), F.pad(lora_b, (0, pad))
         lora_b = lora_b.contiguous()
         r = _cabi.host().lora_linear(
             _codes("x", x) if x_scale is not None else _layer.rows("x", x), _codes("w", w), _layer.parameter("w_scale", w_scale, (N,), x),
             lora_a.contiguous(), lora_b if lora_b.data_ptr() % 16 == 0 else lora_b.clone(), _layer.integers("adapters", adapters.reshape(-1), lead.numel(), x).view(lead),
-            _layer.parameter("scaling", scaling, (lora_a.shape[0],), x) if torch.is_tensor(scaling) and scaling.dim() else None if scaling is None else float(scaling),
+            _layer.parameter("scaling", scaling, (lora_a.shape[0],), x) if torch.is_tensor(scaling) else None if scaling is None else float(scaling),
             _layer.parameter("x_scale", x_scale, lead, x), _layer.parameter("bias", bias, (N,), x), out_dtype)
     return _layer.result(r, "lora_linear_fwd")
