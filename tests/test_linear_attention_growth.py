@@ -15,7 +15,7 @@ def seed():
     torch.manual_seed(17)
 
 
-def lost(q, k, v, g, scale, dtype):
+def lost(q, k, v, g, scale, dtype, initial=None):
     """What fp16 does not hold beside the largest value of a set that goes under one power of two: the largest is 2^14 at least, half the
     distance of the smallest numbers 2^-25, so 2^-39 of the largest at most for each value, times the other operand. The sets: a row of
     decayed q k^T; what a chunk adds to the state, decayed to the chunk's end (v on tcgen05, k on warp MMA: the larger bound of both); the state
@@ -26,7 +26,7 @@ def lost(q, k, v, g, scale, dtype):
     if dtype != F16:
         return o, h
     q, k, v = (x.double().repeat_interleave(H // x.shape[2], 2).movedim(2, 1) for x in (q, k, v))
-    g, state, part = g.double().movedim(2, 1).clamp(min=-1e3), h.clone(), 2.0**-39
+    g, state, part = g.double().movedim(2, 1).clamp(min=-1e3), h.clone() if initial is None else initial.double(), 2.0**-39
     for t in range(0, T, 64):
         qc, kc, vc, G = q[:, :, t:t + 64], k[:, :, t:t + 64], v[:, :, t:t + 64], g[:, :, t:t + 64].cumsum(-1)
         C = G.shape[-1]
