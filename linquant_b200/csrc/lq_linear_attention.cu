@@ -555,7 +555,7 @@ __global__ void __launch_bounds__(sizeof(T) == 4 && KP <= 128 ? 256 : 128, sizeo
 #pragma unroll
       for (int j = 0; j < NT; ++j)
         to[(m * NT + j) * S::THREADS + tid] = make_float4(st[m][j][0] * back, st[m][j][1] * back, st[m][j][2] * back, st[m][j][3] * back);
-    if (vt == 0 && tid == 0) seg.decays[(size_t)blockIdx.y * (gridDim.x / vts) + bh] = ex2(total.hi);
+    if (vt == 0 && tid == 0) seg.decays[(size_t)blockIdx.y * (gridDim.x / vts) + bh] = total.hi;
   } else {
     if (p.final_state != nullptr && (int)blockIdx.y == (n > 0 ? (n - 1) / seg.tokens : 0)) {
       float* to = p.final_state + (size_t)bh * p.K * p.V + v0;
@@ -580,6 +580,7 @@ __global__ void __launch_bounds__(sizeof(T) == 4 && KP <= 128 ? 256 : 128, sizeo
 }
 
 // What leaves a segment: its own state and, decayed, what entered it. One thread has four values of all segments, eight of them on their way.
+// The decay goes in by its square root, twice: tokens that grow may multiply a segment by more than fp32 holds where what they multiply is small, or zero.
 __global__ void __launch_bounds__(128) segment_states_kernel(const Segments seg, int heads, long long values, int values_a_head) {
   constexpr int U = 8;
   pdl_enter();
@@ -594,13 +595,14 @@ __global__ void __launch_bounds__(128) segment_states_kernel(const Segments seg,
     for (int u = 0; u < U; ++u) {
       const int k = min(k0 + u, last);
       own[u] = *reinterpret_cast<const float4*>(seg.states + (size_t)k * values + i);
-      a[u] = __ldg(seg.decays + (size_t)k * heads + bh);
+      a[u] = ex2(0.5f * __ldg(seg.decays + (size_t)k * heads + bh));
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int k = k0 + u;
       if (k > last) break;
-      s = k == 0 ? own[u] : make_float4(fmaf(a[u], s.x, own[u].x), fmaf(a[u], s.y, own[u].y), fmaf(a[u], s.z, own[u].z), fmaf(a[u], s.w, own[u].w));
+      auto on = [&](float before, float own) { return before == 0.f ? own : fmaf(a[u], a[u] * before, own); };
+      s = k == 0 ? own[u] : make_float4(on(s.x, own[u].x), on(s.y, own[u].y), on(s.z, own[u].z), on(s.w, own[u].w));
       if (k > 0) *reinterpret_cast<float4*>(seg.states + (size_t)k * values + i) = s;
     }
   }

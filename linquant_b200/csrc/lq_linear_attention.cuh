@@ -48,7 +48,7 @@ __device__ __forceinline__ int exponent(float m) {
 struct Segments {
   int count, tokens;  // of a segment: a multiple of 64
   float* states;      // [count - 1][B * H][V tiles][floats of a tile]: what leaves a segment
-  float* decays;      // [count - 1][B * H]
+  float* decays;      // [count - 1][B * H]: log2 of a segment's decay, which may leave fp32 itself
 };
 
 // The log-decays of a chunk's tokens from t0, C / 32 a lane; none behind the sequence's n tokens

@@ -593,7 +593,7 @@ __global__ void __launch_bounds__(32 * WARPS, 1) linear_attention_tc_kernel(cons
   __syncthreads();
   if (STATES && vt == 0 && tid == 0) {
     const Pair even(lds_f32(s0 + S::SUM), lds_f32(s0 + S::SUM + 4)), odd(lds_f32(s0 + S::SUM + 8), lds_f32(s0 + S::SUM + 12));
-    seg.decays[(size_t)blockIdx.y * (gridDim.x / vts) + bh] = ex2((even + odd).hi);
+    seg.decays[(size_t)blockIdx.y * (gridDim.x / vts) + bh] = (even + odd).hi;
   }
   if (warp == ISSUER) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tbase), "r"(512u) : "memory");
 }

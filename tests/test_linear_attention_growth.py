@@ -117,3 +117,35 @@ def test_a_reset_behind_large_values(K, V, pad, large):
     rel = OUT[F16] + chunks * CHUNK
     outputs(o, wo, mag + lo / rel, rel)
     ref.check(state, h, m + lh / (chunks * CHUNK), chunks * CHUNK)
+
+
+@gpu
+@pytest.mark.parametrize("start", [0.0, 1e-36])
+@pytest.mark.parametrize("dtype,K", [(F16, 128), (BF16, 128), (BF16, 200), (F32, 64)])
+def test_a_segment_that_grows_by_more_than_fp32_holds(dtype, K, start):
+    """e^102 over 128 tokens, where the state is nothing, or so little that what comes of it is a number."""
+    from linquant_b200.kernels.layer import linear_attention_fwd
+
+    T, V = 2000, 64
+    q, k, v, _ = inputs(1, T, 1, 1, K, V, dtype)
+    g = torch.full((1, T, 1), -0.05, device="cuda")
+    g[0, 256:384] = 0.8
+    k[:, :400] = 0
+    s0 = torch.randn(1, 1, K, V, device="cuda") * start
+    scale = 1e-7 if start else 1.0
+    wo, mag, h, m = recurrence(q, k, v, g, scale, s0, None)
+    o, state = linear_attention_fwd(q, k, v, g, scale=scale, initial_state=s0, output_final_state=True)
+    lo, lh = lost(q, k, v, g, scale, dtype, s0)
+    chunks = T // 64 + 2
+    rel = OUT[dtype] + chunks * CHUNK
+    # A state of 1e-36 has come down to 3e-42 when it starts to grow, below what fp32 (2^-126) and its bf16 pieces hold in full: an fp32 product or sum there
+    # is off by 2^-150, four of them a chunk, and what q reads by half of bf16's smallest number, 2^-134. Both grow from there like the state itself. Outputs in front
+    # of the growth, 1e-43, are off by half of their type's smallest number.
+    G, low_state, low_read = g.double().flatten(), 0.0, torch.zeros(1, T, 1, 1, device="cuda", dtype=torch.float64)
+    for t in range(0, T, 64):
+        up = torch.exp(G[t:t + 64].cumsum(0))
+        low_read[0, t:t + 64, 0, 0] = up * (low_state + 2.0**-134)
+        low_state = float(up[-1]) * low_state + 2.0**-148
+    lo = lo + abs(scale) * low_read * q.double().abs().sum(-1, keepdim=True) + {F16: 0.0, BF16: 2.0**-134, F32: 2.0**-150}[dtype]
+    ref.check(o, wo, mag + lo / rel, rel)
+    ref.check(state, h, m + (lh + low_state) / (chunks * CHUNK), chunks * CHUNK)
