@@ -13,7 +13,7 @@
 // three; codes or fp16 with fp16 as they are), six products for fp32.
 // Both kernels let their successors start at once (pdl_trigger()): the product's loads and sums run beside them, and wait for t or the share where
 // it is added. 3 tokens, 5120 -> 2560, rank 16: 11.4 us in a row, 15.6 without, 9.3 the product alone.
-// t of 333 x 2560 codes, rank 32, 24 adapters in runs of 7: 11 us, bound by latency, a tile's adapters one after the other; of 16384 x 2560, rank 16:
+// 16384 tokens, 2560 -> 10576, rank 16: 514 us in a row, the product alone 310. t of 333 x 2560 codes, rank 32, 24 adapters in runs of 7: 11 us, bound by latency, a tile's adapters one after the other; of 16384 x 2560, rank 16:
 // 22 us (42 MB of codes from HBM or L2, half of the issue slots).
 #include "lq_lora.cuh"
 #include "lq_tc.cuh"
@@ -492,7 +492,7 @@ struct Slabs {
     count = (M + most - 1) / most;
   }
   int start(long long i) const { return i >= count ? (int)M : (int)(M * i / count & ~31ll); }
-  size_t bytes() const { return (size_t)((M + count - 1) / count / 32 + 2) * 32 * blocks * 16; }
+  size_t bytes() const { return (size_t)(count == 1 ? (M + 31) / 32 : M / count / 32 + 2) * 32 * blocks * 16; }  // a slab: M / count + 31 tokens at most
 };
 
 }  // namespace lora

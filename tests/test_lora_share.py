@@ -103,6 +103,7 @@ def share_bytes(M, N, out):
 
 def test_scratch_of_the_share():
     assert share_bytes(16, 4096, 1) == 0 and share_bytes(40, 4096, 2) == 0 and share_bytes(17, 0, 1) == 0  # few tokens; fp32 outputs; nothing
+    assert share_bytes(17, 1000, 1) == 32 * 1000 * 4 and share_bytes(16384, 10576, 0) == 16384 * 10576 * 4  # one slab: whole blocks of 32 tokens
     for M, N in ((17, 1), (33, 77), (16384, 10576), (150_001, 4100), (2_100_003, 1032), (2**31 - 9000, 7), (2**31 - 9000, 2**20)):
         n = share_bytes(M, N, 1)
         pitch = (N + 3) // 4 * 4
