@@ -10,8 +10,8 @@
 // and sum of squared distances (a channel's values by eights around their own mean, merged by the exact formula for two
 // sets, then channels, tokens and tiles the same way); the second merges the tiles of its sequence and writes y, reading x from
 // L2 where it fits there. All sums are fp32, in a fixed order.
-// 32768 x 2048 fp16 in 16 groups with a gate: 86 us, 4.7 TB/s (half of HBM's cycles, 56 % of the issue slots: two exponentials and reciprocals a value with
-// activation and gate); without a gate, bf16: 62 us, 4.3 TB/s. Over 6 x 1499 tokens x 1026 channels, ragged: 23 us, the latency of two kernels whose
+// 32768 x 2048 fp16 in 16 groups with a gate: 86 us, 4.7 TB/s (half of HBM's cycles, 56 % of the issue slots); without a gate, bf16: 62 to 68 us, 4.0 to 4.3 TB/s. No
+// unit is full: a team requests its next rows behind the two sums of these. Over 6 x 1499 tokens x 1026 channels, ragged: 23 us, the latency of two kernels whose
 // accesses are 4 bytes wide, as rows of 2052 bytes allow; a round of CTAs is best (tiles of half the tokens, two rounds: 27).
 #include "lq_layer.cuh"
 

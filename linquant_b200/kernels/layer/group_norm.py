@@ -11,8 +11,8 @@ from ... import _cabi
 
 def group_norm_fwd(x, num_groups, weight=None, bias=None, activation=None, gate=None, eps=1e-5, over_tokens=False, lengths=None):
     """x (.., D) f16/bf16/f32; mean and variance over the D / num_groups channels of each group, for each token by itself. With
-    ``over_tokens`` x is (B,T,D) and they are taken over all tokens of a sequence as well; ``lengths`` (B,): tokens of each sequence
-    that count, y is zero behind them and nothing there is read. weight, bias (D,). ``activation`` "silu" or None. ``gate``, shaped
+    ``over_tokens`` x is (B,T,D) and they are taken over all tokens of a sequence as well (for encoders: later tokens reach earlier ones);
+    ``lengths`` (B,): tokens of each sequence that count, y is zero behind them and nothing there is read. weight, bias (D,). ``activation`` "silu" or None. ``gate``, shaped
     and typed like x, may be a slice of a wider projection: y is multiplied by its SiLU, after the activation.
 
     Returns y, dense, in x's type. Sums are fp32, around each group's own mean."""
