@@ -14,7 +14,7 @@
 // as three bf16 pieces (all 24 bits; fp16: two pieces under a power of two of the largest of them, 22 bits), the state that q
 // reads and the decayed products q.k as two pieces (16 or 22 bits). fp32 operands are three bf16 pieces each, six products.
 //
-// 16-bit prompts whose rows TMA takes run in lq_linear_attention_tc.cu (4 x 4096 x 16 heads of 128 x 128, bf16: 91 us, 334 here, 600 with heads off 16-byte
+// 16-bit prompts whose rows TMA takes run in lq_linear_attention_tc.cu (4 x 4096 x 16 heads of 128 x 128, bf16: 102 us, 334 here, 600 with heads off 16-byte
 // boundaries, whose values come one by one; of 256 x 128 968, fp32 957). What is left is bound by warp MMA's own latencies: 5 x 611 x 6 heads of 72 x 100, fp32, 87 us with the call, tensor pipe 29 % busy, HBM 1 %.
 #include <math_constants.h>
 

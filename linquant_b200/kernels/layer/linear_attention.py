@@ -41,9 +41,7 @@ def linear_attention_fwd(q, k, v, g=None, scale=None, initial_state=None, length
     An infinity or NaN in q, k, v or g may reach every token of its chunk of 64, the ones before it too, and those that follow. Log-decays may be
     minus infinity (what came before is forgotten) or positive, up to 88 in all between two tokens of a chunk.
 
-    Returns (o (B,T,H,V), final_state (B,H,K,V) fp32 or None). States are fp32 throughout. 16-bit prompts of more than 64 tokens with K <= 128 and
-    rows on 16-byte boundaries run on tcgen05, where each term of an output is rounded to the type once, like the output itself; all other calls, fp32
-    ones among them, round outputs alone. In fp16 what a chunk leaves to the state is kept to 2^-39 of the chunk's largest decayed value."""
+    Returns (o (B,T,H,V), final_state (B,H,K,V) fp32 or None). States are fp32 throughout; outputs are rounded once. In fp16 what a chunk leaves to the state is kept to 2^-39 of the chunk's largest decayed value."""
     r = _cabi.host().linear_attention(q, k, v, g, scale, initial_state, lengths, output_final_state)
     if r is None:
         lead, H, V, q, k, v = _heads("linear_attention_fwd", q, k, v, 4)

@@ -1,5 +1,5 @@
-"""The forms of linear attention's prompts, each with the bound that its own roundings give: on tcgen05 (16-bit operands of more than 64
-tokens, K <= 128, rows on 16-byte boundaries) and on warp MMA (the others)."""
+"""The forms of linear attention's prompts, held to what their pieces leave: on tcgen05 (16-bit operands of more than 64 tokens, K <= 128, rows
+on 16-byte boundaries) and on warp MMA (the others)."""
 
 import pytest
 import torch
@@ -10,11 +10,9 @@ from tests.test_linear_attention_growth import lost
 
 gpu = pytest.mark.gpu
 
-# Beside its own rounding an output has those of the terms it is summed of. On tcgen05 a term goes through a decayed q.k or through the
-# state that q reads, each rounded once to the type: half a step. On warp MMA both are two pieces: half a step squared; three pieces
-# of fp32 operands leave 2^-24 a product, four of which meet.
-TC = {BF16: 2.0**-8, F16: 2.0**-11}
-WARP = {BF16: 2.0**-16, F16: 2.0**-22, F32: 2.0**-22}
+# Beside its own rounding an output has those of the terms it is summed of. A term goes through a decayed q.k or through the state that q
+# reads, each in two pieces of the type: half a step squared; three pieces of fp32 operands leave 2^-24 a product, four of which meet.
+TERMS = {BF16: 2.0**-16, F16: 2.0**-22, F32: 2.0**-22}
 
 
 @pytest.fixture(autouse=True)
@@ -29,7 +27,7 @@ def rows(B, T, heads, width, pitch, dtype):
     return x[..., :width]
 
 
-def compare(q, k, v, g, s0, n, terms):
+def compare(q, k, v, g, s0, n):
     from linquant_b200.kernels.layer import linear_attention_fwd
 
     B, T, H, V = v.shape
@@ -43,7 +41,7 @@ def compare(q, k, v, g, s0, n, terms):
                 x[b, max(int(n[b]), 0):] = float("nan")
     o, state = linear_attention_fwd(q, k, v, g, initial_state=s0, lengths=n, output_final_state=True)
     chunks = T // 64 + 2
-    rel = terms[dtype] + chunks * CHUNK
+    rel = TERMS[dtype] + chunks * CHUNK
     ref.check(o, want[0], want[1] + lo / rel, rel)
     ref.check(state, want[2], want[3] + lh / (chunks * CHUNK), chunks * CHUNK)
     for b in range(B):
@@ -68,7 +66,7 @@ def decays(B, T, H):
 ])
 def test_segments_on_tcgen05(B, T, Hk, H, K, V, lengths, initial, dtype):
     q, k, v = rows(B, T, Hk, K, K, dtype), rows(B, T, Hk, K, K, dtype), rows(B, T, H, V, V, dtype)
-    compare(q, k, v, decays(B, T, H), randn(B, H, K, V) if initial else None, None if lengths is None else ints(*lengths), TC)
+    compare(q, k, v, decays(B, T, H), randn(B, H, K, V) if initial else None, None if lengths is None else ints(*lengths))
 
 
 @gpu
@@ -82,7 +80,7 @@ def test_widths_on_tcgen05(T, K, V, lengths, dtype):
     B, Hk, H = 1, 1, 2
     up = lambda n: (n + 7) // 8 * 8  # noqa: E731
     q, k, v = rows(B, T, Hk, K, up(K), dtype), rows(B, T, Hk, K, up(K) + 8, dtype), rows(B, T, H, V, up(V), dtype)
-    compare(q, k, v, decays(B, T, H), None, None if lengths is None else ints(*lengths), TC)
+    compare(q, k, v, decays(B, T, H), None, None if lengths is None else ints(*lengths))
 
 
 @gpu
@@ -93,6 +91,6 @@ def test_widths_on_tcgen05(T, K, V, lengths, dtype):
     (130, 200, 64, 200), (200, 256, 32, 256), (1500, 136, 40, 136),                  # wide heads
 ])
 def test_warp_mma(T, K, V, pitch, dtype):
-    """Calls of one chunk among them, whose outputs are sums of few terms: nothing but their own rounding is of the type's size."""
+    """Calls of one chunk among them."""
     q, k, v = rows(1, T, 2, K, pitch, dtype), rows(1, T, 2, K, pitch, dtype), rows(1, T, 2, V, V, dtype)
-    compare(q, k, v, decays(1, T, 2), None, None, WARP)
+    compare(q, k, v, decays(1, T, 2), None, None)

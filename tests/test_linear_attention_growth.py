@@ -5,9 +5,12 @@ import pytest
 import torch
 
 from tests import layer_reference as ref
-from tests.test_linear_attention import BF16, CHUNK, F16, F32, OUT, inputs, recurrence
+from tests.test_linear_attention import BF16, CHUNK, F16, F32, inputs, recurrence
 
 gpu = pytest.mark.gpu
+
+# Decayed q.k and the state that q reads are two pieces of the type, fp32 operands three: half a step squared, or 2^-24 for each of four products
+OUT = {BF16: 2.0**-16, F16: 2.0**-22, F32: 2.0**-22}
 
 
 @pytest.fixture(autouse=True)
